@@ -33,6 +33,21 @@ class HgkOp(C.Structure):
                 ("offsets", C.c_void_p), ("offset", C.c_int32)]
 
 
+class HgkKvPages(C.Structure):
+    """hgk_kv_pages of include/higgs_hip.h (a pool of key and value pages)."""
+    _fields_ = [("dtype", C.c_int), ("page_size", C.c_int), ("n_pages", C.c_int64),
+                ("kv_heads", C.c_int64), ("head_dim", C.c_int64),
+                ("k", C.c_void_p), ("k_strides", C.c_int64 * 3),
+                ("v", C.c_void_p), ("v_strides", C.c_int64 * 3)]
+
+
+class HgkKvBatch(C.Structure):
+    """hgk_kv_batch of include/higgs_hip.h (a batch's new tokens and its page table)."""
+    _fields_ = [("batch", C.c_int64), ("tokens", C.c_int64), ("block_table", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_width", C.c_int64),
+                ("kv_lens", C.c_void_p), ("q_starts", C.c_void_p)]
+
+
 OP_RMS_NORM, OP_ADD_RMS_NORM, OP_GATED_RMS_NORM, OP_QK_NORM_ROPE, OP_GLU = 0, 1, 2, 3, 4
 
 # name -> (restype, argtypes); kept in the order of include/higgs_hip.h
@@ -76,6 +91,11 @@ PROTOTYPES = {
     "hgk_op_list_bytes": (_i64, [_int]),
     "hgk_op_list_upload": (_int, [_int, C.POINTER(HgkOp), _int, _vp, _i64, _vp]),
     "hgk_op_list_run": (_int, [_int, _vp, _int, _i64, _vp]),
+    "hgk_kv_append": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "hgk_kv_copy_pages": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp]),
+    "hgk_paged_attention": (_int, [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _i64, _i64, _vp, _vp, _vp,
+                                   _i64, _vp]),
+    "hgk_paged_attention_workspace": (_i64, [_vp, _vp, _i64, _i64, _i64]),
     "hgk_st_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "hgk_st_close": (None, [_vp]),
     "hgk_st_count": (_i64, [_vp]),

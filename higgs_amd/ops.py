@@ -20,6 +20,10 @@ Each function keeps the reference call's name and argument meaning:
     QuantizedEmbedding(...).forward_rms_norm(ids, w, eps)
                                              embed_tokens + the first input_layernorm
                                              (transformer.rs:494, 407)
+    kv_append(k, v, k_pages, v_pages, ...)   KeyValueCache::update (cache.rs:4-29, 130-312)
+    kv_copy_pages(k_pages, v_pages, src, dst)   the copy of a cache (prompt_cache.rs:22-307)
+    paged_attention(q, k_pages, v_pages, ...)   fast::scaled_dot_product_attention and its
+                                             masks (utils.rs:28-125; gemma2.rs:219-379)
     OpSequence                               a decode step's per-layer ops in one launch
                                              (the layer loop, qwen3_next.rs:1508-1547)
 
@@ -28,8 +32,10 @@ Every op enqueues on torch's current CUDA/HIP stream and never synchronises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -505,6 +511,166 @@ def gated_delta_gated_norm(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         return out, state_out
     check(st)
     return out, state_out
+
+
+# ---------------------------------------------------------------- paged cache
+# hgk_kv_pages and hgk_kv_batch as one pack call each (native alignment is the
+# C layout): shorter on the host than filling ctypes structures field by field
+_KV_PAGES = struct.Struct("@iiqqqP3qP3q")
+_KV_BATCH = struct.Struct("@qqPqqPP")
+
+
+def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor, what: str):
+    """The packed hgk_kv_pages of pools [n_pages, page_size, Hk, D]."""
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise HgkError(1, f"{what}: pages must be [n_pages, page_size, kv_heads, head_dim], "
+                          "keys and values alike")
+    if k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device:
+        raise HgkError(1, f"{what}: key and value pages must share dtype and device")
+    n, ps, hk, d = k_pages.shape
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise HgkError(1, f"{what}: last axis must be unit-stride")
+    return _KV_PAGES.pack(dtype_code(k_pages.dtype), ps, n, hk, d, k_pages.data_ptr(), *ks[:3],
+                          v_pages.data_ptr(), *vs[:3])
+
+
+def _kv_batch(tokens: int, block_table: torch.Tensor, kv_lens: torch.Tensor, q_starts, device,
+              what: str):
+    """The packed hgk_kv_batch."""
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1 \
+            and block_table.shape[1] > 1:
+        raise HgkError(1, f"{what}: block_table must be int32 [batch, pages] with a unit-stride last axis")
+    batch = block_table.shape[0]
+    if kv_lens.dtype != torch.int32 or kv_lens.shape != (batch,) or not kv_lens.is_contiguous():
+        raise HgkError(1, f"{what}: kv_lens must be contiguous int32[{batch}]")
+    if block_table.device != device or kv_lens.device != device:
+        raise HgkError(1, f"{what}: operands on different devices")
+    if q_starts is not None and (q_starts.dtype != torch.int32 or q_starts.shape != (batch + 1,)
+                                 or not q_starts.is_contiguous() or q_starts.device != device):
+        raise HgkError(1, f"{what}: q_starts must be contiguous int32[{batch + 1}] on {device}")
+    return _KV_BATCH.pack(batch, tokens, block_table.data_ptr(), block_table.stride(0),
+                          block_table.shape[1], kv_lens.data_ptr(),
+                          0 if q_starts is None else q_starts.data_ptr())
+
+
+def _token_rows(t: torch.Tensor, pages: torch.Tensor, what: str, name: str):
+    """(token, head) strides of a [tokens, heads, D] operand, packed."""
+    if t.dim() != 3 or t.shape[2] != pages.shape[3]:
+        raise HgkError(1, f"{what}: {name} must be [tokens, heads, {pages.shape[3]}]")
+    if t.dtype != pages.dtype or t.device != pages.device:
+        raise HgkError(1, f"{what}: {name} must share the pages' dtype and device")
+    st = t.stride()
+    if st[2] != 1:
+        raise HgkError(1, f"{what}: {name}: last axis must be unit-stride")
+    return _TWO.pack(st[0], st[1])
+
+
+_TWO = struct.Struct("@qq")
+
+
+def _on_device(device: torch.device):
+    """The device's guard where it is not the current one: a stream takes
+    launches of its own device only."""
+    if device.type != "cuda":
+        raise HgkError(1, f"operands must be on the GPU, not on {device}")
+    return (_NO_GUARD if device.index == torch.cuda.current_device()
+            else torch.cuda.device(device))
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+              block_table: torch.Tensor, kv_lens: torch.Tensor, *,
+              q_starts: Optional[torch.Tensor] = None) -> None:
+    """Writes new tokens' keys and values, k and v [T, Hk, D] (any token and
+    head strides), into their sequences' pages [n_pages, page_size, Hk, D].
+
+    block_table int32 [B, P] names each sequence's pages in order; kv_lens
+    int32 [B] counts its tokens with the new ones, which are its last. Sequence
+    b owns rows q_starts[b] .. q_starts[b+1]-1 of k and v (int32 [B+1]);
+    without q_starts, row b is its one new token. Rows of no sequence,
+    positions beyond the table and pages outside the pool are skipped."""
+    what = "kv_append"
+    pool = _pool(k_pages, v_pages, what)
+    ks, vs = _token_rows(k, k_pages, what, "k"), _token_rows(v, k_pages, what, "v")
+    if k.shape != v.shape or k.shape[1] != k_pages.shape[2]:
+        raise HgkError(1, f"{what}: k and v must be [tokens, {k_pages.shape[2]}, {k_pages.shape[3]}]")
+    dev = k_pages.device
+    batch = _kv_batch(k.shape[0], block_table, kv_lens, q_starts, dev, what)
+    with _on_device(dev):
+        check(lib().hgk_kv_append(pool, batch, k.data_ptr(), ks, v.data_ptr(), vs, _stream(dev)))
+
+
+def kv_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence[int],
+                  dst: Sequence[int]) -> None:
+    """Copies page src[i] to page dst[i], keys and values, for lists of page
+    indices held on the host. Pages are [n_pages, page_size, Hk, D], or
+    [layers, n_pages, ...] to copy them in every layer. A destination may
+    neither be named twice nor be a source."""
+    what = "kv_copy_pages"
+    layers, strides = 1, None
+    if k_pages.dim() == 5 and k_pages.shape == v_pages.shape:
+        layers = k_pages.shape[0]
+        strides = _TWO.pack(k_pages.stride(0), v_pages.stride(0))
+        if layers == 0:
+            return
+        k_pages, v_pages = k_pages[0], v_pages[0]
+    pool = _pool(k_pages, v_pages, what)
+    if len(src) != len(dst):
+        raise HgkError(1, f"{what}: {len(src)} sources for {len(dst)} destinations")
+    n = len(src)
+    try:
+        s, d = (C.c_int32 * n)(*src), (C.c_int32 * n)(*dst)
+    except TypeError:
+        raise HgkError(1, f"{what}: src and dst must be sequences of page indices") from None
+    for i in range(n):
+        if s[i] != src[i] or d[i] != dst[i]:  # ctypes keeps the low 32 bits
+            raise HgkError(1, f"{what}: pair {i} outside the pages")
+    dev = k_pages.device
+    with _on_device(dev):
+        check(lib().hgk_kv_copy_pages(pool, layers, strides, C.addressof(s), C.addressof(d), n,
+                                      _stream(dev)))
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    block_table: torch.Tensor, kv_lens: torch.Tensor, *,
+                    scale: Optional[float] = None, window: int = 0, sinks: int = 0,
+                    softcap: float = 0.0, q_starts: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of new tokens over their sequences' pages, which hold
+    the new tokens too (kv_append first). q [T, Hq, D] with any token and head
+    strides; pages, block_table, kv_lens and q_starts as in kv_append: prompts
+    of any lengths over any cached prefix, or, without q_starts, one token per
+    sequence. Query head h reads kv head h // (Hq // Hk).
+
+    ``scale`` is 1/sqrt(D) unless given. ``window`` > 0 keeps the last
+    ``window`` keys visible, and of the keys before them the first ``sinks``.
+    ``softcap`` > 0 replaces a score s by softcap * tanh(s / softcap). A query
+    that sees no key gives zeros. Rows of no sequence are not written (without
+    ``out`` they hold whatever the new tensor held). Returns [T, Hq, D]."""
+    what = "paged_attention"
+    pool = _pool(k_pages, v_pages, what)
+    qs = _token_rows(q, k_pages, what, "q")
+    T, hq, d = q.shape
+    if out is None:
+        out = torch.empty((T, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise HgkError(1, f"{what}: out shape {tuple(out.shape)} is not q's")
+    os_ = _token_rows(out, k_pages, what, "out")
+    dev = k_pages.device
+    batch = _kv_batch(T, block_table, kv_lens, q_starts, dev, what)
+    with _on_device(dev):
+        need = lib().hgk_paged_attention_workspace(pool, batch, hq, window, sinks)
+        if need < 0:
+            check(1)
+        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+        check(lib().hgk_paged_attention(pool, batch, q.data_ptr(), qs, hq,
+                                        1.0 / math.sqrt(d) if scale is None else scale, softcap,
+                                        window, sinks, out.data_ptr(), os_, _ptr(ws), need,
+                                        _stream(dev)))
+    return out
 
 
 # ---------------------------------------------------------------- embedding

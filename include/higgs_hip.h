@@ -448,6 +448,99 @@ int hgk_op_list_upload(int dtype, const hgk_op* ops, int n_ops, void* dev_list,
 int hgk_op_list_run(int dtype, const void* dev_list, int n_ops, int64_t tokens, void* stream);
 
 /* ------------------------------------------------------------------------
+ * The paged key-value cache and the attention that reads it.
+ *
+ * Keys and values live in a pool of pages of page_size tokens each; a table
+ * [batch, table_width] names the pages of every sequence in order. Replaces
+ * the per-request KeyValueCache and its update (crates/higgs-models/src/
+ * cache.rs:4-29, 130-312), the clone of a cache per prompt prefix
+ * (crates/higgs-engine/src/prompt_cache.rs:22-307) and the attention over it
+ * (utils.rs:28-125 with mlx_rs::fast::scaled_dot_product_attention; the soft-
+ * capped and sliding-window form gemma2.rs:219-379; the ragged batch of
+ * forward_batched, transformer.rs:747-827).
+ *
+ * Every pointer is 16-byte aligned and every stride a multiple of 8 elements
+ * (int32 arrays: 4-byte aligned, any stride). Metadata on the device (tables,
+ * lengths, starts) is read by the kernels, which check it: a page outside
+ * [0, n_pages), a length beyond the table and a start outside the tokens
+ * reach no memory. Tokens on such a page are seen by no query and written
+ * nowhere.
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int dtype;     /* HGK_BF16 or HGK_F16 */
+  int page_size; /* tokens per page: a power of two, 1..65536 */
+  int64_t n_pages;
+  int64_t kv_heads, head_dim; /* head_dim 64, 96, 128 or 256 */
+  void* k;
+  int64_t k_strides[3]; /* page, token, head */
+  void* v;
+  int64_t v_strides[3];
+} hgk_kv_pages;
+
+/* The new tokens of `batch` sequences, rows of one packed array: sequence b
+ * owns rows q_starts[b] .. q_starts[b+1]-1 (device int32[batch+1], not
+ * decreasing), or row b alone when q_starts is NULL. They are the last tokens of
+ * the sequence: kv_lens[b] (device int32) counts its tokens with them, so row
+ * i of n lies at position kv_lens[b] - n + i. Rows in front of q_starts[0] and
+ * behind q_starts[batch] (a padded batch) belong to no sequence. */
+typedef struct {
+  int64_t batch;
+  int64_t tokens; /* rows of the packed array */
+  const int32_t* block_table;
+  int64_t table_stride, table_width;
+  const int32_t* kv_lens;
+  const int32_t* q_starts;
+} hgk_kv_batch;
+
+/*
+ * Writes the new tokens' keys and values, k and v [tokens, kv_heads, head_dim]
+ * (strides: token, head), to their places in the pages. Rows of no sequence,
+ * positions below zero or beyond the table, and pages outside the pool are
+ * skipped. No two sequences of a call may write to the same place.
+ */
+int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batch, const void* k,
+                  const int64_t k_strides[2], const void* v, const int64_t v_strides[2],
+                  void* stream);
+
+/*
+ * Copies whole pages, keys and values: page src[i] to page dst[i] (HOST
+ * arrays) for i < n, in each of `layers` pools that lie layer_strides[0] (k)
+ * and layer_strides[1] (v) elements apart. Indices outside the pool, a
+ * destination named twice and a destination that is also a source are
+ * refused, so the copies are independent of each other. Used to fork a
+ * sequence whose last page is shared, and to compact a pool.
+ */
+int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers, const int64_t layer_strides[2],
+                      const int32_t* src, const int32_t* dst, int64_t n, void* stream);
+
+/*
+ * Attention of the new tokens over their sequences' pages (which hold the new
+ * tokens too: hgk_kv_append first). q and out [tokens, q_heads, head_dim]
+ * (strides: token, head); query head h reads kv head h / (q_heads / kv_heads).
+ *   s_j = scale * (q . k_j), softcap > 0: softcap * tanh(s_j / softcap)
+ *   out = sum_j softmax(s)_j v_j over the keys j that the query at position p
+ * sees: j <= p, and with window > 0 either j > p - window or j < sinks (the
+ * last `window` keys and the first `sinks`). A query that sees no key gives a
+ * row of zeros; keys and values that a query does not see, infinities and NaN
+ * among them, do not touch its row. Rows of no sequence are left as they are.
+ * Sums and softmax statistics are f32; the probabilities are rounded to the
+ * dtype for the product with v; the result is rounded once.
+ * `workspace`: device memory of hgk_paged_attention_workspace() bytes (NULL
+ * if that is 0), 16-byte aligned, used until the call's work on `stream` is
+ * done and by no other call meanwhile (two calls on different streams, and
+ * two captured graphs that may run side by side, need one each).
+ */
+int hgk_paged_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch, const void* q,
+                        const int64_t q_strides[2], int64_t q_heads, float scale, float softcap,
+                        int64_t window, int64_t sinks, void* out, const int64_t out_strides[2],
+                        void* workspace, int64_t workspace_bytes, void* stream);
+/* Bytes of device memory that call needs (0: none; -1 for sizes it refuses).
+ * Depends on the sizes alone: batch, tokens, table_width, whether q_starts is
+ * given, the pages' sizes, q_heads, window and sinks. */
+int64_t hgk_paged_attention_workspace(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                      int64_t q_heads, int64_t window, int64_t sinks);
+
+/* ------------------------------------------------------------------------
  * Checkpoint files: the safetensors files MLX 4-bit checkpoints ship in
  * (u32-packed `.weight`, bf16/f16 `.scales`/`.biases`, bf16 norm weights).
  * Replaces Array::load_safetensors as used by load_quantized_safetensors_weights
