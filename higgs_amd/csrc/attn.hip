@@ -8,6 +8,7 @@ namespace hgk {
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -38,9 +39,14 @@ template <> struct Mx<BF16> {
     return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a),
                                                      __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
   }
+  static __device__ inline f32x16 mma32x16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
   static __device__ inline uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
   }
+  static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u, k128 = 0x4300u, k16384 = 0x4680u;
 };
 template <> struct Mx<F16> {
   static __device__ inline f32x4 mma16x32(u32x4 a, u32x4 b, f32x4 c) {
@@ -51,9 +57,15 @@ template <> struct Mx<F16> {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a),
                                                  __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
   }
+  static __device__ inline f32x16 mma32x16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
   static __device__ inline uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
   }
+  // the exponent's bits, and 1, 128 and 16384
+  static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u, k128 = 0x5800u, k16384 = 0x7400u;
 };
 
 constexpr float kLog2e = 1.44269504088896341f;
@@ -79,11 +91,11 @@ __device__ inline Scale fold_scale(const AttnArgs& a) {
   s.flip = 0;
   s.keep = ~0u;
   if constexpr (CAP) {
-    s.c = a.softcap * kLog2e;
+    s.c = fminf(a.softcap * kLog2e, 1.0e37f);
     s.inner = a.scale / a.softcap;
   } else {
     s.inner = 0.0f;
-    s.c = fabsf(a.scale) * kLog2e;
+    s.c = fminf(fabsf(a.scale) * kLog2e, 1.0e37f);
     if (a.scale < 0.0f) s.flip = 0x80008000u;
     if (s.c == 0.0f) {
       s.c = 1.0f;
@@ -108,6 +120,13 @@ constexpr float kSlack = 8.0f;
 // The reference of a row that has seen no score: below every score that can
 // occur, and finite times c.
 __device__ inline float lowest_ref(float c) { return -3.0e38f / fmaxf(c, 1.0f); }
+
+// 2^(c (ref - to)) of a reference that moves up. Not below the smallest normal
+// number: an infinite sum (of infinite values) stays infinite, and a finite
+// one that far below is lost in the new one's rounding all the same.
+__device__ inline float shrink(float ref, float to, float c) {
+  return fmaxf(__builtin_amdgcn_exp2f((ref - to) * c), 1.2e-38f);
+}
 
 // ---------------------------------------------------------------- one token
 // The keys that a sequence's last token sees, as one run of n: index i is key
@@ -272,10 +291,10 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
       }
 #pragma unroll
       for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
-      if (__any(top > ref + slack)) {
+      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = fmaxf(ref, top), f = __builtin_amdgcn_exp2f((ref - to) * sc.c);
+        const float to = top > ref + slack ? top : ref, f = shrink(ref, to, sc.c);
         sum *= f;
 #pragma unroll
         for (int t = 0; t < kOut; ++t) o[t] *= f;
@@ -284,11 +303,6 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
       const float base = -ref * sc.c;
 #pragma unroll
       for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
-      if (now != kAll) {
-#pragma unroll
-        for (int i = 0; i < 4 * NS; ++i)
-          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = 0.0f;
-      }
       any |= now != 0;
       uint32_t hi[2 * NS], lo[2 * NS];
 #pragma unroll
@@ -392,59 +406,410 @@ __global__ __launch_bounds__(128) void attn_join_kernel(AttnArgs a) {
       top == -INFINITY ? 0u : T::pack(v0 * r, v1 * r);
 }
 
-// One wave per (row, query head). Lane l scores key base + l, then the lanes
-// share the head's D outputs.
-template <class T>
-__global__ __launch_bounds__(64) void attn_simple_kernel(AttnArgs a) {
-  __shared__ float qs[256], ps[64];
-  const int D = a.p.head_dim, lane = threadIdx.x;
-  const int t = blockIdx.x, h = blockIdx.y, hk = h / a.group;
-  const int seq = kv_row_owner(a.b, t);
-  const KvSeq s = kv_seq(a.b, seq);
-  const int r = t - s.first;
-  if (r < 0 || r >= s.n) return;
-  const int64_t p64 = (int64_t)s.len - s.n + r;
-  const int p = (int)p64;
-  for (int d = lane; d < D; d += 64) qs[d] = load1<T>(a.q, t * a.qst[0] + h * a.qst[1] + d) * a.scale;
-  __syncthreads();
-  float o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0;
-  bool any = false;
-  for (int base = 0; p64 >= 0 && base <= p; base += 64) {
-    const int j = base + lane;
-    bool see = j <= p && (a.window == 0 || j > p - a.window || j < a.sinks);
-    const int page = see ? kv_page(a.p, a.b, seq, j) : -1;
-    see = page >= 0;
-    float sc = -INFINITY;
-    if (see) {
-      const int64_t at = page * a.p.kst[0] + (j & a.p.page_mask) * a.p.kst[1] + hk * a.p.kst[2];
-      sc = 0;
-      for (int d = 0; d < D; ++d) sc = fmaf(qs[d], load1<T>(a.p.k, at + d), sc);
-      if (a.softcap > 0) sc = a.softcap * tanhf(sc / a.softcap);
+// ---------------------------------------------------------------- prompts
+// 16 bytes per lane from memory to LDS at dst + 16 * lane (dst is uniform):
+// from base + off, or from an address of the lane's own. m0 is written inside,
+// and the compiler has to know (it need not warn that nothing preserves it).
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ inline void lds_load(uint32_t dst, const char* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(dst), "v"(off), "s"(base) : "m0", "memory");
+}
+__device__ inline void lds_load(uint32_t dst, const char* p) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(dst), "v"(p) : "m0", "memory");
+}
+#pragma clang diagnostic pop
+__device__ inline uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+// this wave's loads to LDS have landed, then the block's barrier
+__device__ inline void landed_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Where the 16-byte piece c of a tile's row r lies in its row of D/8 pieces.
+// Keys are read 16 rows at a time, one piece each: those go to 16 different
+// places modulo 256 bytes. Values are read transposed, 4 pieces of 8 rows at a
+// time: those cover 256 bytes twice.
+template <int D> __device__ inline int key_place(int r, int c) {
+  if constexpr (D == 64) return c ^ ((r >> 1) & 7);
+  else if constexpr (D == 96) return (c + (r >> 2)) % 12;
+  else return c ^ (r & 15);
+}
+template <int D> __device__ inline int value_place(int r, int c) {
+  if constexpr (D == 64) return c ^ ((r << 1) & 4);
+  else if constexpr (D == 96) return c;
+  else return c ^ ((r & 3) << 2);
+}
+// ... and the piece that lies at place c.
+template <int D> __device__ inline int key_piece(int r, int c) {
+  if constexpr (D == 96) return (c + 24 - (r >> 2)) % 12;
+  else return key_place<D>(r, c);
+}
+
+// The rows of a (sequence, kv head): row r is query token r / group with the
+// kv head's query head r % group, so that all heads of a group, and as many
+// tokens as fit, read a tile of keys once.
+//
+// A non-finite value in a tile that some row sees only in part: a weight of
+// zero times infinity would be NaN. Such a tile's values are counted on the
+// matrix cores (+inf as 1, -inf as 128, NaN as 16384, times 1 where the row
+// sees the key: at most 64 keys a tile, so the sum gives the three counts
+// back), and the product runs with zeros in their place.
+template <class M>
+__device__ inline uint32_t finite_pair(uint32_t w) {
+  uint32_t m = 0;
+  if ((w & M::kExp) != M::kExp) m |= 0xffffu;
+  if (((w >> 16) & M::kExp) != M::kExp) m |= 0xffff0000u;
+  return w & m;
+}
+template <class M>
+__device__ inline uint32_t count_code(uint32_t h) {
+  if ((h & M::kExp) != M::kExp) return 0;
+  if (h & 0x7fffu & ~M::kExp) return M::k16384;
+  return h & 0x8000u ? M::k128 : M::kOne;
+}
+template <class M>
+__device__ inline uint32_t count_pair(uint32_t w) {
+  return count_code<M>(w & 0xffffu) | count_code<M>(w >> 16) << 16;
+}
+// top bits set where a half is not finite
+template <class M>
+__device__ inline uint32_t odd_pair(uint32_t w) {
+  constexpr uint32_t e = M::kExp | M::kExp << 16, one = (M::kExp & -M::kExp) * 0x10001u;
+  return ((w & e) + one) & 0x80008000u;
+}
+
+// Block = (kv head, tile of 32 * NW rows, part of its tiles of BN keys); a wave
+// has 32 rows. As in the decode kernel S^T = K Q^T and O^T = V^T P^T, here on
+// 32x32x16 instructions: a lane has half the scores of one row in registers,
+// its weights are the second product's operand as they stand, and a row's
+// reference and sum are one register each.
+//
+// K and V tiles come straight from memory to LDS, double buffered: the next
+// tile's loads are issued before a tile is computed, one barrier a tile.
+template <class T, int D, int NW, int BN, bool CAP>
+__global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnArgs a) {
+  constexpr int NT = 64 * NW, BM = 32 * NW, CH = D / 8, kUnits = BN * CH / NT;
+  constexpr int kRow = 2 * D, kTile = BN * kRow;
+  constexpr int KT = BN / 32, QS = D / 16, DT = D / 32;
+  static_assert(BN * CH % NT == 0, "whole units per thread");
+  typedef Mx<T> M;
+  __shared__ __align__(16) char lds[4 * kTile];  // keys, values; keys, values
+  __shared__ int odd;  // 1 + index of the last tile found to hold values that are not finite
+
+  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hk = blockIdx.x, G = a.group;
+
+  // which sequence's tile this is: tiles are counted over the sequences, from
+  // the last one on (the longest ones of a prompt first)
+  int seq = -1, tile = 0;
+  KvSeq s{0, 0, 0};
+  {
+    int want = gridDim.y - 1 - blockIdx.y, before = 0;
+    for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
+      const int b = b0 + lane;
+      const KvSeq c = b < a.b.batch ? kv_seq(a.b, b) : KvSeq{0, 0, 0};
+      const int mine = (c.n * G + BM - 1) / BM;
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
+      }
+      const uint64_t has = __ballot(before + upto > want);
+      if (has) {
+        const int l = __builtin_ctzll(has);
+        seq = b0 + l;
+        tile = want - before - __builtin_amdgcn_readlane(upto - mine, l);
+        s.first = __builtin_amdgcn_readlane(c.first, l);
+        s.n = __builtin_amdgcn_readlane(c.n, l);
+        s.len = __builtin_amdgcn_readlane(c.len, l);
+        break;
+      }
+      before += __builtin_amdgcn_readlane(upto, 63);
     }
-    any |= __any(see);
-    float mt = sc;
-    for (int x = 32; x; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x));
-    const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.f : mn;
-    const float pr = see ? expf(sc - ref) : 0.f, f = expf(m - ref);
-    float sum = pr;
-    for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-    l = l * f + sum;
-    m = mn;
-    ps[lane] = pr;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) o[i] *= f;
-    for (int jj = 0; jj < 64; ++jj) {
-      const int pg = __shfl(page, jj);
-      if (pg < 0) continue;
-      const int64_t at = pg * a.p.vst[0] + ((base + jj) & a.p.page_mask) * a.p.vst[1] + hk * a.p.vst[2];
-      for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < D) o[i] = fmaf(ps[jj], load1<T>(a.p.v, at + lane + 64 * i), o[i]);
-    }
-    __syncthreads();
   }
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < D)
-      store1<T>(a.out, t * a.ost[0] + h * a.ost[1] + lane + 64 * i, any ? o[i] / l : 0.f);
+  if (seq < 0) return;
+  const int R = s.n * G, pos0 = s.len - s.n;  // pos0 may be negative: rows in front of the sequence
+
+  // the block's keys, in tiles of BN: those of the first `sinks`, then the window's
+  const int row0 = tile * BM;
+  const int p_first = pos0 + row0 / G, p_last = pos0 + (min(row0 + BM, R) - 1) / G;
+  const int64_t cap = (int64_t)a.b.width << a.p.page_shift;
+  const int hi = (int)min((int64_t)p_last + 1, cap);
+  const int lo = a.window > 0 && p_first >= a.window ? p_first - a.window + 1 : 0;
+  const int t_hi = hi > 0 ? (hi + BN - 1) / BN : 0, t_lo = lo / BN;
+  const int front = min(min((min(a.sinks, lo) + BN - 1) / BN, t_lo), t_hi);
+  const int tiles = a.p.n_pages > 0 ? front + max(t_hi - t_lo, 0) : 0;
+  const int per = (tiles + a.splits - 1) / a.splits;
+  const int it0 = min(per * (int)blockIdx.z, tiles), it1 = min(it0 + per, tiles);
+  auto tile_of = [&](int it) { return it < front ? it : t_lo + it - front; };
+
+  // this lane's row, and the range of the wave's
+  const int wrow0 = row0 + 32 * wave;
+  const int row = min(wrow0 + col, R - 1);
+  const int qi = row / G, head = hk * G + row - qi * G, p = pos0 + qi;
+  const bool in = wrow0 + col < R;
+  const int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
+  const bool idle = wrow0 >= R;
+
+  const Scale sc = fold_scale<CAP>(a);
+  u32x4 qf[QS];
+  {
+    const char* qp = a.q + 2 * ((int64_t)(s.first + qi) * a.qst[0] + head * a.qst[1] + 8 * half);
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      qf[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+      for (int w = 0; w < 4; ++w) qf[i][w] = (qf[i][w] & sc.keep) ^ sc.flip;
+    }
+  }
+
+  // lane l looks up key l of a tile
+  const int32_t* table = a.b.table + (int64_t)seq * a.b.table_stride;
+  const char* kbase = a.p.k + 2 * hk * a.p.kst[2];
+  const char* vbase = a.p.v + 2 * hk * a.p.vst[2];
+  auto look_up = [&](int it) -> int32_t {
+    if (it >= it1) return -1;
+    const int key = tile_of(it) * BN + (lane & (BN - 1));
+    const int32_t page = key < hi ? table[key >> a.p.page_shift] : -1;
+    return (uint32_t)page < (uint32_t)a.p.n_pages ? page : -1;
+  };
+  // One load instruction takes 64 pieces, of rows that lie in one page when
+  // pages have 16 tokens or more: its page is then scalar, and the lanes'
+  // offsets are the same for every tile. A key that does not exist reads what
+  // is there (a page's end, or page 0); its score is masked and its value, if
+  // not finite, taken out.
+  const bool whole = a.p.page_shift >= 4 && a.p.kst[1] < (1 << 24) && a.p.vst[1] < (1 << 24);
+  uint32_t koff[kUnits], voff[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int u0 = i * NT + 64 * wave, u = u0 + lane, r = u / CH, c = u - r * CH, r0 = u0 / CH;
+    koff[i] = 2 * ((r - r0) * (uint32_t)a.p.kst[1] + 8 * key_piece<D>(r, c));
+    voff[i] = 2 * ((r - r0) * (uint32_t)a.p.vst[1] + 8 * value_place<D>(r, c));
+  }
+  uint64_t there = 0;  // bit i: key i of the tile being loaded exists
+  auto load = [&](int it, int buf, int32_t page) {
+    there = __ballot(page >= 0);
+    if (page < 0) page = 0;
+    const int key0 = tile_of(it) * BN;
+    const uint32_t kt = lds_address(lds) + buf * 2 * kTile + 1024 * wave, vt = kt + kTile;
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int r0 = (i * NT + 64 * wave) / CH;
+        const int64_t pg = __builtin_amdgcn_readlane(page, r0), at = (key0 + r0) & a.p.page_mask;
+        lds_load(kt + 16 * NT * i, kbase + 2 * (pg * a.p.kst[0] + at * a.p.kst[1]), koff[i]);
+        lds_load(vt + 16 * NT * i, vbase + 2 * (pg * a.p.vst[0] + at * a.p.vst[1]), voff[i]);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = i * NT + threadIdx.x, r = u / CH, c = u - r * CH;
+        const int64_t pg = __shfl(page, r), at = (key0 + r) & a.p.page_mask;
+        lds_load(kt + 16 * NT * i, kbase + 2 * (pg * a.p.kst[0] + at * a.p.kst[1] + 8 * key_piece<D>(r, c)));
+        lds_load(vt + 16 * NT * i, vbase + 2 * (pg * a.p.vst[0] + at * a.p.vst[1] + 8 * value_place<D>(r, c)));
+      }
+    }
+  };
+  // does some row of this range see only a part of the tile?
+  auto part_seen = [&](int key0, int first, int last) {
+    return !(key0 + BN - 1 <= first &&
+             (a.window == 0 || key0 > last - a.window || key0 + BN - 1 < a.sinks));
+  };
+  // does this lane's row see key i of the tile?
+  auto sees = [&](int key0, uint64_t exist, int i) {
+    const int key = key0 + i;
+    return key <= p && (a.window == 0 || key > p - a.window || key < a.sinks) && ((exist >> i) & 1);
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = f32x16{};
+  float ref = lowest_ref(sc.c), sum = 0.0f;
+  const float slack = kSlack / sc.c;
+  bool any = false;
+
+  // the transposed reads: value rows 4 half + (lane % 16) / 4, and pieces of
+  // 8 bytes; the place of a piece depends on the row modulo 4 alone
+  const int vr = 4 * half + (lane & 15) / 4, vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  uint32_t vplace[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) vplace[t] = vr * kRow + 16 * value_place<D>(vr, 4 * t + vc) + 8 * (lane & 1);
+
+  if (threadIdx.x == 0) odd = 0;
+  int32_t page = look_up(it0);
+  if (it0 < it1) load(it0, 0, page);
+  page = look_up(it0 + 1);
+  uint64_t now = there;
+  landed_barrier();
+
+  for (int it = it0; it < it1; ++it) {
+    const int buf = (it - it0) & 1;
+    char* kt = lds + buf * 2 * kTile;
+    char* vt = kt + kTile;
+    const int key0 = tile_of(it) * BN;
+    if (it + 1 < it1) {
+      load(it + 1, buf ^ 1, page);
+      page = look_up(it + 2);
+    }
+    const bool exist = BN == 64 ? now == ~0ull : (uint32_t)now == ~0u;  // all keys of the tile do
+    bool strange = false;
+    if (!exist || part_seen(key0, p_first, p_last)) {
+      uint32_t bits = 0;
+#pragma unroll 1
+      for (int i = 0; i < kUnits; ++i) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(vt + 16 * (i * NT + threadIdx.x));
+        bits |= odd_pair<M>(v[0]) | odd_pair<M>(v[1]) | odd_pair<M>(v[2]) | odd_pair<M>(v[3]);
+      }
+      if (bits) odd = it + 1;
+      __syncthreads();
+      strange = odd == it + 1;
+    }
+    const bool none = idle || key0 > pw_last ||
+                      (a.window > 0 && key0 + BN - 1 <= pw_first - a.window && key0 >= a.sinks);
+    u32x4 w[2 * KT];
+    if (!none) {
+      f32x16 x[KT];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        x[t] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < QS; ++i) {
+          const int r = 32 * t + col;
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + r * kRow + 16 * key_place<D>(r, 2 * i + half));
+          x[t] = M::mma32x16(kf, qf[i], x[t]);
+        }
+      }
+      if constexpr (CAP) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[t][e] = fast_tanh(x[t][e] * sc.inner);
+      }
+      if (!exist || part_seen(key0, pw_first, pw_last)) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            if (sees(key0, now, 32 * t + 8 * (e / 4) + 4 * half + e % 4)) any = true;
+            else x[t][e] = -INFINITY;
+          }
+      } else {
+        any = true;
+      }
+      float top = x[0][0];
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[t][e]);
+      if (__any(top > ref + slack)) {  // a row's own scores alone decide for it
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = top > ref + slack ? top : ref, f = shrink(ref, to, sc.c);
+        sum *= f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= f;
+        ref = to;
+      }
+      const float base = -ref * sc.c;
+      float add[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float w0 = __builtin_amdgcn_exp2f(fmaf(x[t][e], sc.c, base));
+          const float w1 = __builtin_amdgcn_exp2f(fmaf(x[t][e + 1], sc.c, base));
+          add[(e / 2) & 3] += w0 + w1;
+          w[2 * t + e / 8][(e / 2) & 3] = M::pack(w0, w1);
+        }
+      sum += (add[0] + add[1]) + (add[2] + add[3]);
+    }
+    if (strange) {
+      if (!none) {
+#pragma unroll 1
+        for (int t = 0; t < DT; ++t) {
+          f32x16 n = f32x16{};
+#pragma unroll 1
+          for (int k = 0; k < 2 * KT; ++k) {
+            const char* vp = vt + 16 * k * kRow + vr * kRow + 16 * value_place<D>(vr, 4 * t + vc) + 8 * (lane & 1);
+            const u32x2 v0 = lds_transposed(vp), v1 = lds_transposed(vp + 8 * kRow);
+            uint32_t see = 0;
+            for (int e = 0; e < 8; ++e)
+              see |= (uint32_t)sees(key0, now, 16 * k + 8 * (e / 4) + 4 * half + e % 4) << e;
+            u32x4 c = {count_pair<M>(v0[0]), count_pair<M>(v0[1]), count_pair<M>(v1[0]), count_pair<M>(v1[1])}, on;
+            for (int i = 0; i < 4; ++i)
+              on[i] = ((see >> (2 * i)) & 1 ? M::kOne : 0u) | ((see >> (2 * i)) & 2 ? M::kOne << 16 : 0u);
+            n = M::mma32x16(c, on, n);
+          }
+          f32x16 f;
+          for (int e = 0; e < 16; ++e) {
+            const int counts = (int)n[e], nan = counts >> 14, neg = (counts >> 7) & 127, pos = counts & 127;
+            f[e] = nan || (neg && pos) ? __builtin_nanf("") : neg ? -INFINITY : pos ? INFINITY : 0.0f;
+          }
+#pragma unroll
+          for (int u = 0; u < DT; ++u)
+            if (u == t) o[u] += f;
+        }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = 0; i < kUnits; ++i) {
+        u32x4* v = reinterpret_cast<u32x4*>(vt + 16 * (i * NT + threadIdx.x));
+        u32x4 t = *v;
+        for (int j = 0; j < 4; ++j) t[j] = finite_pair<M>(t[j]);
+        *v = t;
+      }
+      __syncthreads();
+    }
+    if (!none) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2 * KT; ++k) {
+          const char* vp = vt + vplace[t] + 16 * k * kRow;
+          const u32x2 v0 = lds_transposed(vp), v1 = lds_transposed(vp + 8 * kRow);
+          o[t] = M::mma32x16(u32x4{v0[0], v0[1], v1[0], v1[1]}, w[k], o[t]);
+        }
+    }
+    now = there;
+    landed_barrier();
+  }
+
+  sum += __shfl_xor(sum, 32);
+  any |= __shfl_xor((int)any, 32) != 0;
+  if (a.splits > 1) {
+    const int64_t at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.z;
+    if (!in) return;
+    if (half == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * at) = f32x2{any ? ref * sc.c : -INFINITY, sum};
+    if (!any) return;
+    float* dst = a.part + at * D + 4 * half;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<f32x4*>(dst + 32 * t + 2 * e) = f32x4{o[t][e], o[t][e + 1], o[t][e + 2], o[t][e + 3]};
+    return;
+  }
+  // a lane has 4 of every 8 values of its row: the halves trade, for 16-byte stores
+  const float r = any ? 1.0f / sum : 0.0f;
+  char* dst = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1] + 8 * half);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 16; e += 8) {
+      u32x4 v;
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t b0 = T::pack(o[t][e + 2 * i] * r, o[t][e + 2 * i + 1] * r);
+        const uint32_t b1 = T::pack(o[t][e + 4 + 2 * i] * r, o[t][e + 5 + 2 * i] * r);
+        const auto x = __builtin_amdgcn_permlane32_swap(b0, b1, false, false);
+        v[i] = x[0];
+        v[2 + i] = x[1];
+      }
+      if (in) *reinterpret_cast<u32x4*>(dst + 64 * t + 4 * e) = v;
+    }
 }
 
 // Sizes shared by the call and its workspace query.
@@ -479,9 +844,17 @@ int64_t part_bytes(int64_t rows, int splits, int64_t head_dim) {
   return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
 }
 
+// Rows of a block of the prompt kernel, and the most blocks' tiles that the rows can take.
+int prompt_rows(int64_t head_dim) { return head_dim == 256 ? 256 : 128; }
+int64_t prompt_tiles(const KvBatchView& b, int64_t group, int rows) {
+  return (int64_t)b.tokens * group / rows + std::min(b.batch, b.tokens);
+}
+
 int plan_splits(const KvView& p, const KvBatchView& b, int64_t q_heads, int64_t window, int64_t sinks) {
-  if (b.starts || b.batch == 0) return 1;
+  if (b.batch == 0 || b.tokens == 0) return 1;
   const int64_t group = q_heads / p.kv_heads;
+  if (b.starts)
+    return choose_splits(p, b, p.kv_heads * prompt_tiles(b, group, prompt_rows(p.head_dim)), window, sinks);
   return choose_splits(p, b, (int64_t)b.batch * p.kv_heads * ((group + 15) / 16), window, sinks);
 }
 
@@ -494,6 +867,15 @@ void launch_decode(const AttnArgs& a, hipStream_t stream) {
     HGK_LAUNCH((attn_decode_kernel<T, D, NS, false>), grid, block, 0, stream, a);
 }
 
+template <class T, int D, int NW, int BN>
+void launch_prompt(const AttnArgs& a, hipStream_t stream) {
+  const dim3 grid(a.p.kv_heads, prompt_tiles(a.b, a.group, 32 * NW), a.splits), block(64 * NW);
+  if (a.softcap > 0.0f)
+    HGK_LAUNCH((attn_prompt_kernel<T, D, NW, BN, true>), grid, block, 0, stream, a);
+  else
+    HGK_LAUNCH((attn_prompt_kernel<T, D, NW, BN, false>), grid, block, 0, stream, a);
+}
+
 template <class T>
 int run(const AttnArgs& a, const char* what, hipStream_t stream) {
   if (!a.b.starts) {
@@ -504,7 +886,12 @@ int run(const AttnArgs& a, const char* what, hipStream_t stream) {
       default: launch_decode<T, 256, 1>(a, stream); break;
     }
   } else {
-    HGK_LAUNCH(attn_simple_kernel<T>, dim3(a.b.tokens, a.q_heads), dim3(64), 0, stream, a);
+    switch (a.p.head_dim) {
+      case 64: launch_prompt<T, 64, 4, 64>(a, stream); break;
+      case 96: launch_prompt<T, 96, 4, 64>(a, stream); break;
+      case 128: launch_prompt<T, 128, 4, 64>(a, stream); break;
+      default: launch_prompt<T, 256, 8, 32>(a, stream); break;
+    }
   }
   if (int st = launch_status(what)) return st;
   if (a.splits == 1) return HGK_OK;

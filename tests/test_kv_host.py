@@ -127,6 +127,10 @@ def test_refused_attention_arguments():
         for ws, n in ((None, need), (FAKE, need - 1), (FAKE + 4, need)):
             s, msg = attention(b=long, ws=ws, ws_bytes=n)
             assert s == 1 and "workspace" in msg
+    for b in (batch(batch=0, tokens=0), batch(batch=3, tokens=0, q_starts=FAKE),
+              batch(batch=0, tokens=9, q_starts=FAKE)):
+        assert L.hgk_paged_attention_workspace(C.byref(pages()), C.byref(b), 4, 0, 0) == 0
+        assert attention(b=b, q=None, out=None)[0] == 0
     # nothing to do: no launch, and no data needed
     none = batch(batch=0, tokens=0, block_table=None, kv_lens=None)
     assert attention(b=none, q=None, out=None)[0] == 0
