@@ -32,6 +32,10 @@ CFLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function", "-Wno-unknown-pragmas",
 ]
+# Flags of single files. attn.hip: matrix instructions keep their sums in plain
+# vector registers also where a wave has all 512; otherwise rows of 256 values
+# move every sum between the two halves of the register file for every tile.
+FILE_FLAGS = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def hipcc() -> str:
@@ -43,7 +47,7 @@ def hipcc() -> str:
 
 def _compile(cc: str, src: str) -> str:
     obj = os.path.join(BUILD, os.path.basename(src) + ".o")
-    cmd = [cc, *CFLAGS, "-c", src, "-o", obj]
+    cmd = [cc, *CFLAGS, *FILE_FLAGS.get(os.path.basename(src), []), "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     noise = "is not a recognized feature for this target"
     err = "\n".join(ln for ln in r.stderr.splitlines() if noise not in ln)

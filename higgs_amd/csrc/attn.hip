@@ -1,6 +1,7 @@
 // attn.hip -- attention of new tokens over a paged key-value cache.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv.h"
 
@@ -46,6 +47,11 @@ template <> struct Mx<BF16> {
   static __device__ inline uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
   }
+  // s plus the two values of w
+  static __device__ inline float add_pair(uint32_t w, float s) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3f803f80u), s, false);
+  }
   static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u, k128 = 0x4300u, k16384 = 0x4680u;
 };
 template <> struct Mx<F16> {
@@ -64,11 +70,31 @@ template <> struct Mx<F16> {
   static __device__ inline uint32_t pack(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
   }
+  static __device__ inline float add_pair(uint32_t w, float s) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), s, false);
+  }
   // the exponent's bits, and 1, 128 and 16384
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u, k128 = 0x5800u, k16384 = 0x7400u;
 };
 
 constexpr float kLog2e = 1.44269504088896341f;
+
+// max of three as one instruction (fmaxf would first quiet each operand)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Of this lane's value and that of the lane 32 away: the larger, and the sum.
+__device__ inline float halves_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return max3(u2f(r[0]), u2f(r[1]), u2f(r[1]));
+}
+__device__ inline float halves_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+  return u2f(r[0]) + u2f(r[1]);
+}
 
 // Four 16-bit values of one column from LDS: lane l of each 16 names the row
 // l/4 and the columns 4 (l%4) .. +3, and receives column l of rows 0..3.
@@ -92,7 +118,8 @@ __device__ inline Scale fold_scale(const AttnArgs& a) {
   s.keep = ~0u;
   if constexpr (CAP) {
     s.c = fminf(a.softcap * kLog2e, 1.0e37f);
-    s.inner = a.scale / a.softcap;
+    s.inner = fabsf(a.scale) / a.softcap;
+    if (a.scale < 0.0f) s.flip = 0x80008000u;
   } else {
     s.inner = 0.0f;
     s.c = fminf(fabsf(a.scale) * kLog2e, 1.0e37f);
@@ -465,16 +492,6 @@ __device__ inline uint32_t finite_pair(uint32_t w) {
   if (((w >> 16) & M::kExp) != M::kExp) m |= 0xffff0000u;
   return w & m;
 }
-template <class M>
-__device__ inline uint32_t count_code(uint32_t h) {
-  if ((h & M::kExp) != M::kExp) return 0;
-  if (h & 0x7fffu & ~M::kExp) return M::k16384;
-  return h & 0x8000u ? M::k128 : M::kOne;
-}
-template <class M>
-__device__ inline uint32_t count_pair(uint32_t w) {
-  return count_code<M>(w & 0xffffu) | count_code<M>(w >> 16) << 16;
-}
 // top bits set where a half is not finite
 template <class M>
 __device__ inline uint32_t odd_pair(uint32_t w) {
@@ -482,7 +499,9 @@ __device__ inline uint32_t odd_pair(uint32_t w) {
   return ((w & e) + one) & 0x80008000u;
 }
 
-// Block = (kv head, tile of 32 * NW rows, part of its tiles of BN keys); a wave
+constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
+
+// Block = (kv head, tile of 128 rows, part of its tiles of BN keys); a wave
 // has 32 rows. As in the decode kernel S^T = K Q^T and O^T = V^T P^T, here on
 // 32x32x16 instructions: a lane has half the scores of one row in registers,
 // its weights are the second product's operand as they stand, and a row's
@@ -490,14 +509,15 @@ __device__ inline uint32_t odd_pair(uint32_t w) {
 //
 // K and V tiles come straight from memory to LDS, double buffered: the next
 // tile's loads are issued before a tile is computed, one barrier a tile.
-template <class T, int D, int NW, int BN, bool CAP>
-__global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnArgs a) {
-  constexpr int NT = 64 * NW, BM = 32 * NW, CH = D / 8, kUnits = BN * CH / NT;
+template <class T, int D, int BN, bool CAP>
+__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+  constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
-  constexpr int KT = BN / 32, QS = D / 16, DT = D / 32;
+  constexpr int KT = BN / 32, QS = D / 16, DT = D / 32, kAhead = 2;
+  constexpr bool kPiped = true;
   static_assert(BN * CH % NT == 0, "whole units per thread");
   typedef Mx<T> M;
-  __shared__ __align__(16) char lds[4 * kTile];  // keys, values; keys, values
+  __shared__ __align__(1024) char lds[4 * kTile];  // two tiles of keys, two of values
   __shared__ int odd;  // 1 + index of the last tile found to hold values that are not finite
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
@@ -555,7 +575,6 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnArgs a) {
   const int qi = row / G, head = hk * G + row - qi * G, p = pos0 + qi;
   const bool in = wrow0 + col < R;
   const int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
-  const bool idle = wrow0 >= R;
 
   const Scale sc = fold_scale<CAP>(a);
   u32x4 qf[QS];
@@ -575,55 +594,71 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnArgs a) {
   auto look_up = [&](int it) -> int32_t {
     if (it >= it1) return -1;
     const int key = tile_of(it) * BN + (lane & (BN - 1));
-    const int32_t page = key < hi ? table[key >> a.p.page_shift] : -1;
-    return (uint32_t)page < (uint32_t)a.p.n_pages ? page : -1;
+    return key < hi ? table[key >> a.p.page_shift] : -1;
   };
+  // Looked at a turn after the load was issued: a wait for it is a wait for
+  // the tiles' loads before it.
+  auto checked = [&](int32_t page) { return (uint32_t)page < (uint32_t)a.p.n_pages ? page : -1; };
   // One load instruction takes 64 pieces, of rows that lie in one page when
-  // pages have 16 tokens or more: its page is then scalar, and the lanes'
-  // offsets are the same for every tile. A key that does not exist reads what
-  // is there (a page's end, or page 0); its score is masked and its value, if
-  // not finite, taken out.
+  // pages have 16 tokens or more: the address of its first row is then scalar,
+  // and the lanes' offsets are the same for every tile. A key that does not
+  // exist reads what is there (a page's end, or page 0); its score is masked
+  // and its value, if not finite, taken out.
   const bool whole = a.p.page_shift >= 4 && a.p.kst[1] < (1 << 24) && a.p.vst[1] < (1 << 24);
-  uint32_t koff[kUnits], voff[kUnits];
+  // (rows i * NT / CH apart have the same offsets, where that is a multiple of 16)
+  constexpr int kOffs = NT % (16 * CH) == 0 ? 1 : kUnits;
+  uint32_t koff[kOffs], voff[kOffs];
 #pragma unroll
-  for (int i = 0; i < kUnits; ++i) {
+  for (int i = 0; i < kOffs; ++i) {
     const int u0 = i * NT + 64 * wave, u = u0 + lane, r = u / CH, c = u - r * CH, r0 = u0 / CH;
     koff[i] = 2 * ((r - r0) * (uint32_t)a.p.kst[1] + 8 * key_piece<D>(r, c));
     voff[i] = 2 * ((r - r0) * (uint32_t)a.p.vst[1] + 8 * value_place<D>(r, c));
   }
-  uint64_t there = 0;  // bit i: key i of the tile being loaded exists
-  auto load = [&](int it, int buf, int32_t page) {
-    there = __ballot(page >= 0);
-    if (page < 0) page = 0;
+  const uint32_t lds0 = lds_address(lds) + 1024 * wave;
+  auto load = [&](int it, uint32_t to, int32_t page, const char* base, int64_t page_step, int64_t row_step,
+                  const uint32_t* off, auto piece) {
     const int key0 = tile_of(it) * BN;
-    const uint32_t kt = lds_address(lds) + buf * 2 * kTile + 1024 * wave, vt = kt + kTile;
+    if (page < 0) page = 0;
     if (whole) {
+      const uint64_t at = (uint64_t)(base + 2 * (page * page_step + ((key0 + lane) & a.p.page_mask) * row_step));
+      const int at_lo = (int)(uint32_t)at, at_hi = (int)(uint32_t)(at >> 32);
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
         const int r0 = (i * NT + 64 * wave) / CH;
-        const int64_t pg = __builtin_amdgcn_readlane(page, r0), at = (key0 + r0) & a.p.page_mask;
-        lds_load(kt + 16 * NT * i, kbase + 2 * (pg * a.p.kst[0] + at * a.p.kst[1]), koff[i]);
-        lds_load(vt + 16 * NT * i, vbase + 2 * (pg * a.p.vst[0] + at * a.p.vst[1]), voff[i]);
+        const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, r0) << 32 |
+                             (uint32_t)__builtin_amdgcn_readlane(at_lo, r0);
+        lds_load(to + 16 * NT * i, (const char*)row, off[i % kOffs]);
       }
     } else {
 #pragma unroll 1
       for (int i = 0; i < kUnits; ++i) {
         const int u = i * NT + threadIdx.x, r = u / CH, c = u - r * CH;
         const int64_t pg = __shfl(page, r), at = (key0 + r) & a.p.page_mask;
-        lds_load(kt + 16 * NT * i, kbase + 2 * (pg * a.p.kst[0] + at * a.p.kst[1] + 8 * key_piece<D>(r, c)));
-        lds_load(vt + 16 * NT * i, vbase + 2 * (pg * a.p.vst[0] + at * a.p.vst[1] + 8 * value_place<D>(r, c)));
+        lds_load(to + 16 * NT * i, base + 2 * (pg * page_step + at * row_step + 8 * piece(r, c)));
       }
     }
+  };
+  // keys and values have two slots each: tile it0 + i lies in slot i % 2
+  auto load_keys = [&](int it, int slot, int32_t page) {
+    load(it, lds0 + slot * kTile, page, kbase, a.p.kst[0], a.p.kst[1], koff, key_piece<D>);
+  };
+  auto load_values = [&](int it, int slot, int32_t page) {
+    load(it, lds0 + (2 + slot) * kTile, page, vbase, a.p.vst[0], a.p.vst[1], voff, value_place<D>);
   };
   // does some row of this range see only a part of the tile?
   auto part_seen = [&](int key0, int first, int last) {
     return !(key0 + BN - 1 <= first &&
              (a.window == 0 || key0 > last - a.window || key0 + BN - 1 < a.sinks));
   };
-  // does this lane's row see key i of the tile?
-  auto sees = [&](int key0, uint64_t exist, int i) {
-    const int key = key0 + i;
-    return key <= p && (a.window == 0 || key > p - a.window || key < a.sinks) && ((exist >> i) & 1);
+  // which keys of a tile this lane's row sees (bit i: key key0 + i)
+  auto seen_keys = [&](int key0, uint64_t exist) {
+    auto below = [&](int key) {  // the tile's keys below `key`
+      const int n = key - key0;
+      return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
+    };
+    uint64_t m = p >= 0 ? below(p + 1) & exist : 0ull;
+    if (a.window > 0 && p >= a.window) m &= ~below(p - a.window + 1) | below(a.sinks);
+    return m;
   };
 
   f32x16 o[DT];
@@ -633,153 +668,299 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_prompt_kernel(AttnArgs a) {
   const float slack = kSlack / sc.c;
   bool any = false;
 
-  // the transposed reads: value rows 4 half + (lane % 16) / 4, and pieces of
-  // 8 bytes; the place of a piece depends on the row modulo 4 alone
+  // A lane's places in a tile of keys (row col, piece 2 i + half) and of values
+  // (row 4 half + (lane % 16) / 4, 8-byte pieces, read transposed). Rows are
+  // whole multiples of 64 bytes (D = 96: 192) and the places differ by an
+  // exclusive or, so one address register serves all pieces.
   const int vr = 4 * half + (lane & 15) / 4, vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  uint32_t vplace[DT];
+  const uint32_t kat = col * kRow + 16 * key_place<D>(col, half);
+  const uint32_t vat = vr * kRow + 16 * value_place<D>(vr, vc) + 8 * (lane & 1);
+  auto key_frag = [&](int slot, int t, int i) {
+    const char* kt = lds + slot * kTile + 32 * t * kRow;
+    if constexpr (D == 96) {
+      const int r = 32 * t + col;
+      return *reinterpret_cast<const u32x4*>(kt + col * kRow + 16 * key_place<D>(r, 2 * i + half));
+    } else {
+      return *reinterpret_cast<const u32x4*>(kt + (kat ^ (32 * i)));
+    }
+  };
+  auto value_frag = [&](int slot, int t, int k) {
+    const char* vt = lds + (2 + slot) * kTile + 16 * k * kRow +
+                     (D == 96 ? vat + 64 * t : vat ^ (64 * t));
+    const u32x2 v0 = lds_transposed(vt), v1 = lds_transposed(vt + 8 * kRow);
+    return u32x4{v0[0], v0[1], v1[0], v1[1]};
+  };
+
+  // Scores of tile `it` ready in x: masks them where the wave's rows see only
+  // part of the tile, and moves the references that they pass. Returns the
+  // factor for the sums so far (1 for nearly every tile, then not applied).
+  bool moved;
+  float shrunk;
+  auto settle = [&](f32x16* x, int it, uint64_t exist, bool masked) {
+    if constexpr (CAP) {
 #pragma unroll
-  for (int t = 0; t < DT; ++t) vplace[t] = vr * kRow + 16 * value_place<D>(vr, 4 * t + vc) + 8 * (lane & 1);
-
-  if (threadIdx.x == 0) odd = 0;
-  int32_t page = look_up(it0);
-  if (it0 < it1) load(it0, 0, page);
-  page = look_up(it0 + 1);
-  uint64_t now = there;
-  landed_barrier();
-
-  for (int it = it0; it < it1; ++it) {
-    const int buf = (it - it0) & 1;
-    char* kt = lds + buf * 2 * kTile;
-    char* vt = kt + kTile;
-    const int key0 = tile_of(it) * BN;
-    if (it + 1 < it1) {
-      load(it + 1, buf ^ 1, page);
-      page = look_up(it + 2);
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] = fast_tanh(x[t][e] * sc.inner);
     }
-    const bool exist = BN == 64 ? now == ~0ull : (uint32_t)now == ~0u;  // all keys of the tile do
-    bool strange = false;
-    if (!exist || part_seen(key0, p_first, p_last)) {
-      uint32_t bits = 0;
-#pragma unroll 1
-      for (int i = 0; i < kUnits; ++i) {
-        const u32x4 v = *reinterpret_cast<const u32x4*>(vt + 16 * (i * NT + threadIdx.x));
-        bits |= odd_pair<M>(v[0]) | odd_pair<M>(v[1]) | odd_pair<M>(v[2]) | odd_pair<M>(v[3]);
-      }
-      if (bits) odd = it + 1;
-      __syncthreads();
-      strange = odd == it + 1;
-    }
-    const bool none = idle || key0 > pw_last ||
-                      (a.window > 0 && key0 + BN - 1 <= pw_first - a.window && key0 >= a.sinks);
-    u32x4 w[2 * KT];
-    if (!none) {
-      f32x16 x[KT];
+    if (masked) {
+      float hidden = -INFINITY;
+      asm volatile("" : "+v"(hidden));  // no register for it but here
+      const uint64_t see = seen_keys(tile_of(it) * BN, exist) >> (4 * half);
+      any |= (see & 0x0f0f0f0f0f0f0f0full) != 0;
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        x[t] = f32x16{};
+        const uint32_t m = (uint32_t)(see >> (32 * t));
 #pragma unroll
-        for (int i = 0; i < QS; ++i) {
-          const int r = 32 * t + col;
-          const u32x4 kf = *reinterpret_cast<const u32x4*>(kt + r * kRow + 16 * key_place<D>(r, 2 * i + half));
-          x[t] = M::mma32x16(kf, qf[i], x[t]);
-        }
+        for (int e = 0; e < 16; ++e) x[t][e] = m & (1u << (8 * (e / 4) + e % 4)) ? x[t][e] : hidden;
       }
-      if constexpr (CAP) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[t][e] = fast_tanh(x[t][e] * sc.inner);
-      }
-      if (!exist || part_seen(key0, pw_first, pw_last)) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (sees(key0, now, 32 * t + 8 * (e / 4) + 4 * half + e % 4)) any = true;
-            else x[t][e] = -INFINITY;
-          }
-      } else {
-        any = true;
-      }
-      float top = x[0][0];
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) top = fmaxf(top, x[t][e]);
-      if (__any(top > ref + slack)) {  // a row's own scores alone decide for it
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = top > ref + slack ? top : ref, f = shrink(ref, to, sc.c);
-        sum *= f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] *= f;
-        ref = to;
-      }
-      const float base = -ref * sc.c;
-      float add[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float w0 = __builtin_amdgcn_exp2f(fmaf(x[t][e], sc.c, base));
-          const float w1 = __builtin_amdgcn_exp2f(fmaf(x[t][e + 1], sc.c, base));
-          add[(e / 2) & 3] += w0 + w1;
-          w[2 * t + e / 8][(e / 2) & 3] = M::pack(w0, w1);
-        }
-      sum += (add[0] + add[1]) + (add[2] + add[3]);
+    } else {
+      any = true;
     }
-    if (strange) {
-      if (!none) {
-#pragma unroll 1
-        for (int t = 0; t < DT; ++t) {
-          f32x16 n = f32x16{};
-#pragma unroll 1
-          for (int k = 0; k < 2 * KT; ++k) {
-            const char* vp = vt + 16 * k * kRow + vr * kRow + 16 * value_place<D>(vr, 4 * t + vc) + 8 * (lane & 1);
-            const u32x2 v0 = lds_transposed(vp), v1 = lds_transposed(vp + 8 * kRow);
-            uint32_t see = 0;
-            for (int e = 0; e < 8; ++e)
-              see |= (uint32_t)sees(key0, now, 16 * k + 8 * (e / 4) + 4 * half + e % 4) << e;
-            u32x4 c = {count_pair<M>(v0[0]), count_pair<M>(v0[1]), count_pair<M>(v1[0]), count_pair<M>(v1[1])}, on;
-            for (int i = 0; i < 4; ++i)
-              on[i] = ((see >> (2 * i)) & 1 ? M::kOne : 0u) | ((see >> (2 * i)) & 2 ? M::kOne << 16 : 0u);
-            n = M::mma32x16(c, on, n);
-          }
-          f32x16 f;
-          for (int e = 0; e < 16; ++e) {
-            const int counts = (int)n[e], nan = counts >> 14, neg = (counts >> 7) & 127, pos = counts & 127;
-            f[e] = nan || (neg && pos) ? __builtin_nanf("") : neg ? -INFINITY : pos ? INFINITY : 0.0f;
-          }
+    float part[4];
 #pragma unroll
-          for (int u = 0; u < DT; ++u)
-            if (u == t) o[u] += f;
-        }
-      }
-      __syncthreads();
-#pragma unroll 1
-      for (int i = 0; i < kUnits; ++i) {
-        u32x4* v = reinterpret_cast<u32x4*>(vt + 16 * (i * NT + threadIdx.x));
-        u32x4 t = *v;
-        for (int j = 0; j < 4; ++j) t[j] = finite_pair<M>(t[j]);
-        *v = t;
-      }
-      __syncthreads();
+    for (int e = 0; e < 4; ++e) part[e] = max3(x[0][e], x[0][e + 4], x[0][e + 8]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[e] = KT == 1 ? fmaxf(part[e], x[0][e + 12]) : max3(part[e], x[0][e + 12], x[KT - 1][e]);
+    if constexpr (KT == 2) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) part[e] = max3(part[e], x[1][e + 4], x[1][e + 8]);
+      part[0] = max3(part[0], x[1][12], x[1][13]);
+      part[1] = max3(part[1], x[1][14], x[1][15]);
     }
-    if (!none) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-#pragma unroll
-        for (int k = 0; k < 2 * KT; ++k) {
-          const char* vp = vt + vplace[t] + 16 * k * kRow;
-          const u32x2 v0 = lds_transposed(vp), v1 = lds_transposed(vp + 8 * kRow);
-          o[t] = M::mma32x16(u32x4{v0[0], v0[1], v1[0], v1[1]}, w[k], o[t]);
-        }
+    float top = max3(max3(part[0], part[1], part[2]), part[3], part[3]);
+    moved = __any(top > ref + slack);
+    if (moved) {  // a row's own scores alone decide for it
+      top = halves_max(top);
+      const float to = top > ref + slack ? top : ref;
+      shrunk = shrink(ref, to, sc.c);
+      sum *= shrunk;
+      ref = to;
     }
-    now = there;
+  };
+  // Weights of scores 2 i and 2 i + 1, rounded to the type; the sum takes the
+  // rounded ones, so that a row's weights add up to one as they are used.
+  float add[4];
+  auto weigh = [&](const f32x16* x, int i) {
+    const float base = -ref * sc.c;
+    const float w0 = __builtin_amdgcn_exp2f(fmaf(x[i / 8][2 * i % 16], sc.c, base));
+    const float w1 = __builtin_amdgcn_exp2f(fmaf(x[i / 8][2 * i % 16 + 1], sc.c, base));
+    const uint32_t pair = M::pack(w0, w1);
+    add[i & 3] = M::add_pair(pair, i < 4 ? 0.0f : add[i & 3]);
+    return pair;
+  };
+  // values of tile `it` that are not finite, where some row sees only part of the tile
+  auto odd_values = [&](int it, int slot, uint64_t exist, bool all) {
+    const int key0 = tile_of(it) * BN;
+    if (all && !part_seen(key0, p_first, p_last)) return;
+    char* vt = lds + (2 + slot) * kTile;
+    uint32_t bits = 0;
+#pragma unroll 1
+    for (int i = 0; i < kUnits; ++i) {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(vt + 16 * (i * NT + threadIdx.x));
+      bits |= odd_pair<M>(v[0]) | odd_pair<M>(v[1]) | odd_pair<M>(v[2]) | odd_pair<M>(v[3]);
+    }
+    if (bits) odd = it + 1;
+    __syncthreads();
+    if (odd != it + 1) return;
+    // constants of this path, kept out of the loop's registers
+    uint32_t one = M::kOne, c128 = M::k128, c16384 = M::k16384, inf = 0x7f800000u;
+    asm volatile("" : "+s"(one), "+s"(c128), "+s"(c16384), "+s"(inf));
+    auto code = [&](uint32_t h) {
+      const uint32_t e = h & M::kExp, f = h & 0x7fffu & ~M::kExp;
+      return e != M::kExp ? 0u : f ? c16384 : h & 0x8000u ? c128 : one;
+    };
+    const uint64_t see = seen_keys(key0, exist) >> (4 * half);
+#pragma unroll 1
+    for (int t = 0; t < DT; ++t) {
+      f32x16 n = f32x16{};
+#pragma unroll 1
+      for (int k = 0; k < 2 * KT; ++k) {
+        const u32x4 v = value_frag(slot, t, k);
+        u32x4 c, on;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t two = (uint32_t)(see >> (16 * k + 8 * (i / 2) + 2 * (i & 1)));
+          c[i] = code(v[i] & 0xffffu) | code(v[i] >> 16) << 16;
+          on[i] = (two & 1 ? one : 0u) | (two & 2 ? one << 16 : 0u);
+        }
+        n = M::mma32x16(c, on, n);
+      }
+      f32x16 f;
+      for (int e = 0; e < 16; ++e) {
+        const int counts = (int)n[e], nan = counts >> 14, neg = (counts >> 7) & 127, pos = counts & 127;
+        const uint32_t bits = nan || (neg && pos) ? inf | 0x400000u : neg ? inf | 0x80000000u : pos ? inf : 0u;
+        f[e] = u2f(bits);
+      }
+#pragma unroll
+      for (int u = 0; u < DT; ++u)
+        if (u == t) o[u] += f;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = 0; i < kUnits; ++i) {
+      u32x4* v = reinterpret_cast<u32x4*>(vt + 16 * (i * NT + threadIdx.x));
+      u32x4 t = *v;
+      for (int j = 0; j < 4; ++j) t[j] = finite_pair<M>(t[j]);
+      *v = t;
+    }
+    __syncthreads();
+  };
+  auto all_of = [&](uint64_t exist) { return BN == 64 ? exist == ~0ull : (uint32_t)exist == ~0u; };
+
+  // One step: the product of tile it - 1 with its weights w, the weights wn of
+  // tile `it`, whose scores x are ready, and the scores of tile it + 1 into y:
+  // independent pieces, so that the matrix cores and the vector units have
+  // work side by side from every wave. The product comes first, so that w is
+  // done with when y begins. Before the first tile the weights are zero; behind
+  // the last one the scores are of stale keys and not used.
+  // The operands of the matrix instructions are read kAhead ahead; nothing
+  // moves across a pair of weights, or the reads would all come first and spill.
+  constexpr int kPairs = 8 * KT, kQ = KT * QS, kP = DT * 2 * KT;
+  auto step = [&](const f32x16* x, f32x16* y, const u32x4* w, u32x4* wn, int slot) {
+    u32x4 f[kAhead + 1];
+    auto frag = [&](int n) {
+      return n < kP ? value_frag(slot ^ 1, n % DT, n / DT) : key_frag(slot ^ 1, (n - kP) / QS, (n - kP) % QS);
+    };
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) f[j] = frag(j);
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = i * (kQ + kP) / kPairs; n < (i + 1) * (kQ + kP) / kPairs; ++n) {
+        if (n + kAhead < kQ + kP) f[(n + kAhead) % (kAhead + 1)] = frag(n + kAhead);
+        const u32x4& v = f[n % (kAhead + 1)];
+        const int j = n - kP;
+        if (j < 0)
+          o[n % DT] = M::mma32x16(v, w[n / DT], o[n % DT]);
+        else
+          y[j / QS] = M::mma32x16(v, qf[j % QS], j % QS ? y[j / QS] : f32x16{});
+      }
+      wn[i / 4][i & 3] = weigh(x, i);
+      if (i % 4 == 3) {  // here, and not where they are used
+        asm volatile("" : "+v"(wn[i / 4]));
+        asm volatile("" : "+v"(add[0]), "+v"(add[1]), "+v"(add[2]), "+v"(add[3]));
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    sum += (add[0] + add[1]) + (add[2] + add[3]);
+  };
+
+  if (threadIdx.x == 0) odd = 0;
+  if constexpr (kPiped) if (it0 < it1) {
+    // pages of the tiles it, it + 1 and it + 2, and which keys of it - 1 and it exist
+    int32_t page0 = checked(look_up(it0)), page1 = checked(look_up(it0 + 1)), next = look_up(it0 + 2);
+    uint64_t exist = __ballot(page0 >= 0), exist1 = 0;
+    load_keys(it0, 0, page0);
+    if (it0 + 1 < it1) load_keys(it0 + 1, 1, page1);
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i)  // the values in front of the first tile
+      *reinterpret_cast<u32x4*>(lds + 3 * kTile + 16 * (i * NT + threadIdx.x)) = u32x4{0, 0, 0, 0};
     landed_barrier();
+    f32x16 xa[KT], xb[KT];
+    u32x4 wa[2 * KT], wb[2 * KT];
+#pragma unroll
+    for (int k = 0; k < 2 * KT; ++k) wb[k] = u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      xa[t] = f32x16{};
+#pragma unroll
+      for (int i = 0; i < QS; ++i) xa[t] = M::mma32x16(key_frag(0, t, i), qf[i], xa[t]);
+    }
+    __syncthreads();  // its slot is loaded again below
+
+    auto turn = [&](f32x16* x, f32x16* y, const u32x4* w, u32x4* wn, int it, int slot) {
+      const int32_t page2 = checked(next);
+      next = look_up(it + 3);
+      load_values(it, slot, page0);
+      if (it + 2 < it1) load_keys(it + 2, slot, page2);
+      page0 = page1;
+      page1 = page2;
+      const bool masked = !all_of(exist) || part_seen(tile_of(it) * BN, pw_first, pw_last);
+      settle(x, it, exist, masked);
+      if (it > it0) odd_values(it - 1, slot ^ 1, exist1, all_of(exist1));
+      step(x, y, w, wn, slot);
+      if (moved) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= shrunk;
+      }
+      exist1 = exist;
+      exist = __ballot(page0 >= 0);
+      landed_barrier();
+    };
+    auto drain = [&](const u32x4* w, int slot) {
+      odd_values(it1 - 1, slot, exist1, all_of(exist1));
+#pragma unroll
+      for (int j = 0; j < kP; ++j) o[j % DT] = M::mma32x16(value_frag(slot, j % DT, j / DT), w[j / DT], o[j % DT]);
+    };
+    // two turns a round, so that no score or weight is moved between registers
+    int it = it0;
+    for (; it + 1 < it1; it += 2) {
+      turn(xa, xb, wb, wa, it, 0);
+      turn(xb, xa, wa, wb, it + 1, 1);
+    }
+    if (it < it1) {
+      turn(xa, xb, wb, wa, it, 0);
+      drain(wa, 0);
+    } else {
+      drain(wb, 1);
+    }
+  }
+  // Rows of 256 values leave no registers for a second tile's scores: scores,
+  // weights and product of a tile one after the other.
+  if constexpr (!kPiped) if (it0 < it1) {
+    int32_t page0 = checked(look_up(it0)), next = look_up(it0 + 1);
+    uint64_t exist = __ballot(page0 >= 0);
+    load_keys(it0, 0, page0);
+    load_values(it0, 0, page0);
+    landed_barrier();
+    auto turn = [&](int it, int slot) {
+      page0 = checked(next);
+      next = look_up(it + 2);
+      if (it + 1 < it1) {
+        load_keys(it + 1, slot ^ 1, page0);
+        load_values(it + 1, slot ^ 1, page0);
+      }
+      f32x16 x[KT];
+      u32x4 w[2 * KT], f[kAhead + 1];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) f[j] = key_frag(slot, j / QS, j % QS);
+#pragma unroll
+      for (int j = 0; j < kQ; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int n = j + kAhead;
+        if (n < kQ) f[n % (kAhead + 1)] = key_frag(slot, n / QS, n % QS);
+        x[j / QS] = M::mma32x16(f[j % (kAhead + 1)], qf[j % QS], j % QS ? x[j / QS] : f32x16{});
+      }
+      settle(x, it, exist, !all_of(exist) || part_seen(tile_of(it) * BN, pw_first, pw_last));
+      if (moved) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t) o[t] *= shrunk;
+      }
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) w[i / 4][i & 3] = weigh(x, i);
+      sum += (add[0] + add[1]) + (add[2] + add[3]);
+      odd_values(it, slot, exist, all_of(exist));
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) f[j] = value_frag(slot, j % DT, j / DT);
+#pragma unroll
+      for (int j = 0; j < kP; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int n = j + kAhead;
+        if (n < kP) f[n % (kAhead + 1)] = value_frag(slot, n % DT, n / DT);
+        o[j % DT] = M::mma32x16(f[j % (kAhead + 1)], w[j / DT], o[j % DT]);
+      }
+      exist = __ballot(page0 >= 0);
+      landed_barrier();
+    };
+    for (int it = it0; it < it1; it += 2) {
+      turn(it, 0);
+      if (it + 1 < it1) turn(it + 1, 1);
+    }
   }
 
-  sum += __shfl_xor(sum, 32);
-  any |= __shfl_xor((int)any, 32) != 0;
+  sum = halves_sum(sum);
+  any = halves_sum(any ? 1.0f : 0.0f) != 0.0f;
   if (a.splits > 1) {
     const int64_t at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.z;
     if (!in) return;
@@ -844,17 +1025,16 @@ int64_t part_bytes(int64_t rows, int splits, int64_t head_dim) {
   return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
 }
 
-// Rows of a block of the prompt kernel, and the most blocks' tiles that the rows can take.
-int prompt_rows(int64_t head_dim) { return head_dim == 256 ? 256 : 128; }
-int64_t prompt_tiles(const KvBatchView& b, int64_t group, int rows) {
-  return (int64_t)b.tokens * group / rows + std::min(b.batch, b.tokens);
+// The most tiles that the rows of a call can take.
+int64_t prompt_tiles(const KvBatchView& b, int64_t group) {
+  return (int64_t)b.tokens * group / kPromptRows + std::min(b.batch, b.tokens);
 }
 
 int plan_splits(const KvView& p, const KvBatchView& b, int64_t q_heads, int64_t window, int64_t sinks) {
   if (b.batch == 0 || b.tokens == 0) return 1;
   const int64_t group = q_heads / p.kv_heads;
   if (b.starts)
-    return choose_splits(p, b, p.kv_heads * prompt_tiles(b, group, prompt_rows(p.head_dim)), window, sinks);
+    return choose_splits(p, b, p.kv_heads * prompt_tiles(b, group), window, sinks);
   return choose_splits(p, b, (int64_t)b.batch * p.kv_heads * ((group + 15) / 16), window, sinks);
 }
 
@@ -867,13 +1047,13 @@ void launch_decode(const AttnArgs& a, hipStream_t stream) {
     HGK_LAUNCH((attn_decode_kernel<T, D, NS, false>), grid, block, 0, stream, a);
 }
 
-template <class T, int D, int NW, int BN>
+template <class T, int D, int BN>
 void launch_prompt(const AttnArgs& a, hipStream_t stream) {
-  const dim3 grid(a.p.kv_heads, prompt_tiles(a.b, a.group, 32 * NW), a.splits), block(64 * NW);
+  const dim3 grid(a.p.kv_heads, prompt_tiles(a.b, a.group), a.splits), block(2 * kPromptRows);
   if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_prompt_kernel<T, D, NW, BN, true>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, true>), grid, block, 0, stream, a);
   else
-    HGK_LAUNCH((attn_prompt_kernel<T, D, NW, BN, false>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, false>), grid, block, 0, stream, a);
 }
 
 template <class T>
@@ -887,10 +1067,10 @@ int run(const AttnArgs& a, const char* what, hipStream_t stream) {
     }
   } else {
     switch (a.p.head_dim) {
-      case 64: launch_prompt<T, 64, 4, 64>(a, stream); break;
-      case 96: launch_prompt<T, 96, 4, 64>(a, stream); break;
-      case 128: launch_prompt<T, 128, 4, 64>(a, stream); break;
-      default: launch_prompt<T, 256, 8, 32>(a, stream); break;
+      case 64: launch_prompt<T, 64, 64>(a, stream); break;
+      case 96: launch_prompt<T, 96, 64>(a, stream); break;
+      case 128: launch_prompt<T, 128, 64>(a, stream); break;
+      default: launch_prompt<T, 256, 64>(a, stream); break;
     }
   }
   if (int st = launch_status(what)) return st;
