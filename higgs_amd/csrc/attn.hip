@@ -514,7 +514,6 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
   constexpr int KT = BN / 32, QS = D / 16, DT = D / 32, kAhead = 2;
-  constexpr bool kPiped = true;
   static_assert(BN * CH % NT == 0, "whole units per thread");
   typedef Mx<T> M;
   __shared__ __align__(1024) char lds[4 * kTile];  // two tiles of keys, two of values
@@ -577,15 +576,6 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   const int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
 
   const Scale sc = fold_scale<CAP>(a);
-  u32x4 qf[QS];
-  {
-    const char* qp = a.q + 2 * ((int64_t)(s.first + qi) * a.qst[0] + head * a.qst[1] + 8 * half);
-#pragma unroll
-    for (int i = 0; i < QS; ++i) {
-      qf[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
-      for (int w = 0; w < 4; ++w) qf[i][w] = (qf[i][w] & sc.keep) ^ sc.flip;
-    }
-  }
 
   // lane l looks up key l of a tile
   const int32_t* table = a.b.table + (int64_t)seq * a.b.table_stride;
@@ -661,6 +651,15 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     return m;
   };
 
+  u32x4 qf[QS];
+  auto load_rows = [&]() {  // behind the first keys' loads: one wait for both
+    const char* qp = a.q + 2 * ((int64_t)(s.first + qi) * a.qst[0] + head * a.qst[1] + 8 * half);
+#pragma unroll
+    for (int i = 0; i < QS; ++i) {
+      qf[i] = *reinterpret_cast<const u32x4*>(qp + 32 * i);
+      for (int w = 0; w < 4; ++w) qf[i][w] = (qf[i][w] & sc.keep) ^ sc.flip;
+    }
+  };
   f32x16 o[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) o[t] = f32x16{};
@@ -847,12 +846,15 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   };
 
   if (threadIdx.x == 0) odd = 0;
-  if constexpr (kPiped) if (it0 < it1) {
+  if (it0 < it1) {
     // pages of the tiles it, it + 1 and it + 2, and which keys of it - 1 and it exist
-    int32_t page0 = checked(look_up(it0)), page1 = checked(look_up(it0 + 1)), next = look_up(it0 + 2);
+    int32_t page0 = look_up(it0), page1 = look_up(it0 + 1), next = look_up(it0 + 2);
+    page0 = checked(page0);
+    page1 = checked(page1);
     uint64_t exist = __ballot(page0 >= 0), exist1 = 0;
     load_keys(it0, 0, page0);
     if (it0 + 1 < it1) load_keys(it0 + 1, 1, page1);
+    load_rows();
 #pragma unroll
     for (int i = 0; i < kUnits; ++i)  // the values in front of the first tile
       *reinterpret_cast<u32x4*>(lds + 3 * kTile + 16 * (i * NT + threadIdx.x)) = u32x4{0, 0, 0, 0};
@@ -870,6 +872,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     __syncthreads();  // its slot is loaded again below
 
     auto turn = [&](f32x16* x, f32x16* y, const u32x4* w, u32x4* wn, int it, int slot) {
+      asm volatile("" : "+v"(next));  // waits here if it must, in front of the tiles' loads
       const int32_t page2 = checked(next);
       next = look_up(it + 3);
       load_values(it, slot, page0);
@@ -906,59 +909,6 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
       drain(wb, 1);
     }
   }
-  // Rows of 256 values leave no registers for a second tile's scores: scores,
-  // weights and product of a tile one after the other.
-  if constexpr (!kPiped) if (it0 < it1) {
-    int32_t page0 = checked(look_up(it0)), next = look_up(it0 + 1);
-    uint64_t exist = __ballot(page0 >= 0);
-    load_keys(it0, 0, page0);
-    load_values(it0, 0, page0);
-    landed_barrier();
-    auto turn = [&](int it, int slot) {
-      page0 = checked(next);
-      next = look_up(it + 2);
-      if (it + 1 < it1) {
-        load_keys(it + 1, slot ^ 1, page0);
-        load_values(it + 1, slot ^ 1, page0);
-      }
-      f32x16 x[KT];
-      u32x4 w[2 * KT], f[kAhead + 1];
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) f[j] = key_frag(slot, j / QS, j % QS);
-#pragma unroll
-      for (int j = 0; j < kQ; ++j) {
-        __builtin_amdgcn_sched_barrier(0);
-        const int n = j + kAhead;
-        if (n < kQ) f[n % (kAhead + 1)] = key_frag(slot, n / QS, n % QS);
-        x[j / QS] = M::mma32x16(f[j % (kAhead + 1)], qf[j % QS], j % QS ? x[j / QS] : f32x16{});
-      }
-      settle(x, it, exist, !all_of(exist) || part_seen(tile_of(it) * BN, pw_first, pw_last));
-      if (moved) {
-#pragma unroll
-        for (int t = 0; t < DT; ++t) o[t] *= shrunk;
-      }
-#pragma unroll
-      for (int i = 0; i < kPairs; ++i) w[i / 4][i & 3] = weigh(x, i);
-      sum += (add[0] + add[1]) + (add[2] + add[3]);
-      odd_values(it, slot, exist, all_of(exist));
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) f[j] = value_frag(slot, j % DT, j / DT);
-#pragma unroll
-      for (int j = 0; j < kP; ++j) {
-        __builtin_amdgcn_sched_barrier(0);
-        const int n = j + kAhead;
-        if (n < kP) f[n % (kAhead + 1)] = value_frag(slot, n % DT, n / DT);
-        o[j % DT] = M::mma32x16(f[j % (kAhead + 1)], w[j / DT], o[j % DT]);
-      }
-      exist = __ballot(page0 >= 0);
-      landed_barrier();
-    };
-    for (int it = it0; it < it1; it += 2) {
-      turn(it, 0);
-      if (it + 1 < it1) turn(it + 1, 1);
-    }
-  }
-
   sum = halves_sum(sum);
   any = halves_sum(any ? 1.0f : 0.0f) != 0.0f;
   if (a.splits > 1) {
