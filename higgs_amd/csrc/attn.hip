@@ -24,9 +24,12 @@ struct AttnArgs {
   int32_t q_heads, group;  // group = q heads per kv head
   float scale, softcap;
   int32_t window, sinks;
-  int32_t splits;  // parts of the cache; more than one: joined from the workspace
-  float* part;     // [tokens * q_heads][splits][head_dim], not normalised
-  float* stat;     // [tokens * q_heads][splits][2]: reference (log2 domain), sum
+  // Parts of the keys; more than one are joined from the workspace. Prompts: of
+  // every row, [tokens * q_heads][splits]. One token: blocks that share the work,
+  // [row tiles][splits][2][16].
+  int32_t splits;
+  float* part;  // [...][head_dim], not normalised
+  float* stat;  // [...][2]: reference (log2 domain), sum
 };
 
 // Matrix instructions, pair packing and the non-finite test of the two types.
@@ -178,10 +181,75 @@ __device__ inline Seen seen_by_last(const AttnArgs& a, int32_t len) {
 
 constexpr int kDecWaves = 4;
 
-// One new token per sequence: block = (part of the cache, 16 of a kv head's
-// query heads, sequence and kv head). Each wave walks its own tiles of NS * 16
-// keys with a softmax of its own; nothing is shared until the end, so no wave
-// waits for another.
+// Keys of a decode tile, and the fewest tiles that a block takes (two a wave).
+template <int D> constexpr int dec_keys() { return D == 256 ? 16 : 32; }
+constexpr int kDecMinTiles = 2 * kDecWaves;
+
+// The tiles of all (sequence, kv head) pairs, one after the other, dealt out to
+// the blocks in equal runs, whatever the lengths: no block is left with a long
+// sequence, and a short one in a wide table is still spread. A run may end in
+// the middle of a pair; its part is then joined with the neighbours' by
+// attn_decode_join_kernel. Every wave of both kernels works this out for itself.
+struct Deal {
+  int64_t before;  // tiles in front of the sequence's
+  int64_t share;   // tiles of a block
+  int32_t seq, tiles;  // tiles of one pair of the sequence
+  Seen seen;
+};
+// Of the sequence that has tile `want` (or of sequence `seq`, where that is given).
+template <int KEYS>
+__device__ inline Deal deal_out(const AttnArgs& a, int blocks, int64_t block, int seq) {
+  const int lane = threadIdx.x & 63;
+  auto tiles_of = [&](int b, Seen& s) {
+    s = b < a.b.batch ? seen_by_last(a, a.b.lens[b]) : Seen{0, 0, 0};
+    return (s.n + KEYS - 1) / KEYS;
+  };
+  Deal d{0, 0, -1, 0, {0, 0, 0}};
+  Seen s;
+  int64_t total = 0, upto = 0;
+  for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
+    upto = (int64_t)tiles_of(b0 + lane, s) * a.p.kv_heads;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t v = __shfl_up(upto, o);
+      if (lane >= o) upto += v;
+    }
+    total += __shfl(upto, 63);
+  }
+  d.share = (total + blocks - 1) / blocks;
+  if (d.share < kDecMinTiles) d.share = kDecMinTiles;
+  const int64_t want = block * d.share;
+  if (seq < 0 && want >= total) return d;
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
+    const int tiles = tiles_of(b0 + lane, s);
+    const int64_t mine = (int64_t)tiles * a.p.kv_heads;
+    if (a.b.batch > 64) {
+      upto = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t v = __shfl_up(upto, o);
+        if (lane >= o) upto += v;
+      }
+    }
+    const uint64_t has = __ballot(seq < 0 ? before + upto > want : b0 + lane == seq);
+    if (has) {
+      const int l = __builtin_ctzll(has);
+      d.seq = b0 + l;
+      d.before = before + __shfl(upto - mine, l);
+      d.tiles = __shfl(tiles, l);
+      d.seen = Seen{__shfl(s.n, l), __shfl(s.sinks, l), __shfl(s.skip, l)};
+      return d;
+    }
+    before += __shfl(upto, 63);
+  }
+  return d;
+}
+
+// One new token per sequence: block = (16 of a kv head's query heads; a run of
+// tiles, or with one part a (sequence, kv head)). Each wave walks its own tiles
+// of NS * 16 keys with a softmax of its own; nothing is shared until a pair's
+// end, so no wave waits for another.
 //
 // A tile's scores are S^T = K Q^T on 16x16x32 matrix instructions: keys are
 // the rows, so K's 16-byte pieces go from memory straight into the operand,
@@ -192,9 +260,9 @@ constexpr int kDecWaves = 4;
 //
 // Weights are split in two 16-bit parts (hi + lo, both multiplied): the
 // matrix cores have time to spare, and the result is as good as f32 weights.
-template <class T, int D, int NS, bool CAP>
+template <class T, int D, bool CAP>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs a) {
-  constexpr int kKeys = 16 * NS, kStep = D / 32, kOut = D / 16;
+  constexpr int NS = dec_keys<D>() / 16, kKeys = 16 * NS, kStep = D / 32, kOut = D / 16;
   // V rows 32 bytes apart in banks: 16 rows of a transposed read cover each bank twice
   constexpr int kRow = 2 * D + 32, kTile = kKeys * kRow;
   constexpr int kJoin = kDecWaves * 16 * D * 4;
@@ -204,18 +272,43 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m = lane & 15, j = lane >> 4;
-  const int seq = blockIdx.x / a.p.kv_heads, hk = blockIdx.x - seq * a.p.kv_heads, part = blockIdx.z;
-  const int h0 = hk * a.group + blockIdx.y * 16;  // first of this block's heads
-  const int heads = min(16, a.group - (int)blockIdx.y * 16);
   const Scale sc = fold_scale<CAP>(a);
+  const int heads = min(16, a.group - (int)blockIdx.y * 16);
 
-  // this block's keys: whole tiles, as even as they go
-  const Seen seen = seen_by_last(a, a.b.lens[seq]);
-  const int tiles = (seen.n + kKeys - 1) / kKeys;
-  int per = (tiles + a.splits - 1) / a.splits;
-  if (per < 2 * kDecWaves) per = 2 * kDecWaves;
-  const int first = min((int64_t)per * part, (int64_t)tiles);
-  const int last = min(first + per, tiles);
+  Deal deal;
+  int64_t at_tile = 0, end_tile = 0;
+  if (a.splits > 1) {
+    deal = deal_out<kKeys>(a, a.splits, blockIdx.x, -1);
+    if (deal.seq < 0) return;
+    at_tile = blockIdx.x * deal.share;
+    end_tile = at_tile + deal.share;
+  } else {
+    deal.seq = blockIdx.x / a.p.kv_heads;
+    deal.seen = seen_by_last(a, a.b.lens[deal.seq]);
+    deal.tiles = (deal.seen.n + kKeys - 1) / kKeys;
+    deal.before = 0;
+    at_tile = (int64_t)(blockIdx.x - deal.seq * a.p.kv_heads) * deal.tiles;
+  }
+  for (bool head_of_run = true;; head_of_run = false) {
+  // this pair, and the tiles of it that fall to this block
+  const int seq = __builtin_amdgcn_readfirstlane(deal.seq), tiles = __builtin_amdgcn_readfirstlane(deal.tiles);
+  const Seen seen{__builtin_amdgcn_readfirstlane(deal.seen.n), __builtin_amdgcn_readfirstlane(deal.seen.sinks),
+                  __builtin_amdgcn_readfirstlane(deal.seen.skip)};
+  int hk, first, last;
+  if (a.splits > 1) {
+    hk = (int)((at_tile - deal.before) / tiles);
+    first = (int)(at_tile - deal.before - (int64_t)hk * tiles);
+    last = (int)min((int64_t)tiles, first + end_tile - at_tile);
+  } else {
+    hk = blockIdx.x - seq * a.p.kv_heads;
+    first = 0;
+    last = tiles;
+  }
+  hk = __builtin_amdgcn_readfirstlane(hk);
+  first = __builtin_amdgcn_readfirstlane(first);
+  last = __builtin_amdgcn_readfirstlane(last);
+  const bool whole = first == 0 && last == tiles;
+  const int h0 = hk * a.group + blockIdx.y * 16;  // first of this block's heads
 
   u32x4 qf[kStep];
   {
@@ -373,6 +466,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   __syncthreads();
   bool some = false;
   for (int w = 0; w < kDecWaves; ++w) some |= wseen[w] != 0;
+  // a part of the run's first pair, or of its last
+  const int64_t slot = (((int64_t)blockIdx.y * a.splits + blockIdx.x) * 2 + (head_of_run ? 0 : 1)) * 16;
   for (int idx = threadIdx.x; idx < heads * (D / 2); idx += 64 * kDecWaves) {
     const int h = idx / (D / 2), d = 2 * (idx - h * (D / 2));
     float top = wref[0][h];
@@ -385,52 +480,141 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
       v0 = fmaf(src[0], f, v0);
       v1 = fmaf(src[1], f, v1);
     }
-    const int64_t row = (int64_t)seq * a.q_heads + h0 + h;
-    if (a.splits > 1) {
-      if (some) {
-        float* p = a.part + (row * a.splits + part) * D + d;
-        *reinterpret_cast<f32x2*>(p) = f32x2{v0, v1};
-      }
-      if (d == 0) {
-        float* st = a.stat + 2 * (row * a.splits + part);
-        st[0] = some ? top * sc.c : -INFINITY;
-        st[1] = l;
-      }
-    } else {
+    if (whole) {
       const float r = 1.0f / l;
       *reinterpret_cast<uint32_t*>(a.out + 2 * (seq * a.ost[0] + (h0 + h) * a.ost[1] + d)) =
           some ? T::pack(v0 * r, v1 * r) : 0u;
+    } else {
+      *reinterpret_cast<f32x2*>(a.part + (slot + h) * D + d) = f32x2{v0, v1};
+      if (d == 0)
+        *reinterpret_cast<f32x2*>(a.stat + 2 * (slot + h)) = f32x2{some ? top * sc.c : -INFINITY, l};
     }
+  }
+  if (a.splits == 1) return;
+  // the run's next pair: the sequence's next head, or the next sequence that sees anything
+  at_tile += last - first;
+  if (at_tile >= end_tile) return;
+  if (at_tile - deal.before >= (int64_t)tiles * a.p.kv_heads) {
+    deal.before = at_tile;
+    do {
+      if (++deal.seq >= a.b.batch) return;
+      deal.seen = seen_by_last(a, a.b.lens[deal.seq]);
+      deal.tiles = (deal.seen.n + kKeys - 1) / kKeys;
+    } while (deal.tiles == 0);
+  }
+  __syncthreads();  // the waves' sums are read; V tiles may be written again
   }
 }
 
-// Joins the parts of one row (token and query head) per block: out =
-// sum_s 2^(ref_s - max) part_s / sum_s 2^(ref_s - max) sum_s. Parts that saw
-// no key (ref = -inf) were not written.
-template <class T>
-__global__ __launch_bounds__(128) void attn_join_kernel(AttnArgs a) {
-  const int t = blockIdx.x, h = blockIdx.y, D = a.p.head_dim, d = 2 * threadIdx.x;
-  const KvSeq s = kv_seq(a.b, kv_row_owner(a.b, t));
-  if (t < s.first || t >= s.first + s.n) return;
-  const int64_t row = (int64_t)t * a.q_heads + h;
-  const float* stat = a.stat + 2 * row * a.splits;
-  float top = -INFINITY;
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, stat[2 * i]);
-  if (d >= D) return;
-  float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
-  const float* part = a.part + row * a.splits * D + d;
+// Joins the parts of a (sequence, query head): out = sum 2^(ref - max) part /
+// sum 2^(ref - max) sum over the blocks whose runs meet in its pair (parts that
+// saw no key have ref = -inf). Pairs that one block had are written already;
+// a sequence that sees nothing gets its zeros here.
+template <class T, int D>
+__global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
+  __shared__ f32x4 vs[kGroups][kLanes];
+  __shared__ float ls[kGroups];
+  const int seq = blockIdx.x, h = blockIdx.y, hk = h / a.group, in = h - hk * a.group;
+  const Deal d = deal_out<dec_keys<D>()>(a, a.splits, 0, seq);
+  const int g = threadIdx.x / kLanes, c = threadIdx.x - g * kLanes;
+  char* out = a.out + 2 * (seq * a.ost[0] + h * a.ost[1] + 4 * c);
+  if (d.tiles == 0) {
+    if (g == 0) *reinterpret_cast<u32x2*>(out) = u32x2{0u, 0u};
+    return;
+  }
+  const int64_t t0 = d.before + (int64_t)hk * d.tiles;
+  const int b0 = (int)(t0 / d.share), b1 = (int)((t0 + d.tiles - 1) / d.share);
+  if (b0 == b1) return;
+  auto slot = [&](int b) {
+    return (((int64_t)(in >> 4) * a.splits + b) * 2 + (b * d.share < t0 ? 1 : 0)) * 16 + (in & 15);
+  };
+  const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat);
+  float top = -INFINITY, l = 0.0f;
+  for (int b = b0 + (threadIdx.x & 63); b <= b1; b += 64) top = fmaxf(top, stat[slot(b)][0]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  f32x4 v = {0, 0, 0, 0};
+  if (g < kGroups) {
 #pragma unroll 4
-  for (int i = 0; i < a.splits; ++i) {
-    if (stat[2 * i] == -INFINITY) continue;
-    const float f = __builtin_amdgcn_exp2f(stat[2 * i] - top);
-    const f32x2 v = *reinterpret_cast<const f32x2*>(part + (int64_t)i * D);
-    l = fmaf(stat[2 * i + 1], f, l);
-    v0 = fmaf(v[0], f, v0);
-    v1 = fmaf(v[1], f, v1);
+    for (int b = b0 + g; b <= b1; b += kGroups) {
+      const int64_t at = slot(b);
+      const f32x2 st = stat[at];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * c);
+      const float f = st[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[0] - top);
+      l = fmaf(st[1], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+    }
+    vs[g][c] = v;
+    if (c == 0) ls[g] = l;
+  }
+  __syncthreads();
+  if (g > 0) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) {
+    l += ls[i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += vs[i][c][e];
   }
   const float r = 1.0f / l;
-  *reinterpret_cast<uint32_t*>(a.out + 2 * (t * a.ost[0] + h * a.ost[1] + d)) =
-      top == -INFINITY ? 0u : T::pack(v0 * r, v1 * r);
+  u32x2 w = {0u, 0u};
+  if (top != -INFINITY) w = u32x2{T::pack(v[0] * r, v[1] * r), T::pack(v[2] * r, v[3] * r)};
+  *reinterpret_cast<u32x2*>(out) = w;
+}
+
+// Joins the parts of rows (token and query head): out =
+// sum_s 2^(ref_s - max) part_s / sum_s 2^(ref_s - max) sum_s. Parts that saw
+// no key (ref = -inf) were not written. A thread has 4 values of a row; G
+// groups of D/4 threads share a row's parts, and a block has the rows that fit
+// 256 threads (many rows of few parts: G = 1; few rows of many: one row a block).
+template <class T, int D, int G>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t rows) {
+  constexpr uint32_t kLanes = D / 4, kRows = 256 / (kLanes * G);
+  __shared__ f32x4 vs[G][kLanes];
+  __shared__ float ls[G];
+  const uint32_t mine = threadIdx.x / kLanes, c = threadIdx.x - mine * kLanes, g = G > 1 ? mine : 0;
+  const uint32_t row = G > 1 ? blockIdx.x : blockIdx.x * kRows + mine;
+  const bool work = mine < G * kRows && row < rows;
+  const int t = row / a.q_heads, h = row - (uint32_t)t * a.q_heads;
+  const KvSeq s = work ? kv_seq(a.b, kv_row_owner(a.b, t)) : KvSeq{0, 0, 0};
+  const bool owned = t >= s.first && t < s.first + s.n;
+  const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat) + (int64_t)row * a.splits;
+  float top = -INFINITY, l = 0.0f;
+  f32x4 v = {0, 0, 0, 0};
+  if (owned) {
+    for (int i = 0; i < a.splits; ++i) top = fmaxf(top, stat[i][0]);
+    const float* part = a.part + (int64_t)row * a.splits * D + 4 * c;
+#pragma unroll 4
+    for (int i = g; i < a.splits; i += G) {
+      const f32x2 st = stat[i];
+      if (st[0] == -INFINITY) continue;
+      const float f = __builtin_amdgcn_exp2f(st[0] - top);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(part + (int64_t)i * D);
+      l = fmaf(st[1], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+    }
+  }
+  if constexpr (G > 1) {
+    if (mine < G) {
+      vs[g][c] = v;
+      if (c == 0) ls[g] = l;
+    }
+    __syncthreads();
+    if (mine > 0) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i) {
+      l += ls[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += vs[i][c][e];
+    }
+  }
+  if (!owned) return;
+  const float r = 1.0f / l;
+  u32x2 w = {0u, 0u};
+  if (top != -INFINITY) w = u32x2{T::pack(v[0] * r, v[1] * r), T::pack(v[2] * r, v[3] * r)};
+  *reinterpret_cast<u32x2*>(a.out + 2 * (t * a.ost[0] + h * a.ost[1] + 4 * c)) = w;
 }
 
 // ---------------------------------------------------------------- prompts
@@ -521,14 +705,14 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int hk = blockIdx.x, G = a.group;
+  const int place = blockIdx.x / a.p.kv_heads, hk = blockIdx.x - place * a.p.kv_heads, G = a.group;
 
   // which sequence's tile this is: tiles are counted over the sequences, from
   // the last one on (the longest ones of a prompt first)
   int seq = -1, tile = 0;
   KvSeq s{0, 0, 0};
   {
-    int want = gridDim.y - 1 - blockIdx.y, before = 0;
+    int want = gridDim.x / a.p.kv_heads - 1 - place, before = 0;
     for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
       const int b = b0 + lane;
       const KvSeq c = b < a.b.batch ? kv_seq(a.b, b) : KvSeq{0, 0, 0};
@@ -565,7 +749,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   const int front = min(min((min(a.sinks, lo) + BN - 1) / BN, t_lo), t_hi);
   const int tiles = a.p.n_pages > 0 ? front + max(t_hi - t_lo, 0) : 0;
   const int per = (tiles + a.splits - 1) / a.splits;
-  const int it0 = min(per * (int)blockIdx.z, tiles), it1 = min(it0 + per, tiles);
+  const int it0 = min(per * (int)blockIdx.y, tiles), it1 = min(it0 + per, tiles);
   auto tile_of = [&](int it) { return it < front ? it : t_lo + it - front; };
 
   // this lane's row, and the range of the wave's
@@ -912,7 +1096,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   sum = halves_sum(sum);
   any = halves_sum(any ? 1.0f : 0.0f) != 0.0f;
   if (a.splits > 1) {
-    const int64_t at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.z;
+    const int64_t at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.y;
     if (!in) return;
     if (half == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * at) = f32x2{any ? ref * sc.c : -INFINITY, sum};
     if (!any) return;
@@ -959,61 +1143,72 @@ int check_sizes(const char* what, const hgk_kv_pages* pages, const hgk_kv_batch*
   return HGK_OK;
 }
 
-// Parts that the cache is split into, from the sizes alone (the lengths are on
-// the device): enough blocks to fill the chip, and not so many that a part
-// of the longest sequence that the table holds goes below kMinPart keys.
-constexpr int kMinPart = 256, kWantBlocks = 1024, kMaxSplits = 256;
-int choose_splits(const KvView& p, const KvBatchView& b, int64_t blocks, int64_t window, int64_t sinks) {
-  int64_t keys = (int64_t)b.width << p.page_shift;
-  if (window > 0 && window < keys && sinks < keys - window) keys = window + sinks;
-  int64_t s = (kWantBlocks + blocks - 1) / blocks;
-  s = std::min<int64_t>(s, keys / kMinPart);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(s, kMaxSplits));
-}
-
-int64_t part_bytes(int64_t rows, int splits, int64_t head_dim) {
-  return splits > 1 ? rows * splits * (head_dim + 2) * 4 : 0;
-}
-
 // The most tiles that the rows of a call can take.
 int64_t prompt_tiles(const KvBatchView& b, int64_t group) {
   return (int64_t)b.tokens * group / kPromptRows + std::min(b.batch, b.tokens);
 }
 
+// How the keys are split, from the sizes alone (the lengths are on the device).
+// One token a sequence: the number of blocks that share out all tiles (1: a
+// block per pair). Prompts: the parts of every row's tiles, as many as fill the
+// chip, and not so many that a part goes below kMinPart keys.
+constexpr int kMinPart = 256, kDecodeBlocks = 512, kPromptBlocks = 512, kMaxSplits = 64;
 int plan_splits(const KvView& p, const KvBatchView& b, int64_t q_heads, int64_t window, int64_t sinks) {
   if (b.batch == 0 || b.tokens == 0) return 1;
   const int64_t group = q_heads / p.kv_heads;
-  if (b.starts)
-    return choose_splits(p, b, p.kv_heads * prompt_tiles(b, group), window, sinks);
-  return choose_splits(p, b, (int64_t)b.batch * p.kv_heads * ((group + 15) / 16), window, sinks);
+  int64_t keys = (int64_t)b.width << p.page_shift;
+  if (window > 0 && window < keys && sinks < keys - window) keys = window + sinks;
+  if (!b.starts) return keys <= kMinPart ? 1 : kDecodeBlocks;
+  const int64_t s = std::min(kPromptBlocks / (p.kv_heads * prompt_tiles(b, group)), keys / kMinPart);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, kMaxSplits));
 }
 
-template <class T, int D, int NS>
+// Rows of the workspace: parts of head_dim values, and two statistics each.
+int64_t part_rows(const KvView& p, const KvBatchView& b, int64_t q_heads, int splits) {
+  if (splits == 1) return 0;
+  if (b.starts) return (int64_t)b.tokens * q_heads * splits;
+  return (q_heads / p.kv_heads + 15) / 16 * splits * 2 * 16;
+}
+
+template <class T, int D>
 void launch_decode(const AttnArgs& a, hipStream_t stream) {
-  const dim3 grid(a.b.batch * a.p.kv_heads, (a.group + 15) / 16, a.splits), block(64 * kDecWaves);
+  const unsigned blocks = a.splits > 1 ? a.splits : a.b.batch * a.p.kv_heads;
+  const dim3 grid(blocks, (a.group + 15) / 16), block(64 * kDecWaves);
   if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_decode_kernel<T, D, NS, true>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_decode_kernel<T, D, true>), grid, block, 0, stream, a);
   else
-    HGK_LAUNCH((attn_decode_kernel<T, D, NS, false>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_decode_kernel<T, D, false>), grid, block, 0, stream, a);
+  if (a.splits > 1)
+    HGK_LAUNCH((attn_decode_join_kernel<T, D>), dim3(a.b.batch, a.q_heads), dim3(256), 0, stream, a);
 }
 
 template <class T, int D, int BN>
 void launch_prompt(const AttnArgs& a, hipStream_t stream) {
-  const dim3 grid(a.p.kv_heads, prompt_tiles(a.b, a.group), a.splits), block(2 * kPromptRows);
+  const dim3 grid(a.p.kv_heads * prompt_tiles(a.b, a.group), a.splits), block(2 * kPromptRows);
   if (a.softcap > 0.0f)
     HGK_LAUNCH((attn_prompt_kernel<T, D, BN, true>), grid, block, 0, stream, a);
   else
     HGK_LAUNCH((attn_prompt_kernel<T, D, BN, false>), grid, block, 0, stream, a);
 }
 
+template <class T, int D>
+void launch_join(const AttnArgs& a, hipStream_t stream) {
+  constexpr int kGroups = 256 / (D / 4);
+  const uint32_t rows = (uint32_t)a.b.tokens * a.q_heads;
+  if (a.splits > 8)
+    HGK_LAUNCH((attn_join_kernel<T, D, kGroups>), dim3(rows), dim3(256), 0, stream, a, rows);
+  else
+    HGK_LAUNCH((attn_join_kernel<T, D, 1>), dim3((rows + kGroups - 1) / kGroups), dim3(256), 0, stream, a, rows);
+}
+
 template <class T>
 int run(const AttnArgs& a, const char* what, hipStream_t stream) {
   if (!a.b.starts) {
     switch (a.p.head_dim) {
-      case 64: launch_decode<T, 64, 2>(a, stream); break;
-      case 96: launch_decode<T, 96, 2>(a, stream); break;
-      case 128: launch_decode<T, 128, 2>(a, stream); break;
-      default: launch_decode<T, 256, 1>(a, stream); break;
+      case 64: launch_decode<T, 64>(a, stream); break;
+      case 96: launch_decode<T, 96>(a, stream); break;
+      case 128: launch_decode<T, 128>(a, stream); break;
+      default: launch_decode<T, 256>(a, stream); break;
     }
   } else {
     switch (a.p.head_dim) {
@@ -1024,8 +1219,13 @@ int run(const AttnArgs& a, const char* what, hipStream_t stream) {
     }
   }
   if (int st = launch_status(what)) return st;
-  if (a.splits == 1) return HGK_OK;
-  HGK_LAUNCH(attn_join_kernel<T>, dim3(a.b.tokens, a.q_heads), dim3(128), 0, stream, a);
+  if (a.splits == 1 || !a.b.starts) return HGK_OK;
+  switch (a.p.head_dim) {
+    case 64: launch_join<T, 64>(a, stream); break;
+    case 96: launch_join<T, 96>(a, stream); break;
+    case 128: launch_join<T, 128>(a, stream); break;
+    default: launch_join<T, 256>(a, stream); break;
+  }
   return launch_status(what);
 }
 
@@ -1040,7 +1240,7 @@ extern "C" int64_t hgk_paged_attention_workspace(const hgk_kv_pages* pages, cons
   KvView p;
   KvBatchView b;
   if (check_sizes("hgk_paged_attention_workspace", pages, batch, q_heads, window, sinks, &p, &b)) return -1;
-  return part_bytes((int64_t)b.tokens * q_heads, plan_splits(p, b, q_heads, window, sinks), p.head_dim);
+  return part_rows(p, b, q_heads, plan_splits(p, b, q_heads, window, sinks)) * (p.head_dim + 2) * 4;
 }
 
 extern "C" int hgk_paged_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch, const void* q,
@@ -1067,11 +1267,13 @@ extern "C" int hgk_paged_attention(const hgk_kv_pages* pages, const hgk_kv_batch
   a.softcap = softcap;
   a.window = (int32_t)(window > INT32_MAX ? INT32_MAX : window);
   a.sinks = (int32_t)(sinks > INT32_MAX ? INT32_MAX : sinks);
+  if (a.p.kv_heads * (a.b.starts ? prompt_tiles(a.b, a.group) : (int64_t)a.b.batch) > INT32_MAX)
+    return fail(HGK_ERR_ARG, "%s: %lld rows are too many", what, (long long)T);
   a.splits = plan_splits(a.p, a.b, q_heads, window, sinks);
-  const int64_t need = part_bytes(T * q_heads, a.splits, D);
+  const int64_t rows = part_rows(a.p, a.b, q_heads, a.splits), need = rows * (D + 2) * 4;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(HGK_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
   a.part = static_cast<float*>(workspace);
-  a.stat = a.splits > 1 ? a.part + T * q_heads * a.splits * D : nullptr;
+  a.stat = rows > 0 ? a.part + rows * D : nullptr;
   return pages->dtype == DT_BF16 ? run<BF16>(a, what, as_stream(stream)) : run<F16>(a, what, as_stream(stream));
 }
