@@ -1152,13 +1152,22 @@ int64_t prompt_tiles(const KvBatchView& b, int64_t group) {
 // One token a sequence: the number of blocks that share out all tiles (1: a
 // block per pair). Prompts: the parts of every row's tiles, as many as fill the
 // chip, and not so many that a part goes below kMinPart keys.
-constexpr int kMinPart = 256, kDecodeBlocks = 512, kPromptBlocks = 512, kMaxSplits = 64;
+constexpr int kMinPart = 256, kPromptBlocks = 512, kMaxSplits = 64;
+
+// Blocks that share out the tiles of single tokens. Rows of 256 values take two
+// blocks a CU (64 sequences of 16384 tokens, 2 kv heads: 378 us, one: 417). Rows
+// up to 128 stream better from one (32 sequences of 8192, 8 kv heads of 64: 106
+// us, two: 127), until the pairs are so many that a run holds several and the
+// gaps between them show (64 ragged sequences up to 2048: 57 us, two: 47).
+int decode_blocks(const KvView& p, const KvBatchView& b) {
+  return p.head_dim == 256 || (int64_t)b.batch * p.kv_heads >= 512 ? 512 : 256;
+}
 int plan_splits(const KvView& p, const KvBatchView& b, int64_t q_heads, int64_t window, int64_t sinks) {
   if (b.batch == 0 || b.tokens == 0) return 1;
   const int64_t group = q_heads / p.kv_heads;
   int64_t keys = (int64_t)b.width << p.page_shift;
   if (window > 0 && window < keys && sinks < keys - window) keys = window + sinks;
-  if (!b.starts) return keys <= kMinPart ? 1 : kDecodeBlocks;
+  if (!b.starts) return keys <= kMinPart ? 1 : decode_blocks(p, b);
   const int64_t s = std::min(kPromptBlocks / (p.kv_heads * prompt_tiles(b, group)), keys / kMinPart);
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, kMaxSplits));
 }

@@ -32,7 +32,6 @@ Every op enqueues on torch's current CUDA/HIP stream and never synchronises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import math
 import struct
@@ -569,16 +568,16 @@ def _token_rows(t: torch.Tensor, pages: torch.Tensor, what: str, name: str):
 _TWO = struct.Struct("@qq")
 
 
-def _on_device(device: torch.device):
-    """The device's guard where it is not the current one: a stream takes
-    launches of its own device only."""
+def _kv_call(device: torch.device, fn, *args):
+    """fn(*args, stream) with the device current, as a launch needs: a stream
+    takes launches of its own device only."""
     if device.type != "cuda":
         raise HgkError(1, f"operands must be on the GPU, not on {device}")
-    return (_NO_GUARD if device.index == torch.cuda.current_device()
-            else torch.cuda.device(device))
-
-
-_NO_GUARD = contextlib.nullcontext()
+    if device.index == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -599,8 +598,7 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
         raise HgkError(1, f"{what}: k and v must be [tokens, {k_pages.shape[2]}, {k_pages.shape[3]}]")
     dev = k_pages.device
     batch = _kv_batch(k.shape[0], block_table, kv_lens, q_starts, dev, what)
-    with _on_device(dev):
-        check(lib().hgk_kv_append(pool, batch, k.data_ptr(), ks, v.data_ptr(), vs, _stream(dev)))
+    _kv_call(dev, lib().hgk_kv_append, pool, batch, k.data_ptr(), ks, v.data_ptr(), vs)
 
 
 def kv_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence[int],
@@ -629,9 +627,7 @@ def kv_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence[in
         if s[i] != src[i] or d[i] != dst[i]:  # ctypes keeps the low 32 bits
             raise HgkError(1, f"{what}: pair {i} outside the pages")
     dev = k_pages.device
-    with _on_device(dev):
-        check(lib().hgk_kv_copy_pages(pool, layers, strides, C.addressof(s), C.addressof(d), n,
-                                      _stream(dev)))
+    _kv_call(dev, lib().hgk_kv_copy_pages, pool, layers, strides, C.addressof(s), C.addressof(d), n)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -661,15 +657,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     os_ = _token_rows(out, k_pages, what, "out")
     dev = k_pages.device
     batch = _kv_batch(T, block_table, kv_lens, q_starts, dev, what)
-    with _on_device(dev):
-        need = lib().hgk_paged_attention_workspace(pool, batch, hq, window, sinks)
-        if need < 0:
-            check(1)
-        ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-        check(lib().hgk_paged_attention(pool, batch, q.data_ptr(), qs, hq,
-                                        1.0 / math.sqrt(d) if scale is None else scale, softcap,
-                                        window, sinks, out.data_ptr(), os_, _ptr(ws), need,
-                                        _stream(dev)))
+    L = lib()
+    need = L.hgk_paged_attention_workspace(pool, batch, hq, window, sinks)
+    if need < 0:
+        check(1)
+    # a workspace of the call's own, from the current stream's pool of memory
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _kv_call(dev, L.hgk_paged_attention, pool, batch, q.data_ptr(), qs, hq,
+             1.0 / math.sqrt(d) if scale is None else scale, softcap, window, sinks,
+             out.data_ptr(), os_, None if ws is None else ws.data_ptr(), need)
     return out
 
 
