@@ -57,6 +57,8 @@ class PagedKVCache:
             raise HgkError(1, f"PagedKVCache: {layers} layers of {n_pages} pages")
         if page_size < 1 or page_size > 65536 or page_size & (page_size - 1):
             raise HgkError(1, f"PagedKVCache: page_size={page_size} must be a power of two in 1..65536")
+        if dtype not in (torch.bfloat16, torch.float16) or head_dim not in (64, 96, 128, 256):
+            raise HgkError(2, f"PagedKVCache: {dtype} of head_dim {head_dim} (bf16 or f16; 64, 96, 128 or 256)")
         shape = (layers, n_pages, page_size, kv_heads, head_dim)
         self.k_pages = torch.empty(shape, dtype=dtype, device=device)
         self.v_pages = torch.empty(shape, dtype=dtype, device=device)

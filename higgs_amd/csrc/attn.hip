@@ -1131,7 +1131,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
 int check_sizes(const char* what, const hgk_kv_pages* pages, const hgk_kv_batch* batch, int64_t q_heads,
                 int64_t window, int64_t sinks, KvView* p, KvBatchView* b) {
   if (int st = kv_check_pages(what, pages, p)) return st;
-  if (int st = kv_check_batch(what, batch, b)) return st;
+  if (int st = kv_check_batch(what, *p, batch, b)) return st;
   if (q_heads < 1 || q_heads > 65535 || q_heads % p->kv_heads)
     return fail(HGK_ERR_ARG, "%s: %lld query heads for %d kv heads", what, (long long)q_heads, p->kv_heads);
   if ((int64_t)b->batch * p->kv_heads > INT32_MAX || (int64_t)b->tokens * q_heads > INT32_MAX)
@@ -1274,9 +1274,9 @@ extern "C" int hgk_paged_attention(const hgk_kv_pages* pages, const hgk_kv_batch
   a.group = (int32_t)(q_heads / a.p.kv_heads);
   a.scale = scale;
   a.softcap = softcap;
-  a.window = (int32_t)(window > INT32_MAX ? INT32_MAX : window);
+  a.window = (int32_t)(window >= INT32_MAX ? 0 : window);  // every key of any sequence
   a.sinks = (int32_t)(sinks > INT32_MAX ? INT32_MAX : sinks);
-  if (a.p.kv_heads * (a.b.starts ? prompt_tiles(a.b, a.group) : (int64_t)a.b.batch) > INT32_MAX)
+  if (a.p.kv_heads * (a.b.starts ? prompt_tiles(a.b, a.group) : (int64_t)a.b.batch) > kMaxBlocks)
     return fail(HGK_ERR_ARG, "%s: %lld rows are too many", what, (long long)T);
   a.splits = plan_splits(a.p, a.b, q_heads, window, sinks);
   const int64_t rows = part_rows(a.p, a.b, q_heads, a.splits), need = rows * (D + 2) * 4;

@@ -25,15 +25,15 @@ struct KvBatchView {
   int32_t batch, tokens;
 };
 
-// Rows [first, first + n) of a sequence and its length. Whatever the arrays
-// hold, the rows lie within the packed array.
+// Rows [first, first + n) of a sequence and its length (a negative one counts
+// as none). Whatever the arrays hold, the rows lie within the packed array.
 struct KvSeq {
   int32_t first, n, len;
 };
 
 __host__ __device__ inline KvSeq kv_seq(const KvBatchView& b, int seq) {
   KvSeq s;
-  s.len = b.lens[seq];
+  s.len = b.lens[seq] < 0 ? 0 : b.lens[seq];
   if (!b.starts) {
     s.first = seq;
     s.n = seq < b.tokens ? 1 : 0;
@@ -73,7 +73,10 @@ __host__ __device__ inline int kv_row_owner(const KvBatchView& b, int t) {
 
 // Checks of the pool and the batch; on success the views are filled in.
 int kv_check_pages(const char* what, const hgk_kv_pages* p, KvView* out);
-int kv_check_batch(const char* what, const hgk_kv_batch* b, KvBatchView* out);
+int kv_check_batch(const char* what, const KvView& p, const hgk_kv_batch* b, KvBatchView* out);
+
+// A grid of 256-thread blocks has at most this many (2^31 threads).
+constexpr int64_t kMaxBlocks = 1 << 23;
 
 // A [tokens, heads, head_dim] operand: pointer and strides usable by 16-byte
 // accesses (the stride of an axis of one element is not looked at, and comes

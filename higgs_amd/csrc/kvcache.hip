@@ -45,9 +45,9 @@ int kv_check_pages(const char* what, const hgk_kv_pages* p, KvView* out) {
   return HGK_OK;
 }
 
-int kv_check_batch(const char* what, const hgk_kv_batch* b, KvBatchView* out) {
+int kv_check_batch(const char* what, const KvView& p, const hgk_kv_batch* b, KvBatchView* out) {
   if (!b) return fail(HGK_ERR_ARG, "%s: null batch", what);
-  if (b->batch < 0 || b->batch > (1 << 24) || b->tokens < 0 || b->tokens > INT32_MAX)
+  if (b->batch < 0 || b->batch > kMaxBlocks || b->tokens < 0 || b->tokens > INT32_MAX)
     return fail(HGK_ERR_ARG, "%s: batch=%lld, tokens=%lld out of range", what, (long long)b->batch,
                 (long long)b->tokens);
   if (!b->q_starts && b->tokens != b->batch)
@@ -55,6 +55,9 @@ int kv_check_batch(const char* what, const hgk_kv_batch* b, KvBatchView* out) {
                 (long long)b->tokens, (long long)b->batch);
   if (b->table_width < 0 || b->table_width > INT32_MAX || b->table_stride < 0)
     return fail(HGK_ERR_ARG, "%s: bad table width or stride", what);
+  if (b->table_width > (int64_t)1 << (30 - p.page_shift))
+    return fail(HGK_ERR_ARG, "%s: a table of %lld pages of %d tokens is too wide (2^30 tokens)", what,
+                (long long)b->table_width, p.page_mask + 1);
   if (b->batch > 0 && b->tokens > 0 && (!b->kv_lens || (!b->block_table && b->table_width > 0)))
     return fail(HGK_ERR_ARG, "%s: null table or lengths", what);
   out->table = b->block_table;
@@ -211,7 +214,7 @@ extern "C" int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batc
   KvView p;
   KvBatchView b;
   if (int st = kv_check_pages("hgk_kv_append", pages, &p)) return st;
-  if (int st = kv_check_batch("hgk_kv_append", batch, &b)) return st;
+  if (int st = kv_check_batch("hgk_kv_append", p, batch, &b)) return st;
   if (b.batch == 0 || b.tokens == 0 || p.n_pages == 0) return HGK_OK;
   if (int st = kv_check_written_pages("hgk_kv_append", p)) return st;
   RowsView x{static_cast<const char*>(k), static_cast<const char*>(v), {}, {}};
@@ -224,8 +227,10 @@ extern "C" int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batc
   if (units > INT32_MAX / kMaxTokens) return fail(HGK_ERR_ARG, "hgk_kv_append: too many kv heads");
   // a token a block until the chip is full of blocks, then 16
   const int per = b.tokens <= 2048 ? 1 : kMaxTokens;
-  HGK_LAUNCH(kv_append_kernel, dim3((unsigned)((b.tokens + (int64_t)per - 1) / per)), dim3(kThreads), 0,
-             as_stream(stream), p, b, x, (uint32_t)units, chunks, per);
+  const int64_t blocks = (b.tokens + (int64_t)per - 1) / per;
+  if (blocks > kMaxBlocks) return fail(HGK_ERR_ARG, "hgk_kv_append: %d rows are too many", b.tokens);
+  HGK_LAUNCH(kv_append_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, as_stream(stream), p, b, x,
+             (uint32_t)units, chunks, per);
   return launch_status("hgk_kv_append");
 }
 

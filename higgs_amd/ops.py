@@ -34,6 +34,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import struct
 from typing import Optional, Sequence
 
@@ -620,12 +621,12 @@ def kv_copy_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, src: Sequence[in
         raise HgkError(1, f"{what}: {len(src)} sources for {len(dst)} destinations")
     n = len(src)
     try:
-        s, d = (C.c_int32 * n)(*src), (C.c_int32 * n)(*dst)
+        pairs = [operator.index(i) for i in (*src, *dst)]
     except TypeError:
         raise HgkError(1, f"{what}: src and dst must be sequences of page indices") from None
-    for i in range(n):
-        if s[i] != src[i] or d[i] != dst[i]:  # ctypes keeps the low 32 bits
-            raise HgkError(1, f"{what}: pair {i} outside the pages")
+    if n and not -2 ** 31 <= min(pairs) <= max(pairs) < 2 ** 31:  # ctypes would keep the low 32 bits
+        raise HgkError(1, f"{what}: a page index outside the pages")
+    s, d = (C.c_int32 * n)(*pairs[:n]), (C.c_int32 * n)(*pairs[n:])
     dev = k_pages.device
     _kv_call(dev, lib().hgk_kv_copy_pages, pool, layers, strides, C.addressof(s), C.addressof(d), n)
 
@@ -645,7 +646,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``window`` keys visible, and of the keys before them the first ``sinks``.
     ``softcap`` > 0 replaces a score s by softcap * tanh(s / softcap). A query
     that sees no key gives zeros. Rows of no sequence are not written (without
-    ``out`` they hold whatever the new tensor held). Returns [T, Hq, D]."""
+    ``out`` they hold whatever the new tensor held). ``out`` must not share
+    memory with the other operands. Returns [T, Hq, D]."""
     what = "paged_attention"
     pool = _pool(k_pages, v_pages, what)
     qs = _token_rows(q, k_pages, what, "q")
@@ -654,6 +656,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty((T, hq, d), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape:
         raise HgkError(1, f"{what}: out shape {tuple(out.shape)} is not q's")
+    if not (0 <= window < 2 ** 63 and 0 <= sinks < 2 ** 63):
+        raise HgkError(1, f"{what}: window={window}, sinks={sinks}")
     os_ = _token_rows(out, k_pages, what, "out")
     dev = k_pages.device
     batch = _kv_batch(T, block_table, kv_lens, q_starts, dev, what)

@@ -464,7 +464,7 @@ int hgk_op_list_run(int dtype, const void* dev_list, int n_ops, int64_t tokens, 
  * lengths, starts) is read by the kernels, which check it: a page outside
  * [0, n_pages), a length beyond the table and a start outside the tokens
  * reach no memory. Tokens on such a page are seen by no query and written
- * nowhere.
+ * nowhere; a negative length counts as zero. A table holds at most 2^30 tokens.
  * ------------------------------------------------------------------------ */
 typedef struct {
   int dtype;     /* HGK_BF16 or HGK_F16 */
@@ -523,6 +523,7 @@ int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers, const int64_t l
  * last `window` keys and the first `sinks`). A query that sees no key gives a
  * row of zeros; keys and values that a query does not see, infinities and NaN
  * among them, do not touch its row. Rows of no sequence are left as they are.
+ * out must not overlap the other operands.
  * Sums and softmax statistics are f32; the probabilities are rounded to the
  * dtype for the product with v; the result is rounded once.
  * `workspace`: device memory of hgk_paged_attention_workspace() bytes (NULL

@@ -214,6 +214,41 @@ def test_infinite_scores_follow_the_formula(dev):
         assert torch.isnan(R.call(H, R.to(x, dev)).cpu()[1]).all()
 
 
+@pytest.mark.parametrize("news", [None, [3]])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_small_weights_beside_a_large_one(dev, news, dtype):
+    """One key of weight 1 and 6000 of about e^-10 each, subnormal in f16: their
+    sum is a quarter of the whole and none of it may be lost. Bound as ever."""
+    x = R.make(31, [6001], news=news, heads=4, kv_heads=2, head_dim=64, page=64, dtype=dtype)
+    x["q"][:] = 0
+    x["q"][..., 0] = 8.0
+    for e in range(x["table"].shape[1]):
+        x["k_pages"][int(x["table"][0, e]), :, :, 0] = 0.0
+    x["k_pages"][int(x["table"][0, 1]), 5, :, 0] = 10.0  # score 80 / 8 = 10, the others 0
+    run(dev, x)
+
+
+@pytest.mark.parametrize("news", [None, [4, 70]])
+def test_lengths_at_the_ends_of_their_type(dev, news):
+    """Lengths far beyond the table (its keys, all in front of the queries, are
+    seen without a window, and not with one) and below zero."""
+    lens = [4, 100]
+    x = R.make(32, lens, news=news, heads=4, kv_heads=2, head_dim=64, page=16, dtype=BF16)
+    x["k_pages"][:], x["v_pages"][:] = (torch.randn(x["k_pages"].shape).to(BF16) for _ in range(2))
+    d = R.to(x, dev)
+    for far in (2 ** 31 - 1, 2 ** 30 + 5):
+        d["lens"].fill_(far)
+        y = R.call(H, d).cpu()
+        for window, same in ((0, True), (2 ** 31 - 1, True), (2 ** 31, True), (1000, False)):
+            z = R.call(H, d, window=window).cpu()
+            assert torch.equal(z, y) if same else (z == 0).all()
+        k = x["table"].shape[1] * 16
+        short = {**x, "lens": torch.tensor([k + 200, k + 200], dtype=torch.int32)}
+        R.check(y, R.reference(short))
+    d["lens"].fill_(-2 ** 31)
+    assert (R.call(H, d).cpu() == 0).all()
+
+
 # ---------------------------------------------------------------- layouts
 @pytest.mark.parametrize("news", [None, [40, 1, 130]])
 @pytest.mark.parametrize("head_major", [False, True])

@@ -95,7 +95,7 @@ def test_refused_pages(kw, status, text):
 
 @pytest.mark.parametrize("kw,text", [
     (dict(batch=-1, tokens=-1), "out of range"), (dict(tokens=-1, q_starts=FAKE), "out of range"),
-    (dict(tokens=3), "3 rows for 2"), (dict(table_width=-1), "table"), (dict(table_stride=-4), "table"),
+    (dict(tokens=3), "3 rows for 2"), (dict(table_width=1 << 27), "too wide"), (dict(table_width=-1), "table"), (dict(table_stride=-4), "table"),
     (dict(kv_lens=None), "null"), (dict(block_table=None), "null"), (dict(tokens=1 << 31, q_starts=FAKE), "out of range"),
 ])
 def test_refused_batches(kw, text):
@@ -175,7 +175,8 @@ def test_refusals_of_the_python_calls():
         lambda: H.paged_attention(q.transpose(1, 2), p, p, t, n), lambda: H.paged_attention(q, p[0], p[0], t, n),
         lambda: H.kv_append(k, k[:1], p, p, t, n), lambda: H.kv_append(k[:, :1], k[:, :1], p, p, t, n),
         lambda: H.kv_append(k.float(), k, p, p, t, n), lambda: H.kv_copy_pages(p, p, [0], [1, 2]),
-        lambda: H.kv_copy_pages(p, p, [0], [2 ** 32 + 1]), lambda: H.kv_copy_pages(p, p, [0.5], [1]),
+        lambda: H.kv_copy_pages(p, p, [0], [2 ** 32 + 1]), lambda: H.paged_attention(q, p, p, t, n, window=2 ** 64),
+        lambda: H.paged_attention(q, p, p, t, n, sinks=-1), lambda: H.kv_copy_pages(p, p, [0.5], [1]),
         # nothing of this is on a GPU
         lambda: H.paged_attention(q, p, p, t, n), lambda: H.kv_append(k, k, p, p, t, n),
         lambda: H.kv_copy_pages(p, p, [0], [1]),
@@ -338,6 +339,9 @@ def test_refused_sequences(cpu_copies):
     for kw in ((0, 4, 4), (2, 0, 4), (2, 4, 3), (2, 4, 0)):
         with pytest.raises(HgkError):
             H.PagedKVCache(*kw, 1, 64, device="cpu")
+    for kw in ({"dtype": torch.float32}, {"head_dim": 80}):
+        with pytest.raises(HgkError):
+            H.PagedKVCache(2, 4, 4, 1, **{"head_dim": 64, "device": "cpu", **kw})
 
 
 def test_batches(cpu_copies):
