@@ -698,7 +698,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
   constexpr int KT = BN / 32, QS = D / 16, DT = D / 32, kAhead = 2;
-  static_assert(BN * CH % NT == 0, "whole units per thread");
+  static_assert(BN == 64 && BN * CH % NT == 0, "two tiles of 32 keys, whole units per thread");
   typedef Mx<T> M;
   __shared__ __align__(1024) char lds[4 * kTile];  // two tiles of keys, two of values
   __shared__ int odd;  // 1 + index of the last tile found to hold values that are not finite
@@ -874,44 +874,52 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     return u32x4{v0[0], v0[1], v1[0], v1[1]};
   };
 
-  // Scores of tile `it` ready in x: masks them where the wave's rows see only
-  // part of the tile, and moves the references that they pass. Returns the
-  // factor for the sums so far (1 for nearly every tile, then not applied).
+  // Scores of tile `it` ready in x: hides those that the wave's rows do not see,
+  // and moves the references that others pass; `shrunk` is then the factor for
+  // the sums so far (few tiles move any: most leave `moved` false).
   bool moved;
   float shrunk;
+  uint32_t see[KT];  // CAP, masked: the 32 keys' bits, at 8 (e / 4) + e % 4 for score e
   auto settle = [&](f32x16* x, int it, uint64_t exist, bool masked) {
-    if constexpr (CAP) {
+    auto top_of = [&](const f32x16* x) {
+      float part[4];
 #pragma unroll
-      for (int t = 0; t < KT; ++t)
+      for (int e = 0; e < 4; ++e) part[e] = max3(x[0][e], x[0][e + 4], x[0][e + 8]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = fast_tanh(x[t][e] * sc.inner);
-    }
-    if (masked) {
-      float hidden = -INFINITY;
-      asm volatile("" : "+v"(hidden));  // no register for it but here
-      const uint64_t see = seen_keys(tile_of(it) * BN, exist) >> (4 * half);
-      any |= (see & 0x0f0f0f0f0f0f0f0full) != 0;
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const uint32_t m = (uint32_t)(see >> (32 * t));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = m & (1u << (8 * (e / 4) + e % 4)) ? x[t][e] : hidden;
-      }
-    } else {
-      any = true;
-    }
-    float part[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[e] = max3(x[0][e], x[0][e + 4], x[0][e + 8]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) part[e] = KT == 1 ? fmaxf(part[e], x[0][e + 12]) : max3(part[e], x[0][e + 12], x[KT - 1][e]);
-    if constexpr (KT == 2) {
+      for (int e = 0; e < 4; ++e) part[e] = max3(part[e], x[0][e + 12], x[1][e]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) part[e] = max3(part[e], x[1][e + 4], x[1][e + 8]);
       part[0] = max3(part[0], x[1][12], x[1][13]);
       part[1] = max3(part[1], x[1][14], x[1][15]);
+      return max3(max3(part[0], part[1], part[2]), part[3], part[3]);
+    };
+    float top;
+    if (masked) {
+      float hidden = -INFINITY;
+      asm volatile("" : "+v"(hidden));  // no register for it but here
+      const uint64_t bits = seen_keys(tile_of(it) * BN, exist) >> (4 * half);
+      const bool some = (bits & 0x0f0f0f0f0f0f0f0full) != 0;
+      any |= some;
+      f32x16 h[KT];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        see[t] = (uint32_t)(bits >> (32 * t));
+#pragma unroll
+        for (int e = 0; e < 16; ++e) h[t][e] = see[t] & (1u << (8 * (e / 4) + e % 4)) ? x[t][e] : hidden;
+      }
+      top = top_of(h);
+      if constexpr (CAP) {
+        // the scores stay: under tanh a hidden one would count, so the weights are cleared instead
+        top = some ? fast_tanh(top * sc.inner) : hidden;
+      } else {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) x[t] = h[t];
+      }
+    } else {
+      any = true;
+      top = top_of(x);
+      if constexpr (CAP) top = fast_tanh(top * sc.inner);
     }
-    float top = max3(max3(part[0], part[1], part[2]), part[3], part[3]);
     moved = __any(top > ref + slack);
     if (moved) {  // a row's own scores alone decide for it
       top = halves_max(top);
@@ -926,8 +934,13 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   float add[4];
   auto weigh = [&](const f32x16* x, int i) {
     const float base = -ref * sc.c;
-    const float w0 = __builtin_amdgcn_exp2f(fmaf(x[i / 8][2 * i % 16], sc.c, base));
-    const float w1 = __builtin_amdgcn_exp2f(fmaf(x[i / 8][2 * i % 16 + 1], sc.c, base));
+    float s0 = x[i / 8][2 * i % 16], s1 = x[i / 8][2 * i % 16 + 1];
+    if constexpr (CAP) {
+      s0 = fast_tanh(s0 * sc.inner);
+      s1 = fast_tanh(s1 * sc.inner);
+    }
+    const float w0 = __builtin_amdgcn_exp2f(fmaf(s0, sc.c, base));
+    const float w1 = __builtin_amdgcn_exp2f(fmaf(s1, sc.c, base));
     const uint32_t pair = M::pack(w0, w1);
     add[i & 3] = M::add_pair(pair, i < 4 ? 0.0f : add[i & 3]);
     return pair;
@@ -988,7 +1001,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     }
     __syncthreads();
   };
-  auto all_of = [&](uint64_t exist) { return BN == 64 ? exist == ~0ull : (uint32_t)exist == ~0u; };
+  auto all_of = [&](uint64_t exist) { return exist == ~0ull; };
 
   // One step: the product of tile it - 1 with its weights w, the weights wn of
   // tile `it`, whose scores x are ready, and the scores of tile it + 1 into y:
@@ -1066,7 +1079,19 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
       const bool masked = !all_of(exist) || part_seen(tile_of(it) * BN, pw_first, pw_last);
       settle(x, it, exist, masked);
       if (it > it0) odd_values(it - 1, slot ^ 1, exist1, all_of(exist1));
+      const float before = sum;
       step(x, y, w, wn, slot);
+      if (CAP && masked) {
+        sum = before;
+#pragma unroll
+        for (int k = 0; k < 2 * KT; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t two = see[k / 2] >> (16 * (k & 1) + 8 * (i / 2) + 2 * (i & 1));
+            wn[k][i] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+            sum = M::add_pair(wn[k][i], sum);
+          }
+      }
       if (moved) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) o[t] *= shrunk;
@@ -1151,8 +1176,11 @@ int64_t prompt_tiles(const KvBatchView& b, int64_t group) {
 // How the keys are split, from the sizes alone (the lengths are on the device).
 // One token a sequence: the number of blocks that share out all tiles (1: a
 // block per pair). Prompts: the parts of every row's tiles, as many as fill the
-// chip, and not so many that a part goes below kMinPart keys.
-constexpr int kMinPart = 256, kPromptBlocks = 512, kMaxSplits = 64;
+// chip, and not so many that a part goes below kMinPart keys. Writing and
+// joining the parts costs as much as half the work of a few hundred blocks, so
+// rows are split only where they make less than half a block a CU (ragged turns
+// over 20000 tokens, 250 blocks: unsplit 41 us, in two 43, in three 50).
+constexpr int kMinPart = 256, kPromptBlocks = 256, kMaxSplits = 64;
 
 // Blocks that share out the tiles of single tokens. Rows of 256 values take two
 // blocks a CU (64 sequences of 16384 tokens, 2 kv heads: 378 us, one: 417). Rows
