@@ -70,6 +70,23 @@ int kv_check_batch(const char* what, const KvView& p, const hgk_kv_batch* b, KvB
   return HGK_OK;
 }
 
+namespace {
+// Do rows of `d` elements, stepped along these axes, lie on each other? (Taken to
+// where an axis's step does not clear the whole of the axes with smaller ones.)
+bool rows_overlap(const int64_t* stride, const int64_t* extent, int axes, int64_t d) {
+  int order[4] = {0, 1, 2, 3};
+  std::sort(order, order + axes, [&](int x, int y) { return stride[x] < stride[y]; });
+  __int128 span = d;
+  for (int i = 0; i < axes; ++i) {
+    const int x = order[i];
+    if (extent[x] <= 1) continue;
+    if (stride[x] < span) return true;
+    span += (__int128)stride[x] * (extent[x] - 1);
+  }
+  return false;
+}
+}  // namespace
+
 int kv_check_rows(const char* what, const char* name, const void* p, const int64_t strides[2],
                   int64_t tokens, int64_t heads, int64_t head_dim, bool written, int64_t out[2]) {
   if (!p || !strides) return fail(HGK_ERR_ARG, "%s: null %s", what, name);
@@ -79,17 +96,17 @@ int kv_check_rows(const char* what, const char* name, const void* p, const int64
     out[i] = extent[i] > 1 ? strides[i] : 0;
     if (out[i] < 0 || (out[i] & 7))
       return fail(HGK_ERR_ARG, "%s: %s strides must be multiples of 8 elements", what, name);
-    if (written && extent[i] > 1 && out[i] < head_dim)
-      return fail(HGK_ERR_ARG, "%s: %s rows overlap (stride %lld)", what, name, (long long)out[i]);
   }
+  if (written && rows_overlap(out, extent, 2, head_dim))
+    return fail(HGK_ERR_ARG, "%s: %s rows overlap (strides %lld, %lld)", what, name, (long long)out[0],
+                (long long)out[1]);
   return HGK_OK;
 }
 
 int kv_check_written_pages(const char* what, const KvView& p) {
   const int64_t extent[3] = {p.n_pages, (int64_t)p.page_mask + 1, p.kv_heads};
-  for (int i = 0; i < 3; ++i)
-    if (extent[i] > 1 && (p.kst[i] < p.head_dim || p.vst[i] < p.head_dim))
-      return fail(HGK_ERR_ARG, "%s: rows of the pages overlap", what);
+  if (rows_overlap(p.kst, extent, 3, p.head_dim) || rows_overlap(p.vst, extent, 3, p.head_dim))
+    return fail(HGK_ERR_ARG, "%s: rows of the pages overlap", what);
   return HGK_OK;
 }
 
@@ -264,7 +281,10 @@ extern "C" int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers,
   }
   if (n == 0 || layers == 0) return HGK_OK;
   if (int st = kv_check_written_pages(what, p)) return st;
-  if (layers > 1 && (layer_strides[0] < p.head_dim || layer_strides[1] < p.head_dim))
+  const int64_t extent[4] = {p.n_pages, (int64_t)p.page_mask + 1, p.kv_heads, layers};
+  const int64_t ks[4] = {p.kst[0], p.kst[1], p.kst[2], layers > 1 ? layer_strides[0] : 0};
+  const int64_t vs[4] = {p.vst[0], p.vst[1], p.vst[2], layers > 1 ? layer_strides[1] : 0};
+  if (rows_overlap(ks, extent, 4, p.head_dim) || rows_overlap(vs, extent, 4, p.head_dim))
     return fail(HGK_ERR_ARG, "%s: the layers' pages overlap", what);
   CopyView c;
   c.base[0] = static_cast<char*>(pages->k);

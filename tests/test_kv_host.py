@@ -113,7 +113,8 @@ def test_refused_attention_arguments():
                      (dict(softcap=float("nan")), "softcap"), (dict(softcap=float("inf")), "softcap"),
                      (dict(q=None), "null q"), (dict(out=None), "null out"), (dict(q=FAKE + 8), "aligned"),
                      (dict(qs=(256, 60)), "multiples"), (dict(os_=(256, -64)), "multiples"),
-                     (dict(os_=(0, 64)), "overlap"), (dict(os_=(256, 56)), "overlap")):
+                     (dict(os_=(0, 64)), "overlap"), (dict(os_=(256, 56)), "overlap"),
+                     (dict(os_=(64, 64)), "overlap"), (dict(os_=(192, 64)), "overlap")):
         s, msg = attention(**kw)
         assert s == 1 and text in msg, (kw, msg)
     L = _lib.lib()
@@ -155,7 +156,13 @@ def test_refused_copies():
     assert copy([0], [1], layers=-1)[0] == 1 and copy([0], [1], layers=2)[0] == 1
     assert copy([0], [1], layers=2, strides=st(60, 64))[0] == 1
     assert "overlap" in copy([0], [1], layers=2, strides=st(0, 1 << 20))[1]
-    assert "overlap" in copy([0], [1], k_strides=st(0, 128, 64))[1]
+    for lk, lv in ((64, 1 << 20), (1 << 20, 8192), (2048, 1 << 20)):  # layers inside each other
+        assert "overlap" in copy([0], [1], layers=2, strides=st(lk, lv))[1], (lk, lv)
+    for k in ((0, 128, 64), (2048, 128, 56), (2048, 64, 64), (1024, 128, 64), (2048, 64, 512)):
+        assert "overlap" in copy([0], [1], k_strides=st(*k))[1], k
+    for k in ((2048, 128, 64), (2048, 64, 1024), (64, 1024, 512), (64, 512, 8192)):  # any order of the axes
+        assert L.hgk_kv_append(C.byref(pages(v_strides=st(*k))), C.byref(batch()), None, st(128, 64), FAKE,
+                               st(128, 64), None) == 1 and "null k" in L.hgk_last_error().decode(), k
     assert copy([], []) == (0, "") and copy([0], [1], layers=0)[0] == 0
 
 
