@@ -184,66 +184,60 @@ constexpr int kDecWaves = 4;
 // Keys of a decode tile, and the fewest tiles that a block takes (two a wave).
 template <int D> constexpr int dec_keys() { return D == 256 ? 16 : 32; }
 constexpr int kDecMinTiles = 2 * kDecWaves;
+constexpr int kDecJoinBlocks = 2048;  // of the join, about: 2048 sequences get a block each
 
-// The tiles of all (sequence, kv head) pairs, one after the other, dealt out to
-// the blocks in equal runs, whatever the lengths: no block is left with a long
-// sequence, and a short one in a wide table is still spread. A run may end in
-// the middle of a pair; its part is then joined with the neighbours' by
-// attn_decode_join_kernel. Every wave of both kernels works this out for itself.
-struct Deal {
-  int64_t before;  // tiles in front of the sequence's
-  int64_t share;   // tiles of a block
-  int32_t seq, tiles;  // tiles of one pair of the sequence
-  Seen seen;
+// The sequence that has item `want` when every sequence b has count(b) items,
+// one after the other, and how many lie in front of its own (seq -1: there are
+// fewer). `want_of(total)` gives the item. Each wave does this for itself: a
+// lane sums a run of sequences, the wave scans the sums, then the run that has
+// the item.
+struct Owner {
+  int64_t before;
+  int32_t seq;
 };
-// Of the sequence that has tile `want` (or of sequence `seq`, where that is given).
-template <int KEYS>
-__device__ inline Deal deal_out(const AttnArgs& a, int blocks, int64_t block, int seq) {
+__device__ inline int64_t scan64(int64_t v) {
   const int lane = threadIdx.x & 63;
-  auto tiles_of = [&](int b, Seen& s) {
-    s = b < a.b.batch ? seen_by_last(a, a.b.lens[b]) : Seen{0, 0, 0};
-    return (s.n + KEYS - 1) / KEYS;
-  };
-  Deal d{0, 0, -1, 0, {0, 0, 0}};
-  Seen s;
-  int64_t total = 0, upto = 0;
-  for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
-    upto = (int64_t)tiles_of(b0 + lane, s) * a.p.kv_heads;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(upto, o);
-      if (lane >= o) upto += v;
-    }
-    total += __shfl(upto, 63);
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t u = __shfl_up(v, o);
+    if (lane >= o) v += u;
   }
-  d.share = (total + blocks - 1) / blocks;
-  if (d.share < kDecMinTiles) d.share = kDecMinTiles;
-  const int64_t want = block * d.share;
-  if (seq < 0 && want >= total) return d;
-  int64_t before = 0;
-  for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
-    const int tiles = tiles_of(b0 + lane, s);
-    const int64_t mine = (int64_t)tiles * a.p.kv_heads;
-    if (a.b.batch > 64) {
-      upto = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int64_t v = __shfl_up(upto, o);
-        if (lane >= o) upto += v;
-      }
-    }
-    const uint64_t has = __ballot(seq < 0 ? before + upto > want : b0 + lane == seq);
+  return v;
+}
+template <class C, class W>
+__device__ inline Owner find_owner(int batch, C count, W want_of) {
+  const int lane = threadIdx.x & 63, run = (batch + 63) / 64, b0 = min(lane * run, batch), b1 = min(b0 + run, batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += count(b);
+  int64_t upto = scan64(mine);
+  const int64_t total = __shfl(upto, 63), want = want_of(total);
+  if (want < 0 || want >= total) return Owner{0, -1};
+  int l = __builtin_ctzll(__ballot(upto > want));
+  int64_t before = __shfl(upto - mine, l);
+  if (run == 1) return Owner{before, l};
+  const int stop = min((l + 1) * run, batch);
+  for (int b = l * run; b < stop; b += 64) {
+    mine = b + lane < stop ? count(b + lane) : 0;
+    upto = scan64(mine);
+    const uint64_t has = __ballot(before + upto > want);
     if (has) {
-      const int l = __builtin_ctzll(has);
-      d.seq = b0 + l;
-      d.before = before + __shfl(upto - mine, l);
-      d.tiles = __shfl(tiles, l);
-      d.seen = Seen{__shfl(s.n, l), __shfl(s.sinks, l), __shfl(s.skip, l)};
-      return d;
+      l = __builtin_ctzll(has);
+      return Owner{before + __shfl(upto - mine, l), b + l};
     }
     before += __shfl(upto, 63);
   }
-  return d;
+  return Owner{0, -1};
+}
+
+// The tiles of all (sequence, kv head) pairs, one after the other, are dealt out
+// to the blocks in equal runs, whatever the lengths: no block is left with a
+// long sequence, and a short one in a wide table is still spread. A run may end
+// in the middle of a pair; its part is then joined with the neighbours' by
+// attn_decode_join_kernel.
+template <int KEYS>
+__device__ inline int decode_tiles(const Seen& s) { return (s.n + KEYS - 1) / KEYS; }
+__device__ inline int64_t decode_share(int64_t total, int blocks) {
+  return max((total + blocks - 1) / blocks, (int64_t)kDecMinTiles);
 }
 
 // One new token per sequence: block = (16 of a kv head's query heads; a run of
@@ -260,6 +254,12 @@ __device__ inline Deal deal_out(const AttnArgs& a, int blocks, int64_t block, in
 //
 // Weights are split in two 16-bit parts (hi + lo, both multiplied): the
 // matrix cores have time to spare, and the result is as good as f32 weights.
+//
+// Bound by the reading of the cache. 64 ragged sequences of up to 32768 tokens,
+// 16/2 heads of 256 bf16 (2.2 GB): 395 us with the join, 5.5 TB/s, where a
+// streaming read reaches 6.1; a block per (pair, fixed part) took 527 us, its
+// longest pair last. One sequence of 131071, 32/8 heads of 128: 107 us, 5.0
+// TB/s. One of 127: 11 us, a launch and a chain of dependent loads.
 template <class T, int D, bool CAP>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs a) {
   constexpr int NS = dec_keys<D>() / 16, kKeys = 16 * NS, kStep = D / 32, kOut = D / 16;
@@ -275,29 +275,37 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   const Scale sc = fold_scale<CAP>(a);
   const int heads = min(16, a.group - (int)blockIdx.y * 16);
 
-  Deal deal;
-  int64_t at_tile = 0, end_tile = 0;
+  // the pair's sequence, and what its last token sees; the tiles in front of the sequence's, and this run
+  int32_t of_seq, of_tiles;
+  Seen of_seen;
+  int64_t before = 0, at_tile = 0, end_tile = 0;
   if (a.splits > 1) {
-    deal = deal_out<kKeys>(a, a.splits, blockIdx.x, -1);
-    if (deal.seq < 0) return;
-    at_tile = blockIdx.x * deal.share;
-    end_tile = at_tile + deal.share;
+    const Owner w = find_owner(
+        a.b.batch,
+        [&](int b) { return (int64_t)decode_tiles<kKeys>(seen_by_last(a, a.b.lens[b])) * a.p.kv_heads; },
+        [&](int64_t total) {
+          const int64_t share = decode_share(total, a.splits);
+          at_tile = blockIdx.x * share;
+          end_tile = min(at_tile + share, total);
+          return at_tile;
+        });
+    if (w.seq < 0) return;
+    of_seq = w.seq;
+    before = w.before;
   } else {
-    deal.seq = blockIdx.x / a.p.kv_heads;
-    deal.seen = seen_by_last(a, a.b.lens[deal.seq]);
-    deal.tiles = (deal.seen.n + kKeys - 1) / kKeys;
-    deal.before = 0;
-    at_tile = (int64_t)(blockIdx.x - deal.seq * a.p.kv_heads) * deal.tiles;
+    of_seq = blockIdx.x / a.p.kv_heads;
   }
+  of_seen = seen_by_last(a, a.b.lens[of_seq]);
+  of_tiles = decode_tiles<kKeys>(of_seen);
   for (bool head_of_run = true;; head_of_run = false) {
   // this pair, and the tiles of it that fall to this block
-  const int seq = __builtin_amdgcn_readfirstlane(deal.seq), tiles = __builtin_amdgcn_readfirstlane(deal.tiles);
-  const Seen seen{__builtin_amdgcn_readfirstlane(deal.seen.n), __builtin_amdgcn_readfirstlane(deal.seen.sinks),
-                  __builtin_amdgcn_readfirstlane(deal.seen.skip)};
+  const int seq = __builtin_amdgcn_readfirstlane(of_seq), tiles = __builtin_amdgcn_readfirstlane(of_tiles);
+  const Seen seen{__builtin_amdgcn_readfirstlane(of_seen.n), __builtin_amdgcn_readfirstlane(of_seen.sinks),
+                  __builtin_amdgcn_readfirstlane(of_seen.skip)};
   int hk, first, last;
   if (a.splits > 1) {
-    hk = (int)((at_tile - deal.before) / tiles);
-    first = (int)(at_tile - deal.before - (int64_t)hk * tiles);
+    hk = (int)((at_tile - before) / tiles);
+    first = (int)(at_tile - before - (int64_t)hk * tiles);
     last = (int)min((int64_t)tiles, first + end_tile - at_tile);
   } else {
     hk = blockIdx.x - seq * a.p.kv_heads;
@@ -494,13 +502,13 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   // the run's next pair: the sequence's next head, or the next sequence that sees anything
   at_tile += last - first;
   if (at_tile >= end_tile) return;
-  if (at_tile - deal.before >= (int64_t)tiles * a.p.kv_heads) {
-    deal.before = at_tile;
+  if (at_tile - before >= (int64_t)tiles * a.p.kv_heads) {
+    before = at_tile;
     do {
-      if (++deal.seq >= a.b.batch) return;
-      deal.seen = seen_by_last(a, a.b.lens[deal.seq]);
-      deal.tiles = (deal.seen.n + kKeys - 1) / kKeys;
-    } while (deal.tiles == 0);
+      if (++of_seq >= a.b.batch) return;
+      of_seen = seen_by_last(a, a.b.lens[of_seq]);
+      of_tiles = decode_tiles<kKeys>(of_seen);
+    } while (of_tiles == 0);
   }
   __syncthreads();  // the waves' sums are read; V tiles may be written again
   }
@@ -509,25 +517,54 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 // Joins the parts of a (sequence, query head): out = sum 2^(ref - max) part /
 // sum 2^(ref - max) sum over the blocks whose runs meet in its pair (parts that
 // saw no key have ref = -inf). Pairs that one block had are written already;
-// a sequence that sees nothing gets its zeros here.
+// a sequence that sees nothing gets its zeros here. A block has the query heads
+// blockIdx.y, blockIdx.y + gridDim.y, ...: with many sequences most pairs are
+// written already, and counting the sequences' tiles is what a block costs
+// (1024 sequences of up to 512 tokens, 32 query heads: a block per head 63 us,
+// two blocks a sequence 19 us).
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ f32x4 vs[kGroups][kLanes];
   __shared__ float ls[kGroups];
-  const int seq = blockIdx.x, h = blockIdx.y, hk = h / a.group, in = h - hk * a.group;
-  const Deal d = deal_out<dec_keys<D>()>(a, a.splits, 0, seq);
+  const int seq = blockIdx.x;
+  const int tiles = decode_tiles<dec_keys<D>()>(seen_by_last(a, a.b.lens[seq]));
   const int g = threadIdx.x / kLanes, c = threadIdx.x - g * kLanes;
-  char* out = a.out + 2 * (seq * a.ost[0] + h * a.ost[1] + 4 * c);
-  if (d.tiles == 0) {
-    if (g == 0) *reinterpret_cast<u32x2*>(out) = u32x2{0u, 0u};
+  char* out = a.out + 2 * (seq * a.ost[0] + 4 * c);
+  if (tiles == 0) {
+    if (g == 0)
+      for (int h = blockIdx.y; h < a.q_heads; h += gridDim.y)
+        *reinterpret_cast<u32x2*>(out + 2 * h * a.ost[1]) = u32x2{0u, 0u};
     return;
   }
-  const int64_t t0 = d.before + (int64_t)hk * d.tiles;
-  const int b0 = (int)(t0 / d.share), b1 = (int)((t0 + d.tiles - 1) / d.share);
-  if (b0 == b1) return;
+  // all tiles, and those in front of the sequence's
+  __shared__ int64_t part_total[4], part_before[4];
+  int64_t total = 0, before = 0;
+  for (int b = threadIdx.x; b < a.b.batch; b += 256) {
+    const int64_t n = decode_tiles<dec_keys<D>()>(seen_by_last(a, a.b.lens[b]));
+    total += n;
+    if (b < seq) before += n;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    total += __shfl_xor(total, o);
+    before += __shfl_xor(before, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    part_total[threadIdx.x >> 6] = total;
+    part_before[threadIdx.x >> 6] = before;
+  }
+  __syncthreads();
+  total = (part_total[0] + part_total[1] + part_total[2] + part_total[3]) * a.p.kv_heads;
+  before = (part_before[0] + part_before[1] + part_before[2] + part_before[3]) * a.p.kv_heads;
+  const int64_t share = decode_share(total, a.splits);
+  for (int h = blockIdx.y; h < a.q_heads; h += gridDim.y) {
+  const int hk = h / a.group, in = h - hk * a.group;
+  const int64_t t0 = before + (int64_t)hk * tiles;
+  const int b0 = (int)(t0 / share), b1 = (int)((t0 + tiles - 1) / share);
+  if (b0 == b1) continue;
   auto slot = [&](int b) {
-    return (((int64_t)(in >> 4) * a.splits + b) * 2 + (b * d.share < t0 ? 1 : 0)) * 16 + (in & 15);
+    return (((int64_t)(in >> 4) * a.splits + b) * 2 + (b * share < t0 ? 1 : 0)) * 16 + (in & 15);
   };
   const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat);
   float top = -INFINITY, l = 0.0f;
@@ -535,6 +572,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
   f32x4 v = {0, 0, 0, 0};
+  __syncthreads();  // the last head's parts are read
   if (g < kGroups) {
 #pragma unroll 4
     for (int b = b0 + g; b <= b1; b += kGroups) {
@@ -550,7 +588,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
     if (c == 0) ls[g] = l;
   }
   __syncthreads();
-  if (g > 0) return;
+  if (g > 0) continue;
 #pragma unroll
   for (int i = 1; i < kGroups; ++i) {
     l += ls[i];
@@ -560,7 +598,8 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   const float r = 1.0f / l;
   u32x2 w = {0u, 0u};
   if (top != -INFINITY) w = u32x2{T::pack(v[0] * r, v[1] * r), T::pack(v[2] * r, v[3] * r)};
-  *reinterpret_cast<u32x2*>(out) = w;
+  *reinterpret_cast<u32x2*>(out + 2 * h * a.ost[1]) = w;
+  }
 }
 
 // Joins the parts of rows (token and query head): out =
@@ -568,6 +607,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
 // no key (ref = -inf) were not written. A thread has 4 values of a row; G
 // groups of D/4 threads share a row's parts, and a block has the rows that fit
 // 256 threads (many rows of few parts: G = 1; few rows of many: one row a block).
+// Bound by the reading of the parts, which the prompt kernel has just written.
 template <class T, int D, int G>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t rows) {
   constexpr uint32_t kLanes = D / 4, kRows = 256 / (kLanes * G);
@@ -693,6 +733,16 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 //
 // K and V tiles come straight from memory to LDS, double buffered: the next
 // tile's loads are issued before a tile is computed, one barrier a tile.
+//
+// 8 sequences of 2048, 32/8 heads of 128 bf16, causal (275 GFLOP): 336 to 346
+// us, 800 to 820 TFLOP/s, where a large library product reaches 1260 (a card
+// that clocks lower: up to 410). With two waves a SIMD the matrix units work 42
+// % of the time and the vector units 49 (a score takes a multiply-add, an exp
+// and half a conversion), each wave's own step one after the other. 8191 tokens
+// in a window of 4096, soft cap, 16/8 heads of 256 (412 GFLOP): 582 to 640 us;
+// registers allow one wave a SIMD there, and the tile's load instructions and
+// its barrier stand beside the step. Deeper rings of tiles, 256 rows a block
+// and loads spread over the step were no faster.
 template <class T, int D, int BN, bool CAP>
 __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
@@ -709,34 +759,16 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
 
   // which sequence's tile this is: tiles are counted over the sequences, from
   // the last one on (the longest ones of a prompt first)
-  int seq = -1, tile = 0;
-  KvSeq s{0, 0, 0};
-  {
-    int want = gridDim.x / a.p.kv_heads - 1 - place, before = 0;
-    for (int b0 = 0; b0 < a.b.batch; b0 += 64) {
-      const int b = b0 + lane;
-      const KvSeq c = b < a.b.batch ? kv_seq(a.b, b) : KvSeq{0, 0, 0};
-      const int mine = (c.n * G + BM - 1) / BM;
-      int upto = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(upto, o);
-        if (lane >= o) upto += v;
-      }
-      const uint64_t has = __ballot(before + upto > want);
-      if (has) {
-        const int l = __builtin_ctzll(has);
-        seq = b0 + l;
-        tile = want - before - __builtin_amdgcn_readlane(upto - mine, l);
-        s.first = __builtin_amdgcn_readlane(c.first, l);
-        s.n = __builtin_amdgcn_readlane(c.n, l);
-        s.len = __builtin_amdgcn_readlane(c.len, l);
-        break;
-      }
-      before += __builtin_amdgcn_readlane(upto, 63);
-    }
-  }
-  if (seq < 0) return;
+  const int64_t want = gridDim.x / a.p.kv_heads - 1 - place;
+  const Owner w = find_owner(
+      a.b.batch, [&](int b) { return ((int64_t)kv_seq(a.b, b).n * G + BM - 1) / BM; }, [&](int64_t) { return want; });
+  if (w.seq < 0) return;
+  const int seq = __builtin_amdgcn_readfirstlane(w.seq);
+  const int tile = __builtin_amdgcn_readfirstlane((int)(want - w.before));
+  KvSeq s = kv_seq(a.b, seq);
+  s.first = __builtin_amdgcn_readfirstlane(s.first);
+  s.n = __builtin_amdgcn_readfirstlane(s.n);
+  s.len = __builtin_amdgcn_readfirstlane(s.len);
   const int R = s.n * G, pos0 = s.len - s.n;  // pos0 may be negative: rows in front of the sequence
 
   // the block's keys, in tiles of BN: those of the first `sinks`, then the window's
@@ -1159,7 +1191,7 @@ int check_sizes(const char* what, const hgk_kv_pages* pages, const hgk_kv_batch*
   if (int st = kv_check_batch(what, *p, batch, b)) return st;
   if (q_heads < 1 || q_heads > 65535 || q_heads % p->kv_heads)
     return fail(HGK_ERR_ARG, "%s: %lld query heads for %d kv heads", what, (long long)q_heads, p->kv_heads);
-  if ((int64_t)b->batch * p->kv_heads > INT32_MAX || (int64_t)b->tokens * q_heads > INT32_MAX)
+  if ((int64_t)b->batch * p->kv_heads > INT32_MAX || (int64_t)b->tokens * q_heads > 1 << 30)
     return fail(HGK_ERR_ARG, "%s: %lld rows of %lld heads are too many", what, (long long)b->tokens,
                 (long long)q_heads);
   if (window < 0 || sinks < 0)
@@ -1216,7 +1248,8 @@ void launch_decode(const AttnArgs& a, hipStream_t stream) {
   else
     HGK_LAUNCH((attn_decode_kernel<T, D, false>), grid, block, 0, stream, a);
   if (a.splits > 1)
-    HGK_LAUNCH((attn_decode_join_kernel<T, D>), dim3(a.b.batch, a.q_heads), dim3(256), 0, stream, a);
+    HGK_LAUNCH((attn_decode_join_kernel<T, D>),
+               dim3(a.b.batch, std::clamp<int>(kDecJoinBlocks / a.b.batch, 1, a.q_heads)), dim3(256), 0, stream, a);
 }
 
 template <class T, int D, int BN>

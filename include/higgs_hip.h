@@ -523,7 +523,8 @@ int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers, const int64_t l
  * last `window` keys and the first `sinks`). A query that sees no key gives a
  * row of zeros; keys and values that a query does not see, infinities and NaN
  * among them, do not touch its row. Rows of no sequence are left as they are.
- * out must not overlap the other operands.
+ * out must not overlap the other operands, nor its rows each other; tokens * q_heads
+ * is at most 2^30.
  * Sums and softmax statistics are f32; the probabilities are rounded to the
  * dtype for the product with v; the result is rounded once.
  * `workspace`: device memory of hgk_paged_attention_workspace() bytes (NULL

@@ -45,6 +45,20 @@ def test_decode_long_and_wide(dev, batch, length):
     run(dev, x)
 
 
+@pytest.mark.parametrize("prompts", [False, True])
+def test_many_sequences(dev, prompts):
+    """More sequences than a wave has lanes, several times over, empty ones among them."""
+    g = torch.Generator().manual_seed(5)
+    news = torch.randint(0, 4, (700,), generator=g).tolist() if prompts else None
+    lens = torch.randint(0, 90, (700,), generator=g).tolist()
+    lens[0] = lens[1] = lens[699] = 0
+    lens[350] = 3000
+    if prompts:
+        lens = [n + m for n, m in zip(lens, news)]
+    x = R.make(33, lens, news=news, heads=4, kv_heads=2, head_dim=64, page=16, dtype=BF16)
+    run(dev, x)
+
+
 @pytest.mark.parametrize("softcap", [0.0, 50.0, 1.5])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 0), (100, 4), (100, 90), (64, 1000),
                                           (1000, 0), (1000, 4), (2 ** 40, 0), (0, 5)])
@@ -170,15 +184,26 @@ def test_starts_outside_the_rows_reach_nothing(dev):
 @pytest.mark.parametrize("head_dim,dtype", [(64, BF16), (128, F16), (256, BF16)])
 def test_values_that_are_not_seen_do_not_reach_a_row(dev, bad, head_dim, dtype):
     """A key or value that is no number: rows that do not see it keep their bits."""
+    unseen(dev, bad, head_dim, dtype, 16, ({}, {"window": 40, "sinks": 3}))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("head_dim,dtype,page", [(64, BF16, 4), (96, F16, 2), (128, BF16, 16), (256, F16, 4)])
+def test_values_that_are_not_seen_with_a_soft_cap(dev, bad, head_dim, dtype, page):
+    """The same, capped, and with pages that end inside a tile's rows."""
+    unseen(dev, bad, head_dim, dtype, page, ({"softcap": 50.0}, {"softcap": 2.0, "window": 40, "sinks": 3}))
+
+
+def unseen(dev, bad, head_dim, dtype, page, masks):
     news, lens = [150, 90], [150, 400]
-    x = R.make(17, lens, news=news, heads=4, kv_heads=2, head_dim=head_dim, page=16, dtype=dtype)
-    for kw in ({}, {"window": 40, "sinks": 3}):
+    x = R.make(17, lens, news=news, heads=4, kv_heads=2, head_dim=head_dim, page=page, dtype=dtype)
+    for kw in masks:
         clean = run(dev, x, **kw)
         for pool in ("k_pages", "v_pages"):
             for b, j in ((0, 77), (0, 149), (1, 330)):
                 y = dict(x)
                 y[pool] = x[pool].clone()
-                y[pool][int(x["table"][b, j // 16]), j % 16, :, 5] = bad
+                y[pool][int(x["table"][b, j // page]), j % page, :, 5] = bad
                 got = R.call(H, R.to(y, dev), **kw).cpu()
                 for s, (n, length) in enumerate(zip(news, lens)):
                     first = 0 if s == 0 else news[0]
