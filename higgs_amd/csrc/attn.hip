@@ -521,7 +521,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 // blockIdx.y, blockIdx.y + gridDim.y, ...: with many sequences most pairs are
 // written already, and counting the sequences' tiles is what a block costs
 // (1024 sequences of up to 512 tokens, 32 query heads: a block per head 63 us,
-// two blocks a sequence 19 us).
+// two blocks a sequence 20 us).
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
