@@ -520,8 +520,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 // a sequence that sees nothing gets its zeros here. A block has the query heads
 // blockIdx.y, blockIdx.y + gridDim.y, ...: with many sequences most pairs are
 // written already, and counting the sequences' tiles is what a block costs
-// (1024 sequences of up to 512 tokens, 32 query heads: a block per head 63 us,
-// two blocks a sequence 20 us).
+// (1024 sequences of up to 512 tokens in a wide table, 32 query heads: a block
+// per head 63 us, two blocks a sequence 20 us).
 template <class T, int D>
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
@@ -1206,28 +1206,37 @@ int64_t prompt_tiles(const KvBatchView& b, int64_t group) {
 }
 
 // How the keys are split, from the sizes alone (the lengths are on the device).
-// One token a sequence: the number of blocks that share out all tiles (1: a
-// block per pair). Prompts: the parts of every row's tiles, as many as fill the
+// One token a sequence: see decode_blocks. Prompts: the parts of every row's tiles, as many as fill the
 // chip, and not so many that a part goes below kMinPart keys. Writing and
 // joining the parts costs as much as half the work of a few hundred blocks, so
 // rows are split only where they make less than half a block a CU (ragged turns
 // over 20000 tokens, 250 blocks: unsplit 41 us, in two 43, in three 50).
 constexpr int kMinPart = 256, kPromptBlocks = 256, kMaxSplits = 64;
 
-// Blocks that share out the tiles of single tokens. Rows of 256 values take two
-// blocks a CU (64 sequences of 16384 tokens, 2 kv heads: 378 us, one: 417). Rows
-// up to 128 stream better from one (32 sequences of 8192, 8 kv heads of 64: 106
-// us, two: 127), until the pairs are so many that a run holds several and the
-// gaps between them show (64 ragged sequences up to 2048: 57 us, two: 47).
-int decode_blocks(const KvView& p, const KvBatchView& b) {
-  return p.head_dim == 256 || (int64_t)b.batch * p.kv_heads >= 512 ? 512 : 256;
+// Blocks that share out the tiles of single tokens; 1: a block per pair and no
+// join. That is for caches whose longest pair, as the table and the window allow
+// it, is a block's work of about 20 us, or half of that where the pairs are fewer
+// than the CUs: finding the run, the ends of pairs inside it and the join cost
+// more than unequal pairs (in us, ragged lengths, a block per pair and dealt out:
+// 256 pairs of up to 1024 keys of 128 values 23, 33; 1024 pairs of up to 512 33,
+// 65; 512 pairs of up to 2048 keys of 64 36, 47; past the rule 256 pairs of up to
+// 2048 keys of 256 74, 64; 64 of 1024 of 128 21, 18).
+// Rows of 256 values take two blocks a CU (64 sequences of 16384 tokens, 2 kv
+// heads: 378 us, one: 417). Rows up to 128 stream better from one (32 sequences
+// of 8192, 8 kv heads of 64: 106 us, two: 127), until the pairs are so many that
+// a run holds several and the gaps between them show (64 sequences, 8 kv heads of
+// 64, ragged up to 4096: 82 us, two: 70; all 4096 long: 107, two: 125).
+int decode_blocks(const KvView& p, const KvBatchView& b, int64_t keys) {
+  const int64_t pairs = (int64_t)b.batch * p.kv_heads;
+  if (keys * p.head_dim <= (pairs >= 256 ? 1 << 17 : 1 << 16)) return 1;
+  return p.head_dim == 256 || pairs >= 512 ? 512 : 256;
 }
 int plan_splits(const KvView& p, const KvBatchView& b, int64_t q_heads, int64_t window, int64_t sinks) {
   if (b.batch == 0 || b.tokens == 0) return 1;
   const int64_t group = q_heads / p.kv_heads;
   int64_t keys = (int64_t)b.width << p.page_shift;
   if (window > 0 && window < keys && sinks < keys - window) keys = window + sinks;
-  if (!b.starts) return keys <= kMinPart ? 1 : decode_blocks(p, b);
+  if (!b.starts) return decode_blocks(p, b, keys);
   const int64_t s = std::min(kPromptBlocks / (p.kv_heads * prompt_tiles(b, group)), keys / kMinPart);
   return (int)std::max<int64_t>(1, std::min<int64_t>(s, kMaxSplits));
 }

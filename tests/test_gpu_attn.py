@@ -45,6 +45,21 @@ def test_decode_long_and_wide(dev, batch, length):
     run(dev, x)
 
 
+@pytest.mark.parametrize("kw", [{}, {"softcap": 2.0}, {"window": 1500, "sinks": 3}])
+@pytest.mark.parametrize("heads,kv_heads,head_dim,dtype", [(32, 8, 64, BF16), (4, 1, 96, F16), (16, 8, 128, BF16),
+                                                           (40, 2, 128, F16), (16, 2, 256, BF16)])
+def test_decode_short_sequences_in_a_wide_table(dev, heads, kv_heads, head_dim, dtype, kw):
+    """A table with room for long sequences: runs of tiles that end inside a pair or hold several."""
+    lens = [1, 300, 0, 2, 257, 1700, 31, 0, 512, 640, 17, 900]
+    x = R.make(34, lens, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page=16, dtype=dtype)
+    x["table"] = torch.nn.functional.pad(x["table"], (0, 256), value=-1)
+    run(dev, x, **kw)
+    many = [1 + 37 * i % 90 for i in range(150)]
+    x = R.make(35, many, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page=16, dtype=dtype)
+    x["table"] = torch.nn.functional.pad(x["table"], (0, 256), value=-1)
+    run(dev, x, **kw)
+
+
 @pytest.mark.parametrize("prompts", [False, True])
 def test_many_sequences(dev, prompts):
     """More sequences than a wave has lanes, several times over, empty ones among them."""
