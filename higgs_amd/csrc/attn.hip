@@ -778,7 +778,8 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   const int hi = (int)min((int64_t)p_last + 1, cap);
   const int lo = a.window > 0 && p_first >= a.window ? p_first - a.window + 1 : 0;
   const int t_hi = hi > 0 ? (hi + BN - 1) / BN : 0, t_lo = lo / BN;
-  const int front = min(min((min(a.sinks, lo) + BN - 1) / BN, t_lo), t_hi);
+  // (at most 2^30 before it is rounded up: sinks and lo may both end at int32's end)
+  const int front = min((min(min(a.sinks, lo), max(hi, 0)) + BN - 1) / BN, t_lo);
   const int tiles = a.p.n_pages > 0 ? front + max(t_hi - t_lo, 0) : 0;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int it0 = min(per * (int)blockIdx.y, tiles), it1 = min(it0 + per, tiles);
