@@ -151,6 +151,14 @@ constexpr float kSlack = 8.0f;
 // occur, and finite times c.
 __device__ inline float lowest_ref(float c) { return -3.0e38f / fmaxf(c, 1.0f); }
 
+// A weight is 2^(c x + base), base = -c ref. That product is rounded, by up to
+// 2^-8 at 2^16: no matter, all of the row's weights share it. Far above, the
+// rounding alone would take weights beyond f32: there a weight is 2^(c (x - ref)),
+// as the difference is exact next to the reference. Prompts look at the base of
+// every tile; single tokens, where one more branch a tile costs 3 % of a long
+// cache, at their last base and their sums, and then walk their tiles again.
+constexpr float kBaseMax = 65536.0f;
+
 // 2^(c (ref - to)) of a reference that moves up. Not below the smallest normal
 // number: an infinite sum (of infinite values) stays infinite, and a finite
 // one that far below is lost in the new one's rounding all the same.
@@ -365,103 +373,116 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   };
 
   f32x4 o[kOut];
-#pragma unroll
-  for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
-  float ref = lowest_ref(sc.c), sum = 0.0f;
+  float ref, sum;
   const float slack = kSlack / sc.c;
-  bool any = false;
+  bool any;
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   char* vt = lds + wave * kTile;
 
-  int32_t page[NS], at[NS];
-  if (a.p.n_pages > 0 && first + wave < last) {
-    look_up(first + wave, page, at);
-    load(page, at);
-    look_up(first + wave + kDecWaves, page, at);
-    for (int tile = first + wave; tile < last; tile += kDecWaves) {
-      // scores
-      f32x4 s[NS];
+  auto walk = [&](auto exact) {  // this wave's tiles
 #pragma unroll
-      for (int h = 0; h < NS; ++h) {
-        s[h] = f32x4{0, 0, 0, 0};
+    for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
+    ref = lowest_ref(sc.c);
+    sum = 0.0f;
+    any = false;
+    int32_t page[NS], at[NS];
+    if (a.p.n_pages > 0 && first + wave < last) {
+      look_up(first + wave, page, at);
+      load(page, at);
+      look_up(first + wave + kDecWaves, page, at);
+      for (int tile = first + wave; tile < last; tile += kDecWaves) {
+        // scores
+        f32x4 s[NS];
 #pragma unroll
-        for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
-      }
-      const uint32_t now = there;
-      if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
+        for (int h = 0; h < NS; ++h) {
+          s[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
+        }
+        const uint32_t now = there;
+        if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
+#pragma unroll
+          for (int h = 0; h < NS; ++h)
+            if (!((now >> (16 * h + m)) & 1))
+#pragma unroll
+              for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int h = 0; h < NS; ++h)
-          if (!((now >> (16 * h + m)) & 1))
 #pragma unroll
-            for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
-      }
+          for (int k = 0; k < kStep; ++k)
+            *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
+        if (tile + kDecWaves < last) {
+          load(page, at);
+          look_up(tile + 2 * kDecWaves, page, at);
+        }
+        // weights
+        float x[4 * NS], top = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < NS; ++h)
+        for (int i = 0; i < 4 * NS; ++i) {
+          x[i] = s[i / 4][i % 4];
+          if constexpr (CAP) x[i] = fast_tanh(x[i] * sc.inner);
+        }
+        const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
+        if (now != kAll) {
 #pragma unroll
-        for (int k = 0; k < kStep; ++k)
-          *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
-      if (tile + kDecWaves < last) {
-        load(page, at);
-        look_up(tile + 2 * kDecWaves, page, at);
-      }
-      // weights
-      float x[4 * NS], top = -INFINITY;
+          for (int i = 0; i < 4 * NS; ++i)
+            if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
+        }
 #pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) {
-        x[i] = s[i / 4][i % 4];
-        if constexpr (CAP) x[i] = fast_tanh(x[i] * sc.inner);
-      }
-      const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
-      if (now != kAll) {
+        for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
+        if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
+          const float to = top > ref + slack ? top : ref, f = shrink(ref, to, sc.c);
+          sum *= f;
+#pragma unroll
+          for (int t = 0; t < kOut; ++t) o[t] *= f;
+          ref = to;
+        }
+        const float base = -ref * sc.c;
 #pragma unroll
         for (int i = 0; i < 4 * NS; ++i)
-          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
-      }
+          x[i] = __builtin_amdgcn_exp2f(exact() ? (x[i] - ref) * sc.c : fmaf(x[i], sc.c, base));
+        any |= now != 0;
+        uint32_t hi[2 * NS], lo[2 * NS];
 #pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
-      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = top > ref + slack ? top : ref, f = shrink(ref, to, sc.c);
-        sum *= f;
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) o[t] *= f;
-        ref = to;
-      }
-      const float base = -ref * sc.c;
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
-      any |= now != 0;
-      uint32_t hi[2 * NS], lo[2 * NS];
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) {
-        sum += x[2 * i] + x[2 * i + 1];
-        hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
-        lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
-      }
-      // O^T += V^T P^T
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int t = 0; t < kOut; ++t) {
-        const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
-        const u32x2 v0 = lds_transposed(p);
-        if constexpr (NS == 2) {
-          const u32x2 v1 = lds_transposed(p + 16 * kRow);
-          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-          o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
-          o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
-        } else {
-          o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
-          o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
+        for (int i = 0; i < 2 * NS; ++i) {
+          sum += x[2 * i] + x[2 * i + 1];
+          hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
+          lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
         }
+        // O^T += V^T P^T
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < kOut; ++t) {
+          const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
+          const u32x2 v0 = lds_transposed(p);
+          if constexpr (NS == 2) {
+            const u32x2 v1 = lds_transposed(p + 16 * kRow);
+            const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
+            o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
+            o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
+          } else {
+            o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
+            o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_wave_barrier();
     }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+  };
+  walk(std::false_type{});
+  {
+    float all = sum;  // not finite where one of them is not
+#pragma unroll
+    for (int t = 0; t < kOut; ++t) all += (o[t][0] + o[t][1]) + (o[t][2] + o[t][3]);
+    if (__any(any && !(fabsf(ref * sc.c) <= kBaseMax && fabsf(all) < INFINITY))) walk(std::true_type{});
   }
 
   // join the waves
-  sum += __shfl_xor(sum, 16);
-  sum += __shfl_xor(sum, 32);
   __syncthreads();  // every wave is done with its V tile
   float* wo = reinterpret_cast<float*>(lds) + wave * 16 * D;
 #pragma unroll
@@ -911,7 +932,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   // and moves the references that others pass; `shrunk` is then the factor for
   // the sums so far (few tiles move any: most leave `moved` false).
   bool moved;
-  float shrunk;
+  float shrunk, base;  // base: of the weights' exponents, c x + base
   uint32_t see[KT];  // CAP, masked: the 32 keys' bits, at 8 (e / 4) + e % 4 for score e
   auto settle = [&](f32x16* x, int it, uint64_t exist, bool masked) {
     auto top_of = [&](const f32x16* x) {
@@ -961,12 +982,21 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
       sum *= shrunk;
       ref = to;
     }
+    base = -ref * sc.c;
+    if constexpr (!CAP) {
+      if (__any(fabsf(base) > kBaseMax)) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[t][e] -= ref;
+        base = 0.0f;
+      }
+    }
   };
   // Weights of scores 2 i and 2 i + 1, rounded to the type; the sum takes the
   // rounded ones, so that a row's weights add up to one as they are used.
   float add[4];
   auto weigh = [&](const f32x16* x, int i) {
-    const float base = -ref * sc.c;
     float s0 = x[i / 8][2 * i % 16], s1 = x[i / 8][2 * i % 16 + 1];
     if constexpr (CAP) {
       s0 = fast_tanh(s0 * sc.inner);
