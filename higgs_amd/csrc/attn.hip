@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   f32x4 o[kOut];
   float ref, sum;
   const float slack = kSlack / sc.c;
-  bool any;
+  bool any, again;
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   char* vt = lds + wave * kTile;
 
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
         const float base = -ref * sc.c;
 #pragma unroll
         for (int i = 0; i < 4 * NS; ++i)
-          x[i] = __builtin_amdgcn_exp2f(exact() ? (x[i] - ref) * sc.c : fmaf(x[i], sc.c, base));
+          x[i] = __builtin_amdgcn_exp2f(exact() && again ? (x[i] - ref) * sc.c : fmaf(x[i], sc.c, base));
         any |= now != 0;
         uint32_t hi[2 * NS], lo[2 * NS];
 #pragma unroll
@@ -479,7 +479,11 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
     float all = sum;  // not finite where one of them is not
 #pragma unroll
     for (int t = 0; t < kOut; ++t) all += (o[t][0] + o[t][1]) + (o[t][2] + o[t][3]);
-    if (__any(any && !(fabsf(ref * sc.c) <= kBaseMax && fabsf(all) < INFINITY))) walk(std::true_type{});
+    all += __shfl_xor(all, 16);
+    all += __shfl_xor(all, 32);
+    // a head's own scores and values alone decide for it
+    again = any && !(fabsf(ref * sc.c) <= kBaseMax && fabsf(all) < INFINITY);
+    if (__any(again)) walk(std::true_type{});
   }
 
   // join the waves
@@ -988,8 +992,8 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[t][e] -= ref;
-        base = 0.0f;
+          for (int e = 0; e < 16; ++e) x[t][e] -= fabsf(base) > kBaseMax ? ref : 0.0f;
+        base = fabsf(base) > kBaseMax ? 0.0f : base;
       }
     }
   };
