@@ -55,6 +55,8 @@ template <> struct Mx<BF16> {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), __builtin_bit_cast(v2, 0x3f803f80u), s, false);
   }
+  // slack and bias of the weights' exponents, prompts' and single tokens'
+  static constexpr float kSlack = 8.0f, kBias = 0.0f, kDecSlack = 8.0f, kDecBias = 0.0f;
   static constexpr uint32_t kExp = 0x7f80u, kOne = 0x3f80u, k128 = 0x4300u, k16384 = 0x4680u;
 };
 template <> struct Mx<F16> {
@@ -76,6 +78,7 @@ template <> struct Mx<F16> {
   static __device__ inline float add_pair(uint32_t w, float s) {
     return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w), __builtin_bit_cast(f16x2, 0x3c003c00u), s, false);
   }
+  static constexpr float kSlack = 8.0f, kBias = 7.0f, kDecSlack = 0.0f, kDecBias = 15.0f;
   // the exponent's bits, and 1, 128 and 16384
   static constexpr uint32_t kExp = 0x7c00u, kOne = 0x3c00u, k128 = 0x5800u, k16384 = 0x7400u;
 };
@@ -143,18 +146,22 @@ __device__ inline float fast_tanh(float x) {
 }
 
 // The running maximum only has to keep exp2 in range, so a row's reference
-// moves when a raw score passes it by more than 2^kSlack in weight, and not
-// with every new maximum: f32 sums and 16-bit weights up to 2^kSlack lose nothing.
-constexpr float kSlack = 8.0f;
+// moves when a raw score passes it by more than 2^slack in weight, and not with
+// every new maximum. A weight carries a factor 2^bias, which the division by the
+// sum takes out again. bf16 holds every weight of f32. f16 ends at 2^16 and holds
+// multiples of 2^-24: its bias puts the largest weight at 2^15, so that a weight
+// is off by 2^-32 of the reference's at the most (a million keys of it are 2^-12
+// of the row). Single tokens, whose tiles leave the time, move their references
+// with every new maximum: 2^-40.
 
 // The reference of a row that has seen no score: below every score that can
 // occur, and finite times c.
 __device__ inline float lowest_ref(float c) { return -3.0e38f / fmaxf(c, 1.0f); }
 
-// A weight is 2^(c x + base), base = -c ref. That product is rounded, by up to
+// A weight is 2^(c x + base), base = bias - c ref. That product is rounded, by up to
 // 2^-8 at 2^16: no matter, all of the row's weights share it. Far above, the
-// rounding alone would take weights beyond f32: there a weight is 2^(c (x - ref)),
-// as the difference is exact next to the reference. Prompts look at the base of
+// rounding alone would take weights beyond f32: there a weight is 2^(c (x - ref) +
+// bias), as the difference is exact next to the reference. Prompts look at the base of
 // every tile; single tokens, where one more branch a tile costs 3 % of a long
 // cache, at their last base and their sums, and then walk their tiles again.
 constexpr float kBaseMax = 65536.0f;
@@ -261,7 +268,8 @@ __device__ inline int64_t decode_share(int64_t total, int blocks) {
 // are in flight while a tile is computed.
 //
 // Weights are split in two 16-bit parts (hi + lo, both multiplied): the
-// matrix cores have time to spare, and the result is as good as f32 weights.
+// matrix cores have time to spare, and two parts keep 16 bits of a weight in
+// bf16 and 22 in f16, well below the result's own rounding.
 //
 // Bound by the reading of the cache. 64 ragged sequences of up to 32768 tokens,
 // 16/2 heads of 256 bf16 (2.2 GB): 395 us with the join, 5.5 TB/s, where a
@@ -374,7 +382,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 
   f32x4 o[kOut];
   float ref, sum;
-  const float slack = kSlack / sc.c;
+  const float slack = Mx<T>::kDecSlack / sc.c;
   bool any, again;
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   char* vt = lds + wave * kTile;
@@ -440,10 +448,11 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
           for (int t = 0; t < kOut; ++t) o[t] *= f;
           ref = to;
         }
-        const float base = -ref * sc.c;
+        const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
 #pragma unroll
         for (int i = 0; i < 4 * NS; ++i)
-          x[i] = __builtin_amdgcn_exp2f(exact() && again ? (x[i] - ref) * sc.c : fmaf(x[i], sc.c, base));
+          x[i] = __builtin_amdgcn_exp2f(exact() && again ? fmaf(x[i] - ref, sc.c, Mx<T>::kDecBias)
+                                                         : fmaf(x[i], sc.c, base));
         any |= now != 0;
         uint32_t hi[2 * NS], lo[2 * NS];
 #pragma unroll
@@ -906,7 +915,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
 #pragma unroll
   for (int t = 0; t < DT; ++t) o[t] = f32x16{};
   float ref = lowest_ref(sc.c), sum = 0.0f;
-  const float slack = kSlack / sc.c;
+  const float slack = M::kSlack / sc.c;
   bool any = false;
 
   // A lane's places in a tile of keys (row col, piece 2 i + half) and of values
@@ -986,14 +995,14 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
       sum *= shrunk;
       ref = to;
     }
-    base = -ref * sc.c;
+    base = fmaf(-ref, sc.c, M::kBias);
     if constexpr (!CAP) {
       if (__any(fabsf(base) > kBaseMax)) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
           for (int e = 0; e < 16; ++e) x[t][e] -= fabsf(base) > kBaseMax ? ref : 0.0f;
-        base = fabsf(base) > kBaseMax ? 0.0f : base;
+        base = fabsf(base) > kBaseMax ? M::kBias : base;
       }
     }
   };
