@@ -117,14 +117,16 @@ struct Scale {
   float c, inner;      // inner: scale / softcap
   uint32_t flip, keep; // q word = (q & keep) ^ flip
 };
-template <bool CAP>
+template <int CAP>
 __device__ inline Scale fold_scale(const AttnArgs& a) {
   Scale s;
   s.flip = 0;
   s.keep = ~0u;
   if constexpr (CAP) {
-    s.c = fminf(a.softcap * kLog2e, 1.0e37f);
-    s.inner = fabsf(a.scale) / a.softcap;
+    // (a larger cap is none to scores below 10^26)
+    const float cap = fminf(a.softcap, 1.0e30f);
+    s.c = cap * kLog2e;
+    s.inner = fminf(fabsf(a.scale) / cap, 3.0e38f);  // a score of zero stays zero
     if (a.scale < 0.0f) s.flip = 0x80008000u;
   } else {
     s.inner = 0.0f;
@@ -139,10 +141,32 @@ __device__ inline Scale fold_scale(const AttnArgs& a) {
 }
 
 // tanh from one exp2 and one reciprocal: 1 - 2 / (e^2x + 1). Its absolute
-// error, a few 2^-24, is what matters for softcap * tanh as a score.
+// error is 2^-22 at the most, so a capped score's is softcap times that.
 __device__ inline float fast_tanh(float x) {
   const float e = __builtin_amdgcn_exp2f(x * (2.0f * kLog2e));
   return fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+}
+
+// A soft cap's form (CAP): none, up to kCapMax, and beyond. Up to kCapMax the
+// scores are within 2^-16 with fast_tanh, a 32nd of an f16 rounding. Far beyond
+// it the scores are a small part of the cap, and tanh has to be good to its own
+// size: below 5/8 it is x + x^3 p(x^2), p of degree 4 through the function's
+// values at the Chebyshev points (2^-23.5 of tanh in f32). The caps of models,
+// 30 and 50, do not pay for it (8191 tokens in a window of 4096, 16/8 heads of
+// 256: 580 us, with the wide form 723; eight prompts of 2048, 32/8 heads of 128:
+// 418, 529). Single tokens take it for every cap: it costs them nothing.
+constexpr int kNoCap = 0, kCap = 1, kWideCap = 2;
+constexpr float kCapMax = 64.0f;
+template <int CAP>
+__device__ inline float cap_tanh(float x) {
+  const float t = fast_tanh(x);
+  if constexpr (CAP != kWideCap) return t;
+  const float z = x * x;
+  float p = fmaf(z, -0.00609671418f, 0.0209971797f);
+  p = fmaf(z, p, -0.0538509078f);
+  p = fmaf(z, p, 0.133327693f);
+  p = fmaf(z, p, -0.333333284f);
+  return fabsf(x) < 0.625f ? fmaf(x * z, p, x) : t;
 }
 
 // The running maximum only has to keep exp2 in range, so a row's reference
@@ -276,7 +300,7 @@ __device__ inline int64_t decode_share(int64_t total, int blocks) {
 // streaming read reaches 6.1; a block per (pair, fixed part) took 527 us, its
 // longest pair last. One sequence of 131071, 32/8 heads of 128: 107 us, 5.0
 // TB/s. One of 127: 11 us, a launch and a chain of dependent loads.
-template <class T, int D, bool CAP>
+template <class T, int D, int CAP>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs a) {
   constexpr int NS = dec_keys<D>() / 16, kKeys = 16 * NS, kStep = D / 32, kOut = D / 16;
   // V rows 32 bytes apart in banks: 16 rows of a transposed read cover each bank twice
@@ -429,7 +453,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 #pragma unroll
         for (int i = 0; i < 4 * NS; ++i) {
           x[i] = s[i / 4][i % 4];
-          if constexpr (CAP) x[i] = fast_tanh(x[i] * sc.inner);
+          if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
         }
         const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
         if (now != kAll) {
@@ -777,7 +801,7 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 // registers allow one wave a SIMD there, and the tile's load instructions and
 // its barrier stand beside the step. Deeper rings of tiles, 256 rows a block
 // and loads spread over the step were no faster.
-template <class T, int D, int BN, bool CAP>
+template <class T, int D, int BN, int CAP>
 __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
@@ -977,7 +1001,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
       top = top_of(h);
       if constexpr (CAP) {
         // the scores stay: under tanh a hidden one would count, so the weights are cleared instead
-        top = some ? fast_tanh(top * sc.inner) : hidden;
+        top = some ? cap_tanh<CAP>(top * sc.inner) : hidden;
       } else {
 #pragma unroll
         for (int t = 0; t < KT; ++t) x[t] = h[t];
@@ -985,7 +1009,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     } else {
       any = true;
       top = top_of(x);
-      if constexpr (CAP) top = fast_tanh(top * sc.inner);
+      if constexpr (CAP) top = cap_tanh<CAP>(top * sc.inner);
     }
     moved = __any(top > ref + slack);
     if (moved) {  // a row's own scores alone decide for it
@@ -995,8 +1019,8 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
       sum *= shrunk;
       ref = to;
     }
-    base = fmaf(-ref, sc.c, M::kBias);
-    if constexpr (!CAP) {
+    base = CAP == kWideCap ? M::kBias : fmaf(-ref, sc.c, M::kBias);
+    if constexpr (CAP == kNoCap) {
       if (__any(fabsf(base) > kBaseMax)) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -1012,8 +1036,12 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   auto weigh = [&](const f32x16* x, int i) {
     float s0 = x[i / 8][2 * i % 16], s1 = x[i / 8][2 * i % 16 + 1];
     if constexpr (CAP) {
-      s0 = fast_tanh(s0 * sc.inner);
-      s1 = fast_tanh(s1 * sc.inner);
+      s0 = cap_tanh<CAP>(s0 * sc.inner);
+      s1 = cap_tanh<CAP>(s1 * sc.inner);
+    }
+    if constexpr (CAP == kWideCap) {  // such scores may be past kBaseMax
+      s0 -= ref;
+      s1 -= ref;
     }
     const float w0 = __builtin_amdgcn_exp2f(fmaf(s0, sc.c, base));
     const float w1 = __builtin_amdgcn_exp2f(fmaf(s1, sc.c, base));
@@ -1297,9 +1325,9 @@ void launch_decode(const AttnArgs& a, hipStream_t stream) {
   const unsigned blocks = a.splits > 1 ? a.splits : a.b.batch * a.p.kv_heads;
   const dim3 grid(blocks, (a.group + 15) / 16), block(64 * kDecWaves);
   if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_decode_kernel<T, D, true>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_decode_kernel<T, D, kWideCap>), grid, block, 0, stream, a);
   else
-    HGK_LAUNCH((attn_decode_kernel<T, D, false>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_decode_kernel<T, D, kNoCap>), grid, block, 0, stream, a);
   if (a.splits > 1)
     HGK_LAUNCH((attn_decode_join_kernel<T, D>),
                dim3(a.b.batch, std::clamp<int>(kDecJoinBlocks / a.b.batch, 1, a.q_heads)), dim3(256), 0, stream, a);
@@ -1308,10 +1336,12 @@ void launch_decode(const AttnArgs& a, hipStream_t stream) {
 template <class T, int D, int BN>
 void launch_prompt(const AttnArgs& a, hipStream_t stream) {
   const dim3 grid(a.p.kv_heads * prompt_tiles(a.b, a.group), a.splits), block(2 * kPromptRows);
-  if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, true>), grid, block, 0, stream, a);
+  if (a.softcap > kCapMax)
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kWideCap>), grid, block, 0, stream, a);
+  else if (a.softcap > 0.0f)
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kCap>), grid, block, 0, stream, a);
   else
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, false>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kNoCap>), grid, block, 0, stream, a);
 }
 
 template <class T, int D>

@@ -520,7 +520,8 @@ int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers, const int64_t l
  *   s_j = scale * (q . k_j), softcap > 0: softcap * tanh(s_j / softcap)
  *   out = sum_j softmax(s)_j v_j over the keys j that the query at position p
  * sees: j <= p, and with window > 0 either j > p - window or j < sinks (the
- * last `window` keys and the first `sinks`). A query that sees no key gives a
+ * last `window` keys and the first `sinks`). A soft cap above 1e30 counts as
+ * 1e30. A query that sees no key gives a
  * row of zeros; keys and values that a query does not see, infinities and NaN
  * among them, do not touch its row. Rows of no sequence are left as they are.
  * out must not overlap the other operands, nor its rows each other; tokens * q_heads
