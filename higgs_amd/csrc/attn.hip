@@ -92,6 +92,13 @@ __device__ inline float max3(float a, float b, float c) {
   return r;
 }
 
+// The largest magnitude of three values, NaN if one of them is NaN.
+__device__ inline float peak3(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 // Of this lane's value and that of the lane 32 away: the larger, and the sum.
 __device__ inline float halves_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
@@ -190,12 +197,10 @@ __device__ inline float lowest_ref(float c) { return -3.0e38f / fmaxf(c, 1.0f); 
 // cache, at their last base and their sums, and then walk their tiles again.
 constexpr float kBaseMax = 65536.0f;
 
-// 2^(c (ref - to)) of a reference that moves up. Not below the smallest normal
-// number: an infinite sum (of infinite values) stays infinite, and a finite
-// one that far below is lost in the new one's rounding all the same.
-__device__ inline float shrink(float ref, float to, float c) {
-  return fmaxf(__builtin_amdgcn_exp2f((ref - to) * c), 1.2e-38f);
-}
+// The factor 2^e of sums whose reference gives way to a greater one. Never zero:
+// an infinite sum (of infinite values that a row sees) stays infinite, and of a
+// finite one so little is lost in the greater one's rounding.
+__device__ inline float lesser(float e) { return fmaxf(__builtin_amdgcn_exp2f(e), 1.0e-44f); }
 
 // ---------------------------------------------------------------- one token
 // The keys that a sequence's last token sees, as one run of n: index i is key
@@ -405,121 +410,111 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   };
 
   f32x4 o[kOut];
-  float ref, sum;
+#pragma unroll
+  for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
+  float ref = lowest_ref(sc.c), sum = 0.0f;
   const float slack = Mx<T>::kDecSlack / sc.c;
-  bool any, again;
+  bool any = false;
   constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
   char* vt = lds + wave * kTile;
 
-  auto walk = [&](auto exact) {  // this wave's tiles
+  int32_t page[NS], at[NS];
+  if (a.p.n_pages > 0 && first + wave < last) {
+    look_up(first + wave, page, at);
+    load(page, at);
+    look_up(first + wave + kDecWaves, page, at);
+    for (int tile = first + wave; tile < last; tile += kDecWaves) {
+      // scores
+      f32x4 s[NS];
 #pragma unroll
-    for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
-    ref = lowest_ref(sc.c);
-    sum = 0.0f;
-    any = false;
-    int32_t page[NS], at[NS];
-    if (a.p.n_pages > 0 && first + wave < last) {
-      look_up(first + wave, page, at);
-      load(page, at);
-      look_up(first + wave + kDecWaves, page, at);
-      for (int tile = first + wave; tile < last; tile += kDecWaves) {
-        // scores
-        f32x4 s[NS];
+      for (int h = 0; h < NS; ++h) {
+        s[h] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < NS; ++h) {
-          s[h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
-        }
-        const uint32_t now = there;
-        if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
-#pragma unroll
-          for (int h = 0; h < NS; ++h)
-            if (!((now >> (16 * h + m)) & 1))
-#pragma unroll
-              for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
-        }
+        for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
+      }
+      const uint32_t now = there;
+      if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
 #pragma unroll
         for (int h = 0; h < NS; ++h)
+          if (!((now >> (16 * h + m)) & 1))
 #pragma unroll
-          for (int k = 0; k < kStep; ++k)
-            *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
-        if (tile + kDecWaves < last) {
-          load(page, at);
-          look_up(tile + 2 * kDecWaves, page, at);
-        }
-        // weights
-        float x[4 * NS], top = -INFINITY;
+            for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
+      }
 #pragma unroll
-        for (int i = 0; i < 4 * NS; ++i) {
-          x[i] = s[i / 4][i % 4];
-          if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
-        }
-        const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
-        if (now != kAll) {
+      for (int h = 0; h < NS; ++h)
 #pragma unroll
-          for (int i = 0; i < 4 * NS; ++i)
-            if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
-        }
+        for (int k = 0; k < kStep; ++k)
+          *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
+      if (tile + kDecWaves < last) {
+        load(page, at);
+        look_up(tile + 2 * kDecWaves, page, at);
+      }
+      // weights
+      float x[4 * NS], top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
-        if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
-          top = fmaxf(top, __shfl_xor(top, 16));
-          top = fmaxf(top, __shfl_xor(top, 32));
-          const float to = top > ref + slack ? top : ref, f = shrink(ref, to, sc.c);
-          sum *= f;
-#pragma unroll
-          for (int t = 0; t < kOut; ++t) o[t] *= f;
-          ref = to;
-        }
-        const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
+      for (int i = 0; i < 4 * NS; ++i) {
+        x[i] = s[i / 4][i % 4];
+        if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
+      }
+      const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
+      if (now != kAll) {
 #pragma unroll
         for (int i = 0; i < 4 * NS; ++i)
-          x[i] = __builtin_amdgcn_exp2f(exact() && again ? fmaf(x[i] - ref, sc.c, Mx<T>::kDecBias)
-                                                         : fmaf(x[i], sc.c, base));
-        any |= now != 0;
-        uint32_t hi[2 * NS], lo[2 * NS];
-#pragma unroll
-        for (int i = 0; i < 2 * NS; ++i) {
-          sum += x[2 * i] + x[2 * i + 1];
-          hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
-          lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
-        }
-        // O^T += V^T P^T
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) {
-          const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
-          const u32x2 v0 = lds_transposed(p);
-          if constexpr (NS == 2) {
-            const u32x2 v1 = lds_transposed(p + 16 * kRow);
-            const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-            o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
-            o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
-          } else {
-            o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
-            o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
-          }
-        }
-        __builtin_amdgcn_wave_barrier();
+          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
       }
-    }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-  };
-  walk(std::false_type{});
-  {
-    float all = sum;  // not finite where one of them is not
 #pragma unroll
-    for (int t = 0; t < kOut; ++t) all += (o[t][0] + o[t][1]) + (o[t][2] + o[t][3]);
-    all += __shfl_xor(all, 16);
-    all += __shfl_xor(all, 32);
-    // a head's own scores and values alone decide for it
-    again = any && !(fabsf(ref * sc.c) <= kBaseMax && fabsf(all) < INFINITY);
-    if (__any(again)) walk(std::true_type{});
+      for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
+      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = top > ref + slack ? top : ref, f = lesser((ref - to) * sc.c);
+        sum *= f;
+#pragma unroll
+        for (int t = 0; t < kOut; ++t) o[t] *= f;
+        ref = to;
+      }
+      const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
+#pragma unroll
+      for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
+      any |= now != 0;
+      uint32_t hi[2 * NS], lo[2 * NS];
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
+        sum += x[2 * i] + x[2 * i + 1];
+        hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
+        lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
+      }
+      // O^T += V^T P^T
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < kOut; ++t) {
+        const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
+        const u32x2 v0 = lds_transposed(p);
+        if constexpr (NS == 2) {
+          const u32x2 v1 = lds_transposed(p + 16 * kRow);
+          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
+          o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
+          o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
+        } else {
+          o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
+          o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
   }
 
   // join the waves
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  // Did this head's scores fit the weights' form, and are its sums finite?
+  bool again;
+  {
+    float peak = sum;
+#pragma unroll
+    for (int t = 0; t < kOut; ++t) peak = peak3(peak3(peak, o[t][0], o[t][1]), o[t][2], o[t][3]);
+    again = any && !(fabsf(ref * sc.c) <= kBaseMax && peak < INFINITY);
+  }
   __syncthreads();  // every wave is done with its V tile
   float* wo = reinterpret_cast<float*>(lds) + wave * 16 * D;
 #pragma unroll
@@ -529,6 +524,70 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
     wsum[wave][lane] = sum;
   }
   if (lane == 0) wseen[wave] = any;
+  if (__any(again)) {
+    int mine = again;
+    mine |= __shfl_xor(mine, 16);
+    mine |= __shfl_xor(mine, 32);
+    again = mine != 0;  // all lanes of the head
+    // Such heads' keys once more, one after the other in f32. The reference is the
+    // maximum, subtracted before the scale, and an infinity or NaN among the values
+    // counts however small its key's weight is (the two parts of a weight would
+    // not do: the lesser one may be zero or negative). Lane: head m, a quarter of D.
+    constexpr int kPieces = D / 32;
+    const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1] + j * (D / 4));
+    float acc[D / 4], r = lowest_ref(sc.c), l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 4; ++d) acc[d] = 0.0f;
+#pragma unroll 1
+    for (int n = (first + wave) * kKeys; n < min(last * kKeys, seen.n);
+         n += (n + 1) % kKeys ? 1 : 1 + (kDecWaves - 1) * kKeys) {
+      const int32_t key = n < seen.sinks ? n : n + seen.skip, pg = table[key >> a.p.page_shift];
+      if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
+      const int64_t row = key & a.p.page_mask;
+      const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
+      const char* vp = a.p.v + 2 * (hk * a.p.vst[2] + pg * a.p.vst[0] + row * a.p.vst[1] + j * (D / 4));
+      float x = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + 16 * c), qw = *reinterpret_cast<const u32x4*>(qp + 16 * c);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t qq = (qw[w] & sc.keep) ^ sc.flip;
+          x = fmaf(T::hi(kw[w]), T::hi(qq), fmaf(T::lo(kw[w]), T::lo(qq), x));
+        }
+      }
+      x += __shfl_xor(x, 16);
+      x += __shfl_xor(x, 32);
+      if constexpr (CAP) x = cap_tanh<CAP>(x * sc.inner);
+      if (x > r) {
+        const float f = lesser((r - x) * sc.c);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < D / 4; ++d) acc[d] *= f;
+        r = x;
+      }
+      const float w = __builtin_amdgcn_exp2f(fmaf(x - r, sc.c, Mx<T>::kDecBias));
+      const float odd = x == -INFINITY ? w : fmaxf(w, 1.0e-44f);
+      l += w;
+#pragma unroll
+      for (int c = 0; c < kPieces; ++c) {
+        const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + 16 * c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = e & 1 ? T::hi(vw[e / 2]) : T::lo(vw[e / 2]);
+          acc[8 * c + e] = fmaf(v, fabsf(v) < INFINITY ? w : odd, acc[8 * c + e]);
+        }
+      }
+    }
+    if (again) {
+#pragma unroll
+      for (int d = 0; d < D / 4; ++d) wo[m * D + j * (D / 4) + d] = acc[d];
+      if (j == 0) {
+        wref[wave][m] = r;
+        wsum[wave][m] = l;
+      }
+    }
+  }
   __syncthreads();
   bool some = false;
   for (int w = 0; w < kDecWaves; ++w) some |= wseen[w] != 0;
@@ -540,7 +599,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
     for (int w = 1; w < kDecWaves; ++w) top = fmaxf(top, wref[w][h]);
     float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
     for (int w = 0; w < kDecWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f((wref[w][h] - top) * sc.c);
+      const float f = lesser((wref[w][h] - top) * sc.c);
       const float* src = reinterpret_cast<float*>(lds) + (w * 16 + h) * D + d;
       l = fmaf(wsum[w][h], f, l);
       v0 = fmaf(src[0], f, v0);
@@ -637,7 +696,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
       const int64_t at = slot(b);
       const f32x2 st = stat[at];
       const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * c);
-      const float f = st[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[0] - top);
+      const float f = st[0] == -INFINITY ? 0.0f : lesser(st[0] - top);
       l = fmaf(st[1], f, l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
@@ -687,7 +746,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t row
     for (int i = g; i < a.splits; i += G) {
       const f32x2 st = stat[i];
       if (st[0] == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f(st[0] - top);
+      const float f = lesser(st[0] - top);
       const f32x4 x = *reinterpret_cast<const f32x4*>(part + (int64_t)i * D);
       l = fmaf(st[1], f, l);
 #pragma unroll
@@ -762,11 +821,13 @@ template <int D> __device__ inline int key_piece(int r, int c) {
 // kv head's query head r % group, so that all heads of a group, and as many
 // tokens as fit, read a tile of keys once.
 //
-// A non-finite value in a tile that some row sees only in part: a weight of
-// zero times infinity would be NaN. Such a tile's values are counted on the
-// matrix cores (+inf as 1, -inf as 128, NaN as 16384, times 1 where the row
-// sees the key: at most 64 keys a tile, so the sum gives the three counts
-// back), and the product runs with zeros in their place.
+// A non-finite value in a tile that some row sees only in part, or of a key whose
+// weight is too small for the type: a weight of zero times infinity would be
+// NaN. Such a tile's values are counted on the matrix cores (+inf as 1, -inf as
+// 128, NaN as 16384, times 1 where the row sees the key: at most 64 keys a tile,
+// so the sum gives the three counts back), and the product runs with zeros in
+// their place. Tiles that all rows see whole are looked at only when a block's
+// sums have turned out not finite.
 template <class M>
 __device__ inline uint32_t finite_pair(uint32_t w) {
   uint32_t m = 0;
@@ -809,7 +870,8 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   static_assert(BN == 64 && BN * CH % NT == 0, "two tiles of 32 keys, whole units per thread");
   typedef Mx<T> M;
   __shared__ __align__(1024) char lds[4 * kTile];  // two tiles of keys, two of values
-  __shared__ int odd;  // 1 + index of the last tile found to hold values that are not finite
+  __shared__ int odd;   // 1 + index of the last tile found to hold values that are not finite
+  __shared__ int redo;  // a row's sums are not finite
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1015,7 +1077,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     if (moved) {  // a row's own scores alone decide for it
       top = halves_max(top);
       const float to = top > ref + slack ? top : ref;
-      shrunk = shrink(ref, to, sc.c);
+      shrunk = lesser((ref - to) * sc.c);
       sum *= shrunk;
       ref = to;
     }
@@ -1049,6 +1111,36 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     add[i & 3] = M::add_pair(pair, i < 4 ? 0.0f : add[i & 3]);
     return pair;
   };
+  // Sums of what is not finite among a tile's values 32 t .. 32 t + 31 that the
+  // lane's row sees (`see`): zero, an infinity or NaN.
+  auto odd_sum = [&](int slot, int t, uint64_t see) {
+    // constants of this path, kept out of the loop's registers
+    uint32_t one = M::kOne, c128 = M::k128, c16384 = M::k16384, inf = 0x7f800000u;
+    asm volatile("" : "+s"(one), "+s"(c128), "+s"(c16384), "+s"(inf));
+    auto code = [&](uint32_t h) {
+      const uint32_t e = h & M::kExp, f = h & 0x7fffu & ~M::kExp;
+      return e != M::kExp ? 0u : f ? c16384 : h & 0x8000u ? c128 : one;
+    };
+    f32x16 n = f32x16{};
+#pragma unroll 1
+    for (int k = 0; k < 2 * KT; ++k) {
+      const u32x4 v = value_frag(slot, t, k);
+      u32x4 c, on;
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = (uint32_t)(see >> (16 * k + 8 * (i / 2) + 2 * (i & 1)));
+        c[i] = code(v[i] & 0xffffu) | code(v[i] >> 16) << 16;
+        on[i] = (two & 1 ? one : 0u) | (two & 2 ? one << 16 : 0u);
+      }
+      n = M::mma32x16(c, on, n);
+    }
+    f32x16 f;
+    for (int e = 0; e < 16; ++e) {
+      const int counts = (int)n[e], nan = counts >> 14, neg = (counts >> 7) & 127, pos = counts & 127;
+      const uint32_t bits = nan || (neg && pos) ? inf | 0x400000u : neg ? inf | 0x80000000u : pos ? inf : 0u;
+      f[e] = u2f(bits);
+    }
+    return f;
+  };
   // values of tile `it` that are not finite, where some row sees only part of the tile
   auto odd_values = [&](int it, int slot, uint64_t exist, bool all) {
     const int key0 = tile_of(it) * BN;
@@ -1063,34 +1155,10 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     if (bits) odd = it + 1;
     __syncthreads();
     if (odd != it + 1) return;
-    // constants of this path, kept out of the loop's registers
-    uint32_t one = M::kOne, c128 = M::k128, c16384 = M::k16384, inf = 0x7f800000u;
-    asm volatile("" : "+s"(one), "+s"(c128), "+s"(c16384), "+s"(inf));
-    auto code = [&](uint32_t h) {
-      const uint32_t e = h & M::kExp, f = h & 0x7fffu & ~M::kExp;
-      return e != M::kExp ? 0u : f ? c16384 : h & 0x8000u ? c128 : one;
-    };
     const uint64_t see = seen_keys(key0, exist) >> (4 * half);
 #pragma unroll 1
     for (int t = 0; t < DT; ++t) {
-      f32x16 n = f32x16{};
-#pragma unroll 1
-      for (int k = 0; k < 2 * KT; ++k) {
-        const u32x4 v = value_frag(slot, t, k);
-        u32x4 c, on;
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t two = (uint32_t)(see >> (16 * k + 8 * (i / 2) + 2 * (i & 1)));
-          c[i] = code(v[i] & 0xffffu) | code(v[i] >> 16) << 16;
-          on[i] = (two & 1 ? one : 0u) | (two & 2 ? one << 16 : 0u);
-        }
-        n = M::mma32x16(c, on, n);
-      }
-      f32x16 f;
-      for (int e = 0; e < 16; ++e) {
-        const int counts = (int)n[e], nan = counts >> 14, neg = (counts >> 7) & 127, pos = counts & 127;
-        const uint32_t bits = nan || (neg && pos) ? inf | 0x400000u : neg ? inf | 0x80000000u : pos ? inf : 0u;
-        f[e] = u2f(bits);
-      }
+      const f32x16 f = odd_sum(slot, t, see);
 #pragma unroll
       for (int u = 0; u < DT; ++u)
         if (u == t) o[u] += f;
@@ -1146,7 +1214,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     sum += (add[0] + add[1]) + (add[2] + add[3]);
   };
 
-  if (threadIdx.x == 0) odd = 0;
+  if (threadIdx.x == 0) odd = redo = 0;
   if (it0 < it1) {
     // pages of the tiles it, it + 1 and it + 2, and which keys of it - 1 and it exist
     int32_t page0 = look_up(it0), page1 = look_up(it0 + 1), next = look_up(it0 + 2);
@@ -1224,36 +1292,86 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   }
   sum = halves_sum(sum);
   any = halves_sum(any ? 1.0f : 0.0f) != 0.0f;
-  if (a.splits > 1) {
-    const int64_t at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.y;
-    if (!in) return;
-    if (half == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * at) = f32x2{any ? ref * sc.c : -INFINITY, sum};
-    if (!any) return;
-    float* dst = a.part + at * D + 4 * half;
+  // Sums that are not finite though the row's weights are: its values are not.
+  bool bad;
+  {
+    float peak[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        *reinterpret_cast<f32x4*>(dst + 32 * t + 2 * e) = f32x4{o[t][e], o[t][e + 1], o[t][e + 2], o[t][e + 3]};
-    return;
-  }
-  // a lane has 4 of every 8 values of its row: the halves trade, for 16-byte stores
-  const float r = any ? 1.0f / sum : 0.0f;
-  char* dst = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1] + 8 * half);
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int e = 0; e < 16; e += 8) {
-      u32x4 v;
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t b0 = T::pack(o[t][e + 2 * i] * r, o[t][e + 2 * i + 1] * r);
-        const uint32_t b1 = T::pack(o[t][e + 4 + 2 * i] * r, o[t][e + 5 + 2 * i] * r);
-        const auto x = __builtin_amdgcn_permlane32_swap(b0, b1, false, false);
-        v[i] = x[0];
-        v[2 + i] = x[1];
+      for (int e = 0; e < 16; e += 4) {
+        peak[0] = peak3(peak[0], o[t][e], o[t][e + 1]);
+        peak[1] = peak3(peak[1], o[t][e + 2], o[t][e + 3]);
       }
-      if (in) *reinterpret_cast<u32x4*>(dst + 64 * t + 4 * e) = v;
+    bad = !(peak[0] < INFINITY && peak[1] < INFINITY) && sum > 0.0f && sum < INFINITY;
+  }
+  auto tell = [&]() {  // the block, whether a row is bad; without a wait for stores
+    if (bad) redo = 1;
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  // (in front of the stores 168 registers do for rows of 64, a third block a CU;
+  // rows of 256 would move 32 of their sums to memory)
+  if constexpr (D < 256) tell();
+  const int64_t part_at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.y;
+  char* out_row = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1]);
+  if (a.splits > 1) {
+    if (in && half == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * part_at) = f32x2{any ? ref * sc.c : -INFINITY, sum};
+    if (in && any) {
+      float* dst = a.part + part_at * D + 4 * half;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<f32x4*>(dst + 32 * t + 2 * e) = f32x4{o[t][e], o[t][e + 1], o[t][e + 2], o[t][e + 3]};
     }
+  } else {
+    // a lane has 4 of every 8 values of its row: the halves trade, for 16-byte stores
+    const float r = any ? 1.0f / sum : 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; e += 8) {
+        u32x4 v;
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t b0 = T::pack(o[t][e + 2 * i] * r, o[t][e + 2 * i + 1] * r);
+          const uint32_t b1 = T::pack(o[t][e + 4 + 2 * i] * r, o[t][e + 5 + 2 * i] * r);
+          const auto x = __builtin_amdgcn_permlane32_swap(b0, b1, false, false);
+          v[i] = x[0];
+          v[2 + i] = x[1];
+        }
+        if (in) *reinterpret_cast<u32x4*>(out_row + 16 * half + 64 * t + 4 * e) = v;
+      }
+  }
+
+  // Rows over values that are not finite, of which a weight may have been rounded
+  // to zero: every column that holds such a value among the keys that the row sees
+  // is written again, from the counts of every tile.
+  if constexpr (D == 256) tell();
+  if (!redo) return;
+#pragma unroll 1
+  for (int t = 0; t < DT; ++t) {
+    f32x16 f = f32x16{};
+#pragma unroll 1
+    for (int it = it0; it < it1; ++it) {
+      const int32_t page = checked(look_up(it));
+      const uint64_t exist = __ballot(page >= 0);
+      load_values(it, 0, page);
+      landed_barrier();
+      f += odd_sum(0, t, seen_keys(tile_of(it) * BN, exist) >> (4 * half));
+      __syncthreads();
+    }
+    if (!bad || !in) continue;
+#pragma unroll 1
+    for (int e = 0; e < 16; e += 4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = e == 0 ? f[i] : e == 4 ? f[4 + i] : e == 8 ? f[8 + i] : f[12 + i];
+        const int d = 32 * t + 2 * e + 4 * half + i;
+        if (x == 0.0f) continue;
+        if (a.splits > 1) a.part[part_at * D + d] = x;
+        else *reinterpret_cast<uint16_t*>(out_row + 2 * d) = (uint16_t)T::pack(x, x);
+      }
+  }
 }
 
 // Sizes shared by the call and its workspace query.

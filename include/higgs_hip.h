@@ -521,9 +521,12 @@ int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers, const int64_t l
  *   out = sum_j softmax(s)_j v_j over the keys j that the query at position p
  * sees: j <= p, and with window > 0 either j > p - window or j < sinks (the
  * last `window` keys and the first `sinks`). A soft cap above 1e30 counts as
- * 1e30. A query that sees no key gives a
- * row of zeros; keys and values that a query does not see, infinities and NaN
- * among them, do not touch its row. Rows of no sequence are left as they are.
+ * 1e30. A query that sees no key gives a row of zeros; keys and values that a
+ * query does not see, infinities and NaN among them, do not touch its row. Of
+ * the values that it sees, one infinity in a column makes the row's value that
+ * infinity, infinities of both signs or a NaN make it NaN, and the other columns
+ * are what they were. (Finite bf16 values above 1e30 may overflow a row's f32
+ * sums.) Rows of no sequence are left as they are.
  * out must not overlap the other operands, nor its rows each other; tokens * q_heads
  * is at most 2^30.
  * Sums and softmax statistics are f32; the probabilities are rounded to the

@@ -50,3 +50,23 @@ def test_the_highest_score_takes_the_row(dev, heads, kv_heads, head_dim, news, d
                         clear += 1
                         assert torch.equal(row[h, g], v[int(s[h, g].argmax()), h]), (b, i, h, g)
     assert clear > starts[-1] * heads // 2
+
+
+@pytest.mark.parametrize("dtype,size", [(BF16, 1e20), (F16, 6e4), (BF16, float("nan")), (F16, float("inf"))])
+@pytest.mark.parametrize("news", [None, [1, 40, 70]])
+@pytest.mark.parametrize("kw", [{}, {"softcap": 50.0}, {"softcap": 1e4}])
+def test_other_rows_keep_their_bits(dev, news, dtype, size, kw):
+    """One query head (in a prompt, of one token) with such scores beside ordinary ones in a wave."""
+    x = R.make(2, [9, 333, 400], news=news, heads=8, kv_heads=2, head_dim=128, page=16, dtype=dtype)
+    d = R.to(x, dev)
+    if dtype == F16 and size == 6e4:
+        d["k_pages"] *= 500.0
+    plain = R.call(H, d, **kw)
+    t = 1 if news is None else 20
+    d["q"][t, 2] = torch.where(d["q"][t, 2] > 0, size, -size)
+    got = R.call(H, d, **kw)
+    keep = torch.ones(got.shape[:2], dtype=torch.bool, device=dev)
+    keep[t, 2] = False
+    assert torch.equal(got[keep], plain[keep])
+    if size == size and size != float("inf"):
+        assert torch.isfinite(got).all() and not torch.equal(got, plain)
