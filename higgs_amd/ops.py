@@ -663,8 +663,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     batch = _kv_batch(T, block_table, kv_lens, q_starts, dev, what)
     L = lib()
     need = L.hgk_paged_attention_workspace(pool, batch, hq, window, sinks)
-    if need < 0:
-        check(1)
+    if need < 0:  # the call refuses the same sizes, with their status
+        check(L.hgk_paged_attention(pool, batch, None, None, hq, 1.0, 0.0, window, sinks, None, None, None, 0, None))
     # a workspace of the call's own, from the current stream's pool of memory
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
     _kv_call(dev, L.hgk_paged_attention, pool, batch, q.data_ptr(), qs, hq,
