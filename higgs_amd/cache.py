@@ -131,8 +131,8 @@ class PagedKVCache:
         found = self._several(seqs, counts)
         ps, refs, copies, need = self.page_size, {}, [], 0
         for s, n in zip(found, counts):
-            if s.length + n > 2 ** 31 - 1:
-                raise HgkError(1, "PagedKVCache: a sequence of more than 2^31 - 1 tokens")
+            if s.length + n > 2 ** 30:  # what a call's table may hold
+                raise HgkError(1, "PagedKVCache: a sequence of more than 2^30 tokens")
             if n and s.length % ps:
                 last = s.pages[-1]
                 shared = refs.get(last, self._refs[last])

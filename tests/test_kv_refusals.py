@@ -24,3 +24,16 @@ def test_what_is_not_supported_says_so(dtype, head_dim):
     with pytest.raises(HgkError, match="heads") as e:
         H.paged_attention(q, p, p, t, n)
     assert e.value.status == 1
+
+
+def test_a_sequence_ends_where_a_table_does():
+    """2^30 tokens are the most that a call's table holds: no pages are given out beyond."""
+    c = H.PagedKVCache(1, 2 ** 14 + 1, 65536, 1, 64, device="meta")
+    a = c.new()
+    c.extend([a], [2 ** 30 - 5])
+    for n in (6, 2 ** 31):
+        with pytest.raises(HgkError, match="2\\^30"):
+            c.extend([a], [n])
+    assert c.length(a) == 2 ** 30 - 5 and c.free_pages == 1
+    c.extend([a], [5])
+    assert c.length(a) == 2 ** 30
