@@ -120,6 +120,23 @@ struct RowsView {
   int64_t kst[2], vst[2];  // token, head
 };
 
+// Do the key pages lie on the value pages? Of pools with the same strides: they
+// are then one array with an axis of two more.
+bool pools_meet(const KvView& p) {
+  if (!std::equal(p.kst, p.kst + 3, p.vst)) return false;
+  const int64_t apart = p.k < p.v ? p.v - p.k : p.k - p.v;
+  const __int128 span = (__int128)p.kst[0] * (p.n_pages - 1) + (__int128)p.kst[1] * p.page_mask +
+                        (__int128)p.kst[2] * (p.kv_heads - 1) + p.head_dim;
+  if (apart / 2 >= span) return false;  // two arrays
+  const int64_t st[4] = {p.kst[0], p.kst[1], p.kst[2], apart / 2};
+  const int64_t extent[4] = {p.n_pages, (int64_t)p.page_mask + 1, p.kv_heads, 2};
+  return rows_overlap(st, extent, 4, p.head_dim);
+}
+// Values that are the keys, in pages that are the keys' pages: written twice alike.
+bool same_rows(const KvView& p, const RowsView& x) {
+  return p.k == p.v && x.k == x.v && x.kst[0] == x.vst[0] && x.kst[1] == x.vst[1];
+}
+
 // Block = `per` tokens. Their places are worked out once, by a thread each (a
 // search of the starts, the length, the table: dependent loads), and kept in
 // LDS; then all threads move the tokens' 2 * Hk * D/8 16-byte units, keys and
@@ -239,6 +256,8 @@ extern "C" int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batc
     return st;
   if (int st = kv_check_rows("hgk_kv_append", "v", v, v_strides, b.tokens, p.kv_heads, p.head_dim, false, x.vst))
     return st;
+  if (pools_meet(p) && !same_rows(p, x))
+    return fail(HGK_ERR_ARG, "hgk_kv_append: the key pages and the value pages overlap");
   const uint32_t chunks = p.head_dim / 8;
   const int64_t units = 2 * (int64_t)p.kv_heads * chunks;
   if (units > INT32_MAX / kMaxTokens) return fail(HGK_ERR_ARG, "hgk_kv_append: too many kv heads");

@@ -591,7 +591,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     int32 [B] counts its tokens with the new ones, which are its last. Sequence
     b owns rows q_starts[b] .. q_starts[b+1]-1 of k and v (int32 [B+1]);
     without q_starts, row b is its one new token. Rows of no sequence,
-    positions beyond the table and pages outside the pool are skipped."""
+    positions beyond the table and pages outside the pool are skipped. The key
+    pages may not lie on the value pages, unless k is v and they are the same."""
     what = "kv_append"
     pool = _pool(k_pages, v_pages, what)
     ks, vs = _token_rows(k, k_pages, what, "k"), _token_rows(v, k_pages, what, "v")

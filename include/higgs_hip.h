@@ -496,7 +496,8 @@ typedef struct {
  * Writes the new tokens' keys and values, k and v [tokens, kv_heads, head_dim]
  * (strides: token, head), to their places in the pages. Rows of no sequence,
  * positions below zero or beyond the table, and pages outside the pool are
- * skipped. No two sequences of a call may write to the same place.
+ * skipped. No two sequences of a call may write to the same place, and the
+ * key pages may not lie on the value pages (but for keys that are the values).
  */
 int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batch, const void* k,
                   const int64_t k_strides[2], const void* v, const int64_t v_strides[2],
