@@ -33,8 +33,10 @@ CFLAGS = [
     "-Wall", "-Wno-unused-function", "-Wno-unknown-pragmas",
 ]
 # Flags of single files. attn.hip: matrix instructions keep their sums in plain
-# vector registers also where a wave has all 512; otherwise rows of 256 values
-# move every sum between the two halves of the register file for every tile.
+# vector registers also where a wave has all 512. Prompts of 256 values a row
+# move fewer of them between the two halves of the register file so (8191 tokens
+# in a window with a soft cap: 575 us, without the flag 652; two prompts of 4096:
+# 352, 373); the other kernels take the same time either way.
 FILE_FLAGS = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 

@@ -301,7 +301,7 @@ __device__ inline int64_t decode_share(int64_t total, int blocks) {
 // bf16 and 22 in f16, well below the result's own rounding.
 //
 // Bound by the reading of the cache. 64 ragged sequences of up to 32768 tokens,
-// 16/2 heads of 256 bf16 (2.2 GB): 395 us with the join, 5.5 TB/s, where a
+// 16/2 heads of 256 bf16 (2.2 GB): 392 us with the join, 5.5 TB/s, where a
 // streaming read reaches 6.1; a block per (pair, fixed part) took 527 us, its
 // longest pair last. One sequence of 131071, 32/8 heads of 128: 107 us, 5.0
 // TB/s. One of 127: 11 us, a launch and a chain of dependent loads.
@@ -858,7 +858,7 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 // that clocks lower: up to 410). With two waves a SIMD the matrix units work 42
 // % of the time and the vector units 49 (a score takes a multiply-add, an exp
 // and half a conversion), each wave's own step one after the other. 8191 tokens
-// in a window of 4096, soft cap, 16/8 heads of 256 (412 GFLOP): 582 to 640 us;
+// in a window of 4096, soft cap, 16/8 heads of 256 (412 GFLOP): 575 to 582 us;
 // registers allow one wave a SIMD there, and the tile's load instructions and
 // its barrier stand beside the step. Deeper rings of tiles, 256 rows a block
 // and loads spread over the step were no faster.
@@ -1007,7 +1007,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   // A lane's places in a tile of keys (row col, piece 2 i + half) and of values
   // (row 4 half + (lane % 16) / 4, 8-byte pieces, read transposed). Rows are
   // whole multiples of 64 bytes (D = 96: 192) and the places differ by an
-  // exclusive or, so one address register serves all pieces.
+  // exclusive or: every piece's address is one register's, xor a constant.
   const int vr = 4 * half + (lane & 15) / 4, vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
   const uint32_t kat = col * kRow + 16 * key_place<D>(col, half);
   const uint32_t vat = vr * kRow + 16 * value_place<D>(vr, vc) + 8 * (lane & 1);

@@ -88,3 +88,20 @@ def test_values_in_pages_that_no_row_sees_stay_out(dev):
     plant(x, [(0, 3, 0, 0, INF), (0, 60, 0, 1, INF), (1, 89, 1, 2, -INF)])  # the places behind the lengths are NaN
     compare(dev, x)
     compare(dev, x, window=20)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("head_dim,dtype", [(64, BF16), (96, F16), (128, F16), (256, BF16)])
+def test_a_single_token_keeps_its_bits_beside_what_it_does_not_see(dev, bad, head_dim, dtype):
+    """Keys and values in front of the window, and another sequence's."""
+    x = R.make(5, [333, 90, 5000], heads=8, kv_heads=2, head_dim=head_dim, page=16, dtype=dtype)
+    kw = {"window": 200, "sinks": 3}
+    clean = R.call(H, R.to(x, dev), **kw).cpu()
+    for pool in ("k_pages", "v_pages"):
+        y = dict(x)
+        y[pool] = x[pool].clone()
+        for b, j in ((0, 3), (0, 100), (0, 132), (1, 60), (2, 4799)):
+            y[pool][int(x["table"][b, j // 16]), j % 16, :, 5] = bad
+        got = R.call(H, R.to(y, dev), **kw).cpu()
+        assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2]), pool
+        assert not torch.isfinite(got[1]).all()
