@@ -343,291 +343,292 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   of_seen = seen_by_last(a, a.b.lens[of_seq]);
   of_tiles = decode_tiles<kKeys>(of_seen);
   for (bool head_of_run = true;; head_of_run = false) {
-  // this pair, and the tiles of it that fall to this block
-  const int seq = __builtin_amdgcn_readfirstlane(of_seq), tiles = __builtin_amdgcn_readfirstlane(of_tiles);
-  const Seen seen{__builtin_amdgcn_readfirstlane(of_seen.n), __builtin_amdgcn_readfirstlane(of_seen.sinks),
-                  __builtin_amdgcn_readfirstlane(of_seen.skip)};
-  int hk, first, last;
-  if (a.splits > 1) {
-    hk = (int)((at_tile - before) / tiles);
-    first = (int)(at_tile - before - (int64_t)hk * tiles);
-    last = (int)min((int64_t)tiles, first + end_tile - at_tile);
-  } else {
-    hk = blockIdx.x - seq * a.p.kv_heads;
-    first = 0;
-    last = tiles;
-  }
-  hk = __builtin_amdgcn_readfirstlane(hk);
-  first = __builtin_amdgcn_readfirstlane(first);
-  last = __builtin_amdgcn_readfirstlane(last);
-  const bool whole = first == 0 && last == tiles;
-  const int h0 = hk * a.group + blockIdx.y * 16;  // first of this block's heads
-
-  u32x4 qf[kStep];
-  {
-    const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1] + 8 * j);
-#pragma unroll
-    for (int s = 0; s < kStep; ++s) {
-      qf[s] = *reinterpret_cast<const u32x4*>(qp + 64 * s);
-      for (int w = 0; w < 4; ++w) qf[s][w] = (qf[s][w] & sc.keep) ^ sc.flip;
+    // this pair, and the tiles of it that fall to this block
+    const int seq = __builtin_amdgcn_readfirstlane(of_seq), tiles = __builtin_amdgcn_readfirstlane(of_tiles);
+    const Seen seen{__builtin_amdgcn_readfirstlane(of_seen.n), __builtin_amdgcn_readfirstlane(of_seen.sinks),
+                    __builtin_amdgcn_readfirstlane(of_seen.skip)};
+    int hk, first, last;
+    if (a.splits > 1) {
+      hk = (int)((at_tile - before) / tiles);
+      first = (int)(at_tile - before - (int64_t)hk * tiles);
+      last = (int)min((int64_t)tiles, first + end_tile - at_tile);
+    } else {
+      hk = blockIdx.x - seq * a.p.kv_heads;
+      first = 0;
+      last = tiles;
     }
-  }
+    hk = __builtin_amdgcn_readfirstlane(hk);
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
+    const bool whole = first == 0 && last == tiles;
+    const int h0 = hk * a.group + blockIdx.y * 16;  // first of this block's heads
 
-  const int32_t* table = a.b.table + (int64_t)seq * a.b.table_stride;
-  const char* kbase = a.p.k + 2 * (hk * a.p.kst[2] + 8 * j);
-  const char* vbase = a.p.v + 2 * (hk * a.p.vst[2] + 8 * j);
-  // page of key i of the run (-1: none) and its place in the page
-  auto look_up = [&](int tile, int32_t* page, int32_t* at) {
+    u32x4 qf[kStep];
+    {
+      const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1] + 8 * j);
 #pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      const int i = tile * kKeys + 16 * h + m;
-      page[h] = -1;
-      at[h] = 0;
-      if (tile < last && i < seen.n) {
-        const int32_t key = i < seen.sinks ? i : i + seen.skip;
-        page[h] = table[key >> a.p.page_shift];
-        at[h] = key & a.p.page_mask;
+      for (int s = 0; s < kStep; ++s) {
+        qf[s] = *reinterpret_cast<const u32x4*>(qp + 64 * s);
+        for (int w = 0; w < 4; ++w) qf[s][w] = (qf[s][w] & sc.keep) ^ sc.flip;
       }
     }
-  };
-  u32x4 kr[NS][kStep], vr[NS][kStep];
-  uint32_t there = 0;  // bit i: key i of the loaded tile exists
-  auto load = [&](const int32_t* page, const int32_t* at) {
-    there = 0;
-#pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      const bool ok = (uint32_t)page[h] < (uint32_t)a.p.n_pages;
-      there |= (uint32_t)(__ballot(ok) & 0xffffu) << (16 * h);
-      // a key that does not exist reads the pool's first row, and is masked below
-      const int64_t pg = ok ? page[h] : 0, r = ok ? at[h] : 0;
-      const char* kp = kbase + 2 * (pg * a.p.kst[0] + r * a.p.kst[1]);
-      const char* vp = vbase + 2 * (pg * a.p.vst[0] + r * a.p.vst[1]);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) kr[h][s] = *reinterpret_cast<const u32x4*>(kp + 64 * s);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) vr[h][s] = *reinterpret_cast<const u32x4*>(vp + 64 * s);
-    }
-  };
 
-  f32x4 o[kOut];
-#pragma unroll
-  for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
-  float ref = lowest_ref(sc.c), sum = 0.0f;
-  const float slack = Mx<T>::kDecSlack / sc.c;
-  bool any = false;
-  constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
-  char* vt = lds + wave * kTile;
-
-  int32_t page[NS], at[NS];
-  if (a.p.n_pages > 0 && first + wave < last) {
-    look_up(first + wave, page, at);
-    load(page, at);
-    look_up(first + wave + kDecWaves, page, at);
-    for (int tile = first + wave; tile < last; tile += kDecWaves) {
-      // scores
-      f32x4 s[NS];
+    const int32_t* table = a.b.table + (int64_t)seq * a.b.table_stride;
+    const char* kbase = a.p.k + 2 * (hk * a.p.kst[2] + 8 * j);
+    const char* vbase = a.p.v + 2 * (hk * a.p.vst[2] + 8 * j);
+    // page of key i of the run (-1: none) and its place in the page
+    auto look_up = [&](int tile, int32_t* page, int32_t* at) {
 #pragma unroll
       for (int h = 0; h < NS; ++h) {
-        s[h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
+        const int i = tile * kKeys + 16 * h + m;
+        page[h] = -1;
+        at[h] = 0;
+        if (tile < last && i < seen.n) {
+          const int32_t key = i < seen.sinks ? i : i + seen.skip;
+          page[h] = table[key >> a.p.page_shift];
+          at[h] = key & a.p.page_mask;
+        }
       }
-      const uint32_t now = there;
-      if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
+    };
+    u32x4 kr[NS][kStep], vr[NS][kStep];
+    uint32_t there = 0;  // bit i: key i of the loaded tile exists
+    auto load = [&](const int32_t* page, const int32_t* at) {
+      there = 0;
+#pragma unroll
+      for (int h = 0; h < NS; ++h) {
+        const bool ok = (uint32_t)page[h] < (uint32_t)a.p.n_pages;
+        there |= (uint32_t)(__ballot(ok) & 0xffffu) << (16 * h);
+        // a key that does not exist reads the pool's first row, and is masked below
+        const int64_t pg = ok ? page[h] : 0, r = ok ? at[h] : 0;
+        const char* kp = kbase + 2 * (pg * a.p.kst[0] + r * a.p.kst[1]);
+        const char* vp = vbase + 2 * (pg * a.p.vst[0] + r * a.p.vst[1]);
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) kr[h][s] = *reinterpret_cast<const u32x4*>(kp + 64 * s);
+#pragma unroll
+        for (int s = 0; s < kStep; ++s) vr[h][s] = *reinterpret_cast<const u32x4*>(vp + 64 * s);
+      }
+    };
+
+    f32x4 o[kOut];
+#pragma unroll
+    for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
+    float ref = lowest_ref(sc.c), sum = 0.0f;
+    const float slack = Mx<T>::kDecSlack / sc.c;
+    bool any = false;
+    constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
+    char* vt = lds + wave * kTile;
+
+    int32_t page[NS], at[NS];
+    if (a.p.n_pages > 0 && first + wave < last) {
+      look_up(first + wave, page, at);
+      load(page, at);
+      look_up(first + wave + kDecWaves, page, at);
+      for (int tile = first + wave; tile < last; tile += kDecWaves) {
+        // scores
+        f32x4 s[NS];
+#pragma unroll
+        for (int h = 0; h < NS; ++h) {
+          s[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
+        }
+        const uint32_t now = there;
+        if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
+#pragma unroll
+          for (int h = 0; h < NS; ++h)
+            if (!((now >> (16 * h + m)) & 1))
+#pragma unroll
+              for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
+        }
 #pragma unroll
         for (int h = 0; h < NS; ++h)
-          if (!((now >> (16 * h + m)) & 1))
 #pragma unroll
-            for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int h = 0; h < NS; ++h)
-#pragma unroll
-        for (int k = 0; k < kStep; ++k)
-          *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
-      if (tile + kDecWaves < last) {
-        load(page, at);
-        look_up(tile + 2 * kDecWaves, page, at);
-      }
-      // weights
-      float x[4 * NS], top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) {
-        x[i] = s[i / 4][i % 4];
-        if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
-      }
-      const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
-      if (now != kAll) {
-#pragma unroll
-        for (int i = 0; i < 4 * NS; ++i)
-          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
-      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = top > ref + slack ? top : ref, f = lesser((ref - to) * sc.c);
-        sum *= f;
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) o[t] *= f;
-        ref = to;
-      }
-      const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
-      any |= now != 0;
-      uint32_t hi[2 * NS], lo[2 * NS];
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) {
-        sum += x[2 * i] + x[2 * i + 1];
-        hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
-        lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
-      }
-      // O^T += V^T P^T
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int t = 0; t < kOut; ++t) {
-        const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
-        const u32x2 v0 = lds_transposed(p);
-        if constexpr (NS == 2) {
-          const u32x2 v1 = lds_transposed(p + 16 * kRow);
-          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-          o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
-          o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
-        } else {
-          o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
-          o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
+          for (int k = 0; k < kStep; ++k)
+            *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
+        if (tile + kDecWaves < last) {
+          load(page, at);
+          look_up(tile + 2 * kDecWaves, page, at);
         }
+        // weights
+        float x[4 * NS], top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i) {
+          x[i] = s[i / 4][i % 4];
+          if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
+        }
+        const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
+        if (now != kAll) {
+#pragma unroll
+          for (int i = 0; i < 4 * NS; ++i)
+            if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
+        if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
+          top = fmaxf(top, __shfl_xor(top, 16));
+          top = fmaxf(top, __shfl_xor(top, 32));
+          const float to = top > ref + slack ? top : ref, f = lesser((ref - to) * sc.c);
+          sum *= f;
+#pragma unroll
+          for (int t = 0; t < kOut; ++t) o[t] *= f;
+          ref = to;
+        }
+        const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
+        any |= now != 0;
+        uint32_t hi[2 * NS], lo[2 * NS];
+#pragma unroll
+        for (int i = 0; i < 2 * NS; ++i) {
+          sum += x[2 * i] + x[2 * i + 1];
+          hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
+          lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
+        }
+        // O^T += V^T P^T
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < kOut; ++t) {
+          const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
+          const u32x2 v0 = lds_transposed(p);
+          if constexpr (NS == 2) {
+            const u32x2 v1 = lds_transposed(p + 16 * kRow);
+            const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
+            o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
+            o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
+          } else {
+            o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
+            o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_wave_barrier();
     }
-  }
 
-  // join the waves
-  sum += __shfl_xor(sum, 16);
-  sum += __shfl_xor(sum, 32);
-  // Did this head's scores fit the weights' form, and are its sums finite?
-  bool again;
-  {
-    float peak = sum;
+    // join the waves
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    // Did this head's scores fit the weights' form, and are its sums finite?
+    bool again;
+    {
+      float peak = sum;
 #pragma unroll
-    for (int t = 0; t < kOut; ++t) peak = peak3(peak3(peak, o[t][0], o[t][1]), o[t][2], o[t][3]);
-    again = any && !(fabsf(ref * sc.c) <= kBaseMax && peak < INFINITY);
-  }
-  __syncthreads();  // every wave is done with its V tile
-  float* wo = reinterpret_cast<float*>(lds) + wave * 16 * D;
+      for (int t = 0; t < kOut; ++t) peak = peak3(peak3(peak, o[t][0], o[t][1]), o[t][2], o[t][3]);
+      again = any && !(fabsf(ref * sc.c) <= kBaseMax && peak < INFINITY);
+    }
+    __syncthreads();  // every wave is done with its V tile
+    float* wo = reinterpret_cast<float*>(lds) + wave * 16 * D;
 #pragma unroll
-  for (int t = 0; t < kOut; ++t) *reinterpret_cast<f32x4*>(wo + m * D + 16 * t + 4 * j) = o[t];
-  if (lane < 16) {
-    wref[wave][lane] = ref;
-    wsum[wave][lane] = sum;
-  }
-  if (lane == 0) wseen[wave] = any;
-  if (__any(again)) {
-    int mine = again;
-    mine |= __shfl_xor(mine, 16);
-    mine |= __shfl_xor(mine, 32);
-    again = mine != 0;  // all lanes of the head
-    // Such heads' keys once more, one after the other in f32. The reference is the
-    // maximum, subtracted before the scale, and an infinity or NaN among the values
-    // counts however small its key's weight is (the two parts of a weight would
-    // not do: the lesser one may be zero or negative). Lane: head m, a quarter of D.
-    constexpr int kPieces = D / 32;
-    const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1] + j * (D / 4));
-    float acc[D / 4], r = lowest_ref(sc.c), l = 0.0f;
+    for (int t = 0; t < kOut; ++t) *reinterpret_cast<f32x4*>(wo + m * D + 16 * t + 4 * j) = o[t];
+    if (lane < 16) {
+      wref[wave][lane] = ref;
+      wsum[wave][lane] = sum;
+    }
+    if (lane == 0) wseen[wave] = any;
+    if (__any(again)) {
+      int mine = again;
+      mine |= __shfl_xor(mine, 16);
+      mine |= __shfl_xor(mine, 32);
+      again = mine != 0;  // all lanes of the head
+      // Such heads' keys once more, one after the other in f32. The reference is the
+      // maximum, subtracted before the scale, and an infinity or NaN among the values
+      // counts however small its key's weight is (the two parts of a weight would
+      // not do: the lesser one may be zero or negative). Lane: head m, a quarter of D.
+      constexpr int kPieces = D / 32;
+      const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1] + j * (D / 4));
+      float acc[D / 4], r = lowest_ref(sc.c), l = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 4; ++d) acc[d] = 0.0f;
+      for (int d = 0; d < D / 4; ++d) acc[d] = 0.0f;
 #pragma unroll 1
-    for (int n = (first + wave) * kKeys; n < min(last * kKeys, seen.n);
-         n += (n + 1) % kKeys ? 1 : 1 + (kDecWaves - 1) * kKeys) {
-      const int32_t key = n < seen.sinks ? n : n + seen.skip, pg = table[key >> a.p.page_shift];
-      if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
-      const int64_t row = key & a.p.page_mask;
-      const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
-      const char* vp = a.p.v + 2 * (hk * a.p.vst[2] + pg * a.p.vst[0] + row * a.p.vst[1] + j * (D / 4));
-      float x = 0.0f;
+      for (int n = (first + wave) * kKeys; n < min(last * kKeys, seen.n);
+           n += (n + 1) % kKeys ? 1 : 1 + (kDecWaves - 1) * kKeys) {
+        const int32_t key = n < seen.sinks ? n : n + seen.skip, pg = table[key >> a.p.page_shift];
+        if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
+        const int64_t row = key & a.p.page_mask;
+        const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
+        const char* vp = a.p.v + 2 * (hk * a.p.vst[2] + pg * a.p.vst[0] + row * a.p.vst[1] + j * (D / 4));
+        float x = 0.0f;
 #pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + 16 * c), qw = *reinterpret_cast<const u32x4*>(qp + 16 * c);
+        for (int c = 0; c < kPieces; ++c) {
+          const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + 16 * c);
+          const u32x4 qw = *reinterpret_cast<const u32x4*>(qp + 16 * c);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t qq = (qw[w] & sc.keep) ^ sc.flip;
-          x = fmaf(T::hi(kw[w]), T::hi(qq), fmaf(T::lo(kw[w]), T::lo(qq), x));
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t qq = (qw[w] & sc.keep) ^ sc.flip;
+            x = fmaf(T::hi(kw[w]), T::hi(qq), fmaf(T::lo(kw[w]), T::lo(qq), x));
+          }
+        }
+        x += __shfl_xor(x, 16);
+        x += __shfl_xor(x, 32);
+        if constexpr (CAP) x = cap_tanh<CAP>(x * sc.inner);
+        if (x > r) {
+          const float f = lesser((r - x) * sc.c);
+          l *= f;
+#pragma unroll
+          for (int d = 0; d < D / 4; ++d) acc[d] *= f;
+          r = x;
+        }
+        const float w = __builtin_amdgcn_exp2f(fmaf(x - r, sc.c, Mx<T>::kDecBias));
+        const float odd = x == -INFINITY ? w : fmaxf(w, 1.0e-44f);
+        l += w;
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+          const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + 16 * c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float v = e & 1 ? T::hi(vw[e / 2]) : T::lo(vw[e / 2]);
+            acc[8 * c + e] = fmaf(v, fabsf(v) < INFINITY ? w : odd, acc[8 * c + e]);
+          }
         }
       }
-      x += __shfl_xor(x, 16);
-      x += __shfl_xor(x, 32);
-      if constexpr (CAP) x = cap_tanh<CAP>(x * sc.inner);
-      if (x > r) {
-        const float f = lesser((r - x) * sc.c);
-        l *= f;
+      if (again) {
 #pragma unroll
-        for (int d = 0; d < D / 4; ++d) acc[d] *= f;
-        r = x;
-      }
-      const float w = __builtin_amdgcn_exp2f(fmaf(x - r, sc.c, Mx<T>::kDecBias));
-      const float odd = x == -INFINITY ? w : fmaxf(w, 1.0e-44f);
-      l += w;
-#pragma unroll
-      for (int c = 0; c < kPieces; ++c) {
-        const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + 16 * c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = e & 1 ? T::hi(vw[e / 2]) : T::lo(vw[e / 2]);
-          acc[8 * c + e] = fmaf(v, fabsf(v) < INFINITY ? w : odd, acc[8 * c + e]);
+        for (int d = 0; d < D / 4; ++d) wo[m * D + j * (D / 4) + d] = acc[d];
+        if (j == 0) {
+          wref[wave][m] = r;
+          wsum[wave][m] = l;
         }
       }
     }
-    if (again) {
-#pragma unroll
-      for (int d = 0; d < D / 4; ++d) wo[m * D + j * (D / 4) + d] = acc[d];
-      if (j == 0) {
-        wref[wave][m] = r;
-        wsum[wave][m] = l;
+    __syncthreads();
+    bool some = false;
+    for (int w = 0; w < kDecWaves; ++w) some |= wseen[w] != 0;
+    // a part of the run's first pair, or of its last
+    const int64_t slot = (((int64_t)blockIdx.y * a.splits + blockIdx.x) * 2 + (head_of_run ? 0 : 1)) * 16;
+    for (int idx = threadIdx.x; idx < heads * (D / 2); idx += 64 * kDecWaves) {
+      const int h = idx / (D / 2), d = 2 * (idx - h * (D / 2));
+      float top = wref[0][h];
+      for (int w = 1; w < kDecWaves; ++w) top = fmaxf(top, wref[w][h]);
+      float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
+      for (int w = 0; w < kDecWaves; ++w) {
+        const float f = lesser((wref[w][h] - top) * sc.c);
+        const float* src = reinterpret_cast<float*>(lds) + (w * 16 + h) * D + d;
+        l = fmaf(wsum[w][h], f, l);
+        v0 = fmaf(src[0], f, v0);
+        v1 = fmaf(src[1], f, v1);
+      }
+      if (whole) {
+        const float r = 1.0f / l;
+        *reinterpret_cast<uint32_t*>(a.out + 2 * (seq * a.ost[0] + (h0 + h) * a.ost[1] + d)) =
+            some ? T::pack(v0 * r, v1 * r) : 0u;
+      } else {
+        *reinterpret_cast<f32x2*>(a.part + (slot + h) * D + d) = f32x2{v0, v1};
+        if (d == 0)
+          *reinterpret_cast<f32x2*>(a.stat + 2 * (slot + h)) = f32x2{some ? top * sc.c : -INFINITY, l};
       }
     }
-  }
-  __syncthreads();
-  bool some = false;
-  for (int w = 0; w < kDecWaves; ++w) some |= wseen[w] != 0;
-  // a part of the run's first pair, or of its last
-  const int64_t slot = (((int64_t)blockIdx.y * a.splits + blockIdx.x) * 2 + (head_of_run ? 0 : 1)) * 16;
-  for (int idx = threadIdx.x; idx < heads * (D / 2); idx += 64 * kDecWaves) {
-    const int h = idx / (D / 2), d = 2 * (idx - h * (D / 2));
-    float top = wref[0][h];
-    for (int w = 1; w < kDecWaves; ++w) top = fmaxf(top, wref[w][h]);
-    float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
-    for (int w = 0; w < kDecWaves; ++w) {
-      const float f = lesser((wref[w][h] - top) * sc.c);
-      const float* src = reinterpret_cast<float*>(lds) + (w * 16 + h) * D + d;
-      l = fmaf(wsum[w][h], f, l);
-      v0 = fmaf(src[0], f, v0);
-      v1 = fmaf(src[1], f, v1);
+    if (a.splits == 1) return;
+    // the run's next pair: the sequence's next head, or the next sequence that sees anything
+    at_tile += last - first;
+    if (at_tile >= end_tile) return;
+    if (at_tile - before >= (int64_t)tiles * a.p.kv_heads) {
+      before = at_tile;
+      do {
+        if (++of_seq >= a.b.batch) return;
+        of_seen = seen_by_last(a, a.b.lens[of_seq]);
+        of_tiles = decode_tiles<kKeys>(of_seen);
+      } while (of_tiles == 0);
     }
-    if (whole) {
-      const float r = 1.0f / l;
-      *reinterpret_cast<uint32_t*>(a.out + 2 * (seq * a.ost[0] + (h0 + h) * a.ost[1] + d)) =
-          some ? T::pack(v0 * r, v1 * r) : 0u;
-    } else {
-      *reinterpret_cast<f32x2*>(a.part + (slot + h) * D + d) = f32x2{v0, v1};
-      if (d == 0)
-        *reinterpret_cast<f32x2*>(a.stat + 2 * (slot + h)) = f32x2{some ? top * sc.c : -INFINITY, l};
-    }
-  }
-  if (a.splits == 1) return;
-  // the run's next pair: the sequence's next head, or the next sequence that sees anything
-  at_tile += last - first;
-  if (at_tile >= end_tile) return;
-  if (at_tile - before >= (int64_t)tiles * a.p.kv_heads) {
-    before = at_tile;
-    do {
-      if (++of_seq >= a.b.batch) return;
-      of_seen = seen_by_last(a, a.b.lens[of_seq]);
-      of_tiles = decode_tiles<kKeys>(of_seen);
-    } while (of_tiles == 0);
-  }
-  __syncthreads();  // the waves' sums are read; V tiles may be written again
+    __syncthreads();  // the waves' sums are read; V tiles may be written again
   }
 }
 
@@ -676,46 +677,46 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   before = (part_before[0] + part_before[1] + part_before[2] + part_before[3]) * a.p.kv_heads;
   const int64_t share = decode_share(total, a.splits);
   for (int h = blockIdx.y; h < a.q_heads; h += gridDim.y) {
-  const int hk = h / a.group, in = h - hk * a.group;
-  const int64_t t0 = before + (int64_t)hk * tiles;
-  const int b0 = (int)(t0 / share), b1 = (int)((t0 + tiles - 1) / share);
-  if (b0 == b1) continue;
-  auto slot = [&](int b) {
-    return (((int64_t)(in >> 4) * a.splits + b) * 2 + (b * share < t0 ? 1 : 0)) * 16 + (in & 15);
-  };
-  const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat);
-  float top = -INFINITY, l = 0.0f;
-  for (int b = b0 + (threadIdx.x & 63); b <= b1; b += 64) top = fmaxf(top, stat[slot(b)][0]);
+    const int hk = h / a.group, in = h - hk * a.group;
+    const int64_t t0 = before + (int64_t)hk * tiles;
+    const int b0 = (int)(t0 / share), b1 = (int)((t0 + tiles - 1) / share);
+    if (b0 == b1) continue;
+    auto slot = [&](int b) {
+      return (((int64_t)(in >> 4) * a.splits + b) * 2 + (b * share < t0 ? 1 : 0)) * 16 + (in & 15);
+    };
+    const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat);
+    float top = -INFINITY, l = 0.0f;
+    for (int b = b0 + (threadIdx.x & 63); b <= b1; b += 64) top = fmaxf(top, stat[slot(b)][0]);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  f32x4 v = {0, 0, 0, 0};
-  __syncthreads();  // the last head's parts are read
-  if (g < kGroups) {
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    f32x4 v = {0, 0, 0, 0};
+    __syncthreads();  // the last head's parts are read
+    if (g < kGroups) {
 #pragma unroll 4
-    for (int b = b0 + g; b <= b1; b += kGroups) {
-      const int64_t at = slot(b);
-      const f32x2 st = stat[at];
-      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * c);
-      const float f = st[0] == -INFINITY ? 0.0f : lesser(st[0] - top);
-      l = fmaf(st[1], f, l);
+      for (int b = b0 + g; b <= b1; b += kGroups) {
+        const int64_t at = slot(b);
+        const f32x2 st = stat[at];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * c);
+        const float f = st[0] == -INFINITY ? 0.0f : lesser(st[0] - top);
+        l = fmaf(st[1], f, l);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+        for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+      }
+      vs[g][c] = v;
+      if (c == 0) ls[g] = l;
     }
-    vs[g][c] = v;
-    if (c == 0) ls[g] = l;
-  }
-  __syncthreads();
-  if (g > 0) continue;
+    __syncthreads();
+    if (g > 0) continue;
 #pragma unroll
-  for (int i = 1; i < kGroups; ++i) {
-    l += ls[i];
+    for (int i = 1; i < kGroups; ++i) {
+      l += ls[i];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += vs[i][c][e];
-  }
-  const float r = 1.0f / l;
-  u32x2 w = {0u, 0u};
-  if (top != -INFINITY) w = u32x2{T::pack(v[0] * r, v[1] * r), T::pack(v[2] * r, v[3] * r)};
-  *reinterpret_cast<u32x2*>(out + 2 * h * a.ost[1]) = w;
+      for (int e = 0; e < 4; ++e) v[e] += vs[i][c][e];
+    }
+    const float r = 1.0f / l;
+    u32x2 w = {0u, 0u};
+    if (top != -INFINITY) w = u32x2{T::pack(v[0] * r, v[1] * r), T::pack(v[2] * r, v[3] * r)};
+    *reinterpret_cast<u32x2*>(out + 2 * h * a.ost[1]) = w;
   }
 }
 
