@@ -854,10 +854,10 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 // K and V tiles come straight from memory to LDS, double buffered: the next
 // tile's loads are issued before a tile is computed, one barrier a tile.
 //
-// 8 sequences of 2048, 32/8 heads of 128 bf16, causal (275 GFLOP): 336 to 346
-// us, 800 to 820 TFLOP/s, where a large library product reaches 1260 (a card
+// 8 sequences of 2048, 32/8 heads of 128 bf16, causal (275 GFLOP): 341 to 352
+// us, 780 to 806 TFLOP/s, where a large library product reaches 1260 (a card
 // that clocks lower: up to 410). With two waves a SIMD the matrix units work 42
-// % of the time and the vector units 49 (a score takes a multiply-add, an exp
+// % of the time and the vector units 50 (a score takes a multiply-add, an exp
 // and half a conversion), each wave's own step one after the other. 8191 tokens
 // in a window of 4096, soft cap, 16/8 heads of 256 (412 GFLOP): 575 to 582 us;
 // registers allow one wave a SIMD there, and the tile's load instructions and
