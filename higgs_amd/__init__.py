@@ -11,5 +11,6 @@ from .cache import PagedKVCache  # noqa: F401
 from .ops import (OpSequence, QuantizedEmbedding, add_rms_norm, gated_rms_norm, gelu_approximate_mul,  # noqa: F401
                   fused_gate_up_swiglu, gather_qmm, gather_qmm_swiglu, gated_delta,
                   gated_delta_gated_norm, gdn_qk_norm_weights,
-                  kv_append, kv_copy_pages, llama3_rope_freqs, paged_attention, qk_norm_rope, quantized_matmul, rms_norm, rope,
-                  rope_inv_freq, silu_mul, swiglu)
+                  kv_append, kv_copy_pages, kv_extend, kv_release, llama3_rope_freqs, moe_combine, moe_route,
+                  paged_attention, qk_norm_rope, quantized_matmul, rms_norm, rope,
+                  rope_inv_freq, shared_prefix_attention, silu_mul, swiglu)

@@ -48,7 +48,16 @@ class HgkKvBatch(C.Structure):
                 ("kv_lens", C.c_void_p), ("q_starts", C.c_void_p)]
 
 
+class HgkKvTables(C.Structure):
+    """hgk_kv_tables of include/higgs_hip.h (resident sequences' tables and the free pages)."""
+    _fields_ = [("page_size", C.c_int), ("rows", C.c_int64), ("tables", C.c_void_p),
+                ("table_stride", C.c_int64), ("table_width", C.c_int64), ("lens", C.c_void_p),
+                ("free_pages", C.c_void_p), ("n_pages", C.c_int64), ("n_free", C.c_void_p)]
+
+
 OP_RMS_NORM, OP_ADD_RMS_NORM, OP_GATED_RMS_NORM, OP_QK_NORM_ROPE, OP_GLU = 0, 1, 2, 3, 4
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+TABLES_PAGES, TABLES_WIDTH, TABLES_SEQUENCE, TABLES_TOKENS = 1, 2, 4, 8
 
 # name -> (restype, argtypes); kept in the order of include/higgs_hip.h
 PROTOTYPES = {
@@ -96,6 +105,16 @@ PROTOTYPES = {
     "hgk_paged_attention": (_int, [_vp, _vp, _vp, _vp, _i64, _f32, _f32, _i64, _i64, _vp, _vp, _vp,
                                    _i64, _vp]),
     "hgk_paged_attention_workspace": (_i64, [_vp, _vp, _i64, _i64, _i64]),
+    "hgk_kv_append_slots": (_int, [_vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "hgk_shared_prefix_attention": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, _f32, _f32, _i64, _i64, _vp,
+                                           _vp, _vp, _i64, _vp]),
+    "hgk_shared_prefix_attention_workspace": (_i64, [_vp, _vp, _i64, _i64, _i64, _i64, _i64]),
+    "hgk_kv_extend": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp]),
+    "hgk_kv_release": (_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "hgk_moe_route": (_int, [_int, _vp, _i64, _vp, _int, _i64, _i64, _i64, _i64, _i64, _int, _int, _f32, _vp, _vp,
+                             _vp]),
+    "hgk_moe_combine": (_int, [_int, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _int, _i64, _vp, _i64, _i64, _i64,
+                               _vp]),
     "hgk_st_open": (_int, [C.c_char_p, C.POINTER(_vp)]),
     "hgk_st_close": (None, [_vp]),
     "hgk_st_count": (_i64, [_vp]),

@@ -29,8 +29,29 @@ struct AttnArgs {
   // [row tiles][splits][2][16].
   int32_t splits;
   float* part;  // [...][head_dim], not normalised
-  float* stat;  // [...][2]: reference (log2 domain), sum
+  float* stat;  // [...][2]: reference (log2 domain; behind a prefix a raw score), sum
+  // A prefix that the sequences share: its pages, which stand for the sequences'
+  // own where key < prefix; and the parts of a row that a pass of its own over those
+  // keys makes (0: there is none, and the sequences' pass takes all keys). That
+  // pass's part i of a row lies at [row][pre_row] + i, and behind them at `pre` the
+  // part of a single token that one block had whole.
+  const int32_t* prefix_table;
+  int32_t prefix_width, prefix, pre, pre_row;
+  float* pre_part;
+  float* pre_stat;
 };
+
+// Which keys a kernel takes of each row: all, of the row's own table; those of the
+// shared prefix, for the rows of all sequences at once; or those behind it (all, if
+// there is no pass over the prefix), with the prefix's table in front of the own one.
+constexpr int kOwn = 0, kPrefix = 1, kBehind = 2;
+
+// The table's entry for a key of a sequence whose first keys are the prefix's.
+__device__ inline int32_t page_behind(const AttnArgs& a, const int32_t* table, int32_t key) {
+  const int32_t e = key >> a.p.page_shift;
+  if (key < a.prefix) return e < a.prefix_width ? a.prefix_table[e] : -1;
+  return e < a.b.width ? table[e] : -1;
+}
 
 // Matrix instructions, pair packing and the non-finite test of the two types.
 template <class T> struct Mx;
@@ -146,6 +167,9 @@ __device__ inline Scale fold_scale(const AttnArgs& a) {
   }
   return s;
 }
+__device__ inline float scale_of(const AttnArgs& a) {
+  return a.softcap > 0.0f ? fold_scale<1>(a).c : fold_scale<0>(a).c;
+}
 
 // tanh from one exp2 and one reciprocal: 1 - 2 / (e^2x + 1). Its absolute
 // error is 2^-22 at the most, so a capped score's is softcap times that.
@@ -208,6 +232,20 @@ __device__ inline float lesser(float e) { return fmaxf(__builtin_amdgcn_exp2f(e)
 struct Seen {
   int32_t n, sinks, skip;
 };
+// ... of those behind the prefix, if a pass of its own takes that: index i is key
+// i + the prefix below `sinks`.
+__device__ inline Seen seen_behind(const AttnArgs& a, int32_t len) {
+  const int32_t from = a.pre > 0 ? a.prefix : 0;
+  const int64_t cap = max((int64_t)a.b.width << a.p.page_shift, (int64_t)a.prefix);
+  if (len < 0) len = 0;
+  const int32_t lo = a.window > 0 && len > a.window ? len - a.window : 0;
+  const int32_t end = (int32_t)min((int64_t)len, cap), at = max(lo, from);
+  Seen s;
+  s.sinks = max(min(min(a.sinks, lo), end) - from, 0);
+  s.skip = at - s.sinks;
+  s.n = s.sinks + max(end - at, 0);
+  return s;
+}
 __device__ inline Seen seen_by_last(const AttnArgs& a, int32_t len) {
   const int64_t cap = (int64_t)a.b.width << a.p.page_shift;
   Seen s;
@@ -221,6 +259,11 @@ __device__ inline Seen seen_by_last(const AttnArgs& a, int32_t len) {
   }
   s.n = s.sinks + (len > lo ? len - lo : 0);
   return s;
+}
+template <int KEYS>
+__device__ inline Seen seen_keys_of(const AttnArgs& a, int seq) {
+  if constexpr (KEYS == kOwn) return seen_by_last(a, a.b.lens[seq]);
+  else return seen_behind(a, a.b.lens[seq]);
 }
 
 constexpr int kDecWaves = 4;
@@ -305,8 +348,9 @@ __device__ inline int64_t decode_share(int64_t total, int blocks) {
 // streaming read reaches 6.1; a block per (pair, fixed part) took 527 us, its
 // longest pair last. One sequence of 131071, 32/8 heads of 128: 107 us, 5.0
 // TB/s. One of 127: 11 us, a launch and a chain of dependent loads.
-template <class T, int D, int CAP>
+template <class T, int D, int CAP, int KEYS>
 __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs a) {
+  static_assert(KEYS != kPrefix, "the prefix is the prompts' kernel's");
   constexpr int NS = dec_keys<D>() / 16, kKeys = 16 * NS, kStep = D / 32, kOut = D / 16;
   // V rows 32 bytes apart in banks: 16 rows of a transposed read cover each bank twice
   constexpr int kRow = 2 * D + 32, kTile = kKeys * kRow;
@@ -327,7 +371,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   if (a.splits > 1) {
     const Owner w = find_owner(
         a.b.batch,
-        [&](int b) { return (int64_t)decode_tiles<kKeys>(seen_by_last(a, a.b.lens[b])) * a.p.kv_heads; },
+        [&](int b) { return (int64_t)decode_tiles<kKeys>(seen_keys_of<KEYS>(a, b)) * a.p.kv_heads; },
         [&](int64_t total) {
           const int64_t share = decode_share(total, a.splits);
           at_tile = blockIdx.x * share;
@@ -340,7 +384,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
   } else {
     of_seq = blockIdx.x / a.p.kv_heads;
   }
-  of_seen = seen_by_last(a, a.b.lens[of_seq]);
+  of_seen = seen_keys_of<KEYS>(a, of_seq);
   of_tiles = decode_tiles<kKeys>(of_seen);
   for (bool head_of_run = true;; head_of_run = false) {
     // this pair, and the tiles of it that fall to this block
@@ -376,6 +420,12 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
     const int32_t* table = a.b.table + (int64_t)seq * a.b.table_stride;
     const char* kbase = a.p.k + 2 * (hk * a.p.kst[2] + 8 * j);
     const char* vbase = a.p.v + 2 * (hk * a.p.vst[2] + 8 * j);
+    const int32_t from = KEYS == kBehind && a.pre > 0 ? a.prefix : 0;
+    auto key_of = [&](int i) { return i < seen.sinks ? i + from : i + seen.skip; };
+    auto page_of = [&](int32_t key) {
+      if constexpr (KEYS == kOwn) return table[key >> a.p.page_shift];
+      else return page_behind(a, table, key);
+    };
     // page of key i of the run (-1: none) and its place in the page
     auto look_up = [&](int tile, int32_t* page, int32_t* at) {
 #pragma unroll
@@ -384,8 +434,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
         page[h] = -1;
         at[h] = 0;
         if (tile < last && i < seen.n) {
-          const int32_t key = i < seen.sinks ? i : i + seen.skip;
-          page[h] = table[key >> a.p.page_shift];
+          const int32_t key = key_of(i);
+          page[h] = page_of(key);
           at[h] = key & a.p.page_mask;
         }
       }
@@ -541,7 +591,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 #pragma unroll 1
       for (int n = (first + wave) * kKeys; n < min(last * kKeys, seen.n);
            n += (n + 1) % kKeys ? 1 : 1 + (kDecWaves - 1) * kKeys) {
-        const int32_t key = n < seen.sinks ? n : n + seen.skip, pg = table[key >> a.p.page_shift];
+        const int32_t key = key_of(n), pg = page_of(key);
         if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
         const int64_t row = key & a.p.page_mask;
         const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
@@ -606,14 +656,24 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
         v0 = fmaf(src[0], f, v0);
         v1 = fmaf(src[1], f, v1);
       }
-      if (whole) {
+      if (whole && (KEYS == kOwn || a.pre == 0)) {
         const float r = 1.0f / l;
         *reinterpret_cast<uint32_t*>(a.out + 2 * (seq * a.ost[0] + (h0 + h) * a.ost[1] + d)) =
             some ? T::pack(v0 * r, v1 * r) : 0u;
       } else {
-        *reinterpret_cast<f32x2*>(a.part + (slot + h) * D + d) = f32x2{v0, v1};
+        float* part = a.part;
+        float* stat = a.stat;
+        int64_t to = slot + h;
+        if constexpr (KEYS == kBehind)
+          if (whole) {
+            part = a.pre_part;
+            stat = a.pre_stat;
+            to = ((int64_t)seq * a.q_heads + h0 + h) * a.pre_row + a.pre;
+          }
+        *reinterpret_cast<f32x2*>(part + to * D + d) = f32x2{v0, v1};
         if (d == 0)
-          *reinterpret_cast<f32x2*>(a.stat + 2 * (slot + h)) = f32x2{some ? top * sc.c : -INFINITY, l};
+          *reinterpret_cast<f32x2*>(stat + 2 * to) =
+              f32x2{some ? (KEYS == kOwn ? top * sc.c : top) : -INFINITY, l};
       }
     }
     if (a.splits == 1) return;
@@ -624,7 +684,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
       before = at_tile;
       do {
         if (++of_seq >= a.b.batch) return;
-        of_seen = seen_by_last(a, a.b.lens[of_seq]);
+        of_seen = seen_keys_of<KEYS>(a, of_seq);
         of_tiles = decode_tiles<kKeys>(of_seen);
       } while (of_tiles == 0);
     }
@@ -640,16 +700,22 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_decode_kernel(AttnArgs
 // written already, and counting the sequences' tiles is what a block costs
 // (1024 sequences of up to 512 tokens in a wide table, 32 query heads: a block
 // per head 63 us, two blocks a sequence 20 us).
-template <class T, int D>
+// Behind a shared prefix every row has that pass's parts too, and nothing is
+// written yet. References are raw scores there, whose differences are scaled: two
+// products would each be rounded, by up to 2^-8 at 2^16. The two passes' weights
+// have biases of their own.
+template <class T, int D, int KEYS>
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;
   __shared__ f32x4 vs[kGroups][kLanes];
   __shared__ float ls[kGroups];
   const int seq = blockIdx.x;
-  const int tiles = decode_tiles<dec_keys<D>()>(seen_by_last(a, a.b.lens[seq]));
+  const int tiles = decode_tiles<dec_keys<D>()>(seen_keys_of<KEYS>(a, seq));
+  const int pre = KEYS == kBehind ? a.pre : 0;
+  const float c2 = KEYS == kOwn ? 1.0f : scale_of(a);
   const int g = threadIdx.x / kLanes, c = threadIdx.x - g * kLanes;
   char* out = a.out + 2 * (seq * a.ost[0] + 4 * c);
-  if (tiles == 0) {
+  if (tiles == 0 && pre == 0) {
     if (g == 0)
       for (int h = blockIdx.y; h < a.q_heads; h += gridDim.y)
         *reinterpret_cast<u32x2*>(out + 2 * h * a.ost[1]) = u32x2{0u, 0u};
@@ -659,7 +725,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   __shared__ int64_t part_total[4], part_before[4];
   int64_t total = 0, before = 0;
   for (int b = threadIdx.x; b < a.b.batch; b += 256) {
-    const int64_t n = decode_tiles<dec_keys<D>()>(seen_by_last(a, a.b.lens[b]));
+    const int64_t n = decode_tiles<dec_keys<D>()>(seen_keys_of<KEYS>(a, b));
     total += n;
     if (b < seq) before += n;
   }
@@ -679,14 +745,27 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
   for (int h = blockIdx.y; h < a.q_heads; h += gridDim.y) {
     const int hk = h / a.group, in = h - hk * a.group;
     const int64_t t0 = before + (int64_t)hk * tiles;
-    const int b0 = (int)(t0 / share), b1 = (int)((t0 + tiles - 1) / share);
-    if (b0 == b1) continue;
+    int b0 = (int)(t0 / share), b1 = (int)((t0 + tiles - 1) / share);
+    if (b0 == b1 && pre == 0) continue;
+    // the row's parts over the prefix, and the one that a block had whole
+    const int64_t row = ((int64_t)seq * a.q_heads + h) * a.pre_row;
+    int more = 0;
+    if constexpr (KEYS == kBehind) {
+      more = pre;
+      if (tiles == 0 || a.splits == 1 || b0 == b1) {
+        more += tiles > 0;
+        b0 = 0;
+        b1 = -1;
+      }
+    }
     auto slot = [&](int b) {
       return (((int64_t)(in >> 4) * a.splits + b) * 2 + (b * share < t0 ? 1 : 0)) * 16 + (in & 15);
     };
     const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat);
     float top = -INFINITY, l = 0.0f;
     for (int b = b0 + (threadIdx.x & 63); b <= b1; b += 64) top = fmaxf(top, stat[slot(b)][0]);
+    if constexpr (KEYS == kBehind)
+      for (int i = threadIdx.x & 63; i < more; i += 64) top = fmaxf(top, a.pre_stat[2 * (row + i)]);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
     f32x4 v = {0, 0, 0, 0};
@@ -697,10 +776,22 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
         const int64_t at = slot(b);
         const f32x2 st = stat[at];
         const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * D + 4 * c);
-        const float f = st[0] == -INFINITY ? 0.0f : lesser(st[0] - top);
+        const float f = st[0] == -INFINITY ? 0.0f : lesser(KEYS == kOwn ? st[0] - top : (st[0] - top) * c2);
         l = fmaf(st[1], f, l);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+      }
+      if constexpr (KEYS == kBehind) {
+#pragma unroll 4
+        for (int i = g; i < more; i += kGroups) {
+          const f32x2 st = *reinterpret_cast<const f32x2*>(a.pre_stat + 2 * (row + i));
+          if (st[0] == -INFINITY) continue;  // not written
+          const f32x4 x = *reinterpret_cast<const f32x4*>(a.pre_part + (row + i) * D + 4 * c);
+          const float f = lesser((st[0] - top) * c2 + (i < pre ? Mx<T>::kDecBias - Mx<T>::kBias : 0.0f));
+          l = fmaf(st[1], f, l);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+        }
       }
       vs[g][c] = v;
       if (c == 0) ls[g] = l;
@@ -726,7 +817,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(AttnArgs a) {
 // groups of D/4 threads share a row's parts, and a block has the rows that fit
 // 256 threads (many rows of few parts: G = 1; few rows of many: one row a block).
 // Bound by the reading of the parts, which the prompt kernel has just written.
-template <class T, int D, int G>
+template <class T, int D, int G, int KEYS>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t rows) {
   constexpr uint32_t kLanes = D / 4, kRows = 256 / (kLanes * G);
   __shared__ f32x4 vs[G][kLanes];
@@ -738,6 +829,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t row
   const KvSeq s = work ? kv_seq(a.b, kv_row_owner(a.b, t)) : KvSeq{0, 0, 0};
   const bool owned = t >= s.first && t < s.first + s.n;
   const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat) + (int64_t)row * a.splits;
+  const float c2 = KEYS == kOwn ? 1.0f : scale_of(a);
   float top = -INFINITY, l = 0.0f;
   f32x4 v = {0, 0, 0, 0};
   if (owned) {
@@ -747,7 +839,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, uint32_t row
     for (int i = g; i < a.splits; i += G) {
       const f32x2 st = stat[i];
       if (st[0] == -INFINITY) continue;
-      const float f = lesser(st[0] - top);
+      const float f = lesser(KEYS == kOwn ? st[0] - top : (st[0] - top) * c2);
       const f32x4 x = *reinterpret_cast<const f32x4*>(part + (int64_t)i * D);
       l = fmaf(st[1], f, l);
 #pragma unroll
@@ -863,7 +955,7 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 // registers allow one wave a SIMD there, and the tile's load instructions and
 // its barrier stand beside the step. Deeper rings of tiles, 256 rows a block
 // and loads spread over the step were no faster.
-template <class T, int D, int BN, int CAP>
+template <class T, int D, int BN, int CAP, int KEYS>
 __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
@@ -881,37 +973,66 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   // which sequence's tile this is: tiles are counted over the sequences, from
   // the last one on (the longest ones of a prompt first)
   const int64_t want = gridDim.x / a.p.kv_heads - 1 - place;
-  const Owner w = find_owner(
-      a.b.batch, [&](int b) { return ((int64_t)kv_seq(a.b, b).n * G + BM - 1) / BM; }, [&](int64_t) { return want; });
-  if (w.seq < 0) return;
-  const int seq = __builtin_amdgcn_readfirstlane(w.seq);
-  const int tile = __builtin_amdgcn_readfirstlane((int)(want - w.before));
-  KvSeq s = kv_seq(a.b, seq);
-  s.first = __builtin_amdgcn_readfirstlane(s.first);
-  s.n = __builtin_amdgcn_readfirstlane(s.n);
-  s.len = __builtin_amdgcn_readfirstlane(s.len);
+  int seq = 0, tile = (int)want;
+  KvSeq s{0, a.b.tokens, 0};  // the prefix: the rows of all sequences
+  if constexpr (KEYS != kPrefix) {
+    const Owner w = find_owner(
+        a.b.batch, [&](int b) { return ((int64_t)kv_seq(a.b, b).n * G + BM - 1) / BM; }, [&](int64_t) { return want; });
+    if (w.seq < 0) return;
+    seq = __builtin_amdgcn_readfirstlane(w.seq);
+    tile = __builtin_amdgcn_readfirstlane((int)(want - w.before));
+    s = kv_seq(a.b, seq);
+    s.first = __builtin_amdgcn_readfirstlane(s.first);
+    s.n = __builtin_amdgcn_readfirstlane(s.n);
+    s.len = __builtin_amdgcn_readfirstlane(s.len);
+  }
   const int R = s.n * G, pos0 = s.len - s.n;  // pos0 may be negative: rows in front of the sequence
 
   // the block's keys, in tiles of BN: those of the first `sinks`, then the window's
   const int row0 = tile * BM;
-  const int p_first = pos0 + row0 / G, p_last = pos0 + (min(row0 + BM, R) - 1) / G;
-  const int64_t cap = (int64_t)a.b.width << a.p.page_shift;
+  // this lane's row, and the positions of the wave's and the block's
+  const int wrow0 = row0 + 32 * wave;
+  const int row = min(wrow0 + col, R - 1);
+  const int qi = row / G, head = hk * G + row - qi * G;
+  const bool in = wrow0 + col < R;
+  int p = pos0 + qi, p_first = pos0 + row0 / G, p_last = pos0 + (min(row0 + BM, R) - 1) / G;
+  int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
+  if constexpr (KEYS == kPrefix) {
+    // every row has a sequence of its own; a row of none sees nothing
+    __shared__ int bounds[2][NT / 64];
+    const KvSeq of = kv_seq(a.b, kv_row_owner(a.b, qi));
+    p = qi >= of.first && qi < of.first + of.n ? of.len - of.n + qi - of.first : -1;
+    int lowest = p, highest = p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {  // (the halves hold the same rows)
+      lowest = min(lowest, __shfl_xor(lowest, o));
+      highest = max(highest, __shfl_xor(highest, o));
+    }
+    pw_first = __builtin_amdgcn_readfirstlane(lowest);
+    pw_last = __builtin_amdgcn_readfirstlane(highest);
+    if (lane == 0) {
+      bounds[0][wave] = pw_first;
+      bounds[1][wave] = pw_last;
+    }
+    __syncthreads();
+    p_first = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
+    p_last = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    p_first = __builtin_amdgcn_readfirstlane(p_first);
+    p_last = __builtin_amdgcn_readfirstlane(p_last);
+  }
+  // keys from .. cap - 1 are the kernel's
+  const int from = KEYS == kBehind && a.pre > 0 ? a.prefix : 0;
+  const int64_t own = (int64_t)a.b.width << a.p.page_shift;
+  const int64_t cap = KEYS == kOwn ? own : KEYS == kPrefix ? (int64_t)a.prefix : max(own, (int64_t)a.prefix);
   const int hi = (int)min((int64_t)p_last + 1, cap);
   const int lo = a.window > 0 && p_first >= a.window ? p_first - a.window + 1 : 0;
-  const int t_hi = hi > 0 ? (hi + BN - 1) / BN : 0, t_lo = lo / BN;
+  const int t_from = from / BN, t_hi = hi > 0 ? (hi + BN - 1) / BN : 0, t_lo = max(lo, from) / BN;
   // (at most 2^30 before it is rounded up: sinks and lo may both end at int32's end)
-  const int front = min((min(min(a.sinks, lo), max(hi, 0)) + BN - 1) / BN, t_lo);
+  const int front = max(min((min(min(a.sinks, lo), max(hi, 0)) + BN - 1) / BN, t_lo) - t_from, 0);
   const int tiles = a.p.n_pages > 0 ? front + max(t_hi - t_lo, 0) : 0;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int it0 = min(per * (int)blockIdx.y, tiles), it1 = min(it0 + per, tiles);
-  auto tile_of = [&](int it) { return it < front ? it : t_lo + it - front; };
-
-  // this lane's row, and the range of the wave's
-  const int wrow0 = row0 + 32 * wave;
-  const int row = min(wrow0 + col, R - 1);
-  const int qi = row / G, head = hk * G + row - qi * G, p = pos0 + qi;
-  const bool in = wrow0 + col < R;
-  const int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
+  auto tile_of = [&](int it) { return it < front ? t_from + it : t_lo + it - front; };
 
   const Scale sc = fold_scale<CAP>(a);
 
@@ -922,6 +1043,11 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   auto look_up = [&](int it) -> int32_t {
     if (it >= it1) return -1;
     const int key = tile_of(it) * BN + (lane & (BN - 1));
+    if constexpr (KEYS == kPrefix) {
+      const int e = key >> a.p.page_shift;
+      return key < hi && e < a.prefix_width ? a.prefix_table[e] : -1;
+    }
+    if constexpr (KEYS == kBehind) return key >= from && key < hi ? page_behind(a, table, key) : -1;
     return key < hi ? table[key >> a.p.page_shift] : -1;
   };
   // Looked at a turn after the load was issued: a wait for it is a wait for
@@ -933,6 +1059,9 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   // exist reads what is there (a page's end, or page 0); its score is masked
   // and its value, if not finite, taken out.
   const bool whole = a.p.page_shift >= 4 && a.p.kst[1] < (1 << 24) && a.p.vst[1] < (1 << 24);
+  // But where the prefix ends inside such a run of rows, the rows in front of its
+  // end and those behind it lie in two pages: that tile goes row by row.
+  const int cut = KEYS == kBehind && (a.prefix & 15) ? a.prefix / BN : -1;
   // (rows i * NT / CH apart have the same offsets, where that is a multiple of 16)
   constexpr int kOffs = NT % (16 * CH) == 0 ? 1 : kUnits;
   uint32_t koff[kOffs], voff[kOffs];
@@ -947,7 +1076,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
                   const uint32_t* off, auto piece) {
     const int key0 = tile_of(it) * BN;
     if (page < 0) page = 0;
-    if (whole) {
+    if (whole && (KEYS != kBehind || tile_of(it) != cut)) {
       const uint64_t at = (uint64_t)(base + 2 * (page * page_step + ((key0 + lane) & a.p.page_mask) * row_step));
       const int at_lo = (int)(uint32_t)at, at_hi = (int)(uint32_t)(at >> 32);
 #pragma unroll
@@ -1316,12 +1445,18 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   // (in front of the stores 168 registers do for rows of 64, a third block a CU;
   // rows of 256 would move 32 of their sums to memory)
   if constexpr (D < 256) tell();
-  const int64_t part_at = ((int64_t)(s.first + qi) * a.q_heads + head) * a.splits + blockIdx.y;
+  // a row's parts over the prefix come first
+  int64_t part_at = (int64_t)(s.first + qi) * a.q_heads + head;
+  if constexpr (KEYS == kOwn) part_at = part_at * a.splits + blockIdx.y;
+  else part_at = part_at * a.pre_row + (KEYS == kBehind ? a.pre : 0) + blockIdx.y;
+  const bool parts = KEYS == kPrefix || a.splits > 1 || (KEYS == kBehind && a.pre > 0);
+  float* const part_to = KEYS == kPrefix ? a.pre_part : a.part;
+  float* const stat_to = KEYS == kPrefix ? a.pre_stat : a.stat;
   char* out_row = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1]);
-  if (a.splits > 1) {
-    if (in && half == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * part_at) = f32x2{any ? ref * sc.c : -INFINITY, sum};
+  if (parts) {
+    if (in && half == 0) *reinterpret_cast<f32x2*>(stat_to + 2 * part_at) = f32x2{any ? (KEYS == kOwn ? ref * sc.c : ref) : -INFINITY, sum};
     if (in && any) {
-      float* dst = a.part + part_at * D + 4 * half;
+      float* dst = part_to + part_at * D + 4 * half;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -1372,7 +1507,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
         const float x = e == 0 ? f[i] : e == 4 ? f[4 + i] : e == 8 ? f[8 + i] : f[12 + i];
         const int d = 32 * t + 2 * e + 4 * half + i;
         if (x == 0.0f) continue;
-        if (a.splits > 1) a.part[part_at * D + d] = x;
+        if (parts) part_to[part_at * D + d] = x;
         else *reinterpret_cast<uint16_t*>(out_row + 2 * d) = (uint16_t)T::pack(x, x);
       }
   }
@@ -1399,13 +1534,18 @@ int64_t prompt_tiles(const KvBatchView& b, int64_t group) {
   return (int64_t)b.tokens * group / kPromptRows + std::min(b.batch, b.tokens);
 }
 
+// ... and of a pass over a prefix, where a tile has rows of any sequences.
+int64_t prefix_tiles(const KvBatchView& b, int64_t group) {
+  return ((int64_t)b.tokens * group + kPromptRows - 1) / kPromptRows;
+}
+
 // How the keys are split, from the sizes alone (the lengths are on the device).
 // One token a sequence: see decode_blocks. Prompts: the parts of every row's tiles, as many as fill the
 // chip, and not so many that a part goes below kMinPart keys. Writing and
 // joining the parts costs as much as half the work of a few hundred blocks, so
 // rows are split only where they make less than half a block a CU (ragged turns
 // over 20000 tokens, 250 blocks: unsplit 41 us, in two 43, in three 50).
-constexpr int kMinPart = 256, kPromptBlocks = 256, kMaxSplits = 64;
+constexpr int64_t kMinPart = 256, kPromptBlocks = 256, kMaxSplits = 64;
 
 // Blocks that share out the tiles of single tokens; 1: a block per pair and no
 // join. That is for caches whose longest pair, as the table and the window allow
@@ -1442,66 +1582,134 @@ int64_t part_rows(const KvView& p, const KvBatchView& b, int64_t q_heads, int sp
   return (q_heads / p.kv_heads + 15) / 16 * splits * 2 * 16;
 }
 
-template <class T, int D>
+template <class T, int D, int KEYS>
 void launch_decode(const AttnArgs& a, hipStream_t stream) {
   const unsigned blocks = a.splits > 1 ? a.splits : a.b.batch * a.p.kv_heads;
   const dim3 grid(blocks, (a.group + 15) / 16), block(64 * kDecWaves);
   if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_decode_kernel<T, D, kWideCap>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_decode_kernel<T, D, kWideCap, KEYS>), grid, block, 0, stream, a);
   else
-    HGK_LAUNCH((attn_decode_kernel<T, D, kNoCap>), grid, block, 0, stream, a);
-  if (a.splits > 1)
-    HGK_LAUNCH((attn_decode_join_kernel<T, D>),
+    HGK_LAUNCH((attn_decode_kernel<T, D, kNoCap, KEYS>), grid, block, 0, stream, a);
+  if (a.splits > 1 || (KEYS == kBehind && a.pre > 0))
+    HGK_LAUNCH((attn_decode_join_kernel<T, D, KEYS>),
                dim3(a.b.batch, std::clamp<int>(kDecJoinBlocks / a.b.batch, 1, a.q_heads)), dim3(256), 0, stream, a);
 }
 
-template <class T, int D, int BN>
+template <class T, int D, int BN, int KEYS>
 void launch_prompt(const AttnArgs& a, hipStream_t stream) {
-  const dim3 grid(a.p.kv_heads * prompt_tiles(a.b, a.group), a.splits), block(2 * kPromptRows);
+  const int64_t tiles = KEYS == kPrefix ? prefix_tiles(a.b, a.group) : prompt_tiles(a.b, a.group);
+  const dim3 grid(a.p.kv_heads * tiles, a.splits), block(2 * kPromptRows);
   if (a.softcap > kCapMax)
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kWideCap>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kWideCap, KEYS>), grid, block, 0, stream, a);
   else if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kCap>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kCap, KEYS>), grid, block, 0, stream, a);
   else
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kNoCap>), grid, block, 0, stream, a);
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kNoCap, KEYS>), grid, block, 0, stream, a);
 }
 
-template <class T, int D>
+template <class T, int D, int KEYS>
 void launch_join(const AttnArgs& a, hipStream_t stream) {
   constexpr int kGroups = 256 / (D / 4);
   const uint32_t rows = (uint32_t)a.b.tokens * a.q_heads;
   if (a.splits > 8)
-    HGK_LAUNCH((attn_join_kernel<T, D, kGroups>), dim3(rows), dim3(256), 0, stream, a, rows);
+    HGK_LAUNCH((attn_join_kernel<T, D, kGroups, KEYS>), dim3(rows), dim3(256), 0, stream, a, rows);
   else
-    HGK_LAUNCH((attn_join_kernel<T, D, 1>), dim3((rows + kGroups - 1) / kGroups), dim3(256), 0, stream, a, rows);
+    HGK_LAUNCH((attn_join_kernel<T, D, 1, KEYS>), dim3((rows + kGroups - 1) / kGroups), dim3(256), 0, stream, a, rows);
 }
 
-template <class T>
-int run(const AttnArgs& a, const char* what, hipStream_t stream) {
+// All launches of a call. Behind a prefix: its keys for all rows, then the
+// sequences' own, then the join of a row's parts.
+template <class T, int D, int KEYS>
+int run_of(const AttnArgs& a, const char* what, hipStream_t stream) {
+  const bool pass = KEYS == kBehind && a.pre > 0;
+  if constexpr (KEYS == kBehind)
+    if (pass) {
+      AttnArgs of = a;
+      of.splits = a.pre;
+      launch_prompt<T, D, 64, kPrefix>(of, stream);
+      if (int st = launch_status(what)) return st;
+    }
   if (!a.b.starts) {
-    switch (a.p.head_dim) {
-      case 64: launch_decode<T, 64>(a, stream); break;
-      case 96: launch_decode<T, 96>(a, stream); break;
-      case 128: launch_decode<T, 128>(a, stream); break;
-      default: launch_decode<T, 256>(a, stream); break;
-    }
-  } else {
-    switch (a.p.head_dim) {
-      case 64: launch_prompt<T, 64, 64>(a, stream); break;
-      case 96: launch_prompt<T, 96, 64>(a, stream); break;
-      case 128: launch_prompt<T, 128, 64>(a, stream); break;
-      default: launch_prompt<T, 256, 64>(a, stream); break;
-    }
+    launch_decode<T, D, KEYS>(a, stream);
+    return launch_status(what);
   }
+  launch_prompt<T, D, 64, KEYS>(a, stream);
   if (int st = launch_status(what)) return st;
-  if (a.splits == 1 || !a.b.starts) return HGK_OK;
-  switch (a.p.head_dim) {
-    case 64: launch_join<T, 64>(a, stream); break;
-    case 96: launch_join<T, 96>(a, stream); break;
-    case 128: launch_join<T, 128>(a, stream); break;
-    default: launch_join<T, 256>(a, stream); break;
-  }
+  if (a.splits == 1 && !pass) return HGK_OK;
+  AttnArgs of = a;
+  if (KEYS == kBehind) of.splits = a.pre_row;
+  launch_join<T, D, KEYS>(of, stream);
   return launch_status(what);
+}
+
+template <class T, int KEYS>
+int run(const AttnArgs& a, const char* what, hipStream_t stream) {
+  switch (a.p.head_dim) {
+    case 64: return run_of<T, 64, KEYS>(a, what, stream);
+    case 96: return run_of<T, 96, KEYS>(a, what, stream);
+    case 128: return run_of<T, 128, KEYS>(a, what, stream);
+    default: return run_of<T, 256, KEYS>(a, what, stream);
+  }
+}
+
+// The operands of both entry points checked and filled in, but for the workspace.
+int check_call(const char* what, AttnArgs* a, const void* q, const int64_t q_strides[2], int64_t q_heads, float scale,
+               float softcap, int64_t window, int64_t sinks, void* out, const int64_t out_strides[2]) {
+  const int64_t T = a->b.tokens, D = a->p.head_dim;
+  if (int st = kv_check_rows(what, "q", q, q_strides, T, q_heads, D, false, a->qst)) return st;
+  if (int st = kv_check_rows(what, "out", out, out_strides, T, q_heads, D, true, a->ost)) return st;
+  a->q = static_cast<const char*>(q);
+  a->out = static_cast<char*>(out);
+  a->q_heads = (int32_t)q_heads;
+  a->group = (int32_t)(q_heads / a->p.kv_heads);
+  a->scale = scale;
+  a->softcap = softcap;
+  a->window = (int32_t)(window >= INT32_MAX ? 0 : window);  // every key of any sequence
+  a->sinks = (int32_t)(sinks > INT32_MAX ? INT32_MAX : sinks);
+  if (a->p.kv_heads * (a->b.starts ? prompt_tiles(a->b, a->group) : (int64_t)a->b.batch) > kMaxBlocks)
+    return fail(HGK_ERR_ARG, "%s: %lld rows are too many", what, (long long)T);
+  return HGK_OK;
+}
+int check_scales(const char* what, float scale, float softcap) {
+  if (!std::isfinite(scale)) return fail(HGK_ERR_ARG, "%s: scale must be finite", what);
+  if (!(softcap >= 0.0f) || !std::isfinite(softcap))
+    return fail(HGK_ERR_ARG, "%s: softcap must be finite and not negative", what);
+  return HGK_OK;
+}
+
+// The split of a call behind a shared prefix, from the sizes alone.
+struct SharedPlan {
+  int pre, splits;              // parts of a row over the prefix, and the sequences' splits
+  int64_t pre_rows, part_rows;  // rows of the workspace: of the prefix's parts, and of single tokens' runs
+};
+SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, int64_t q_heads, int64_t window,
+                       int64_t sinks) {
+  SharedPlan s{0, 1, 0, 0};
+  if (b.batch == 0 || b.tokens == 0) return s;
+  const int64_t group = q_heads / p.kv_heads, width = (int64_t)b.width << p.page_shift;
+  const int64_t tiles = p.kv_heads * prefix_tiles(b, group), keys = std::min(prefix, width);
+  if (b.batch > 1 && keys > 0)
+    s.pre = (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, keys / kMinPart, (int64_t)kMaxSplits}));
+  int64_t rest = std::max(width, prefix) - (s.pre > 0 ? prefix : 0);
+  if (window > 0 && window < rest && sinks < rest - window) rest = window + sinks;
+  if (!b.starts) {
+    s.splits = decode_blocks(p, b, rest);
+    s.part_rows = part_rows(p, b, q_heads, s.splits);
+    if (s.pre > 0) s.pre_rows = (int64_t)b.tokens * q_heads * (s.pre + 1);
+    return s;
+  }
+  const int64_t n = std::min(kPromptBlocks / (p.kv_heads * prompt_tiles(b, group)), rest / kMinPart);
+  s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
+  if (s.pre > 0 || s.splits > 1) s.pre_rows = (int64_t)b.tokens * q_heads * (s.pre + s.splits);
+  return s;
+}
+int check_prefix(const char* what, const KvView& p, int64_t width, int64_t prefix) {
+  if (prefix < 0 || width < 0 || prefix > (int64_t)1 << 30 || width > (int64_t)1 << (30 - p.page_shift))
+    return fail(HGK_ERR_ARG, "%s: a prefix of %lld tokens on %lld pages", what, (long long)prefix, (long long)width);
+  if (((prefix + p.page_mask) >> p.page_shift) > width)
+    return fail(HGK_ERR_ARG, "%s: %lld pages of %d tokens do not hold a prefix of %lld", what, (long long)width,
+                p.page_mask + 1, (long long)prefix);
+  return HGK_OK;
 }
 
 }  // namespace
@@ -1525,30 +1733,67 @@ extern "C" int hgk_paged_attention(const hgk_kv_pages* pages, const hgk_kv_batch
                                    int64_t workspace_bytes, void* stream) {
   const char* what = "hgk_paged_attention";
   clear_error();
-  AttnArgs a;
+  AttnArgs a{};
   if (int st = check_sizes(what, pages, batch, q_heads, window, sinks, &a.p, &a.b)) return st;
-  if (!std::isfinite(scale)) return fail(HGK_ERR_ARG, "%s: scale must be finite", what);
-  if (!(softcap >= 0.0f) || !std::isfinite(softcap))
-    return fail(HGK_ERR_ARG, "%s: softcap must be finite and not negative", what);
+  if (int st = check_scales(what, scale, softcap)) return st;
   if (a.b.batch == 0 || a.b.tokens == 0) return HGK_OK;
-  const int64_t T = a.b.tokens, D = a.p.head_dim;
-  if (int st = kv_check_rows(what, "q", q, q_strides, T, q_heads, D, false, a.qst)) return st;
-  if (int st = kv_check_rows(what, "out", out, out_strides, T, q_heads, D, true, a.ost)) return st;
-  a.q = static_cast<const char*>(q);
-  a.out = static_cast<char*>(out);
-  a.q_heads = (int32_t)q_heads;
-  a.group = (int32_t)(q_heads / a.p.kv_heads);
-  a.scale = scale;
-  a.softcap = softcap;
-  a.window = (int32_t)(window >= INT32_MAX ? 0 : window);  // every key of any sequence
-  a.sinks = (int32_t)(sinks > INT32_MAX ? INT32_MAX : sinks);
-  if (a.p.kv_heads * (a.b.starts ? prompt_tiles(a.b, a.group) : (int64_t)a.b.batch) > kMaxBlocks)
-    return fail(HGK_ERR_ARG, "%s: %lld rows are too many", what, (long long)T);
+  if (int st = check_call(what, &a, q, q_strides, q_heads, scale, softcap, window, sinks, out, out_strides)) return st;
+  const int64_t D = a.p.head_dim;
   a.splits = plan_splits(a.p, a.b, q_heads, window, sinks);
   const int64_t rows = part_rows(a.p, a.b, q_heads, a.splits), need = rows * (D + 2) * 4;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(HGK_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
   a.part = static_cast<float*>(workspace);
   a.stat = rows > 0 ? a.part + rows * D : nullptr;
-  return pages->dtype == DT_BF16 ? run<BF16>(a, what, as_stream(stream)) : run<F16>(a, what, as_stream(stream));
+  return pages->dtype == DT_BF16 ? run<BF16, kOwn>(a, what, as_stream(stream))
+                                 : run<F16, kOwn>(a, what, as_stream(stream));
+}
+
+extern "C" int64_t hgk_shared_prefix_attention_workspace(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                                         int64_t prefix_width, int64_t prefix_len, int64_t q_heads,
+                                                         int64_t window, int64_t sinks) {
+  const char* what = "hgk_shared_prefix_attention_workspace";
+  clear_error();
+  KvView p;
+  KvBatchView b;
+  if (check_sizes(what, pages, batch, q_heads, window, sinks, &p, &b)) return -1;
+  if (check_prefix(what, p, prefix_width, prefix_len)) return -1;
+  const SharedPlan s = plan_shared(p, b, prefix_len, q_heads, window, sinks);
+  return (s.pre_rows + s.part_rows) * (p.head_dim + 2) * 4;
+}
+
+extern "C" int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                           const int32_t* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                                           const void* q, const int64_t q_strides[2], int64_t q_heads, float scale,
+                                           float softcap, int64_t window, int64_t sinks, void* out,
+                                           const int64_t out_strides[2], void* workspace, int64_t workspace_bytes,
+                                           void* stream) {
+  const char* what = "hgk_shared_prefix_attention";
+  clear_error();
+  AttnArgs a{};
+  if (int st = check_sizes(what, pages, batch, q_heads, window, sinks, &a.p, &a.b)) return st;
+  if (int st = check_prefix(what, a.p, prefix_width, prefix_len)) return st;
+  if (int st = check_scales(what, scale, softcap)) return st;
+  if (a.b.batch == 0 || a.b.tokens == 0) return HGK_OK;
+  if (prefix_len > 0 && !prefix_table) return fail(HGK_ERR_ARG, "%s: null prefix table", what);
+  if (int st = check_call(what, &a, q, q_strides, q_heads, scale, softcap, window, sinks, out, out_strides)) return st;
+  const int64_t D = a.p.head_dim;
+  const SharedPlan s = plan_shared(a.p, a.b, prefix_len, q_heads, window, sinks);
+  const int64_t rows = s.pre_rows + s.part_rows, need = rows * (D + 2) * 4;
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(HGK_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
+  a.prefix_table = prefix_table;
+  a.prefix_width = (int32_t)prefix_width;
+  a.prefix = (int32_t)prefix_len;
+  a.pre = s.pre;
+  a.splits = s.splits;
+  a.pre_row = s.pre + (a.b.starts ? s.splits : 1);
+  float* const ws = static_cast<float*>(workspace);
+  a.pre_part = ws;
+  a.pre_stat = ws + rows * D;
+  a.part = a.b.starts ? a.pre_part : ws + s.pre_rows * D;
+  a.stat = a.b.starts ? a.pre_stat : a.pre_stat + 2 * s.pre_rows;
+  if (!ws) a.pre_part = a.pre_stat = a.part = a.stat = nullptr;
+  return pages->dtype == DT_BF16 ? run<BF16, kBehind>(a, what, as_stream(stream))
+                                 : run<F16, kBehind>(a, what, as_stream(stream));
 }

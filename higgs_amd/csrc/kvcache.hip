@@ -144,12 +144,21 @@ bool same_rows(const KvView& p, const RowsView& x) {
 // past the caches, the pages are not written past them: the attention over them
 // comes next. 16384 tokens of 8 heads of 128 (134 MB read and written, nothing
 // cached): 32 us, 4.2 TB/s; with every thread looking up its own units 51 us.
+// With `slots` the places are given.
 constexpr int kMaxTokens = 16;
+template <bool SLOTS>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvView p, KvBatchView b, RowsView x,
-                                                             uint32_t units, uint32_t chunks, int per) {
+                                                             uint32_t units, uint32_t chunks, int per,
+                                                             const int64_t* slots) {
   __shared__ int32_t page_of[kMaxTokens], at_of[kMaxTokens];
   const int t0 = blockIdx.x * per, n = min(per, b.tokens - t0);
-  if ((int)threadIdx.x < n) {
+  if constexpr (SLOTS) {
+    if ((int)threadIdx.x < n) {
+      const int64_t slot = slots[t0 + threadIdx.x], page = slot >> p.page_shift;
+      page_of[threadIdx.x] = page >= 0 && page < p.n_pages ? (int32_t)page : -1;
+      at_of[threadIdx.x] = (int32_t)(slot & p.page_mask);
+    }
+  } else if ((int)threadIdx.x < n) {
     const int t = t0 + threadIdx.x, seq = kv_row_owner(b, t);
     const KvSeq s = kv_seq(b, seq);
     const int r = t - s.first;
@@ -241,6 +250,33 @@ bool whole_page(const int64_t st[3], const hgk_kv_pages* p) {
 
 using namespace hgk;
 
+namespace {
+// The call's operands checked, and the launch; `b` holds at least the tokens.
+int append(const char* what, const KvView& p, const KvBatchView& b, const void* k, const int64_t k_strides[2],
+           const void* v, const int64_t v_strides[2], const int64_t* slots, void* stream) {
+  if (int st = kv_check_written_pages(what, p)) return st;
+  RowsView x{static_cast<const char*>(k), static_cast<const char*>(v), {}, {}};
+  if (int st = kv_check_rows(what, "k", k, k_strides, b.tokens, p.kv_heads, p.head_dim, false, x.kst)) return st;
+  if (int st = kv_check_rows(what, "v", v, v_strides, b.tokens, p.kv_heads, p.head_dim, false, x.vst)) return st;
+  if (pools_meet(p) && !same_rows(p, x))
+    return fail(HGK_ERR_ARG, "%s: the key pages and the value pages overlap", what);
+  const uint32_t chunks = p.head_dim / 8;
+  const int64_t units = 2 * (int64_t)p.kv_heads * chunks;
+  if (units > INT32_MAX / kMaxTokens) return fail(HGK_ERR_ARG, "%s: too many kv heads", what);
+  // a token a block until the chip is full of blocks, then 16
+  const int per = b.tokens <= 2048 ? 1 : kMaxTokens;
+  const int64_t blocks = (b.tokens + (int64_t)per - 1) / per;
+  if (blocks > kMaxBlocks) return fail(HGK_ERR_ARG, "%s: %d rows are too many", what, b.tokens);
+  if (slots)
+    HGK_LAUNCH(kv_append_kernel<true>, dim3((unsigned)blocks), dim3(kThreads), 0, as_stream(stream), p, b, x,
+               (uint32_t)units, chunks, per, slots);
+  else
+    HGK_LAUNCH(kv_append_kernel<false>, dim3((unsigned)blocks), dim3(kThreads), 0, as_stream(stream), p, b, x,
+               (uint32_t)units, chunks, per, slots);
+  return launch_status(what);
+}
+}  // namespace
+
 extern "C" int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batch, const void* k,
                              const int64_t k_strides[2], const void* v, const int64_t v_strides[2],
                              void* stream) {
@@ -250,24 +286,22 @@ extern "C" int hgk_kv_append(const hgk_kv_pages* pages, const hgk_kv_batch* batc
   if (int st = kv_check_pages("hgk_kv_append", pages, &p)) return st;
   if (int st = kv_check_batch("hgk_kv_append", p, batch, &b)) return st;
   if (b.batch == 0 || b.tokens == 0 || p.n_pages == 0) return HGK_OK;
-  if (int st = kv_check_written_pages("hgk_kv_append", p)) return st;
-  RowsView x{static_cast<const char*>(k), static_cast<const char*>(v), {}, {}};
-  if (int st = kv_check_rows("hgk_kv_append", "k", k, k_strides, b.tokens, p.kv_heads, p.head_dim, false, x.kst))
-    return st;
-  if (int st = kv_check_rows("hgk_kv_append", "v", v, v_strides, b.tokens, p.kv_heads, p.head_dim, false, x.vst))
-    return st;
-  if (pools_meet(p) && !same_rows(p, x))
-    return fail(HGK_ERR_ARG, "hgk_kv_append: the key pages and the value pages overlap");
-  const uint32_t chunks = p.head_dim / 8;
-  const int64_t units = 2 * (int64_t)p.kv_heads * chunks;
-  if (units > INT32_MAX / kMaxTokens) return fail(HGK_ERR_ARG, "hgk_kv_append: too many kv heads");
-  // a token a block until the chip is full of blocks, then 16
-  const int per = b.tokens <= 2048 ? 1 : kMaxTokens;
-  const int64_t blocks = (b.tokens + (int64_t)per - 1) / per;
-  if (blocks > kMaxBlocks) return fail(HGK_ERR_ARG, "hgk_kv_append: %d rows are too many", b.tokens);
-  HGK_LAUNCH(kv_append_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, as_stream(stream), p, b, x,
-             (uint32_t)units, chunks, per);
-  return launch_status("hgk_kv_append");
+  return append("hgk_kv_append", p, b, k, k_strides, v, v_strides, nullptr, stream);
+}
+
+extern "C" int hgk_kv_append_slots(const hgk_kv_pages* pages, const int64_t* slots, int64_t tokens, const void* k,
+                                   const int64_t k_strides[2], const void* v, const int64_t v_strides[2],
+                                   void* stream) {
+  const char* what = "hgk_kv_append_slots";
+  clear_error();
+  KvView p;
+  if (int st = kv_check_pages(what, pages, &p)) return st;
+  if (tokens < 0 || tokens > INT32_MAX) return fail(HGK_ERR_ARG, "%s: tokens=%lld out of range", what, (long long)tokens);
+  if (tokens == 0 || p.n_pages == 0) return HGK_OK;
+  if (!slots || (reinterpret_cast<uintptr_t>(slots) & 7)) return fail(HGK_ERR_ARG, "%s: null or unaligned slots", what);
+  KvBatchView b{};
+  b.tokens = (int32_t)tokens;
+  return append(what, p, b, k, k_strides, v, v_strides, slots, stream);
 }
 
 extern "C" int hgk_kv_copy_pages(const hgk_kv_pages* pages, int64_t layers,

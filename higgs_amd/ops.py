@@ -24,6 +24,14 @@ Each function keeps the reference call's name and argument meaning:
     kv_copy_pages(k_pages, v_pages, src, dst)   the copy of a cache (prompt_cache.rs:22-307)
     paged_attention(q, k_pages, v_pages, ...)   fast::scaled_dot_product_attention and its
                                              masks (utils.rs:28-125; gemma2.rs:219-379)
+    shared_prefix_attention(q, ..., prefix_table, prefix_len)
+                                             the same of a batch that begins with one prompt
+                                             (prompt_cache.rs:22-307)
+    kv_extend(tables, lens, ...), kv_release(...)   cache growth, lengths and offsets of a batch
+                                             (cache.rs:130-312; transformer.rs:747-802)
+    moe_route(logits, top_k)                 router softmax + argpartition + weights
+                                             (qwen3_next.rs:949-985; qwen3_moe.rs:293-322)
+    moe_combine(y, weights, shared=...)      the experts' weighted sum (qwen3_next.rs:970-985)
     OpSequence                               a decode step's per-layer ops in one launch
                                              (the layer loop, qwen3_next.rs:1508-1547)
 
@@ -36,13 +44,13 @@ import ctypes as C
 import math
 import operator
 import struct
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from ._lib import (ACT_GELU_TANH, ACT_SILU, BF16, F16, F32, I32, OP_ADD_RMS_NORM, OP_GATED_RMS_NORM,
-                   OP_GLU, OP_QK_NORM_ROPE, OP_RMS_NORM, U32, HgkError, HgkOp, check, f32_array,
-                   i64_array, lib)
+                   OP_GLU, OP_QK_NORM_ROPE, OP_RMS_NORM, SCORE_SIGMOID, SCORE_SOFTMAX, U32, HgkError, HgkOp,
+                   check, f32_array, i64_array, lib)
 
 _DT = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int32: I32}
 if hasattr(torch, "uint32"):
@@ -582,8 +590,8 @@ def _kv_call(device: torch.device, fn, *args):
 
 
 def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-              block_table: torch.Tensor, kv_lens: torch.Tensor, *,
-              q_starts: Optional[torch.Tensor] = None) -> None:
+              block_table: Optional[torch.Tensor] = None, kv_lens: Optional[torch.Tensor] = None, *,
+              q_starts: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None) -> None:
     """Writes new tokens' keys and values, k and v [T, Hk, D] (any token and
     head strides), into their sequences' pages [n_pages, page_size, Hk, D].
 
@@ -592,13 +600,28 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     b owns rows q_starts[b] .. q_starts[b+1]-1 of k and v (int32 [B+1]);
     without q_starts, row b is its one new token. Rows of no sequence,
     positions beyond the table and pages outside the pool are skipped. The key
-    pages may not lie on the value pages, unless k is v and they are the same."""
+    pages may not lie on the value pages, unless k is v and they are the same.
+
+    With ``slots`` (int64 [T], as kv_extend gives them) row t goes to place
+    slots[t] % page_size of page slots[t] // page_size instead, and a slot below
+    zero or past the pool is skipped; no table, lengths or starts are given then."""
     what = "kv_append"
     pool = _pool(k_pages, v_pages, what)
     ks, vs = _token_rows(k, k_pages, what, "k"), _token_rows(v, k_pages, what, "v")
     if k.shape != v.shape or k.shape[1] != k_pages.shape[2]:
         raise HgkError(1, f"{what}: k and v must be [tokens, {k_pages.shape[2]}, {k_pages.shape[3]}]")
     dev = k_pages.device
+    if slots is not None:
+        if block_table is not None or kv_lens is not None or q_starts is not None:
+            raise HgkError(1, f"{what}: slots stand in place of block_table, kv_lens and q_starts")
+        if slots.dtype != torch.int64 or slots.shape != (k.shape[0],) or not slots.is_contiguous() \
+                or slots.device != dev:
+            raise HgkError(1, f"{what}: slots must be contiguous int64[{k.shape[0]}] on {dev}")
+        _kv_call(dev, lib().hgk_kv_append_slots, pool, slots.data_ptr(), k.shape[0], k.data_ptr(), ks,
+                 v.data_ptr(), vs)
+        return
+    if block_table is None or kv_lens is None:
+        raise HgkError(1, f"{what}: block_table and kv_lens, or slots, must be given")
     batch = _kv_batch(k.shape[0], block_table, kv_lens, q_starts, dev, what)
     _kv_call(dev, lib().hgk_kv_append, pool, batch, k.data_ptr(), ks, v.data_ptr(), vs)
 
@@ -671,6 +694,241 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _kv_call(dev, L.hgk_paged_attention, pool, batch, q.data_ptr(), qs, hq,
              1.0 / math.sqrt(d) if scale is None else scale, softcap, window, sinks,
              out.data_ptr(), os_, None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                            block_table: torch.Tensor, kv_lens: torch.Tensor, prefix_table: torch.Tensor,
+                            prefix_len: int, *, scale: Optional[float] = None, window: int = 0, sinks: int = 0,
+                            softcap: float = 0.0, q_starts: Optional[torch.Tensor] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention of sequences that all begin with the same ``prefix_len``
+    tokens (a host number), whose keys and values are on the pages
+    ``prefix_table`` (int32 [P]): they are read and multiplied once for the
+    whole batch. kv_lens, positions, ``window`` and ``sinks`` count from a
+    sequence's first token, prefix included, so the result is paged_attention's;
+    block_table's entries are read from position prefix_len on (one that holds
+    tokens on both sides of it is the sequence's own). A sequence shorter than
+    the prefix sees its beginning. Everything else as paged_attention."""
+    what = "shared_prefix_attention"
+    pool = _pool(k_pages, v_pages, what)
+    qs = _token_rows(q, k_pages, what, "q")
+    T, hq, d = q.shape
+    if out is None:
+        out = torch.empty((T, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise HgkError(1, f"{what}: out shape {tuple(out.shape)} is not q's")
+    if not (0 <= window < 2 ** 63 and 0 <= sinks < 2 ** 63):
+        raise HgkError(1, f"{what}: window={window}, sinks={sinks}")
+    prefix_len = operator.index(prefix_len)
+    if not 0 <= prefix_len < 2 ** 63:
+        raise HgkError(1, f"{what}: prefix_len={prefix_len}")
+    os_ = _token_rows(out, k_pages, what, "out")
+    dev = k_pages.device
+    if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous() \
+            or prefix_table.device != dev:
+        raise HgkError(1, f"{what}: prefix_table must be contiguous int32 [pages] on {dev}")
+    batch = _kv_batch(T, block_table, kv_lens, q_starts, dev, what)
+    L, pw = lib(), prefix_table.shape[0]
+    need = L.hgk_shared_prefix_attention_workspace(pool, batch, pw, prefix_len, hq, window, sinks)
+    if need < 0:  # the call refuses the same sizes, with their status
+        check(L.hgk_shared_prefix_attention(pool, batch, None, pw, prefix_len, None, None, hq, 1.0, 0.0, window,
+                                            sinks, None, None, None, 0, None))
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _kv_call(dev, L.hgk_shared_prefix_attention, pool, batch, prefix_table.data_ptr(), pw, prefix_len, q.data_ptr(),
+             qs, hq, 1.0 / math.sqrt(d) if scale is None else scale, softcap, window, sinks, out.data_ptr(), os_,
+             None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+# ---------------------------------------------------------------- pages on the GPU
+_KV_TABLES = struct.Struct("@iqPqqPPqP")
+
+
+class KVStep(NamedTuple):
+    """What kv_extend gives: a call's table, lengths, starts, places and
+    positions, and the state after it."""
+    block_table: torch.Tensor
+    kv_lens: torch.Tensor
+    q_starts: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    lens: torch.Tensor
+    n_free: torch.Tensor
+    status: torch.Tensor
+
+
+class KVState(NamedTuple):
+    """The state after kv_release."""
+    lens: torch.Tensor
+    n_free: torch.Tensor
+    status: torch.Tensor
+
+
+def _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what):
+    """The packed hgk_kv_tables, and the batch's size."""
+    dev = tables.device
+    if tables.dim() != 2 or tables.dtype != torch.int32 or (tables.shape[1] > 1 and tables.stride(1) != 1):
+        raise HgkError(1, f"{what}: tables must be int32 [sequences, pages] with a unit-stride last axis")
+    rows = tables.shape[0]
+    for name, t, shape in (("lens", lens, (rows,)), ("n_free", n_free, (1,)), ("free_pages", free_pages, None),
+                           ("seqs", seqs, None)):
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (shape and t.shape != shape):
+            raise HgkError(1, f"{what}: {name} must be contiguous int32{list(shape) if shape else '[n]'}")
+        if t.device != dev:
+            raise HgkError(1, f"{what}: operands on different devices")
+    return _KV_TABLES.pack(page_size, rows, tables.data_ptr(), tables.stride(0), tables.shape[1], lens.data_ptr(),
+                           free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr())
+
+
+def _batch_ints(t, batch, dev, what, name):
+    if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous() or t.device != dev:
+        raise HgkError(1, f"{what}: {name} must be contiguous int32[{batch}] on {dev}")
+    return t.data_ptr()
+
+
+def kv_extend(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
+              counts: torch.Tensor, page_size: int, tokens: int, *, seqs: Optional[torch.Tensor] = None,
+              inplace: bool = False) -> KVStep:
+    """Gives sequences room for their new tokens without the host: pages come
+    off a stack on the GPU, and the table, lengths, starts, places and positions
+    of a call over the new tokens are worked out there.
+
+    tables int32 [S, W] (pages of every resident sequence in order; written in
+    place), lens int32 [S] (their tokens), free_pages int32 [N] (a stack: its
+    first n_free[0] entries are free), n_free int32 [1]. ``counts`` int32 [B]
+    new tokens of the sequences in rows ``seqs`` (int32 [B], any order; without
+    it of every row). ``tokens`` rows is what the packed array of new tokens has;
+    those behind the last sequence's belong to none.
+
+    Returns KVStep: block_table [B, W] (the tables themselves without seqs; else
+    a copy of the batch's rows, -1 behind their last page), kv_lens [B],
+    q_starts [B+1], slots int64 [tokens] (page * page_size + place, -1: none),
+    positions [tokens], and the state after: lens [S], n_free [1] (new tensors,
+    or with ``inplace`` the ones given). A call that cannot be done whole changes
+    nothing and gives a step without new tokens; status [1] tells why (a sum of
+    TABLES_PAGES 1, TABLES_WIDTH 2, TABLES_SEQUENCE 4, TABLES_TOKENS 8)."""
+    what = "kv_extend"
+    state = _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what)
+    dev, rows = tables.device, tables.shape[0]
+    batch = counts.shape[0] if counts.dim() == 1 else -1
+    if seqs is not None and seqs.shape[0] != batch or seqs is None and batch != rows:
+        raise HgkError(1, f"{what}: counts for {rows if seqs is None else seqs.shape[0]} sequences expected")
+    c = _batch_ints(counts, batch, dev, what, "counts")
+    tokens = operator.index(tokens)
+    if not 0 <= tokens <= 2 ** 30:
+        raise HgkError(1, f"{what}: tokens={tokens}")
+    sizes = [batch, batch + 1, tokens, 1, batch + 1] + ([] if inplace else [rows, 1])
+    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split(sizes)
+    kv_lens, starts, positions, status, ws = parts[:5]
+    lens_out, n_out = (lens, n_free) if inplace else parts[5:]
+    slots = torch.empty((tokens,), dtype=torch.int64, device=dev)
+    table = tables if seqs is None else torch.empty((batch, tables.shape[1]), dtype=torch.int32, device=dev)
+    _kv_call(dev, lib().hgk_kv_extend, state, _ptr(seqs), c, batch, tokens, lens_out.data_ptr(), n_out.data_ptr(),
+             kv_lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+             None if seqs is None else table.data_ptr(), tables.shape[1], status.data_ptr(), ws.data_ptr())
+    return KVStep(table, kv_lens, starts, slots, positions, lens_out, n_out, status)
+
+
+def kv_release(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
+               page_size: int, *, seqs: Optional[torch.Tensor] = None, keep: Optional[torch.Tensor] = None,
+               owned_from: Optional[torch.Tensor] = None, inplace: bool = False) -> KVState:
+    """Cuts sequences down to their first ``keep`` tokens (int32 [B]; without it
+    to none: they end) and puts the pages that they no longer need on the stack
+    of free ones. tables, lens, free_pages, n_free, seqs and ``inplace`` as
+    kv_extend; the first ``owned_from`` (int32 [S]) pages of a row are not its
+    own and stay. Returns KVState: lens [S], n_free [1], status [1] (as
+    kv_extend; nothing is changed where it is not zero)."""
+    what = "kv_release"
+    state = _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what)
+    dev, rows = tables.device, tables.shape[0]
+    batch = rows if seqs is None else seqs.shape[0]
+    k = None if keep is None else _batch_ints(keep, batch, dev, what, "keep")
+    o = None if owned_from is None else _batch_ints(owned_from, rows, dev, what, "owned_from")
+    sizes = [1, batch + 1] + ([] if inplace else [rows, 1])
+    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split(sizes)
+    lens_out, n_out = (lens, n_free) if inplace else parts[2:]
+    _kv_call(dev, lib().hgk_kv_release, state, _ptr(seqs), k, o, batch, lens_out.data_ptr(), n_out.data_ptr(),
+             parts[0].data_ptr(), parts[1].data_ptr())
+    return KVState(lens_out, n_out, parts[0])
+
+
+# ---------------------------------------------------------------- routed experts
+_SCORES = {"softmax": SCORE_SOFTMAX, "sigmoid": SCORE_SIGMOID}
+
+
+def moe_route(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias: Optional[torch.Tensor] = None,
+              groups: int = 1, top_groups: int = 1, group_top: int = 1, renormalize: bool = False,
+              scale: float = 1.0):
+    """The experts of every token and their weights, from logits [..., E] (bf16,
+    f16 or f32). With s = softmax or sigmoid (``scores``) of a token's logits the
+    top_k greatest s + bias (f32 [E]) are chosen, greatest first, equal ones by
+    the lower index; with ``top_groups`` < ``groups`` only from the best of E /
+    groups experts in a row, a group counting for its greatest s + bias or the
+    sum of its two greatest (``group_top`` 1 or 2). Returns (weights f32 [..., top_k],
+    experts int32 [..., top_k]): weights are scale * s, divided by the token's sum
+    of them first with ``renormalize``. A NaN logit counts as -inf; a token without
+    any logit above -inf has weights of 0 (softmax). E up to 1024, top_k up to 64."""
+    what = "moe_route"
+    if logits.dim() < 1:
+        raise HgkError(1, f"{what}: logits must have at least 1 dimension")
+    if scores not in _SCORES:
+        raise HgkError(1, f"{what}: scores={scores!r} (softmax or sigmoid)")
+    dev = logits.device
+    rows, n, stride = _rows2d(logits)
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()
+                             or bias.device != dev):
+        raise HgkError(1, f"{what}: bias must be contiguous float32[{n}] on {dev}")
+    top_k = operator.index(top_k)
+    if not 1 <= top_k <= n:
+        raise HgkError(1, f"{what}: top_k={top_k} of {n} experts")
+    shape = (*logits.shape[:-1], top_k)
+    weights = torch.empty(shape, dtype=torch.float32, device=dev)
+    experts = torch.empty(shape, dtype=torch.int32, device=dev)
+    _kv_call(dev, lib().hgk_moe_route, dtype_code(logits.dtype), logits.data_ptr(), stride, _ptr(bias),
+             _SCORES[scores], rows, n, top_k, groups, top_groups, group_top, int(renormalize), scale,
+             weights.data_ptr(), experts.data_ptr())
+    return weights, experts
+
+
+def moe_combine(y: torch.Tensor, weights: torch.Tensor, *, shared: Optional[torch.Tensor] = None,
+                shared_gate: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = sum_i weights[t, i] * y[t * top_k + i] + sigmoid(shared_gate[t]) *
+    shared[t]: the experts' outputs y [T * top_k, H] (gather_qmm's, or [..., top_k,
+    H]) under moe_route's weights f32 [..., top_k], and the shared expert's
+    [..., H] with its gate's logits [...] or [..., 1], if given. A pair of weight
+    zero is left out, whatever its row of y holds. Sums are f32, rounded once.
+    Returns [..., H] of y's dtype; ``out`` may be ``shared``."""
+    what = "moe_combine"
+    if weights.dim() < 1 or weights.dtype != torch.float32:
+        raise HgkError(1, f"{what}: weights must be float32 [..., top_k]")
+    dev = y.device
+    rows, n, ys = _rows2d(y)
+    tokens, top_k, ws = _rows2d(weights)
+    if rows != tokens * top_k:
+        raise HgkError(1, f"{what}: {rows} rows of y for {tokens} tokens of {top_k} experts")
+    shape = (*weights.shape[:-1], n)
+    ss = gs = gd = 0
+    if shared is not None:
+        if shared.dtype != y.dtype or shared.shape != shape:
+            raise HgkError(1, f"{what}: shared must be {y.dtype} {list(shape)}")
+        ss = _rows2d(shared)[2]
+    if shared_gate is not None:
+        if shared_gate.numel() != tokens or shared_gate.shape not in (weights.shape[:-1], (*weights.shape[:-1], 1)):
+            raise HgkError(1, f"{what}: shared_gate must be {list(weights.shape[:-1])}")
+        gd = dtype_code(shared_gate.dtype)
+        gs = _rows2d(shared_gate if shared_gate.shape != weights.shape[:-1] else shared_gate.unsqueeze(-1))[2]
+    if out is None:
+        out = torch.empty(shape, dtype=y.dtype, device=dev)
+    elif out.shape != shape or out.dtype != y.dtype:
+        raise HgkError(1, f"{what}: out must be {y.dtype} {list(shape)}")
+    for t in (weights, shared, shared_gate, out):
+        if t is not None and t.device != dev:
+            raise HgkError(1, f"{what}: operands on different devices")
+    _kv_call(dev, lib().hgk_moe_combine, dtype_code(y.dtype), y.data_ptr(), ys, weights.data_ptr(), ws, top_k,
+             _ptr(shared), ss, _ptr(shared_gate), gd, gs, out.data_ptr(), _rows2d(out)[2], tokens, n)
     return out
 
 

@@ -547,6 +547,153 @@ int hgk_paged_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch, co
 int64_t hgk_paged_attention_workspace(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
                                       int64_t q_heads, int64_t window, int64_t sinks);
 
+/*
+ * hgk_kv_append by places: row t of k and v goes to token slots[t] % page_size
+ * of page slots[t] / page_size (device int64, as hgk_kv_extend writes them);
+ * a slot below zero or past the pool is skipped. No two rows may have one
+ * slot. The places are worked out once for all layers.
+ */
+int hgk_kv_append_slots(const hgk_kv_pages* pages, const int64_t* slots, int64_t tokens, const void* k,
+                        const int64_t k_strides[2], const void* v, const int64_t v_strides[2], void* stream);
+
+/*
+ * hgk_paged_attention of sequences that begin with the same tokens: keys 0 ..
+ * prefix_len - 1 of every sequence are those of the pages prefix_table[0 ..]
+ * (device int32, prefix_width entries; prefix_len is known to the host), and
+ * are read and multiplied once for all rows of the call; the sequences' own
+ * tables are read from position prefix_len on. Lengths, positions, window and
+ * sinks count from the sequences' first token, prefix included, and a row sees
+ * of the prefix what it would see of its own table: a sequence shorter than
+ * the prefix sees its beginning. The prefix may end inside a page; its last
+ * tokens are then read from the prefix's page, those behind them from the
+ * sequences' own. Everything else as hgk_paged_attention, but that the prefix's
+ * part of a row has its weights rounded to the dtype once also for single tokens.
+ */
+int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                const int32_t* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                                const void* q, const int64_t q_strides[2], int64_t q_heads, float scale,
+                                float softcap, int64_t window, int64_t sinks, void* out,
+                                const int64_t out_strides[2], void* workspace, int64_t workspace_bytes,
+                                void* stream);
+/* Bytes of device memory that call needs (0: none; -1 for sizes it refuses),
+ * from the sizes alone, as hgk_paged_attention_workspace. */
+int64_t hgk_shared_prefix_attention_workspace(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                              int64_t prefix_width, int64_t prefix_len, int64_t q_heads,
+                                              int64_t window, int64_t sinks);
+
+/* ------------------------------------------------------------------------
+ * Pages given out and taken back on the GPU.
+ *
+ * The host's part of the paged cache (which pages a sequence has, its length)
+ * for steps whose lengths only the GPU knows: tokens accepted of a draft, ends
+ * found by the sampling. Replaces the per-request caches' growth and its
+ * bookkeeping (crates/higgs-models/src/cache.rs:130-312) and the batch's
+ * lengths and offsets (crates/higgs-models/src/transformer.rs:747-802). No call
+ * waits, so a captured step may hold them.
+ *
+ * `tables` [rows, table_width] names the pages of every resident sequence in
+ * order, lens [rows] counts its tokens; free_pages [n_pages] is a stack whose
+ * first *n_free entries are free. All are device int32.
+ *
+ * A call that cannot be done whole is not done: the state stays as it was, the
+ * other outputs are those of a call without new tokens, and *status (device)
+ * tells why, a sum of HGK_TABLES_*.
+ * ------------------------------------------------------------------------ */
+typedef struct {
+  int page_size; /* tokens per page: a power of two, 1..65536 */
+  int64_t rows;  /* resident sequences, at most 2^18 */
+  int32_t* tables;
+  int64_t table_stride, table_width;
+  const int32_t* lens;
+  int32_t* free_pages;
+  int64_t n_pages;
+  const int32_t* n_free;
+} hgk_kv_tables;
+
+typedef enum {
+  HGK_TABLES_PAGES = 1,    /* too few free pages (release: more pages than the stack has room for) */
+  HGK_TABLES_WIDTH = 2,    /* a sequence outgrows its table */
+  HGK_TABLES_SEQUENCE = 4, /* a row outside the tables, or named twice, or a count below zero */
+  HGK_TABLES_TOKENS = 8    /* more new tokens than `tokens` */
+} hgk_tables_status;
+
+/*
+ * Room for counts[i] (device int32 [batch]) more tokens of the sequence in row
+ * seqs[i] (device int32 [batch]; NULL: row i, batch == rows), and what a call
+ * over them takes. Sequence by sequence, position by position, each page that
+ * is begun is taken from the top of the stack and written into the tables.
+ *   lens_out [rows], n_free_out [1]: the new state. They may be lens and n_free.
+ *   kv_lens [batch], q_starts [batch + 1]: as in hgk_kv_batch, of `tokens` rows,
+ *     of which those from q_starts[batch] on belong to no sequence
+ *   slots [tokens] (int64): page * page_size + place of each new token; -1: none
+ *   positions [tokens]: its position in its sequence (the offset of its RoPE); 0
+ *   block_table [batch, table_width], or NULL: the sequences' rows in the order
+ *     of the batch, -1 behind their last page. (Without seqs the tables are that.)
+ *   workspace: batch + 1 int32, of the call's own until its work is done
+ */
+int hgk_kv_extend(const hgk_kv_tables* tables, const int32_t* seqs, const int32_t* counts, int64_t batch,
+                  int64_t tokens, int32_t* lens_out, int32_t* n_free_out, int32_t* kv_lens,
+                  int32_t* q_starts, int64_t* slots, int32_t* positions, int32_t* block_table,
+                  int64_t block_table_stride, int32_t* status, int32_t* workspace, void* stream);
+
+/*
+ * Cuts the sequence in row seqs[i] down to its first keep[i] tokens (device
+ * int32 [batch]; NULL: none; a longer one stays as it is). Pages that then hold
+ * none of its tokens go on the stack, sequence by sequence in order, but for the
+ * first owned_from[row] (device int32 [rows], or NULL) of a row, which are not
+ * its own. The tables' entries are left. lens_out, n_free_out, status and
+ * workspace as hgk_kv_extend.
+ */
+int hgk_kv_release(const hgk_kv_tables* tables, const int32_t* seqs, const int32_t* keep,
+                   const int32_t* owned_from, int64_t batch, int32_t* lens_out, int32_t* n_free_out,
+                   int32_t* status, int32_t* workspace, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Around the routed experts' products (hgk_gather_qmm).
+ * ------------------------------------------------------------------------ */
+typedef enum { HGK_SCORE_SOFTMAX = 0, HGK_SCORE_SIGMOID = 1 } hgk_score;
+
+/*
+ * The experts of every token and their weights, from logits [tokens, n_experts]
+ * in bf16, f16 or f32 (row stride logits_row_stride). With s = softmax or
+ * sigmoid of a token's logits:
+ *   choice = s + bias (bias f32 [n_experts], or NULL: 0)
+ *   groups > top_groups: the experts lie in `groups` equal runs; a run counts
+ *     for its greatest choice, or the sum of its two greatest (group_top 1, 2),
+ *     and only those of the top_groups greatest runs may be chosen
+ *   experts [tokens, top_k] (int32): the top_k greatest choices, greatest first
+ *   weights [tokens, top_k] (f32): scale * s of them; renormalize: divided by
+ *     the sum of those s first
+ * Equal choices, and equal runs, go to the lower index. The order is that of the
+ * logits themselves, or of sums in 64 bits where something is added to scores. A
+ * NaN logit counts as -inf, of score 0; a NaN choice as the lowest. A token
+ * without a logit above -inf has softmax scores of 0. A sum of zero renormalises
+ * to zeros. At most 1024 experts, 64 groups (whose experts fill at most 16 in
+ * each of the group's share of 64 lanes) and a top_k of 64. Replaces
+ * the router of SparseMoeBlock::forward (crates/higgs-models/src/qwen3_next.rs:
+ * 949-985; qwen3_moe.rs:293-322).
+ */
+int hgk_moe_route(int dtype, const void* logits, int64_t logits_row_stride, const float* bias, int scores,
+                  int64_t tokens, int64_t n_experts, int64_t top_k, int64_t groups, int64_t top_groups,
+                  int group_top, int renormalize, float scale, float* weights, int32_t* experts,
+                  void* stream);
+
+/*
+ * The weighted sum of the experts' outputs, with the shared expert's:
+ *   out[t] = sum_i weights[t, i] * y[t * top_k + i]  (+ sigmoid(gate[t]) * shared[t])
+ * y [tokens * top_k, hidden] (as hgk_gather_qmm writes it), shared and out
+ * [tokens, hidden] in `dtype` (bf16, f16 or f32), weights f32 [tokens, top_k],
+ * shared_gate [tokens] in gate_dtype; strides are between rows. A pair whose
+ * weight is zero is left out, whatever its row holds. shared may be NULL, and
+ * shared_gate (then 1). Sums are f32 in the order i = 0, 1, ..., shared last, and
+ * are rounded once. out may be shared itself, and shares memory with nothing
+ * else. Replaces the end of SparseMoeBlock::forward (qwen3_next.rs:970-985).
+ */
+int hgk_moe_combine(int dtype, const void* y, int64_t y_row_stride, const float* weights,
+                    int64_t weights_row_stride, int64_t top_k, const void* shared, int64_t shared_row_stride,
+                    const void* shared_gate, int gate_dtype, int64_t gate_row_stride, void* out,
+                    int64_t out_row_stride, int64_t tokens, int64_t hidden, void* stream);
+
 /* ------------------------------------------------------------------------
  * Checkpoint files: the safetensors files MLX 4-bit checkpoints ship in
  * (u32-packed `.weight`, bf16/f16 `.scales`/`.biases`, bf16 norm weights).
