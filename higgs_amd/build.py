@@ -32,12 +32,12 @@ CFLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function", "-Wno-unknown-pragmas",
 ]
-# Flags of single files. attn.hip: matrix instructions keep their sums in plain
+# Flags of single files. Attention: matrix instructions keep their sums in plain
 # vector registers also where a wave has all 512. Prompts of 256 values a row
 # move fewer of them between the two halves of the register file so (8191 tokens
 # in a window with a soft cap: 575 us, without the flag 652; two prompts of 4096:
 # 352, 373); the other kernels take the same time either way.
-FILE_FLAGS = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for f in ("attn.hip", "attn_prefix.hip")}
 
 
 def hipcc() -> str:

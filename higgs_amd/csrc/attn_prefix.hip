@@ -1,0 +1,389 @@
+// attn_prefix.hip -- attention of sequences that begin with the same tokens: one
+// pass over the prefix for the rows of all sequences, one over each sequence's own
+// keys, and the join of a row's parts.
+#include "attn.h"
+
+namespace hgk {
+namespace {
+
+// References are raw scores here, whose differences are scaled: two products would
+// each be rounded, by up to 2^-8 at 2^16.
+__device__ inline float scale_of(const AttnArgs& a) {
+  return a.softcap > 0.0f ? fold_scale<1>(a).c : fold_scale<0>(a).c;
+}
+
+// The keys that a sequence's last token sees behind the prefix, or all where no pass
+// takes the prefix: index i is key i + the prefix below `sinks`, and key i + skip
+// behind them.
+__device__ inline int32_t first_behind(const AttnArgs& a) { return a.pre > 0 ? a.prefix : 0; }
+__device__ inline Seen seen_behind(const AttnArgs& a, int32_t len) {
+  const int32_t from = first_behind(a);
+  const int64_t cap = max((int64_t)a.b.width << a.p.page_shift, (int64_t)a.prefix);
+  if (len < 0) len = 0;
+  const int32_t lo = a.window > 0 && len > a.window ? len - a.window : 0;
+  const int32_t end = (int32_t)min((int64_t)len, cap), at = max(lo, from);
+  Seen s;
+  s.sinks = max(min(min(a.sinks, lo), end) - from, 0);
+  s.skip = at - s.sinks;
+  s.n = s.sinks + max(end - at, 0);
+  return s;
+}
+
+// Single tokens' own keys: WAVES waves have a chunk of a (sequence, kv head), for 16
+// of its query heads, and make one part of it.
+template <class T, int D, int CAP, int WAVES>
+__global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs a) {
+  constexpr int kKeys = dec_keys<D>(), kStep = D / 32, kTile = kKeys * dec_row<D>();
+  constexpr int kJoin = WAVES > 1 ? kDecWaves * 16 * D * 4 : 0;
+  __shared__ __align__(16) char lds[kTile * kDecWaves > kJoin ? kTile * kDecWaves : kJoin];
+  __shared__ float wref[kDecWaves][16], wsum[kDecWaves][16];
+  __shared__ int wseen[kDecWaves];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m = lane & 15, j = lane >> 4, step = WAVES > 1 ? wave : 0;
+  // chunks in the order of the sequences: those that are not there come last
+  const int unit = WAVES > 1 ? blockIdx.x : blockIdx.x * kDecWaves + wave, pairs = a.b.batch * a.p.kv_heads;
+  const int at_chunk = unit / pairs, pair = unit - at_chunk * pairs;
+  const int seq = pair / a.p.kv_heads, hk = pair - seq * a.p.kv_heads;
+  if (at_chunk >= a.splits) return;
+  Seen seen = seen_behind(a, a.b.lens[seq]);
+  seen.n = __builtin_amdgcn_readfirstlane(seen.n);
+  const int first = at_chunk * a.chunk, last = min(decode_tiles<kKeys>(seen), first + a.chunk);
+  if (first >= last && a.row_parts > 1) return;  // not a part of the row
+
+  const Scale sc = fold_scale<CAP>(a);
+  const int heads = min(16, a.group - (int)blockIdx.y * 16), h0 = hk * a.group + blockIdx.y * 16;
+  const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1]);
+  u32x4 qf[kStep];
+#pragma unroll
+  for (int s = 0; s < kStep; ++s) {
+    qf[s] = *reinterpret_cast<const u32x4*>(qp + 64 * s + 16 * j);
+    for (int w = 0; w < 4; ++w) qf[s][w] = (qf[s][w] & sc.keep) ^ sc.flip;
+  }
+  const int32_t* table = a.b.table + (int64_t)seq * a.b.table_stride;
+  const int32_t from = first_behind(a);
+  auto key_of = [&](int i) { return i < seen.sinks ? i + from : i + seen.skip; };
+  auto page_of = [&](int32_t key) { return page_behind(a, table, key); };
+  const DecodeSums<D> x = decode_walk<T, D, CAP, WAVES>(a, sc, qf, hk, first + step, last, seen.n, lds + wave * kTile,
+                                                        key_of, page_of);
+
+  // the keys of heads that the walk's form does not fit once more: the head's sums
+  // in f32, a quarter of D in each of its lanes
+  bool again = decode_odd(sc, x);
+  float acc[D / 4];
+  f32x2 rl = {x.ref, x.sum};
+  if (__any(again)) {
+    int mine = again;
+    mine |= __shfl_xor(mine, 16);
+    mine |= __shfl_xor(mine, 32);
+    again = mine != 0;
+    const f32x2 other = decode_again<T, D, CAP, WAVES>(a, sc, qp + 2 * j * (D / 4), hk, first + step, last, seen.n, key_of,
+                                                       page_of, acc);
+    if (again) rl = other;
+  }
+
+  char* out = a.out + 2 * (seq * a.ost[0] + h0 * a.ost[1]);
+  // head h's part
+  auto part_of = [&](int h) { return ((int64_t)seq * a.q_heads + h0 + h) * a.row_parts + a.pre + at_chunk; };
+  if constexpr (WAVES == 1) {
+    if (m >= heads) return;
+    if (a.row_parts > 1) {
+      const int64_t to = part_of(m);
+      float* part = a.part + to * D;
+      if (j == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * to) = f32x2{x.any ? rl[0] : -INFINITY, rl[1]};
+      if (again) {
+#pragma unroll
+        for (int d = 0; d < D / 4; ++d) part[j * (D / 4) + d] = acc[d];
+      } else {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4*>(part + 16 * t + 4 * j) = x.o[t];
+      }
+    } else {
+      const float r = x.any ? 1.0f / rl[1] : 0.0f;
+      char* row = out + 2 * m * a.ost[1];
+      if (again) {
+#pragma unroll
+        for (int d = 0; d < D / 4; d += 2)
+          *reinterpret_cast<uint32_t*>(row + 2 * (j * (D / 4) + d)) = T::pack(acc[d] * r, acc[d + 1] * r);
+      } else {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+          *reinterpret_cast<u32x2*>(row + 2 * (16 * t + 4 * j)) =
+              u32x2{T::pack(x.o[t][0] * r, x.o[t][1] * r), T::pack(x.o[t][2] * r, x.o[t][3] * r)};
+      }
+    }
+  } else {
+    __syncthreads();  // every wave is done with its V tile
+    float* wo = reinterpret_cast<float*>(lds) + wave * 16 * D + m * D;
+    if (again) {
+#pragma unroll
+      for (int d = 0; d < D / 4; ++d) wo[j * (D / 4) + d] = acc[d];
+    } else {
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) *reinterpret_cast<f32x4*>(wo + 16 * t + 4 * j) = x.o[t];
+    }
+    if (lane < 16) {
+      wref[wave][lane] = rl[0];
+      wsum[wave][lane] = rl[1];
+    }
+    if (lane == 0) wseen[wave] = x.any;
+    __syncthreads();
+    bool some = false;
+    for (int w = 0; w < kDecWaves; ++w) some |= wseen[w] != 0;
+    for (int idx = threadIdx.x; idx < heads * (D / 2); idx += 64 * kDecWaves) {
+      const int h = idx / (D / 2), d = 2 * (idx - h * (D / 2));
+      float top = wref[0][h];
+      for (int w = 1; w < kDecWaves; ++w) top = fmaxf(top, wref[w][h]);
+      float l = 0.0f, v0 = 0.0f, v1 = 0.0f;
+      for (int w = 0; w < kDecWaves; ++w) {
+        const float f = lesser((wref[w][h] - top) * sc.c);
+        const float* src = reinterpret_cast<float*>(lds) + (w * 16 + h) * D + d;
+        l = fmaf(wsum[w][h], f, l);
+        v0 = fmaf(src[0], f, v0);
+        v1 = fmaf(src[1], f, v1);
+      }
+      if (a.row_parts > 1) {
+        const int64_t to = part_of(h);
+        *reinterpret_cast<f32x2*>(a.part + to * D + d) = f32x2{v0, v1};
+        if (d == 0) *reinterpret_cast<f32x2*>(a.stat + 2 * to) = f32x2{some ? top : -INFINITY, l};
+      } else {
+        const float r = 1.0f / l;
+        *reinterpret_cast<uint32_t*>(out + 2 * (h * a.ost[1] + d)) = some ? T::pack(v0 * r, v1 * r) : 0u;
+      }
+    }
+  }
+}
+
+// out = sum_i w_i part_i / sum_i w_i sum_i over the parts of a row (token and query
+// head), w_i = 2^(c (ref_i - max)); parts that saw no key (ref = -inf) hold nothing.
+// SINGLE: of single tokens, which have the prefix's parts and those of the chunks
+// that their sequence fills, and whose two passes' weights have biases of their own.
+// G groups of D/4 threads share a row's parts, a thread has 4 values of it. The
+// parts' factors are worked out once, side by side, and kept in LDS.
+constexpr int kMaxParts = 256;
+template <int D, int G> constexpr int join_parts() { return G == 1 ? 4 : G == 2 ? 16 : kMaxParts; }
+template <class T, int D, int G, bool SINGLE>
+__global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs a, uint32_t rows) {
+  constexpr uint32_t kLanes = D / 4, kRows = 256 / (kLanes * G), kShare = kLanes * G;
+  constexpr uint32_t kMax = join_parts<D, G>(), kTurns = (kMax + kShare - 1) / kShare;
+  __shared__ f32x4 vs[kRows][G][kLanes];
+  __shared__ float refs[kRows][kMax], sums[kRows][kMax];
+  const uint32_t mine = threadIdx.x / kShare, in = threadIdx.x - mine * kShare, g = in / kLanes, c = in - g * kLanes;
+  const uint32_t row = blockIdx.x * kRows + mine;
+  const bool work = mine < kRows && row < rows;
+  const int t = work ? row / a.q_heads : 0, h = work ? row - (uint32_t)t * a.q_heads : 0;
+  const float c2 = scale_of(a);
+  int n = 0;
+  bool owned = false;
+  if (work) {
+    if constexpr (SINGLE) {
+      const int tiles = decode_tiles<dec_keys<D>()>(seen_behind(a, a.b.lens[t]));
+      n = a.pre + min((tiles + a.chunk - 1) / a.chunk, a.splits);
+      owned = true;
+    } else {
+      const KvSeq s = kv_seq(a.b, kv_row_owner(a.b, t));
+      owned = t >= s.first && t < s.first + s.n;
+      n = owned ? a.row_parts : 0;
+    }
+  }
+  const f32x2* stat = reinterpret_cast<const f32x2*>(a.stat) + (int64_t)row * a.row_parts;
+  f32x2 st[kTurns];
+#pragma unroll
+  for (uint32_t k = 0; k < kTurns; ++k) {
+    const int i = in + k * kShare;
+    if (i < n) {
+      st[k] = stat[i];
+      refs[mine][i] = st[k][0];
+    }
+  }
+  __syncthreads();
+  float top = -INFINITY;
+  for (int i = 0; i < n; ++i) top = fmaxf(top, refs[mine][i]);
+  __syncthreads();
+#pragma unroll
+  for (uint32_t k = 0; k < kTurns; ++k) {
+    const int i = in + k * kShare;
+    if (i < n) {
+      const float bias = SINGLE && i < a.pre ? Mx<T>::kDecBias - Mx<T>::kBias : 0.0f;
+      const float f = st[k][0] == -INFINITY ? 0.0f : lesser((st[k][0] - top) * c2 + bias);
+      refs[mine][i] = f;
+      sums[mine][i] = f == 0.0f ? 0.0f : st[k][1] * f;
+    }
+  }
+  __syncthreads();
+  float sum = 0.0f;
+  for (int i = 0; i < n; ++i) sum += sums[mine][i];
+  f32x4 v = {0, 0, 0, 0};
+  const float* part = a.part + (int64_t)row * a.row_parts * D + 4 * c;
+#pragma unroll 4
+  for (int i = g; i < n; i += G) {
+    const float f = refs[mine][i];
+    if (f == 0.0f) continue;  // not written
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part + (int64_t)i * D);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = fmaf(x[e], f, v[e]);
+  }
+  if constexpr (G > 1) {
+    if (mine < kRows) vs[mine][g][c] = v;
+    __syncthreads();
+    if (g > 0 || mine >= kRows) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += vs[mine][i][c][e];
+  }
+  if (!owned) return;
+  const float r = 1.0f / sum;
+  u32x2 w = {0u, 0u};
+  if (top != -INFINITY) w = u32x2{T::pack(v[0] * r, v[1] * r), T::pack(v[2] * r, v[3] * r)};
+  *reinterpret_cast<u32x2*>(a.out + 2 * (t * a.ost[0] + h * a.ost[1] + 4 * c)) = w;
+}
+
+// The split of a call, from the sizes alone.
+//
+// A pass over the prefix costs two launches more and the writing and joining of its
+// parts, so it has to save the reading of 40 MB: below, the sequences read the prefix
+// one by one, much of it from the caches (8 sequences behind 1000 tokens, 8 kv heads
+// of 64, 14 MB: 20.7 us with the pass, 13.8 without; 16 behind 2000, 8 of 128, 123
+// MB: 26.7, 32.8). Its blocks are as many as the chip holds at once.
+constexpr int64_t kPassBytes = 40 << 20, kUnits = 2048;
+struct SharedPlan {
+  int pre, splits, chunk, waves;
+  int64_t rows() const { return pre + splits > 1 ? pre + splits : 0; }
+};
+SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, int64_t q_heads, int64_t window,
+                       int64_t sinks) {
+  SharedPlan s{0, 1, 1, 1};
+  if (b.batch == 0 || b.tokens == 0) return s;
+  const int64_t group = q_heads / p.kv_heads, width = (int64_t)b.width << p.page_shift;
+  if ((b.batch - 1) * std::min(prefix, width) * p.kv_heads * p.head_dim >= kPassBytes / 4) {
+    const int64_t blocks = p.head_dim == 256 ? 256 : 512, tiles = p.kv_heads * prefix_tiles(b, group);
+    s.pre = (int)std::max<int64_t>(1, std::min<int64_t>({blocks / tiles, prefix / kMinPart, (int64_t)kMaxSplits}));
+  }
+  int64_t rest = std::max(width, prefix) - (s.pre > 0 ? prefix : 0);
+  if (window > 0 && window < rest && sinks < rest - window) rest = window + sinks;
+  if (b.starts) {
+    const int64_t n = std::min(kPromptBlocks / (p.kv_heads * prompt_tiles(b, group)), rest / kMinPart);
+    s.splits = (int)std::max<int64_t>(1, std::min<int64_t>(n, kMaxSplits));
+    return s;
+  }
+  const int64_t keys = p.head_dim == 256 ? 16 : 32, all = std::max<int64_t>((rest + keys - 1) / keys, 1);
+  const int64_t pairs = (int64_t)b.batch * p.kv_heads * ((group + 15) / 16);
+  if (s.pre == 0 && rest * p.head_dim <= (pairs >= 256 ? 1 << 17 : 1 << 16)) {
+    s.waves = kDecWaves;
+    s.chunk = (int)all;
+    return s;
+  }
+  const int64_t most = std::clamp<int64_t>(kUnits / pairs, 1, kMaxParts - kMaxSplits);
+  s.chunk = (int)std::max<int64_t>((all + most - 1) / most, 4);
+  s.splits = (int)((all + s.chunk - 1) / s.chunk);
+  return s;
+}
+int check_prefix(const char* what, const KvView& p, int64_t width, int64_t prefix) {
+  if (prefix < 0 || width < 0 || prefix > (int64_t)1 << 30 || width > (int64_t)1 << (30 - p.page_shift))
+    return fail(HGK_ERR_ARG, "%s: a prefix of %lld tokens on %lld pages", what, (long long)prefix, (long long)width);
+  if (((prefix + p.page_mask) >> p.page_shift) > width)
+    return fail(HGK_ERR_ARG, "%s: %lld pages of %d tokens do not hold a prefix of %lld", what, (long long)width,
+                p.page_mask + 1, (long long)prefix);
+  return HGK_OK;
+}
+
+template <class T, int D, int WAVES>
+void launch_behind(const AttnArgs& a, hipStream_t stream) {
+  const int64_t units = (int64_t)a.b.batch * a.p.kv_heads * a.splits;
+  const dim3 grid((unsigned)(WAVES > 1 ? units : (units + kDecWaves - 1) / kDecWaves), (a.group + 15) / 16);
+  if (a.softcap > 0.0f)
+    HGK_LAUNCH((attn_behind_kernel<T, D, kWideCap, WAVES>), grid, dim3(64 * kDecWaves), 0, stream, a);
+  else
+    HGK_LAUNCH((attn_behind_kernel<T, D, kNoCap, WAVES>), grid, dim3(64 * kDecWaves), 0, stream, a);
+}
+
+template <class T, int D, bool SINGLE>
+void launch_prefix_join(const AttnArgs& a, hipStream_t stream) {
+  constexpr int kGroups = 256 / (D / 4);
+  const uint32_t rows = (uint32_t)a.b.tokens * a.q_heads;
+  auto grid = [&](int g) { const uint32_t n = kGroups / g; return dim3((rows + n - 1) / n); };
+  if (a.row_parts > 16)
+    HGK_LAUNCH((attn_prefix_join_kernel<T, D, kGroups, SINGLE>), grid(kGroups), dim3(256), 0, stream, a, rows);
+  else if (a.row_parts > 4)
+    HGK_LAUNCH((attn_prefix_join_kernel<T, D, 2, SINGLE>), grid(2), dim3(256), 0, stream, a, rows);
+  else
+    HGK_LAUNCH((attn_prefix_join_kernel<T, D, 1, SINGLE>), grid(1), dim3(256), 0, stream, a, rows);
+}
+
+template <class T, int D>
+int run_of(const AttnArgs& a, int waves, const char* what, hipStream_t stream) {
+  if (a.pre > 0) {
+    AttnArgs of = a;
+    of.splits = a.pre;
+    launch_prompt<T, D, 64, kPrefix>(of, stream);
+    if (int st = launch_status(what)) return st;
+  }
+  if (a.b.starts) launch_prompt<T, D, 64, kBehind>(a, stream);
+  else if (waves > 1) launch_behind<T, D, kDecWaves>(a, stream);
+  else launch_behind<T, D, 1>(a, stream);
+  if (int st = launch_status(what)) return st;
+  if (a.row_parts == 1) return HGK_OK;
+  if (a.b.starts) launch_prefix_join<T, D, false>(a, stream);
+  else launch_prefix_join<T, D, true>(a, stream);
+  return launch_status(what);
+}
+
+template <class T>
+int run(const AttnArgs& a, int waves, const char* what, hipStream_t stream) {
+  switch (a.p.head_dim) {
+    case 64: return run_of<T, 64>(a, waves, what, stream);
+    case 96: return run_of<T, 96>(a, waves, what, stream);
+    case 128: return run_of<T, 128>(a, waves, what, stream);
+    default: return run_of<T, 256>(a, waves, what, stream);
+  }
+}
+
+}  // namespace
+}  // namespace hgk
+
+using namespace hgk;
+
+extern "C" int64_t hgk_shared_prefix_attention_workspace(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                                         int64_t prefix_width, int64_t prefix_len, int64_t q_heads,
+                                                         int64_t window, int64_t sinks) {
+  const char* what = "hgk_shared_prefix_attention_workspace";
+  clear_error();
+  KvView p;
+  KvBatchView b;
+  if (check_sizes(what, pages, batch, q_heads, window, sinks, &p, &b)) return -1;
+  if (check_prefix(what, p, prefix_width, prefix_len)) return -1;
+  return plan_shared(p, b, prefix_len, q_heads, window, sinks).rows() * b.tokens * q_heads * (p.head_dim + 2) * 4;
+}
+
+extern "C" int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
+                                           const int32_t* prefix_table, int64_t prefix_width, int64_t prefix_len,
+                                           const void* q, const int64_t q_strides[2], int64_t q_heads, float scale,
+                                           float softcap, int64_t window, int64_t sinks, void* out,
+                                           const int64_t out_strides[2], void* workspace, int64_t workspace_bytes,
+                                           void* stream) {
+  const char* what = "hgk_shared_prefix_attention";
+  clear_error();
+  AttnArgs a{};
+  if (int st = check_sizes(what, pages, batch, q_heads, window, sinks, &a.p, &a.b)) return st;
+  if (int st = check_prefix(what, a.p, prefix_width, prefix_len)) return st;
+  if (int st = check_scales(what, scale, softcap)) return st;
+  if (a.b.batch == 0 || a.b.tokens == 0) return HGK_OK;
+  if (prefix_len > 0 && !prefix_table) return fail(HGK_ERR_ARG, "%s: null prefix table", what);
+  if (int st = check_call(what, &a, q, q_strides, q_heads, scale, softcap, window, sinks, out, out_strides)) return st;
+  const SharedPlan s = plan_shared(a.p, a.b, prefix_len, q_heads, window, sinks);
+  const int64_t rows = s.rows() * a.b.tokens * q_heads, need = rows * (a.p.head_dim + 2) * 4;
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return fail(HGK_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
+  a.prefix_table = prefix_table;
+  a.prefix_width = (int32_t)prefix_width;
+  a.prefix = (int32_t)prefix_len;
+  a.pre = s.pre;
+  a.splits = s.splits;
+  a.chunk = s.chunk;
+  a.row_parts = s.pre + s.splits;
+  a.part = static_cast<float*>(workspace);
+  a.stat = rows > 0 ? a.part + rows * a.p.head_dim : nullptr;
+  return pages->dtype == DT_BF16 ? run<BF16>(a, s.waves, what, as_stream(stream))
+                                 : run<F16>(a, s.waves, what, as_stream(stream));
+}
