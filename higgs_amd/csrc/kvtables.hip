@@ -8,7 +8,7 @@
 namespace hgk {
 namespace {
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kMaxRows = 1 << 18, kFill = 256;
+constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kMaxRows = 1 << 18, kFill = 256, kNear = 4096;
 
 struct TablesView {
   int32_t* table;
@@ -168,9 +168,17 @@ __global__ __launch_bounds__(kFill) void kv_extend_kernel(ExtendArgs x) {
   const PlanArgs& a = x.p;
   const int32_t top = *a.n_free_out + a.page_starts[a.batch];
   if ((int)blockIdx.x < x.token_blocks) {
+    // the starts, where they fit: a search is a chain of reads
+    __shared__ int32_t near[kNear + 1];
+    const bool cached = a.batch <= kNear;
+    if (cached) {
+      for (int i = threadIdx.x; i <= a.batch; i += kFill) near[i] = a.q_starts[i];
+      __syncthreads();
+    }
+    const int32_t* starts = cached ? near : a.q_starts;
     const int t = blockIdx.x * kFill + threadIdx.x;
     if (t >= a.tokens) return;
-    if (t >= a.q_starts[a.batch]) {
+    if (t >= starts[a.batch]) {
       x.slots[t] = -1;
       x.positions[t] = 0;
       return;
@@ -178,10 +186,10 @@ __global__ __launch_bounds__(kFill) void kv_extend_kernel(ExtendArgs x) {
     int lo = 0, hi = a.batch;  // the last sequence that starts at t or before
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (a.q_starts[mid] <= t) lo = mid;
+      if (starts[mid] <= t) lo = mid;
       else hi = mid;
     }
-    const int32_t first = a.q_starts[lo], n = a.q_starts[lo + 1] - first, old = a.kv_lens[lo] - n;
+    const int32_t first = starts[lo], n = starts[lo + 1] - first, old = a.kv_lens[lo] - n;
     const int32_t row = a.seqs ? a.seqs[lo] : lo, pos = old + t - first, e = pos >> a.t.shift;
     const int32_t at = pos & ((1 << a.t.shift) - 1);
     const int32_t page = entry_of(a, top, row, pages_of(a.t, old), a.page_starts[lo], e);

@@ -2,6 +2,7 @@
 // token's experts with their weights, and the weighted sum of their outputs.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/higgs_hip.h"
 #include "hgk_common.h"
@@ -19,7 +20,7 @@ struct RouteArgs {
   int64_t row;  // elements between logits of two tokens
   int64_t tokens;
   int32_t n, top_k, groups, top_groups, group_top, group_size;
-  int32_t sigmoid, renormalize;
+  int32_t sigmoid, renormalize, group_bits, pieces, bias_pieces;
   float scale;
 };
 
@@ -81,18 +82,17 @@ __device__ inline uint32_t fold_min(uint32_t v) {
   return fold<BITS>(v, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
 }
 
-// A choice as whole numbers in the same order, none of them 0: that is a choice
-// that has been taken. NaN counts as the lowest.
+// A choice as whole numbers in the same order, none of them 0 (NaN has been put
+// below all others).
 __device__ inline uint32_t key_of(float x) {
-  if (x != x) x = -INFINITY;
   const uint32_t b = f2u(x == 0.0f ? 0.0f : x);  // one zero
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ inline uint64_t key_of(double x) {
-  if (x != x) x = -INFINITY;
   const uint64_t b = __builtin_bit_cast(uint64_t, x == 0.0 ? 0.0 : x);
   return b >> 63 ? ~b : b | 1ull << 63;
 }
+__device__ inline float value_of(uint32_t key) { return u2f(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
 // Of the 2^BITS lanes' (key, index), the index of the greatest key, the lowest
 // one of several.
@@ -108,93 +108,41 @@ __device__ inline uint32_t best_of(uint64_t key, uint32_t index) {
   return fold_min<BITS>(hi == top && lo == low ? index : ~0u);
 }
 
-template <class V> struct KeyOf;
-template <> struct KeyOf<float> { typedef uint32_t type; };
-template <> struct KeyOf<double> { typedef uint64_t type; };
-
-// 2^BITS lanes have a token; a lane has PER experts in a row, of one group. V:
-// the type of the choices. Where nothing is added to the scores they are in the
-// order of the logits, which are compared as they are; where a bias or a second
-// score is added, two sums may lie closer than f32 holds scores, and are 64 bits.
-// A round takes the best choice left, its expert found by two folds over the
-// lanes, and the lane that had it looks for its next best.
-template <class T, class V, int BITS, int PER>
-__global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
-  typedef typename KeyOf<V>::type Key;
-  constexpr int W = 1 << BITS;
-  const int sub = threadIdx.x & (W - 1);
-  const int64_t token = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
-  const char* row = a.logits + (token < a.tokens ? token : 0) * a.row * T::kBytes;
-
-  // lanes of a group, and this lane's experts
-  int gbits = BITS;
-  while (gbits > 0 && (a.groups << gbits) > W) --gbits;
-  const int group = sub >> gbits, in = (sub & ((1 << gbits) - 1)) * PER;
-  const int e0 = group * a.group_size + in;
-  const int mine = group < a.groups ? min(max(a.group_size - in, 0), PER) : 0;
-
-  float x[PER];
+// The sum of a group's two greatest choices, or its greatest: over a lane's choices,
+// then over the group's 2^gbits lanes.
+template <int BITS, int PER, class V>
+__device__ inline V group_score(const V* c, int gbits, int group_top) {
+  V b1 = -INFINITY, b2 = -INFINITY;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    x[i] = i < mine ? load1<T>(row, e0 + i) : -INFINITY;
-    if (x[i] != x[i]) x[i] = -INFINITY;
+    b2 = fmax(b2, fmin(b1, c[i]));
+    b1 = fmax(b1, c[i]);
   }
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) top = fmaxf(top, x[i]);
-  top = fold<BITS>(top, [](float p, float q) { return fmaxf(p, q); });
+  auto join = [&](V p, V q) {
+    b2 = fmax(fmin(b1, p), fmax(b2, q));
+    b1 = fmax(b1, p);
+  };
+  if (gbits > 0) join(partner<0>(b1), partner<0>(b2));
+  if (gbits > 1) join(partner<1>(b1), partner<1>(b2));
+  if (gbits > 2) join(partner<2>(b1), partner<2>(b2));
+  if (gbits > 3) join(partner<3>(b1), partner<3>(b2));
+  if constexpr (BITS > 4)
+    if (gbits > 4) join(partner<4>(b1), partner<4>(b2));
+  return group_top == 2 ? b1 + b2 : b1;
+}
 
-  // choices
-  V c[PER];
-  double whole = 1.0;  // softmax: the sum over all experts
-  if constexpr (sizeof(V) == 4) {
-#pragma unroll
-    for (int i = 0; i < PER; ++i) c[i] = x[i];
-  } else {
-    if (a.sigmoid) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) c[i] = 1.0 / (1.0 + exp(-(double)x[i]));
-    } else {
-      double part = 0.0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        c[i] = x[i] == -INFINITY ? 0.0 : x[i] == top ? 1.0 : exp((double)x[i] - (double)top);
-        part += c[i];
-      }
-      whole = fold<BITS>(part, [](double p, double q) { return p + q; });
-      if (whole == 0.0) whole = 1.0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) c[i] /= whole;
-    }
-    if (a.bias) {
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i < mine) c[i] += (double)a.bias[e0 + i];
-    }
-  }
+// The choice to the last bit: the keys hold all of it. c: -inf where a lane has no
+// expert. Returns lane r's expert.
+template <int BITS, int PER, class V, class E>
+__device__ __forceinline__ uint32_t choose_exact(const RouteArgs& a, const V (&c)[PER], int sub, int group,
+                                                           int gbits, int mine, E expert_of) {
+  typedef decltype(key_of(V())) Key;
   Key key[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) key[i] = i < mine ? key_of(c[i]) : 0;
-
-  // groups: all but the best are taken out
   if (a.top_groups < a.groups) {
-    V b1 = -INFINITY, b2 = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const V v = i < mine && c[i] == c[i] ? c[i] : -INFINITY;
-      b2 = fmax(b2, fmin(b1, v));
-      b1 = fmax(b1, v);
-    }
-    auto join = [&](V p, V q) {
-      b2 = fmax(fmin(b1, p), fmax(b2, q));
-      b1 = fmax(b1, p);
-    };
-    if (gbits > 0) join(partner<0>(b1), partner<0>(b2));
-    if (gbits > 1) join(partner<1>(b1), partner<1>(b2));
-    if (gbits > 2) join(partner<2>(b1), partner<2>(b2));
-    if (gbits > 3) join(partner<3>(b1), partner<3>(b2));
-    if constexpr (BITS > 4) if (gbits > 4) join(partner<4>(b1), partner<4>(b2));
-    Key left = group < a.groups ? key_of(a.group_top == 2 ? b1 + b2 : b1) : 0;
+    const V score = group_score<BITS, PER>(c, gbits, a.group_top);
+    Key left = group < a.groups ? key_of(score) : 0;
     bool kept = false;
     for (int r = 0; r < a.top_groups; ++r)
       if (best_of<BITS>(left, (uint32_t)group) == (uint32_t)group) {
@@ -204,27 +152,274 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
 #pragma unroll
     for (int i = 0; i < PER; ++i) key[i] = kept ? key[i] : 0;
   }
-
-  Key best = 0;
-  uint32_t at = 0;
-  auto look = [&]() {
-    best = key[0];
-    at = 0;
+  uint32_t got = 0;
+  for (int r = 0; r < a.top_k; ++r) {
+    Key best = 0;
+    uint32_t e = ~0u;
 #pragma unroll
-    for (int i = 1; i < PER; ++i) {
-      at = key[i] > best ? i : at;
+    for (int i = 0; i < PER; ++i) {
+      e = key[i] > best ? expert_of(i) : e;
       best = key[i] > best ? key[i] : best;
     }
-  };
-  look();
-  uint32_t expert = 0;
-  for (int r = 0; r < a.top_k; ++r) {
-    const uint32_t w = best_of<BITS>(best, e0 + at);
-    if (sub == r) expert = w;
-    if (w == e0 + at && best != 0) {
+    const uint32_t w = best_of<BITS>(best, e);
+    if (sub == r) got = w;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) key[i] = at == (uint32_t)i ? 0 : key[i];
-      look();
+    for (int i = 0; i < PER; ++i) key[i] = expert_of(i) == w ? 0 : key[i];
+  }
+  return got;
+}
+
+// 2^BITS lanes have a token, a lane PER experts of one group: pieces of V in a row,
+// side by side over the group's lanes.
+//
+// Where nothing is added to the scores (SUMS false) they are in the order of the
+// logits, and those are compared. Else two sums may lie closer than f32 holds
+// scores: their order is that of 64 bits.
+//
+// Both are first tried on 32-bit keys: 22 bits of the choice and the expert's number,
+// so that one fold over the lanes finds the best choice with its expert, ties by the
+// lower one. The next best is the greatest of (key - last best) modulo 2^32: what
+// has been taken wraps to the bottom. All of a 16-bit logit is in the upper 22 bits
+// of its f32 form. Other choices are brought to 2^22 equal steps of their range;
+// ones that follow each other by less than the steps' and the f32 sums' errors leave
+// the order open: those are put in the order of their whole choices, and where that
+// is not enough (a chain of them reaches past the last one looked at, or groups'
+// scores are as close) the wave takes its tokens again with whole keys.
+//
+// Bound by the folds' and keys' instructions. 16384 tokens of 256 experts in f32, 4
+// of 8 groups, top 8, with a bias: 16 us, of which the reading of the logits would
+// be 3.5; a wave a token and whole keys for all 34.0.
+constexpr int kSpare = 2;
+template <class T, bool SUMS, int BITS, int PER>
+__global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
+  constexpr int W = 1 << BITS, V = PER < 16 / T::kBytes ? PER : 16 / T::kBytes;
+  constexpr bool kWhole = !SUMS && T::kBytes == 2;  // the short keys hold all
+  const int sub = threadIdx.x & (W - 1);
+  const int64_t token = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
+  const char* row = a.logits + (token < a.tokens ? token : 0) * a.row * T::kBytes;
+
+  // lanes of a group, and this lane's experts: its i-th is expert_of(i) for i < mine
+  const int gbits = a.group_bits, group = sub >> gbits, in = sub & ((1 << gbits) - 1);
+  const uint32_t e0 = group * a.group_size + in * V;
+  auto place = [&](int i) { return (i / V) * (V << gbits) + i % V; };  // from e0
+  auto expert_of = [&](int i) { return e0 + place(i); };
+  int mine = 0;
+  if (group < a.groups)
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mine += in * V + place(i) < a.group_size;
+
+  float x[PER];
+  if (a.pieces) {  // whole pieces, aligned
+#pragma unroll
+    for (int i = 0; i < PER; i += V) {
+      const int64_t at = i < mine ? expert_of(i) : 0;
+      if constexpr (V * T::kBytes == 16) {
+        const u32x4 r = ld16<T>(row, at);
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[i + k] = elem<T>(r, k);
+      } else {
+        static_assert(V * T::kBytes == 8, "pieces of 8 or 16 bytes");
+        const u32x2 r = ld_raw<8>(row, at * T::kBytes);
+#pragma unroll
+        for (int k = 0; k < V; ++k) x[i + k] = elem<T>(r, k);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) x[i] = load1<T>(row, i < mine ? expert_of(i) : 0);
+  }
+  float top = -INFINITY;
+  uint32_t lost = 0;  // bits of the logits behind the first 22
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (i >= mine || x[i] != x[i]) x[i] = -INFINITY;
+    top = fmaxf(top, x[i]);
+    lost |= f2u(x[i]);
+  }
+  top = fold<BITS>(top, [](float p, float q) { return fmaxf(p, q); });
+  lost &= 0x3ffu;
+
+  // softmax's sum, where scores themselves count
+  float whole = 0.0f, e[PER];
+  if (!a.sigmoid && (SUMS || !a.renormalize)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      e[i] = x[i] == -INFINITY ? 0.0f : x[i] == top ? 1.0f : exp_f32(x[i] - top);
+      whole += e[i];
+    }
+    whole = fold<BITS>(whole, [](float p, float q) { return p + q; });
+  }
+
+  // choices, to f32's rounding
+  float c[PER], bias[PER];
+  if constexpr (SUMS) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) bias[i] = 0.0f;
+    if (a.bias && a.bias_pieces) {
+#pragma unroll
+      for (int i = 0; i < PER; i += 4) {
+        const u32x4 r = ld16<F32>(a.bias, i < mine ? expert_of(i) : 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bias[i + k] = u2f(r[k]);
+      }
+    } else if (a.bias) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) bias[i] = a.bias[i < mine ? expert_of(i) : 0];
+    }
+    if (a.sigmoid) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i] * -kLog2e));
+    } else {
+      const float r = whole > 0.0f ? __builtin_amdgcn_rcpf(whole) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c[i] = e[i] * r;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      c[i] += bias[i];
+      if (i >= mine || c[i] != c[i]) c[i] = -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) c[i] = x[i];
+  }
+  // 22 bits of every choice: those of its f32 form, or 2^22 steps of the choices'
+  // range (its upper 16, if it is greater)
+  if constexpr (!kWhole && !SUMS) lost = fold<BITS>(lost, [](uint32_t p, uint32_t q) { return p | q; });
+  const bool steps = SUMS || (!kWhole && lost != 0);
+  float low = INFINITY, high = -INFINITY, per = 0.0f, err = 0.0f;  // err: of the sums, in f32
+  if constexpr (!kWhole) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      low = fminf(low, i < mine ? c[i] : INFINITY);
+      high = fmaxf(high, c[i]);
+    }
+    low = fold<BITS>(low, [](float p, float q) { return fminf(p, q); });
+    high = fold<BITS>(high, [](float p, float q) { return fmaxf(p, q); });
+    low = fmaxf(low, high - 16.0f);
+    // a sigmoid is good to 2^-22 (its exponential's 2^-23 counts for a quarter, the sum
+    // and the reciprocal for 2^-24 and 2^-23), a softmax score to 2^-19 (a sum of up
+    // to 1024), and their sum with the bias is rounded
+    if constexpr (SUMS) err = fmaxf(fabsf(low), fabsf(high)) * 0x1p-24f + (a.sigmoid ? 0x1p-22f : 0x1p-19f);
+    per = high > low && high < INFINITY ? 4194200.0f / (high - low) : 0.0f;
+  }
+  const float margin = fmaf(2.0f * err, per, 3.0f);  // in steps: two roundings, and one (NaN beside an infinity)
+  bool again = false;
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    uint32_t k = 0;
+    if constexpr (!kWhole)
+      if (steps) k = 2u + (uint32_t)__builtin_amdgcn_fmed3f((c[i] - low) * per, 0.0f, 4194200.0f);
+    if constexpr (!SUMS)
+      if (!steps) k = key_of(c[i]) >> 10;
+    key[i] = i < mine ? k << 10 | (1023u - expert_of(i)) : 0u;
+  }
+
+  // groups: all but the best are taken out
+  if (a.top_groups < a.groups) {
+    const float score = group_score<BITS, PER>(c, gbits, a.group_top);
+    uint32_t left = group < a.groups ? key_of(score) : 0u;
+    bool kept = false;
+    uint32_t w = 0;
+    for (int r = 0; r < a.top_groups; ++r) {
+      w = fold_max<BITS>(left);
+      if (fold_min<BITS>(left == w ? (uint32_t)group : ~0u) == (uint32_t)group) {
+        kept = true;
+        left = 0;
+      }
+    }
+    if constexpr (SUMS) {  // the best of the others
+      const uint32_t next = fold_max<BITS>(left);
+      const float p = value_of(w), q = value_of(next);
+      if (next) again = !(p - q > fmaf(fabsf(p) + fabsf(q), 0x1p-22f, 5.0f * err));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) key[i] = kept ? key[i] : 0u;
+  }
+
+  // Lane r takes the r-th best, a few more than are asked for where they may have to
+  // change places. chain: how many in front of the last all leave their order open.
+  const int rounds = kWhole ? a.top_k : min(a.top_k + kSpare, W);
+  uint32_t expert = 0, last = 0;
+  int chain = 0;
+  bool swap = false, got = false;
+  for (int r = 0; r < rounds; ++r) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i += 2) best = max(best, max(key[i] - last, key[i + 1] - last));
+    uint32_t w = fold_max<BITS>(best) + last;
+    if (r > 0) {
+      if (w >= last) w = 0;  // nothing is left
+      if constexpr (!kWhole) {
+        const bool open = steps && w && !((float)(last >> 10) - (float)(w >> 10) > margin);
+        swap |= open && r <= a.top_k;
+        chain = open ? chain + 1 : 0;
+      }
+    }
+    if (sub == r) {
+      expert = 1023u - (w & 1023u);
+      got = w != 0;
+    }
+    last = w;
+  }
+  if constexpr (!kWhole) {
+    // the last of them may be one of the best, and so may others behind it
+    again |= last && steps && chain >= rounds - a.top_k;
+    if (__any(swap)) {
+      // those taken in the order of their whole choices
+      typedef typename std::conditional<SUMS, double, float>::type V;
+      V mine_is = got ? (V)load1<T>(row, expert) : (V)-INFINITY;
+      if (mine_is != mine_is) mine_is = -INFINITY;
+      if constexpr (SUMS) {
+        again |= !a.sigmoid;  // (softmax: of a sum over all experts)
+        mine_is = 1.0 / (1.0 + exp(-mine_is));
+        if (a.bias) mine_is += (double)a.bias[got ? expert : 0];
+        if (mine_is != mine_is) mine_is = -INFINITY;
+      }
+      int rank = 0;
+      for (int r = 0; r < rounds; ++r) {
+        const V other = __shfl(mine_is, r, W);
+        const uint32_t of = __shfl(got ? expert : ~0u, r, W);
+        rank += of != ~0u && (other > mine_is || (other == mine_is && of < expert));
+      }
+      // lane r takes the expert of the lane whose rank is r
+      uint32_t sorted = expert;
+      for (int r = 0; r < rounds; ++r) {
+        const int to = __shfl(got ? rank : -1, r, W);
+        const uint32_t of = __shfl(expert, r, W);
+        sorted = to == sub ? of : sorted;
+      }
+      expert = sorted;
+    }
+  }
+  if constexpr (!kWhole) {
+    if (__any(again)) {
+      if constexpr (SUMS) {
+        double d[PER], sum = 0.0;
+        if (a.sigmoid) {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) d[i] = 1.0 / (1.0 + exp(-(double)x[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            d[i] = x[i] == -INFINITY ? 0.0 : x[i] == top ? 1.0 : exp((double)x[i] - (double)top);
+            sum += d[i];
+          }
+          sum = fold<BITS>(sum, [](double p, double q) { return p + q; });
+#pragma unroll
+          for (int i = 0; i < PER; ++i) d[i] = sum > 0.0 ? d[i] / sum : 0.0;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          d[i] += (double)bias[i];
+          if (i >= mine || d[i] != d[i]) d[i] = -INFINITY;
+        }
+        expert = choose_exact<BITS, PER>(a, d, sub, group, gbits, mine, expert_of);
+      } else {
+        expert = choose_exact<BITS, PER>(a, c, sub, group, gbits, mine, expert_of);
+      }
     }
   }
 
@@ -234,22 +429,12 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
   if (l != l) l = -INFINITY;
   if (a.sigmoid) {
     // of a large negative logit the exponential is the score
-    const float e = exp_f32(-fabsf(l));
-    s = (l < 0.0f ? e : 1.0f) / (1.0f + e);
+    const float f = exp_f32(-fabsf(l));
+    s = (l < 0.0f ? f : 1.0f) / (1.0f + f);
   } else {
-    // (renormalised weights are of no sum over all experts)
+    // (renormalised weights need no sum over all experts)
     s = l == -INFINITY ? 0.0f : l == top ? 1.0f : exp_f32(l - top);
-    if (!a.renormalize) {
-      if constexpr (sizeof(V) == 4) {
-        float part = 0.0f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) part += x[i] == -INFINITY ? 0.0f : x[i] == top ? 1.0f : exp_f32(x[i] - top);
-        part = fold<BITS>(part, [](float p, float q) { return p + q; });
-        s = part > 0.0f ? s / part : 0.0f;
-      } else {
-        s /= (float)whole;
-      }
-    }
+    if (!a.renormalize) s = whole > 0.0f ? s / whole : 0.0f;
   }
   if (a.renormalize) {
     const float sum = fold<BITS>(has ? s : 0.0f, [](float p, float q) { return p + q; });
@@ -263,28 +448,43 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
 
 constexpr int kRouteExperts = 1024, kRouteTopK = 64;
 
-template <class T, class V, int BITS, int PER>
-void launch_route(const RouteArgs& a, hipStream_t stream) {
-  constexpr int kTokens = 256 >> BITS;
-  HGK_LAUNCH((moe_route_kernel<T, V, BITS, PER>), dim3((unsigned)((a.tokens + kTokens - 1) / kTokens)), dim3(256), 0,
+// How a token's experts lie on lanes: 2^bits lanes, per of them each.
+struct RoutePlan {
+  int bits, group_bits, per;
+};
+RoutePlan plan_route(int64_t groups, int64_t group_size, int64_t top_k, int bits) {
+  RoutePlan p{bits, bits, 0};
+  while (p.group_bits >= 0 && groups << p.group_bits > 1 << bits) --p.group_bits;
+  // (with the choices looked at beyond the top_k, where there are lanes for them)
+  if (p.group_bits < 0 || (bits < 6 && top_k + kSpare > 1 << bits)) return p;  // per 0: does not fit
+  const int64_t lanes = 1 << p.group_bits, per = (group_size + lanes - 1) / lanes;
+  // pieces of 4 to 8 are whole: such a lane has room for 4, 8 or 16
+  p.per = per <= 4 ? 4 : per <= 8 ? 8 : per <= 16 ? 16 : 0;
+  return p;
+}
+
+template <class T, bool SUMS, int BITS, int PER>
+void launch_route(RouteArgs a, hipStream_t stream) {
+  constexpr int kTokens = 256 >> BITS, V = PER < 16 / T::kBytes ? PER : 16 / T::kBytes;
+  a.pieces = a.group_size % V == 0 && a.row % V == 0 &&
+             (reinterpret_cast<uintptr_t>(a.logits) & (V * T::kBytes - 1)) == 0;
+  a.bias_pieces = a.pieces && aligned16(a.bias);
+  HGK_LAUNCH((moe_route_kernel<T, SUMS, BITS, PER>), dim3((unsigned)((a.tokens + kTokens - 1) / kTokens)), dim3(256), 0,
              stream, a);
 }
-template <class T, class V>
-void route_of(const RouteArgs& a, hipStream_t stream) {
-  // experts that a lane of 64 has, when groups keep to lanes of their own
-  int lanes = 64;
-  while (lanes > 1 && a.groups * lanes > 64) lanes >>= 1;
-  const int per = (a.group_size + lanes - 1) / lanes;
-  if (per <= 1) launch_route<T, V, 6, 1>(a, stream);
-  else if (per <= 2) launch_route<T, V, 6, 2>(a, stream);
-  else if (per <= 4) launch_route<T, V, 6, 4>(a, stream);
-  else if (per <= 8) launch_route<T, V, 6, 8>(a, stream);
-  else launch_route<T, V, 6, 16>(a, stream);
+template <class T, bool SUMS>
+void route_of(const RouteArgs& a, const RoutePlan& p, hipStream_t stream) {
+  if (p.bits == 4 && p.per == 4) launch_route<T, SUMS, 4, 4>(a, stream);
+  else if (p.bits == 4 && p.per == 8) launch_route<T, SUMS, 4, 8>(a, stream);
+  else if (p.bits == 4) launch_route<T, SUMS, 4, 16>(a, stream);
+  else if (p.bits == 5) launch_route<T, SUMS, 5, 16>(a, stream);
+  else if (p.per == 4) launch_route<T, SUMS, 6, 4>(a, stream);
+  else launch_route<T, SUMS, 6, 16>(a, stream);
 }
 template <class T>
-void route_as(const RouteArgs& a, bool wide, hipStream_t stream) {
-  if (wide) route_of<T, double>(a, stream);
-  else route_of<T, float>(a, stream);
+void route_as(const RouteArgs& a, const RoutePlan& p, bool sums, hipStream_t stream) {
+  if (sums) route_of<T, true>(a, p, stream);
+  else route_of<T, false>(a, p, stream);
 }
 
 // ---------------------------------------------------------------- the sum
@@ -308,7 +508,7 @@ __device__ inline float gate_of(const CombineArgs& a, int64_t t) {
 
 // Block = (token, columns); a thread sums a 16-byte piece of the token's rows, up
 // to kRows of them in flight. The rows are read once: past the caches.
-constexpr int kCombineThreads = 128, kRows = 4;
+constexpr int kCombineThreads = 64, kRows = 8;
 template <class T>
 __global__ __launch_bounds__(kCombineThreads) void moe_combine_kernel(CombineArgs a, uint32_t pieces, int64_t blocks) {
   constexpr int N = Vec<T>::N;
@@ -398,10 +598,11 @@ extern "C" int hgk_moe_route(int dtype, const void* logits, int64_t logits_row_s
     return fail(HGK_ERR_ARG, "%s: group_top=%d of groups of %lld", what, group_top, (long long)(n_experts / groups));
   if (!std::isfinite(scale)) return fail(HGK_ERR_ARG, "%s: scale must be finite", what);
   if (logits_row_stride < 0) return fail(HGK_ERR_ARG, "%s: negative row stride", what);
-  // lanes of a group hold at most 16 experts each
-  int lanes = 64;
-  while (groups * lanes > 64) lanes >>= 1;
-  if ((n_experts / groups + lanes - 1) / lanes > 16)
+  // As few lanes a token as hold its experts: rounds of a small fold, tokens side by
+  // side. (Not by the tokens' number: a token's bits are the same in every batch.)
+  RoutePlan plan{};
+  for (int bits = 4; bits <= 6 && !plan.per; ++bits) plan = plan_route(groups, n_experts / groups, top_k, bits);
+  if (!plan.per)
     return fail(HGK_ERR_UNSUPPORTED, "%s: %lld groups of %lld experts", what, (long long)groups, (long long)(n_experts / groups));
   if (tokens > INT32_MAX) return fail(HGK_ERR_ARG, "%s: %lld tokens are too many", what, (long long)tokens);
   if (tokens == 0) return HGK_OK;
@@ -410,12 +611,12 @@ extern "C" int hgk_moe_route(int dtype, const void* logits, int64_t logits_row_s
     return fail(HGK_ERR_ARG, "%s: operands must be aligned to their elements", what);
   RouteArgs a{static_cast<const char*>(logits), bias, weights, experts, logits_row_stride, tokens, (int32_t)n_experts,
               (int32_t)top_k, (int32_t)groups, (int32_t)top_groups, group_top, (int32_t)(n_experts / groups),
-              scores == HGK_SCORE_SIGMOID, renormalize != 0, scale};
-  const bool wide = bias || (group_top == 2 && top_groups < groups);
+              scores == HGK_SCORE_SIGMOID, renormalize != 0, plan.group_bits, 0, 0, scale};
+  const bool sums = bias || (group_top == 2 && top_groups < groups);
   switch (dtype) {
-    case DT_BF16: route_as<BF16>(a, wide, as_stream(stream)); break;
-    case DT_F16: route_as<F16>(a, wide, as_stream(stream)); break;
-    default: route_as<F32>(a, wide, as_stream(stream)); break;
+    case DT_BF16: route_as<BF16>(a, plan, sums, as_stream(stream)); break;
+    case DT_F16: route_as<F16>(a, plan, sums, as_stream(stream)); break;
+    default: route_as<F32>(a, plan, sums, as_stream(stream)); break;
   }
   return launch_status(what);
 }

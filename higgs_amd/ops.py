@@ -770,6 +770,8 @@ def _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what):
     dev = tables.device
     if tables.dim() != 2 or tables.dtype != torch.int32 or (tables.shape[1] > 1 and tables.stride(1) != 1):
         raise HgkError(1, f"{what}: tables must be int32 [sequences, pages] with a unit-stride last axis")
+    if not 1 <= page_size <= 65536:
+        raise HgkError(1, f"{what}: page_size={page_size} must be a power of two in 1..65536")
     rows = tables.shape[0]
     for name, t, shape in (("lens", lens, (rows,)), ("n_free", n_free, (1,)), ("free_pages", free_pages, None),
                            ("seqs", seqs, None)):
@@ -820,15 +822,21 @@ def kv_extend(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor
     tokens = operator.index(tokens)
     if not 0 <= tokens <= 2 ** 30:
         raise HgkError(1, f"{what}: tokens={tokens}")
-    sizes = [batch, batch + 1, tokens, 1, batch + 1] + ([] if inplace else [rows, 1])
-    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split(sizes)
-    kv_lens, starts, positions, status, ws = parts[:5]
-    lens_out, n_out = (lens, n_free) if inplace else parts[5:]
+    # one array for the small results, and the call's workspace at its end
+    sizes = [batch, batch + 1, tokens, 1] if inplace else [batch, batch + 1, tokens, 1, rows, 1]
+    ints = torch.empty((sum(sizes) + batch + 1,), dtype=torch.int32, device=dev)
+    parts = ints.split_with_sizes([*sizes, batch + 1])
+    kv_lens, starts, positions, status = parts[:4]
+    lens_out, n_out = (lens, n_free) if inplace else parts[4:6]
     slots = torch.empty((tokens,), dtype=torch.int64, device=dev)
-    table = tables if seqs is None else torch.empty((batch, tables.shape[1]), dtype=torch.int32, device=dev)
-    _kv_call(dev, lib().hgk_kv_extend, state, _ptr(seqs), c, batch, tokens, lens_out.data_ptr(), n_out.data_ptr(),
+    if seqs is None:
+        table, rows_of = tables, 0
+    else:
+        table = torch.empty((batch, tables.shape[1]), dtype=torch.int32, device=dev)
+        rows_of = seqs.data_ptr()
+    _kv_call(dev, lib().hgk_kv_extend, state, rows_of, c, batch, tokens, lens_out.data_ptr(), n_out.data_ptr(),
              kv_lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-             None if seqs is None else table.data_ptr(), tables.shape[1], status.data_ptr(), ws.data_ptr())
+             table.data_ptr() if rows_of else 0, tables.shape[1], status.data_ptr(), parts[-1].data_ptr())
     return KVStep(table, kv_lens, starts, slots, positions, lens_out, n_out, status)
 
 
@@ -847,8 +855,8 @@ def kv_release(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tenso
     batch = rows if seqs is None else seqs.shape[0]
     k = None if keep is None else _batch_ints(keep, batch, dev, what, "keep")
     o = None if owned_from is None else _batch_ints(owned_from, rows, dev, what, "owned_from")
-    sizes = [1, batch + 1] + ([] if inplace else [rows, 1])
-    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split(sizes)
+    sizes = [1, batch + 1] if inplace else [1, batch + 1, rows, 1]
+    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split_with_sizes(sizes)
     lens_out, n_out = (lens, n_free) if inplace else parts[2:]
     _kv_call(dev, lib().hgk_kv_release, state, _ptr(seqs), k, o, batch, lens_out.data_ptr(), n_out.data_ptr(),
              parts[0].data_ptr(), parts[1].data_ptr())
