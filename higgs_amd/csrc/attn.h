@@ -43,10 +43,10 @@ struct AttnArgs {
   int32_t chunk;  // single tokens: tiles of a part
 };
 
-// Which keys a kernel takes of each row: all, of the row's own table; those of the
+// Which keys a block takes: all of each row, of the row's own table; those of the
 // shared prefix, for the rows of all sequences at once; or those behind it (all, if
 // there is no pass over the prefix), with the prefix's table in front of the own one.
-constexpr int kOwn = 0, kPrefix = 1, kBehind = 2;
+enum Keys { kOwn, kPrefix, kBehind };
 
 // The table's entry for a key of a sequence whose first keys are the prefix's.
 __device__ inline int32_t page_behind(const AttnArgs& a, const int32_t* table, int32_t key) {
@@ -617,27 +617,33 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 // registers allow one wave a SIMD there, and the tile's load instructions and
 // its barrier stand beside the step. Deeper rings of tiles, 256 rows a block
 // and loads spread over the step were no faster.
-template <class T, int D, int BN, int CAP, int KEYS>
-__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+//
+// lds: prompt_lds<D>() bytes, 1024-byte aligned; words: kPromptWords. x of grid_x
+// and y are the block's place, `splits` the y there are.
+constexpr int kPromptWords = 2 + 2 * (2 * kPromptRows / 64);
+template <int D> constexpr int prompt_lds() { return 4 * 64 * 2 * D; }
+template <class T, int D, int BN, int CAP>
+__device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* lds, int* words, int x, int grid_x,
+                                            int y, int splits) {
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
   constexpr int KT = BN / 32, QS = D / 16, DT = D / 32, kAhead = 2;
   static_assert(BN == 64 && BN * CH % NT == 0, "two tiles of 32 keys, whole units per thread");
   typedef Mx<T> M;
-  __shared__ __align__(1024) char lds[4 * kTile];  // two tiles of keys, two of values
-  __shared__ int odd;   // 1 + index of the last tile found to hold values that are not finite
-  __shared__ int redo;  // a row's sums are not finite
+  static_assert(prompt_lds<D>() == 4 * kTile, "two tiles of keys, two of values");
+  int& odd = words[0];   // 1 + index of the last tile found to hold values that are not finite
+  int& redo = words[1];  // a row's sums are not finite
 
   const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int place = blockIdx.x / a.p.kv_heads, hk = blockIdx.x - place * a.p.kv_heads, G = a.group;
+  const int place = x / a.p.kv_heads, hk = x - place * a.p.kv_heads, G = a.group;
 
   // which sequence's tile this is: tiles are counted over the sequences, from
   // the last one on (the longest ones of a prompt first)
-  const int64_t want = gridDim.x / a.p.kv_heads - 1 - place;
+  const int64_t want = grid_x / a.p.kv_heads - 1 - place;
   int seq = 0, tile = (int)want;
   KvSeq s{0, a.b.tokens, 0};  // the prefix: the rows of all sequences
-  if constexpr (KEYS != kPrefix) {
+  if (keys != kPrefix) {
     const Owner w = find_owner(
         a.b.batch, [&](int b) { return ((int64_t)kv_seq(a.b, b).n * G + BM - 1) / BM; }, [&](int64_t) { return want; });
     if (w.seq < 0) return;
@@ -659,9 +665,10 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   const bool in = wrow0 + col < R;
   int p = pos0 + qi, p_first = pos0 + row0 / G, p_last = pos0 + (min(row0 + BM, R) - 1) / G;
   int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
-  if constexpr (KEYS == kPrefix) {
+  if (keys == kPrefix) {
     // every row has a sequence of its own; a row of none sees nothing
-    __shared__ int bounds[2][NT / 64];
+    int* const lowest_of = words + 2;
+    int* const highest_of = lowest_of + NT / 64;
     const KvSeq of = kv_seq(a.b, kv_row_owner(a.b, qi));
     p = qi >= of.first && qi < of.first + of.n ? of.len - of.n + qi - of.first : -1;
     int lowest = p, highest = p;
@@ -673,27 +680,27 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
     pw_first = __builtin_amdgcn_readfirstlane(lowest);
     pw_last = __builtin_amdgcn_readfirstlane(highest);
     if (lane == 0) {
-      bounds[0][wave] = pw_first;
-      bounds[1][wave] = pw_last;
+      lowest_of[wave] = pw_first;
+      highest_of[wave] = pw_last;
     }
     __syncthreads();
-    p_first = min(min(bounds[0][0], bounds[0][1]), min(bounds[0][2], bounds[0][3]));
-    p_last = max(max(bounds[1][0], bounds[1][1]), max(bounds[1][2], bounds[1][3]));
+    p_first = min(min(lowest_of[0], lowest_of[1]), min(lowest_of[2], lowest_of[3]));
+    p_last = max(max(highest_of[0], highest_of[1]), max(highest_of[2], highest_of[3]));
     p_first = __builtin_amdgcn_readfirstlane(p_first);
     p_last = __builtin_amdgcn_readfirstlane(p_last);
   }
   // keys from .. cap - 1 are the kernel's
-  const int from = KEYS == kBehind && a.pre > 0 ? a.prefix : 0;
+  const int from = keys == kBehind && a.pre > 0 ? a.prefix : 0;
   const int64_t own = (int64_t)a.b.width << a.p.page_shift;
-  const int64_t cap = KEYS == kOwn ? own : KEYS == kPrefix ? (int64_t)a.prefix : max(own, (int64_t)a.prefix);
+  const int64_t cap = keys == kOwn ? own : keys == kPrefix ? (int64_t)a.prefix : max(own, (int64_t)a.prefix);
   const int hi = (int)min((int64_t)p_last + 1, cap);
   const int lo = a.window > 0 && p_first >= a.window ? p_first - a.window + 1 : 0;
   const int t_from = from / BN, t_hi = hi > 0 ? (hi + BN - 1) / BN : 0, t_lo = max(lo, from) / BN;
   // (at most 2^30 before it is rounded up: sinks and lo may both end at int32's end)
   const int front = max(min((min(min(a.sinks, lo), max(hi, 0)) + BN - 1) / BN, t_lo) - t_from, 0);
   const int tiles = a.p.n_pages > 0 ? front + max(t_hi - t_lo, 0) : 0;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int it0 = min(per * (int)blockIdx.y, tiles), it1 = min(it0 + per, tiles);
+  const int per = (tiles + splits - 1) / splits;
+  const int it0 = min(per * y, tiles), it1 = min(it0 + per, tiles);
   auto tile_of = [&](int it) { return it < front ? t_from + it : t_lo + it - front; };
 
   const Scale sc = fold_scale<CAP>(a);
@@ -705,11 +712,11 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   auto look_up = [&](int it) -> int32_t {
     if (it >= it1) return -1;
     const int key = tile_of(it) * BN + (lane & (BN - 1));
-    if constexpr (KEYS == kPrefix) {
+    if (keys == kPrefix) {
       const int e = key >> a.p.page_shift;
       return key < hi && e < a.prefix_width ? a.prefix_table[e] : -1;
     }
-    if constexpr (KEYS == kBehind) return key >= from && key < hi ? page_behind(a, table, key) : -1;
+    if (keys == kBehind) return key >= from && key < hi ? page_behind(a, table, key) : -1;
     return key < hi ? table[key >> a.p.page_shift] : -1;
   };
   // Looked at a turn after the load was issued: a wait for it is a wait for
@@ -723,7 +730,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   const bool whole = a.p.page_shift >= 4 && a.p.kst[1] < (1 << 24) && a.p.vst[1] < (1 << 24);
   // But where the prefix ends inside such a run of rows, the rows in front of its
   // end and those behind it lie in two pages: that tile goes row by row.
-  const int cut = KEYS == kBehind && (a.prefix & 15) ? a.prefix / BN : -1;
+  const int cut = keys == kBehind && (a.prefix & 15) ? a.prefix / BN : -1;
   // (rows i * NT / CH apart have the same offsets, where that is a multiple of 16)
   constexpr int kOffs = NT % (16 * CH) == 0 ? 1 : kUnits;
   uint32_t koff[kOffs], voff[kOffs];
@@ -738,7 +745,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
                   const uint32_t* off, auto piece) {
     const int key0 = tile_of(it) * BN;
     if (page < 0) page = 0;
-    if (whole && (KEYS != kBehind || tile_of(it) != cut)) {
+    if (whole && (keys != kBehind || tile_of(it) != cut)) {
       const uint64_t at = (uint64_t)(base + 2 * (page * page_step + ((key0 + lane) & a.p.page_mask) * row_step));
       const int at_lo = (int)(uint32_t)at, at_hi = (int)(uint32_t)(at >> 32);
 #pragma unroll
@@ -1109,13 +1116,13 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   if constexpr (D < 256) tell();
   // (a row's parts over the prefix come first)
   int64_t part_at = (int64_t)(s.first + qi) * a.q_heads + head;
-  if constexpr (KEYS == kOwn) part_at = part_at * a.splits + blockIdx.y;
-  else part_at = part_at * a.row_parts + (KEYS == kBehind ? a.pre : 0) + blockIdx.y;
-  const bool parts = KEYS == kOwn ? a.splits > 1 : a.row_parts > 1;
+  if (keys == kOwn) part_at = part_at * splits + y;
+  else part_at = part_at * a.row_parts + (keys == kBehind ? a.pre : 0) + y;
+  const bool parts = keys == kOwn ? splits > 1 : a.row_parts > 1;
   char* out_row = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1]);
   if (parts) {
     if (in && half == 0)
-      *reinterpret_cast<f32x2*>(a.stat + 2 * part_at) = f32x2{any ? (KEYS == kOwn ? ref * sc.c : ref) : -INFINITY, sum};
+      *reinterpret_cast<f32x2*>(a.stat + 2 * part_at) = f32x2{any ? (keys == kOwn ? ref * sc.c : ref) : -INFINITY, sum};
     if (in && any) {
       float* dst = a.part + part_at * D + 4 * half;
 #pragma unroll
@@ -1203,18 +1210,6 @@ int64_t prefix_tiles(const KvBatchView& b, int64_t group) {
 // The fewest keys of a part; the blocks that prompts are split to fill; the most parts.
 constexpr int64_t kMinPart = 256, kPromptBlocks = 256;
 constexpr int kMaxSplits = 64;
-
-template <class T, int D, int BN, int KEYS>
-void launch_prompt(const AttnArgs& a, hipStream_t stream) {
-  const int64_t tiles = KEYS == kPrefix ? prefix_tiles(a.b, a.group) : prompt_tiles(a.b, a.group);
-  const dim3 grid(a.p.kv_heads * tiles, a.splits), block(2 * kPromptRows);
-  if (a.softcap > kCapMax)
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kWideCap, KEYS>), grid, block, 0, stream, a);
-  else if (a.softcap > 0.0f)
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kCap, KEYS>), grid, block, 0, stream, a);
-  else
-    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kNoCap, KEYS>), grid, block, 0, stream, a);
-}
 
 // The operands of both entry points checked and filled in, but for the workspace.
 int check_call(const char* what, AttnArgs* a, const void* q, const int64_t q_strides[2], int64_t q_heads, float scale,

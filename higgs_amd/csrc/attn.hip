@@ -369,6 +369,24 @@ void launch_decode(const AttnArgs& a, hipStream_t stream) {
                dim3(a.b.batch, std::clamp<int>(kDecJoinBlocks / a.b.batch, 1, a.q_heads)), dim3(256), 0, stream, a);
 }
 
+template <class T, int D, int BN, int CAP>
+__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
+  __shared__ __align__(1024) char lds[prompt_lds<D>()];
+  __shared__ int words[kPromptWords];
+  attn_prompt<T, D, BN, CAP>(kOwn, a, lds, words, blockIdx.x, gridDim.x, blockIdx.y, a.splits);
+}
+
+template <class T, int D, int BN>
+void launch_prompt(const AttnArgs& a, hipStream_t stream) {
+  const dim3 grid(a.p.kv_heads * prompt_tiles(a.b, a.group), a.splits), block(2 * kPromptRows);
+  if (a.softcap > kCapMax)
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kWideCap>), grid, block, 0, stream, a);
+  else if (a.softcap > 0.0f)
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kCap>), grid, block, 0, stream, a);
+  else
+    HGK_LAUNCH((attn_prompt_kernel<T, D, BN, kNoCap>), grid, block, 0, stream, a);
+}
+
 template <class T, int D>
 void launch_join(const AttnArgs& a, hipStream_t stream) {
   constexpr int kGroups = 256 / (D / 4);
@@ -390,10 +408,10 @@ int run(const AttnArgs& a, const char* what, hipStream_t stream) {
     }
   } else {
     switch (a.p.head_dim) {
-      case 64: launch_prompt<T, 64, 64, kOwn>(a, stream); break;
-      case 96: launch_prompt<T, 96, 64, kOwn>(a, stream); break;
-      case 128: launch_prompt<T, 128, 64, kOwn>(a, stream); break;
-      default: launch_prompt<T, 256, 64, kOwn>(a, stream); break;
+      case 64: launch_prompt<T, 64, 64>(a, stream); break;
+      case 96: launch_prompt<T, 96, 64>(a, stream); break;
+      case 128: launch_prompt<T, 128, 64>(a, stream); break;
+      default: launch_prompt<T, 256, 64>(a, stream); break;
     }
   }
   if (int st = launch_status(what)) return st;

@@ -31,18 +31,19 @@ __device__ inline Seen seen_behind(const AttnArgs& a, int32_t len) {
 
 // Single tokens' own keys: WAVES waves have a chunk of a (sequence, kv head), for 16
 // of its query heads, and make one part of it.
+// lds: behind_lds<D, WAVES>() bytes, 16-byte aligned. x counts the blocks, y the 16s of
+// query heads.
+template <int D, int WAVES> constexpr int behind_lds() {
+  constexpr int kTiles = kDecWaves * dec_keys<D>() * dec_row<D>(), kJoin = WAVES > 1 ? kDecWaves * 16 * D * 4 : 0;
+  return kTiles > kJoin ? kTiles : kJoin;
+}
 template <class T, int D, int CAP, int WAVES>
-__global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_behind(const AttnArgs& a, char* lds, int block, int y) {
   constexpr int kKeys = dec_keys<D>(), kStep = D / 32, kTile = kKeys * dec_row<D>();
-  constexpr int kJoin = WAVES > 1 ? kDecWaves * 16 * D * 4 : 0;
-  __shared__ __align__(16) char lds[kTile * kDecWaves > kJoin ? kTile * kDecWaves : kJoin];
-  __shared__ float wref[kDecWaves][16], wsum[kDecWaves][16];
-  __shared__ int wseen[kDecWaves];
-
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, j = lane >> 4, step = WAVES > 1 ? wave : 0;
   // chunks in the order of the sequences: those that are not there come last
-  const int unit = WAVES > 1 ? blockIdx.x : blockIdx.x * kDecWaves + wave, pairs = a.b.batch * a.p.kv_heads;
+  const int unit = WAVES > 1 ? block : block * kDecWaves + wave, pairs = a.b.batch * a.p.kv_heads;
   const int at_chunk = unit / pairs, pair = unit - at_chunk * pairs;
   const int seq = pair / a.p.kv_heads, hk = pair - seq * a.p.kv_heads;
   if (at_chunk >= a.splits) return;
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs
   if (first >= last && a.row_parts > 1) return;  // not a part of the row
 
   const Scale sc = fold_scale<CAP>(a);
-  const int heads = min(16, a.group - (int)blockIdx.y * 16), h0 = hk * a.group + blockIdx.y * 16;
+  const int heads = min(16, a.group - y * 16), h0 = hk * a.group + y * 16;
   const char* qp = a.q + 2 * (seq * a.qst[0] + (h0 + (m < heads ? m : 0)) * a.qst[1]);
   u32x4 qf[kStep];
 #pragma unroll
@@ -113,6 +114,8 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs
       }
     }
   } else {
+    __shared__ float wref[kDecWaves][16], wsum[kDecWaves][16];
+    __shared__ int wseen[kDecWaves];
     __syncthreads();  // every wave is done with its V tile
     float* wo = reinterpret_cast<float*>(lds) + wave * 16 * D + m * D;
     if (again) {
@@ -152,6 +155,69 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs
       }
     }
   }
+}
+
+template <class T, int D, int CAP, int WAVES>
+__global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs a) {
+  __shared__ __align__(16) char lds[behind_lds<D, WAVES>()];
+  attn_behind<T, D, CAP, WAVES>(a, lds, blockIdx.x, blockIdx.y);
+}
+
+// Which rows and which part of its keys block `id` of the pass over the prefix takes.
+// The blocks of a part are put on one XCD, whose L2 then holds its keys, where the
+// parts share out evenly.
+struct PrefixBlock {
+  int x, grid_x, split;
+};
+__device__ inline PrefixBlock prefix_block(const AttnArgs& a, int id, int blocks) {
+  const int parts = a.pre * a.p.kv_heads, places = blocks / parts;
+  int part = id / places, place = id - part * places;
+  if (parts % 8 == 0) {
+    const int k = id >> 3;
+    part = k / places * 8 + (id & 7);
+    place = k % places;
+  }
+  const int split = part / a.p.kv_heads, hk = part - split * a.p.kv_heads;
+  return PrefixBlock{place * a.p.kv_heads + hk, places * a.p.kv_heads, split};
+}
+
+// Both passes of single tokens in one launch: the blocks that take the prefix, which
+// the matrix instructions bound, and then those of the sequences' own keys, which the
+// memory does, so that either finds CUs, or places on them, that the other leaves.
+// With the join, in us: 256 sequences of up to 200 tokens behind 4001, 32/8 heads of
+// 128 (17 GFLOP, 126 MB): 47, as two launches 66; 64 of up to 1500 behind 8192, 16/2
+// heads of 256 (9 GFLOP, 117 MB): 54, as two 72; every sequence over a table of its
+// own (paged_attention's kernels): 496 and 149.
+template <class T, int D, int CAP>
+__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_kernel(AttnArgs a, int prefix_blocks,
+                                                                                          int behind_blocks) {
+  static_assert(2 * kPromptRows == 64 * kDecWaves && prompt_lds<D>() >= behind_lds<D, 1>(), "one kind of block");
+  __shared__ __align__(1024) char lds[prompt_lds<D>()];
+  const int id = blockIdx.x;
+  if (id < prefix_blocks) {
+    __shared__ int words[kPromptWords];
+    const PrefixBlock p = prefix_block(a, id, prefix_blocks);
+    attn_prompt<T, D, 64, CAP>(kPrefix, a, lds, words, p.x, p.grid_x, p.split, a.pre);
+  } else {
+    const int b = id - prefix_blocks, y = b / behind_blocks;
+    attn_behind<T, D, CAP == kNoCap ? kNoCap : kWideCap, 1>(a, lds, b - y * behind_blocks, y);
+  }
+}
+
+// Both passes of prompts in one launch. 32 sequences of up to 33 + 100 tokens behind
+// 16384, 32/8 heads of 128 f16 (148 GFLOP): 212 us with the join, 700 TFLOP/s.
+template <class T, int D, int CAP>
+__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_prompt_kernel(AttnArgs a,
+                                                                                                 int prefix_blocks,
+                                                                                                 int behind_x) {
+  __shared__ __align__(1024) char lds[prompt_lds<D>()];
+  __shared__ int words[kPromptWords];
+  const int id = blockIdx.x, b = id - prefix_blocks;
+  const bool prefix = b < 0;
+  PrefixBlock p{b % behind_x, behind_x, b / behind_x};
+  if (prefix) p = prefix_block(a, id, prefix_blocks);
+  attn_prompt<T, D, 64, CAP>(prefix ? kPrefix : kBehind, a, lds, words, p.x, p.grid_x, p.split,
+                             prefix ? a.pre : a.splits);
 }
 
 // out = sum_i w_i part_i / sum_i w_i sum_i over the parts of a row (token and query
@@ -241,11 +307,11 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs a, uint3
 
 // The split of a call, from the sizes alone.
 //
-// A pass over the prefix costs two launches more and the writing and joining of its
+// A pass over the prefix costs a launch more and the writing and joining of its
 // parts, so it has to save the reading of 40 MB: below, the sequences read the prefix
 // one by one, much of it from the caches (8 sequences behind 1000 tokens, 8 kv heads
-// of 64, 14 MB: 20.7 us with the pass, 13.8 without; 16 behind 2000, 8 of 128, 123
-// MB: 26.7, 32.8). Its blocks are as many as the chip holds at once.
+// of 64, 14 MB: 20 us with the pass, 14.7 without; 16 behind 2000, 8 of 128, 123 MB:
+// 18.3, 32.8).
 constexpr int64_t kPassBytes = 40 << 20, kUnits = 2048;
 struct SharedPlan {
   int pre, splits, chunk, waves;
@@ -257,8 +323,15 @@ SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, in
   if (b.batch == 0 || b.tokens == 0) return s;
   const int64_t group = q_heads / p.kv_heads, width = (int64_t)b.width << p.page_shift;
   if ((b.batch - 1) * std::min(prefix, width) * p.kv_heads * p.head_dim >= kPassBytes / 4) {
-    const int64_t blocks = p.head_dim == 256 ? 256 : 512, tiles = p.kv_heads * prefix_tiles(b, group);
-    s.pre = (int)std::max<int64_t>(1, std::min<int64_t>({blocks / tiles, prefix / kMinPart, (int64_t)kMaxSplits}));
+    // Places on the chip, shared out by the two passes' work: a tile of 64 keys takes 3 us
+    // of a block with rows of 256, one a CU, and in proportion less of narrower ones, two
+    // a CU and 2.2 us each at 128; own keys, half of what the tables allow, come at 5 TB/s.
+    const int64_t places = p.head_dim == 256 ? 256 : 512, tiles = p.kv_heads * prefix_tiles(b, group);
+    const double own = (double)b.batch * std::max<int64_t>(width - prefix, 0) * p.kv_heads * p.head_dim * 2 / 5e6;
+    const double pass = (double)tiles * prefix / 64 * (p.head_dim == 256 ? 3.0 : 2.2 * p.head_dim / 128) / places;
+    const int64_t blocks = b.starts ? places : (int64_t)(places * pass / (pass + own));
+    s.pre = (int)std::clamp<int64_t>((blocks + (b.starts ? 0 : tiles - 1)) / tiles, 1,
+                                     std::max<int64_t>(std::min<int64_t>(prefix / kMinPart, kMaxSplits), 1));
   }
   int64_t rest = std::max(width, prefix) - (s.pre > 0 ? prefix : 0);
   if (window > 0 && window < rest && sinks < rest - window) rest = window + sinks;
@@ -274,6 +347,7 @@ SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, in
     s.chunk = (int)all;
     return s;
   }
+  // chunks of as many tiles as leave 2048 waves, two a SIMD, if every table is full
   const int64_t most = std::clamp<int64_t>(kUnits / pairs, 1, kMaxParts - kMaxSplits);
   s.chunk = (int)std::max<int64_t>((all + most - 1) / most, 4);
   s.splits = (int)((all + s.chunk - 1) / s.chunk);
@@ -312,16 +386,43 @@ void launch_prefix_join(const AttnArgs& a, hipStream_t stream) {
 }
 
 template <class T, int D>
+void launch_shared(const AttnArgs& a, hipStream_t stream) {
+  const int64_t units = (int64_t)a.b.batch * a.p.kv_heads * a.splits;
+  const int prefix = (int)(a.p.kv_heads * prefix_tiles(a.b, a.group) * a.pre);
+  const int behind = (int)((units + kDecWaves - 1) / kDecWaves), heads = (a.group + 15) / 16;
+  const dim3 grid(prefix + behind * heads), block(2 * kPromptRows);
+  if (a.softcap > kCapMax)
+    HGK_LAUNCH((attn_shared_kernel<T, D, kWideCap>), grid, block, 0, stream, a, prefix, behind);
+  else if (a.softcap > 0.0f)
+    HGK_LAUNCH((attn_shared_kernel<T, D, kCap>), grid, block, 0, stream, a, prefix, behind);
+  else
+    HGK_LAUNCH((attn_shared_kernel<T, D, kNoCap>), grid, block, 0, stream, a, prefix, behind);
+}
+
+template <class T, int D>
+void launch_shared_prompts(const AttnArgs& a, hipStream_t stream) {
+  const int prefix = (int)(a.p.kv_heads * prefix_tiles(a.b, a.group) * a.pre);
+  const int behind = (int)(a.p.kv_heads * prompt_tiles(a.b, a.group));
+  const dim3 grid(prefix + behind * a.splits), block(2 * kPromptRows);
+  if (a.softcap > kCapMax)
+    HGK_LAUNCH((attn_shared_prompt_kernel<T, D, kWideCap>), grid, block, 0, stream, a, prefix, behind);
+  else if (a.softcap > 0.0f)
+    HGK_LAUNCH((attn_shared_prompt_kernel<T, D, kCap>), grid, block, 0, stream, a, prefix, behind);
+  else
+    HGK_LAUNCH((attn_shared_prompt_kernel<T, D, kNoCap>), grid, block, 0, stream, a, prefix, behind);
+}
+
+template <class T, int D>
 int run_of(const AttnArgs& a, int waves, const char* what, hipStream_t stream) {
-  if (a.pre > 0) {
-    AttnArgs of = a;
-    of.splits = a.pre;
-    launch_prompt<T, D, 64, kPrefix>(of, stream);
-    if (int st = launch_status(what)) return st;
+  if (a.b.starts) {
+    launch_shared_prompts<T, D>(a, stream);
+  } else if (a.pre > 0) {
+    launch_shared<T, D>(a, stream);
+  } else if (waves > 1) {
+    launch_behind<T, D, kDecWaves>(a, stream);
+  } else {
+    launch_behind<T, D, 1>(a, stream);
   }
-  if (a.b.starts) launch_prompt<T, D, 64, kBehind>(a, stream);
-  else if (waves > 1) launch_behind<T, D, kDecWaves>(a, stream);
-  else launch_behind<T, D, 1>(a, stream);
   if (int st = launch_status(what)) return st;
   if (a.row_parts == 1) return HGK_OK;
   if (a.b.starts) launch_prefix_join<T, D, false>(a, stream);
@@ -372,6 +473,11 @@ extern "C" int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_
   if (prefix_len > 0 && !prefix_table) return fail(HGK_ERR_ARG, "%s: null prefix table", what);
   if (int st = check_call(what, &a, q, q_strides, q_heads, scale, softcap, window, sinks, out, out_strides)) return st;
   const SharedPlan s = plan_shared(a.p, a.b, prefix_len, q_heads, window, sinks);
+  const int64_t heads = a.b.starts ? 1 : (a.group + 15) / 16;
+  const int64_t blocks = a.p.kv_heads * (s.pre * prefix_tiles(a.b, a.group) +
+                                         s.splits * heads * (a.b.starts ? prompt_tiles(a.b, a.group) : a.b.batch));
+  if (blocks > kMaxBlocks)
+    return fail(HGK_ERR_ARG, "%s: %lld rows are too many", what, (long long)a.b.tokens);
   const int64_t rows = s.rows() * a.b.tokens * q_heads, need = rows * (a.p.head_dim + 2) * 4;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return fail(HGK_ERR_ARG, "%s: needs a 16-byte aligned workspace of %lld bytes", what, (long long)need);
