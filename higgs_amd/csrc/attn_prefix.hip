@@ -322,7 +322,8 @@ SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, in
   SharedPlan s{0, 1, 1, 1};
   if (b.batch == 0 || b.tokens == 0) return s;
   const int64_t group = q_heads / p.kv_heads, width = (int64_t)b.width << p.page_shift;
-  if ((b.batch - 1) * std::min(prefix, width) * p.kv_heads * p.head_dim >= kPassBytes / 4) {
+  const int64_t seen = window > 0 && window < prefix && sinks < prefix - window ? window + sinks : prefix;
+  if ((b.batch - 1) * std::min(seen, width) * p.kv_heads * p.head_dim >= kPassBytes / 4) {
     // Places on the chip, shared out by the two passes' work: a tile of 64 keys takes 3 us
     // of a block with rows of 256, one a CU, and in proportion less of narrower ones, two
     // a CU and 2.2 us each at 128; own keys, half of what the tables allow, come at 5 TB/s.

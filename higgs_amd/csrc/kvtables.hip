@@ -8,7 +8,9 @@
 namespace hgk {
 namespace {
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kMaxRows = 1 << 18, kFill = 256, kNear = 4096;
+constexpr int kPlanThreads = 1024, kMaxRows = 1 << 18, kFill = 256, kNear = 4096;
+// Calls in one launch: at most so many sequences, resident ones and blocks.
+constexpr int kOneBatch = 1024, kOneRows = 1 << 15, kOneBlocks = 512;
 
 struct TablesView {
   int32_t* table;
@@ -69,28 +71,32 @@ struct Pair {
 };
 __device__ inline int64_t shift_up(int64_t v, int by) { return __shfl_up(v, by); }
 
-// One block: a thread has a run of the batch's sequences. Sums them, and if
-// nothing stands against the call writes every sequence's part and the new state.
-// The state may be written where it was read: each of its values is read by the
-// thread that writes it, or before a barrier.
-__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
-  __shared__ uint32_t named[kMaxRows / 32];
-  __shared__ int64_t wave_pages[kPlanWaves], wave_tokens[kPlanWaves];
+// What a block finds out about a call: a thread has the run i0 .. i1 - 1 of the
+// batch's sequences; the pages and tokens of all in front of it, and of all.
+struct Sums {
+  int i0, i1;
+  int32_t status, n_free;
+  Pair before, total;
+};
+template <int THREADS, int ROWS>
+__device__ inline Sums sums_of(const PlanArgs& a) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ uint32_t named[ROWS / 32];
+  __shared__ int64_t wave_pages[kWaves], wave_tokens[kWaves];
   __shared__ int32_t bad;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int run = (a.batch + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min(tid * run, a.batch), i1 = min(i0 + run, a.batch);
+  const int run = (a.batch + THREADS - 1) / THREADS;
+  Sums s;
+  s.i0 = min(tid * run, a.batch);
+  s.i1 = min(s.i0 + run, a.batch);
+  s.n_free = min(max(*a.t.n_free, 0), a.t.n_pages);
   if (tid == 0) bad = 0;
   if (a.seqs)
-    for (int w = tid; w < (a.t.rows + 31) / 32; w += kPlanThreads) named[w] = 0;
-  const int32_t n_free = min(max(*a.t.n_free, 0), a.t.n_pages);
-  if (a.lens_out != a.t.lens)
-    for (int r = tid; r < a.t.rows; r += kPlanThreads) a.lens_out[r] = a.t.lens[r];
+    for (int w = tid; w < (a.t.rows + 31) / 32; w += THREADS) named[w] = 0;
   __syncthreads();
-
   Pair mine{0, 0};
   int32_t status = 0;
-  for (int i = i0; i < i1; ++i) {
+  for (int i = s.i0; i < s.i1; ++i) {
     const Ask k = ask_of(a, i);
     mine.pages += k.pages;
     mine.tokens += k.tokens;
@@ -113,20 +119,34 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
   }
   if (status) atomicOr(&bad, status);
   __syncthreads();
-  Pair before{upto.pages - mine.pages, upto.tokens - mine.tokens}, total{0, 0};
-  for (int w = 0; w < kPlanWaves; ++w) {
+  s.before = Pair{upto.pages - mine.pages, upto.tokens - mine.tokens};
+  s.total = Pair{0, 0};
+  for (int w = 0; w < kWaves; ++w) {
     if (w < wave) {
-      before.pages += wave_pages[w];
-      before.tokens += wave_tokens[w];
+      s.before.pages += wave_pages[w];
+      s.before.tokens += wave_tokens[w];
     }
-    total.pages += wave_pages[w];
-    total.tokens += wave_tokens[w];
+    s.total.pages += wave_pages[w];
+    s.total.tokens += wave_tokens[w];
   }
-  status = bad;
-  if (total.pages > (a.release ? a.t.n_pages - n_free : n_free)) status |= HGK_TABLES_PAGES;
-  if (total.tokens > a.tokens) status |= HGK_TABLES_TOKENS;
-  const bool go = status == 0;
-  for (int i = i0; i < i1; ++i) {
+  s.status = bad;
+  if (s.total.pages > (a.release ? a.t.n_pages - s.n_free : s.n_free)) s.status |= HGK_TABLES_PAGES;
+  if (s.total.tokens > a.tokens) s.status |= HGK_TABLES_TOKENS;
+  return s;
+}
+
+// Writes the new state and the sequences' small results, by one block. The state may
+// be written where it was read: each of its values is read by the thread that writes
+// it, or before a barrier.
+template <int THREADS>
+__device__ inline void write_plan(const PlanArgs& a, const Sums& s) {
+  const bool go = s.status == 0;
+  if (a.lens_out != a.t.lens) {
+    for (int r = threadIdx.x; r < a.t.rows; r += THREADS) a.lens_out[r] = a.t.lens[r];
+    __syncthreads();
+  }
+  Pair before = s.before;
+  for (int i = s.i0; i < s.i1; ++i) {
     const Ask k = ask_of(a, i);
     a.page_starts[i] = go ? (int32_t)before.pages : 0;
     if (!a.release) {
@@ -137,13 +157,18 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
     before.pages += k.pages;
     before.tokens += k.tokens;
   }
-  if (tid == 0) {
-    a.page_starts[a.batch] = go ? (int32_t)total.pages : 0;
-    if (!a.release) a.q_starts[a.batch] = go ? (int32_t)total.tokens : 0;
-    const int32_t moved = go ? (int32_t)total.pages : 0;
-    *a.n_free_out = n_free + (a.release ? moved : -moved);
-    *a.status = status;
+  if (threadIdx.x == 0) {
+    a.page_starts[a.batch] = go ? (int32_t)s.total.pages : 0;
+    if (!a.release) a.q_starts[a.batch] = go ? (int32_t)s.total.tokens : 0;
+    const int32_t moved = go ? (int32_t)s.total.pages : 0;
+    *a.n_free_out = s.n_free + (a.release ? moved : -moved);
+    *a.status = s.status;
   }
+}
+
+// The first of two launches: what the second one's blocks read.
+__global__ __launch_bounds__(kPlanThreads) void kv_plan_kernel(PlanArgs a) {
+  write_plan<kPlanThreads>(a, sums_of<kPlanThreads, kMaxRows>(a));
 }
 
 struct ExtendArgs {
@@ -152,7 +177,7 @@ struct ExtendArgs {
   int32_t* positions;
   int32_t* block_table;  // null: the tables themselves
   int64_t block_stride;
-  int32_t token_blocks, row_blocks;  // blocks over tokens; of a row of block_table
+  int32_t token_blocks, row_blocks, blocks;  // blocks over tokens; of a row of block_table; all
 };
 
 // The page of entry e of a sequence that had `had` pages and whose new ones begin
@@ -161,24 +186,25 @@ __device__ inline int32_t entry_of(const PlanArgs& a, int32_t top, int32_t row, 
   return e < had ? a.t.table[row * a.t.stride + e] : a.t.free_pages[top - 1 - (from + e - had)];
 }
 
-// Blocks over the tokens, each thread with one: its sequence, position and place;
+// What the blocks of a call read of its sequences: the pages and tokens in front of
+// each, and its row; the length is worked out of them.
+struct Seqs {
+  const int32_t* pages;   // [batch + 1]
+  const int32_t* tokens;  // [batch + 1]
+  int32_t top;            // free pages before the call
+};
+
+// Block `block` over the tokens, each thread with one: its sequence, position and place;
 // the first token of a page writes the page into the table. Then blocks over the
-// rows of the batch's own table, if it has one.
-__global__ __launch_bounds__(kFill) void kv_extend_kernel(ExtendArgs x) {
+// rows of the batch's own table, if it has one. old(i, row): sequence i's tokens
+// before the call.
+template <class Old>
+__device__ inline void extend_block(const ExtendArgs& x, int block, const Seqs& q, Old old) {
   const PlanArgs& a = x.p;
-  const int32_t top = *a.n_free_out + a.page_starts[a.batch];
-  if ((int)blockIdx.x < x.token_blocks) {
-    // the starts, where they fit: a search is a chain of reads
-    __shared__ int32_t near[kNear + 1];
-    const bool cached = a.batch <= kNear;
-    if (cached) {
-      for (int i = threadIdx.x; i <= a.batch; i += kFill) near[i] = a.q_starts[i];
-      __syncthreads();
-    }
-    const int32_t* starts = cached ? near : a.q_starts;
-    const int t = blockIdx.x * kFill + threadIdx.x;
+  if (block < x.token_blocks) {
+    const int t = block * kFill + threadIdx.x;
     if (t >= a.tokens) return;
-    if (t >= starts[a.batch]) {
+    if (t >= q.tokens[a.batch]) {
       x.slots[t] = -1;
       x.positions[t] = 0;
       return;
@@ -186,36 +212,87 @@ __global__ __launch_bounds__(kFill) void kv_extend_kernel(ExtendArgs x) {
     int lo = 0, hi = a.batch;  // the last sequence that starts at t or before
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (starts[mid] <= t) lo = mid;
+      if (q.tokens[mid] <= t) lo = mid;
       else hi = mid;
     }
-    const int32_t first = starts[lo], n = starts[lo + 1] - first, old = a.kv_lens[lo] - n;
-    const int32_t row = a.seqs ? a.seqs[lo] : lo, pos = old + t - first, e = pos >> a.t.shift;
-    const int32_t at = pos & ((1 << a.t.shift) - 1);
-    const int32_t page = entry_of(a, top, row, pages_of(a.t, old), a.page_starts[lo], e);
+    const int32_t row = a.seqs ? a.seqs[lo] : lo, had = old(lo, row), pos = had + t - q.tokens[lo];
+    const int32_t e = pos >> a.t.shift, at = pos & ((1 << a.t.shift) - 1);
+    const int32_t page = entry_of(a, q.top, row, pages_of(a.t, had), q.pages[lo], e);
     if (at == 0) a.t.table[row * a.t.stride + e] = page;
     x.slots[t] = ((int64_t)page << a.t.shift) + at;
     x.positions[t] = pos;
     return;
   }
-  const int b = blockIdx.x - x.token_blocks, i = b / x.row_blocks;
+  const int b = block - x.token_blocks, i = b / x.row_blocks;
   const int e = (b - i * x.row_blocks) * kFill + threadIdx.x;
   if (e >= a.t.width) return;
-  const int32_t row = a.seqs[i], len = a.kv_lens[i], old = len - (a.q_starts[i + 1] - a.q_starts[i]);
+  const int32_t row = a.seqs[i];
   int32_t page = -1;
-  if (e < pages_of(a.t, len) && (uint32_t)row < (uint32_t)a.t.rows)
-    page = entry_of(a, top, row, pages_of(a.t, old), a.page_starts[i], e);
+  if ((uint32_t)row < (uint32_t)a.t.rows) {
+    const int32_t had = old(i, row);
+    if (e < pages_of(a.t, (int64_t)had + q.tokens[i + 1] - q.tokens[i]))
+      page = entry_of(a, q.top, row, pages_of(a.t, had), q.pages[i], e);
+  }
   x.block_table[i * x.block_stride + e] = page;
+}
+__global__ __launch_bounds__(kFill) void kv_extend_kernel(ExtendArgs x) {
+  const PlanArgs& a = x.p;
+  // the starts, where they fit: a search is a chain of reads
+  __shared__ int32_t near[kNear + 1];
+  const bool cached = a.batch <= kNear && (int)blockIdx.x < x.token_blocks;
+  if (cached) {
+    for (int i = threadIdx.x; i <= a.batch; i += kFill) near[i] = a.q_starts[i];
+    __syncthreads();
+  }
+  const Seqs q{a.page_starts, cached ? near : a.q_starts, *a.n_free_out + a.page_starts[a.batch]};
+  extend_block(x, blockIdx.x, q, [&](int i, int32_t) { return a.kv_lens[i] - (q.tokens[i + 1] - q.tokens[i]); });
 }
 
 // Block = sequence: its pages that are no longer needed go on the stack, in order.
+__device__ inline void release_row(const PlanArgs& a, int i, int32_t keeps, int32_t from, int32_t n, int32_t base) {
+  if (n == 0) return;
+  const int32_t row = a.seqs ? a.seqs[i] : i, first = max(pages_of(a.t, keeps), a.owned ? a.owned[row] : 0);
+  for (int j = threadIdx.x; j < n; j += kFill) a.t.free_pages[base + from + j] = a.t.table[row * a.t.stride + first + j];
+}
 __global__ __launch_bounds__(kFill) void kv_release_kernel(PlanArgs a) {
   const int i = blockIdx.x;
   const int32_t from = a.page_starts[i], n = a.page_starts[i + 1] - from;
-  if (n == 0) return;
-  const int32_t row = a.seqs ? a.seqs[i] : i, base = *a.n_free_out - a.page_starts[a.batch] + from;
-  const int32_t first = max(pages_of(a.t, a.lens_out[row]), a.owned ? a.owned[row] : 0);
-  for (int j = threadIdx.x; j < n; j += kFill) a.t.free_pages[base + j] = a.t.table[row * a.t.stride + first + j];
+  if (n > 0)
+    release_row(a, i, a.lens_out[a.seqs ? a.seqs[i] : i], from, n, *a.n_free_out - a.page_starts[a.batch]);
+}
+
+// A call in one launch: every block works the sums out for itself, which takes few
+// sequences no longer than a second launch, and the state must not be written where
+// other blocks still read it. (64 sequences of 1024-page tables: 4.9 us, in two
+// launches 6.5.)
+template <bool RELEASE>
+__global__ __launch_bounds__(kFill) void kv_one_kernel(ExtendArgs x) {
+  __shared__ int32_t pages[kOneBatch + 1], tokens[kOneBatch + 1];
+  const PlanArgs& a = x.p;
+  const Sums s = sums_of<kFill, kOneRows>(a);
+  const bool go = s.status == 0;
+  Pair before = s.before;
+  for (int i = s.i0; i < s.i1; ++i) {
+    const Ask k = ask_of(a, i);
+    pages[i] = go ? (int32_t)before.pages : 0;
+    tokens[i] = go ? (int32_t)before.tokens : 0;
+    before.pages += k.pages;
+    before.tokens += k.tokens;
+  }
+  if (threadIdx.x == 0) {
+    pages[a.batch] = go ? (int32_t)s.total.pages : 0;
+    tokens[a.batch] = go ? (int32_t)s.total.tokens : 0;
+  }
+  if (blockIdx.x == 0) write_plan<kFill>(a, s);
+  __syncthreads();
+  if constexpr (RELEASE) {
+    for (int i = blockIdx.x; i < a.batch; i += gridDim.x)
+      if (pages[i + 1] > pages[i])
+        release_row(a, i, (int32_t)ask_of(a, i).now, pages[i], pages[i + 1] - pages[i], s.n_free);
+  } else if ((int)blockIdx.x < x.blocks) {
+    const Seqs q{pages, tokens, s.n_free};
+    extend_block(x, blockIdx.x, q, [&](int, int32_t row) { return max(a.t.lens[row], 0); });
+  }
 }
 
 int check_tables(const char* what, const hgk_kv_tables* t, int64_t batch, TablesView* out) {
@@ -251,6 +328,11 @@ int check_batch(const char* what, const TablesView& t, const int32_t* seqs, int6
   return HGK_OK;
 }
 
+// One launch will do: few sequences, and a state that is not written in place.
+bool in_one(const PlanArgs& a) {
+  return a.batch <= kOneBatch && a.t.rows <= kOneRows && a.lens_out != a.t.lens && a.n_free_out != a.t.n_free;
+}
+
 }  // namespace
 }  // namespace hgk
 
@@ -284,9 +366,14 @@ extern "C" int hgk_kv_extend(const hgk_kv_tables* tables, const int32_t* seqs, c
   a.status = status;
   a.page_starts = workspace;
   ExtendArgs x{a, slots, positions, block_table, block_table_stride, (int32_t)((tokens + kFill - 1) / kFill),
-               (a.t.width + kFill - 1) / kFill};
+               (a.t.width + kFill - 1) / kFill, 0};
   const int64_t blocks = x.token_blocks + (block_table ? batch * x.row_blocks : 0);
   if (blocks > kMaxBlocks) return fail(HGK_ERR_ARG, "%s: %lld rows of %d pages are too many", what, (long long)batch, a.t.width);
+  x.blocks = (int32_t)blocks;
+  if (in_one(a) && blocks <= kOneBlocks) {
+    HGK_LAUNCH(kv_one_kernel<false>, dim3((unsigned)std::max<int64_t>(blocks, 1)), dim3(kFill), 0, as_stream(stream), x);
+    return launch_status(what);
+  }
   HGK_LAUNCH(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, as_stream(stream), a);
   if (int st = launch_status(what)) return st;
   if (blocks == 0) return HGK_OK;
@@ -312,6 +399,13 @@ extern "C" int hgk_kv_release(const hgk_kv_tables* tables, const int32_t* seqs, 
   a.n_free_out = n_free_out;
   a.status = status;
   a.page_starts = workspace;
+  if (in_one(a)) {
+    ExtendArgs x{};
+    x.p = a;
+    const int64_t blocks = std::clamp<int64_t>(batch, 1, kOneBlocks);
+    HGK_LAUNCH(kv_one_kernel<true>, dim3((unsigned)blocks), dim3(kFill), 0, as_stream(stream), x);
+    return launch_status(what);
+  }
   HGK_LAUNCH(kv_plan_kernel, dim3(1), dim3(kPlanThreads), 0, as_stream(stream), a);
   if (int st = launch_status(what)) return st;
   if (batch == 0) return HGK_OK;

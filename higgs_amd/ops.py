@@ -765,30 +765,28 @@ class KVState(NamedTuple):
     status: torch.Tensor
 
 
-def _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what):
-    """The packed hgk_kv_tables, and the batch's size."""
-    dev = tables.device
-    if tables.dim() != 2 or tables.dtype != torch.int32 or (tables.shape[1] > 1 and tables.stride(1) != 1):
-        raise HgkError(1, f"{what}: tables must be int32 [sequences, pages] with a unit-stride last axis")
+def _ints(t: torch.Tensor, n: int, dev, what: str, name: str) -> int:
+    """The address of a contiguous int32 [n] (n < 0: of any length) on dev."""
+    if t.dtype != torch.int32 or t.dim() != 1 or t.device != dev:
+        raise HgkError(1, f"{what}: {name} must be int32 [{'n' if n < 0 else n}] on {dev}")
+    m = t.shape[0]
+    if (m != n and n >= 0) or (m > 1 and t.stride(0) != 1):
+        raise HgkError(1, f"{what}: {name} must be contiguous int32[{'n' if n < 0 else n}]")
+    return t.data_ptr()
+
+
+def _kv_tables(tables, lens, free_pages, n_free, page_size, what):
+    """The packed hgk_kv_tables, the rows and the pages of a row."""
+    if tables.dim() != 2 or tables.dtype != torch.int32:
+        raise HgkError(1, f"{what}: tables must be int32 [sequences, pages]")
+    dev, (rows, width), (stride, unit) = tables.device, tables.shape, tables.stride()
+    if unit != 1 and width > 1:
+        raise HgkError(1, f"{what}: tables: last axis must be unit-stride")
     if not 1 <= page_size <= 65536:
         raise HgkError(1, f"{what}: page_size={page_size} must be a power of two in 1..65536")
-    rows = tables.shape[0]
-    for name, t, shape in (("lens", lens, (rows,)), ("n_free", n_free, (1,)), ("free_pages", free_pages, None),
-                           ("seqs", seqs, None)):
-        if t is None:
-            continue
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (shape and t.shape != shape):
-            raise HgkError(1, f"{what}: {name} must be contiguous int32{list(shape) if shape else '[n]'}")
-        if t.device != dev:
-            raise HgkError(1, f"{what}: operands on different devices")
-    return _KV_TABLES.pack(page_size, rows, tables.data_ptr(), tables.stride(0), tables.shape[1], lens.data_ptr(),
-                           free_pages.data_ptr(), free_pages.shape[0], n_free.data_ptr())
-
-
-def _batch_ints(t, batch, dev, what, name):
-    if t.dtype != torch.int32 or t.shape != (batch,) or not t.is_contiguous() or t.device != dev:
-        raise HgkError(1, f"{what}: {name} must be contiguous int32[{batch}] on {dev}")
-    return t.data_ptr()
+    return _KV_TABLES.pack(page_size, rows, tables.data_ptr(), stride, width, _ints(lens, rows, dev, what, "lens"),
+                           _ints(free_pages, -1, dev, what, "free_pages"), free_pages.shape[0],
+                           _ints(n_free, 1, dev, what, "n_free")), rows, width
 
 
 def kv_extend(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor, n_free: torch.Tensor,
@@ -813,30 +811,29 @@ def kv_extend(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor
     nothing and gives a step without new tokens; status [1] tells why (a sum of
     TABLES_PAGES 1, TABLES_WIDTH 2, TABLES_SEQUENCE 4, TABLES_TOKENS 8)."""
     what = "kv_extend"
-    state = _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what)
-    dev, rows = tables.device, tables.shape[0]
-    batch = counts.shape[0] if counts.dim() == 1 else -1
-    if seqs is not None and seqs.shape[0] != batch or seqs is None and batch != rows:
-        raise HgkError(1, f"{what}: counts for {rows if seqs is None else seqs.shape[0]} sequences expected")
-    c = _batch_ints(counts, batch, dev, what, "counts")
+    state, rows, width = _kv_tables(tables, lens, free_pages, n_free, page_size, what)
+    dev = tables.device
+    batch = rows if seqs is None else seqs.shape[0] if seqs.dim() == 1 else -1
+    c = _ints(counts, batch, dev, what, "counts")
+    s = 0 if seqs is None else _ints(seqs, batch, dev, what, "seqs")
     tokens = operator.index(tokens)
     if not 0 <= tokens <= 2 ** 30:
         raise HgkError(1, f"{what}: tokens={tokens}")
-    # one array for the small results, and the call's workspace at its end
-    sizes = [batch, batch + 1, tokens, 1] if inplace else [batch, batch + 1, tokens, 1, rows, 1]
-    ints = torch.empty((sum(sizes) + batch + 1,), dtype=torch.int32, device=dev)
-    parts = ints.split_with_sizes([*sizes, batch + 1])
-    kv_lens, starts, positions, status = parts[:4]
-    lens_out, n_out = (lens, n_free) if inplace else parts[4:6]
-    slots = torch.empty((tokens,), dtype=torch.int64, device=dev)
-    if seqs is None:
-        table, rows_of = tables, 0
+    # one array for the small results, the call's workspace of batch + 1 at its end
+    small = 3 * batch + tokens + 3
+    if inplace:
+        ints = torch.empty((small,), dtype=torch.int32, device=dev)
+        kv_lens, starts, positions, status, ws = ints.split_with_sizes([batch, batch + 1, tokens, 1, batch + 1])
+        lens_out, n_out = lens, n_free
     else:
-        table = torch.empty((batch, tables.shape[1]), dtype=torch.int32, device=dev)
-        rows_of = seqs.data_ptr()
-    _kv_call(dev, lib().hgk_kv_extend, state, rows_of, c, batch, tokens, lens_out.data_ptr(), n_out.data_ptr(),
+        ints = torch.empty((small + rows + 1,), dtype=torch.int32, device=dev)
+        kv_lens, starts, positions, status, lens_out, n_out, ws = ints.split_with_sizes(
+            [batch, batch + 1, tokens, 1, rows, 1, batch + 1])
+    slots = torch.empty((tokens,), dtype=torch.int64, device=dev)
+    table = tables if seqs is None else torch.empty((batch, width), dtype=torch.int32, device=dev)
+    _kv_call(dev, lib().hgk_kv_extend, state, s, c, batch, tokens, lens_out.data_ptr(), n_out.data_ptr(),
              kv_lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-             table.data_ptr() if rows_of else 0, tables.shape[1], status.data_ptr(), parts[-1].data_ptr())
+             0 if seqs is None else table.data_ptr(), width, status.data_ptr(), ws.data_ptr())
     return KVStep(table, kv_lens, starts, slots, positions, lens_out, n_out, status)
 
 
@@ -850,17 +847,21 @@ def kv_release(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tenso
     own and stay. Returns KVState: lens [S], n_free [1], status [1] (as
     kv_extend; nothing is changed where it is not zero)."""
     what = "kv_release"
-    state = _kv_tables(tables, lens, free_pages, n_free, page_size, seqs, what)
-    dev, rows = tables.device, tables.shape[0]
-    batch = rows if seqs is None else seqs.shape[0]
-    k = None if keep is None else _batch_ints(keep, batch, dev, what, "keep")
-    o = None if owned_from is None else _batch_ints(owned_from, rows, dev, what, "owned_from")
-    sizes = [1, batch + 1] if inplace else [1, batch + 1, rows, 1]
-    parts = torch.empty((sum(sizes),), dtype=torch.int32, device=dev).split_with_sizes(sizes)
-    lens_out, n_out = (lens, n_free) if inplace else parts[2:]
-    _kv_call(dev, lib().hgk_kv_release, state, _ptr(seqs), k, o, batch, lens_out.data_ptr(), n_out.data_ptr(),
-             parts[0].data_ptr(), parts[1].data_ptr())
-    return KVState(lens_out, n_out, parts[0])
+    state, rows, _ = _kv_tables(tables, lens, free_pages, n_free, page_size, what)
+    dev = tables.device
+    batch = rows if seqs is None else seqs.shape[0] if seqs.dim() == 1 else -1
+    s = 0 if seqs is None else _ints(seqs, batch, dev, what, "seqs")
+    k = 0 if keep is None else _ints(keep, batch, dev, what, "keep")
+    o = 0 if owned_from is None else _ints(owned_from, rows, dev, what, "owned_from")
+    if inplace:
+        status, ws = torch.empty((batch + 2,), dtype=torch.int32, device=dev).split_with_sizes([1, batch + 1])
+        lens_out, n_out = lens, n_free
+    else:
+        status, lens_out, n_out, ws = torch.empty((batch + rows + 3,), dtype=torch.int32, device=dev).split_with_sizes(
+            [1, rows, 1, batch + 1])
+    _kv_call(dev, lib().hgk_kv_release, state, s, k, o, batch, lens_out.data_ptr(), n_out.data_ptr(),
+             status.data_ptr(), ws.data_ptr())
+    return KVState(lens_out, n_out, status)
 
 
 # ---------------------------------------------------------------- routed experts
@@ -924,19 +925,23 @@ def moe_combine(y: torch.Tensor, weights: torch.Tensor, *, shared: Optional[torc
             raise HgkError(1, f"{what}: shared must be {y.dtype} {list(shape)}")
         ss = _rows2d(shared)[2]
     if shared_gate is not None:
-        if shared_gate.numel() != tokens or shared_gate.shape not in (weights.shape[:-1], (*weights.shape[:-1], 1)):
-            raise HgkError(1, f"{what}: shared_gate must be {list(weights.shape[:-1])}")
-        gd = dtype_code(shared_gate.dtype)
-        gs = _rows2d(shared_gate if shared_gate.shape != weights.shape[:-1] else shared_gate.unsqueeze(-1))[2]
+        lead = shape[:-1]
+        if shared_gate.shape != (*lead, 1):
+            if shared_gate.shape != lead:
+                raise HgkError(1, f"{what}: shared_gate must be {list(lead)} or {[*lead, 1]}")
+            shared_gate = shared_gate.unsqueeze(-1)
+        gd, gs = dtype_code(shared_gate.dtype), _rows2d(shared_gate)[2]
+    if weights.device != dev or (shared is not None and shared.device != dev) \
+            or (shared_gate is not None and shared_gate.device != dev) or (out is not None and out.device != dev):
+        raise HgkError(1, f"{what}: operands on different devices")
     if out is None:
-        out = torch.empty(shape, dtype=y.dtype, device=dev)
+        out, os_ = torch.empty(shape, dtype=y.dtype, device=dev), n
     elif out.shape != shape or out.dtype != y.dtype:
         raise HgkError(1, f"{what}: out must be {y.dtype} {list(shape)}")
-    for t in (weights, shared, shared_gate, out):
-        if t is not None and t.device != dev:
-            raise HgkError(1, f"{what}: operands on different devices")
+    else:
+        os_ = _rows2d(out)[2]
     _kv_call(dev, lib().hgk_moe_combine, dtype_code(y.dtype), y.data_ptr(), ys, weights.data_ptr(), ws, top_k,
-             _ptr(shared), ss, _ptr(shared_gate), gd, gs, out.data_ptr(), _rows2d(out)[2], tokens, n)
+             _ptr(shared), ss, _ptr(shared_gate), gd, gs, out.data_ptr(), os_, tokens, n)
     return out
 
 
