@@ -34,24 +34,40 @@ struct AttnArgs {
   int32_t splits;
   float* part;  // [...][head_dim], not normalised
   float* stat;  // [...][2]: reference (log2 domain; behind a prefix a raw score), sum
-  // A prefix that the sequences share: its pages, which stand for the sequences'
-  // own where key < prefix, and the parts that a row has of a pass of its own over
-  // those keys (0: there is none, and the sequences' pass takes all keys). With
-  // prefix_table the parts of a row lie at [row][row_parts], the prefix's first.
+};
+
+// Of a call whose sequences share a prefix: its pages, which stand for the sequences'
+// own where key < prefix; the parts that a row has of a pass of its own over those
+// keys (0: there is none, and the sequences' pass takes all keys); and all parts of a
+// row, which lie at [row][row_parts], the prefix's first. (Not in AttnArgs: the kernels
+// without a prefix are compiled otherwise with it, and slower by up to 4 %.)
+struct PrefixArgs : AttnArgs {
   const int32_t* prefix_table;
   int32_t prefix_width, prefix, pre, row_parts;
   int32_t chunk;  // single tokens: tiles of a part
 };
+__device__ inline int32_t prefix_of(const AttnArgs&) { return 0; }
+__device__ inline int32_t prefix_of(const PrefixArgs& a) { return a.prefix; }
+__device__ inline int32_t pre_of(const AttnArgs&) { return 0; }
+__device__ inline int32_t pre_of(const PrefixArgs& a) { return a.pre; }
+__device__ inline int32_t row_parts_of(const AttnArgs&) { return 1; }
+__device__ inline int32_t row_parts_of(const PrefixArgs& a) { return a.row_parts; }
 
 // Which keys a block takes: all of each row, of the row's own table; those of the
 // shared prefix, for the rows of all sequences at once; or those behind it (all, if
 // there is no pass over the prefix), with the prefix's table in front of the own one.
 enum Keys { kOwn, kPrefix, kBehind };
 
-// The table's entry for a key of a sequence whose first keys are the prefix's.
-__device__ inline int32_t page_behind(const AttnArgs& a, const int32_t* table, int32_t key) {
+// The prefix's table's entry for a key, and the table's of a sequence that begins with it.
+__device__ inline int32_t page_of_prefix(const AttnArgs&, int32_t) { return -1; }
+__device__ inline int32_t page_of_prefix(const PrefixArgs& a, int32_t key) {
   const int32_t e = key >> a.p.page_shift;
-  if (key < a.prefix) return e < a.prefix_width ? a.prefix_table[e] : -1;
+  return e < a.prefix_width ? a.prefix_table[e] : -1;
+}
+template <class Args>
+__device__ inline int32_t page_behind(const Args& a, const int32_t* table, int32_t key) {
+  if (key < prefix_of(a)) return page_of_prefix(a, key);
+  const int32_t e = key >> a.p.page_shift;
   return e < a.b.width ? table[e] : -1;
 }
 
@@ -298,237 +314,6 @@ __device__ inline Owner find_owner(int batch, C count, W want_of) {
 template <int KEYS>
 __device__ inline int decode_tiles(const Seen& s) { return (s.n + KEYS - 1) / KEYS; }
 
-// Sums of 16 heads over some keys. A lane has 4 values, 16 t + 4 (lane / 16) .., of head
-// lane % 16.
-template <int D> struct DecodeSums {
-  f32x4 o[D / 16];
-  float ref, sum;
-  bool any;  // has the wave seen a key?
-};
-
-// One wave's walk over the tiles first, first + STEP, ... below last of a run of n
-// keys of a kv head; key_of(i) is the position of key i, page_of(position) its page.
-//
-// A tile's scores are S^T = K Q^T on 16x16x32 matrix instructions: keys are
-// the rows, so K's 16-byte pieces go from memory straight into the operand,
-// and a lane ends with 4 keys each of one head. That is also where the second
-// product O^T = V^T P^T wants its weights: no weight crosses lanes. V^T comes
-// through LDS (written row by row, read transposed). K and V of the next tile
-// are in flight while a tile is computed.
-//
-// Weights are split in two 16-bit parts (hi + lo, both multiplied): the
-// matrix cores have time to spare, and two parts keep 16 bits of a weight in
-// bf16 and 22 in f16, well below the result's own rounding.
-template <class T, int D, int CAP, int STEP, class Key, class Page>
-__device__ __forceinline__ DecodeSums<D> decode_walk(const AttnArgs& a, const Scale& sc, const u32x4 (&qf)[D / 32],
-                                                     int hk, int first, int last, int n, char* vt, Key key_of,
-                                                     Page page_of) {
-  constexpr int NS = dec_keys<D>() / 16, kKeys = 16 * NS, kStep = D / 32, kOut = D / 16, kRow = dec_row<D>();
-  const int lane = threadIdx.x & 63, m = lane & 15, j = lane >> 4;
-  const char* kbase = a.p.k + 2 * (hk * a.p.kst[2] + 8 * j);
-  const char* vbase = a.p.v + 2 * (hk * a.p.vst[2] + 8 * j);
-  // page of key i of the run (-1: none) and its place in the page
-  auto look_up = [&](int tile, int32_t* page, int32_t* at) {
-#pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      const int i = tile * kKeys + 16 * h + m;
-      page[h] = -1;
-      at[h] = 0;
-      if (tile < last && i < n) {
-        const int32_t key = key_of(i);
-        page[h] = page_of(key);
-        at[h] = key & a.p.page_mask;
-      }
-    }
-  };
-  u32x4 kr[NS][kStep], vr[NS][kStep];
-  uint32_t there = 0;  // bit i: key i of the loaded tile exists
-  auto load = [&](const int32_t* page, const int32_t* at) {
-    there = 0;
-#pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      const bool ok = (uint32_t)page[h] < (uint32_t)a.p.n_pages;
-      there |= (uint32_t)(__ballot(ok) & 0xffffu) << (16 * h);
-      // a key that does not exist reads the pool's first row, and is masked below
-      const int64_t pg = ok ? page[h] : 0, r = ok ? at[h] : 0;
-      const char* kp = kbase + 2 * (pg * a.p.kst[0] + r * a.p.kst[1]);
-      const char* vp = vbase + 2 * (pg * a.p.vst[0] + r * a.p.vst[1]);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) kr[h][s] = *reinterpret_cast<const u32x4*>(kp + 64 * s);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) vr[h][s] = *reinterpret_cast<const u32x4*>(vp + 64 * s);
-    }
-  };
-
-  DecodeSums<D> acc;
-  f32x4(&o)[kOut] = acc.o;
-#pragma unroll
-  for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
-  float ref = lowest_ref(sc.c), sum = 0.0f;
-  const float slack = Mx<T>::kDecSlack / sc.c;
-  bool any = false;
-  constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
-
-  int32_t page[NS], at[NS];
-  if (a.p.n_pages > 0 && first < last) {
-    look_up(first, page, at);
-    load(page, at);
-    look_up(first + STEP, page, at);
-    for (int tile = first; tile < last; tile += STEP) {
-      // scores
-      f32x4 s[NS];
-#pragma unroll
-      for (int h = 0; h < NS; ++h) {
-        s[h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
-      }
-      const uint32_t now = there;
-      if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
-#pragma unroll
-        for (int h = 0; h < NS; ++h)
-          if (!((now >> (16 * h + m)) & 1))
-#pragma unroll
-            for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int h = 0; h < NS; ++h)
-#pragma unroll
-        for (int k = 0; k < kStep; ++k)
-          *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
-      if (tile + STEP < last) {
-        load(page, at);
-        look_up(tile + 2 * STEP, page, at);
-      }
-      // weights
-      float x[4 * NS], top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) {
-        x[i] = s[i / 4][i % 4];
-        if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
-      }
-      const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
-      if (now != kAll) {
-#pragma unroll
-        for (int i = 0; i < 4 * NS; ++i)
-          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
-      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = top > ref + slack ? top : ref, f = lesser((ref - to) * sc.c);
-        sum *= f;
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) o[t] *= f;
-        ref = to;
-      }
-      const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
-      any |= now != 0;
-      uint32_t hi[2 * NS], lo[2 * NS];
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) {
-        sum += x[2 * i] + x[2 * i + 1];
-        hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
-        lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
-      }
-      // O^T += V^T P^T
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int t = 0; t < kOut; ++t) {
-        const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
-        const u32x2 v0 = lds_transposed(p);
-        if constexpr (NS == 2) {
-          const u32x2 v1 = lds_transposed(p + 16 * kRow);
-          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-          o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
-          o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
-        } else {
-          o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
-          o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
-    }
-  }
-  sum += __shfl_xor(sum, 16);
-  sum += __shfl_xor(sum, 32);
-  acc.ref = ref;
-  acc.sum = sum;
-  acc.any = any;
-  return acc;
-}
-
-// Did this lane's head's scores not fit the weights' form, or are its sums not finite?
-template <int D>
-__device__ __forceinline__ bool decode_odd(const Scale& sc, const DecodeSums<D>& x) {
-  float peak = x.sum;
-#pragma unroll
-  for (int t = 0; t < D / 16; ++t) peak = peak3(peak3(peak, x.o[t][0], x.o[t][1]), x.o[t][2], x.o[t][3]);
-  return x.any && !(fabsf(x.ref * sc.c) <= kBaseMax && peak < INFINITY);
-}
-
-// Such heads' keys once more, one after the other in f32. The reference is the
-// maximum, subtracted before the scale, and an infinity or NaN among the values
-// counts however small its key's weight is (the two parts of a weight would
-// not do: the lesser one may be zero or negative). Lane: head m, a quarter of D.
-// qp: the lane's head's q from its quarter on. Returns the head's reference and sum.
-template <class T, int D, int CAP, int STEP, class Key, class Page>
-__device__ __forceinline__ f32x2 decode_again(const AttnArgs& a, const Scale& sc, const char* qp, int hk, int first,
-                                              int last, int n, Key key_of, Page page_of, float (&acc)[D / 4]) {
-  constexpr int kKeys = dec_keys<D>();
-  const int j = (threadIdx.x & 63) >> 4;
-  constexpr int kPieces = D / 32;
-  float r = lowest_ref(sc.c), l = 0.0f;
-#pragma unroll
-  for (int d = 0; d < D / 4; ++d) acc[d] = 0.0f;
-#pragma unroll 1
-  for (int i = first * kKeys; i < min(last * kKeys, n); i += (i + 1) % kKeys ? 1 : 1 + (STEP - 1) * kKeys) {
-    const int32_t key = key_of(i), pg = page_of(key);
-    if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
-    const int64_t row = key & a.p.page_mask;
-    const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
-    const char* vp = a.p.v + 2 * (hk * a.p.vst[2] + pg * a.p.vst[0] + row * a.p.vst[1] + j * (D / 4));
-    float x = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-      const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + 16 * c);
-      const u32x4 qw = *reinterpret_cast<const u32x4*>(qp + 16 * c);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t qq = (qw[w] & sc.keep) ^ sc.flip;
-        x = fmaf(T::hi(kw[w]), T::hi(qq), fmaf(T::lo(kw[w]), T::lo(qq), x));
-      }
-    }
-    x += __shfl_xor(x, 16);
-    x += __shfl_xor(x, 32);
-    if constexpr (CAP) x = cap_tanh<CAP>(x * sc.inner);
-    if (x > r) {
-      const float f = lesser((r - x) * sc.c);
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < D / 4; ++d) acc[d] *= f;
-      r = x;
-    }
-    const float w = __builtin_amdgcn_exp2f(fmaf(x - r, sc.c, Mx<T>::kDecBias));
-    const float odd = x == -INFINITY ? w : fmaxf(w, 1.0e-44f);
-    l += w;
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-      const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + 16 * c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = e & 1 ? T::hi(vw[e / 2]) : T::lo(vw[e / 2]);
-        acc[8 * c + e] = fmaf(v, fabsf(v) < INFINITY ? w : odd, acc[8 * c + e]);
-      }
-    }
-  }
-  return f32x2{r, l};
-}
-
 // ---------------------------------------------------------------- prompts
 // 16 bytes per lane from memory to LDS at dst + 16 * lane (dst is uniform):
 // from base + off, or from an address of the lane's own. m0 is written inside,
@@ -622,8 +407,8 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 // and y are the block's place, `splits` the y there are.
 constexpr int kPromptWords = 2 + 2 * (2 * kPromptRows / 64);
 template <int D> constexpr int prompt_lds() { return 4 * 64 * 2 * D; }
-template <class T, int D, int BN, int CAP>
-__device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* lds, int* words, int x, int grid_x,
+template <class T, int D, int BN, int CAP, class Args>
+__device__ __forceinline__ void attn_prompt(Keys keys, const Args& a, char* lds, int* words, uint32_t x, uint32_t grid_x,
                                             int y, int splits) {
   constexpr int NT = 2 * kPromptRows, BM = kPromptRows, CH = D / 8, kUnits = BN * CH / NT;
   constexpr int kRow = 2 * D, kTile = BN * kRow;
@@ -656,15 +441,14 @@ __device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* 
   }
   const int R = s.n * G, pos0 = s.len - s.n;  // pos0 may be negative: rows in front of the sequence
 
-  // the block's keys, in tiles of BN: those of the first `sinks`, then the window's
   const int row0 = tile * BM;
-  // this lane's row, and the positions of the wave's and the block's
+  int p_first = pos0 + row0 / G, p_last = pos0 + (min(row0 + BM, R) - 1) / G;
+  // this lane's row
   const int wrow0 = row0 + 32 * wave;
   const int row = min(wrow0 + col, R - 1);
   const int qi = row / G, head = hk * G + row - qi * G;
   const bool in = wrow0 + col < R;
-  int p = pos0 + qi, p_first = pos0 + row0 / G, p_last = pos0 + (min(row0 + BM, R) - 1) / G;
-  int pw_first = pos0 + min(wrow0, R - 1) / G, pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
+  int p = pos0 + qi, pw_first = 0, pw_last = 0;
   if (keys == kPrefix) {
     // every row has a sequence of its own; a row of none sees nothing
     int* const lowest_of = words + 2;
@@ -689,19 +473,26 @@ __device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* 
     p_first = __builtin_amdgcn_readfirstlane(p_first);
     p_last = __builtin_amdgcn_readfirstlane(p_last);
   }
-  // keys from .. cap - 1 are the kernel's
-  const int from = keys == kBehind && a.pre > 0 ? a.prefix : 0;
+  // the block's keys, in tiles of BN: those of the first `sinks`, then the window's,
+  // of the keys from .. cap - 1 that are the call's
+  const int from = keys == kBehind && pre_of(a) > 0 ? prefix_of(a) : 0;
   const int64_t own = (int64_t)a.b.width << a.p.page_shift;
-  const int64_t cap = keys == kOwn ? own : keys == kPrefix ? (int64_t)a.prefix : max(own, (int64_t)a.prefix);
+  const int64_t cap = keys == kOwn ? own : keys == kPrefix ? (int64_t)prefix_of(a) : max(own, (int64_t)prefix_of(a));
   const int hi = (int)min((int64_t)p_last + 1, cap);
   const int lo = a.window > 0 && p_first >= a.window ? p_first - a.window + 1 : 0;
-  const int t_from = from / BN, t_hi = hi > 0 ? (hi + BN - 1) / BN : 0, t_lo = max(lo, from) / BN;
+  const int t_from = from / BN, t_hi = hi > 0 ? (hi + BN - 1) / BN : 0;
+  const int t_lo = (keys == kBehind ? max(lo, from) : lo) / BN;
   // (at most 2^30 before it is rounded up: sinks and lo may both end at int32's end)
-  const int front = max(min((min(min(a.sinks, lo), max(hi, 0)) + BN - 1) / BN, t_lo) - t_from, 0);
+  int front = min((min(min(a.sinks, lo), max(hi, 0)) + BN - 1) / BN, t_lo);
+  if (keys == kBehind) front = max(front - t_from, 0);
   const int tiles = a.p.n_pages > 0 ? front + max(t_hi - t_lo, 0) : 0;
   const int per = (tiles + splits - 1) / splits;
   const int it0 = min(per * y, tiles), it1 = min(it0 + per, tiles);
   auto tile_of = [&](int it) { return it < front ? t_from + it : t_lo + it - front; };
+  if (keys != kPrefix) {  // the range of the wave's rows
+    pw_first = pos0 + min(wrow0, R - 1) / G;
+    pw_last = pos0 + min(wrow0 + 31, R - 1) / G;
+  }
 
   const Scale sc = fold_scale<CAP>(a);
 
@@ -712,10 +503,7 @@ __device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* 
   auto look_up = [&](int it) -> int32_t {
     if (it >= it1) return -1;
     const int key = tile_of(it) * BN + (lane & (BN - 1));
-    if (keys == kPrefix) {
-      const int e = key >> a.p.page_shift;
-      return key < hi && e < a.prefix_width ? a.prefix_table[e] : -1;
-    }
+    if (keys == kPrefix) return key < hi ? page_of_prefix(a, key) : -1;
     if (keys == kBehind) return key >= from && key < hi ? page_behind(a, table, key) : -1;
     return key < hi ? table[key >> a.p.page_shift] : -1;
   };
@@ -730,7 +518,7 @@ __device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* 
   const bool whole = a.p.page_shift >= 4 && a.p.kst[1] < (1 << 24) && a.p.vst[1] < (1 << 24);
   // But where the prefix ends inside such a run of rows, the rows in front of its
   // end and those behind it lie in two pages: that tile goes row by row.
-  const int cut = keys == kBehind && (a.prefix & 15) ? a.prefix / BN : -1;
+  const int cut = keys == kBehind && (prefix_of(a) & 15) ? prefix_of(a) / BN : -1;
   // (rows i * NT / CH apart have the same offsets, where that is a multiple of 16)
   constexpr int kOffs = NT % (16 * CH) == 0 ? 1 : kUnits;
   uint32_t koff[kOffs], voff[kOffs];
@@ -1117,8 +905,8 @@ __device__ __forceinline__ void attn_prompt(Keys keys, const AttnArgs& a, char* 
   // (a row's parts over the prefix come first)
   int64_t part_at = (int64_t)(s.first + qi) * a.q_heads + head;
   if (keys == kOwn) part_at = part_at * splits + y;
-  else part_at = part_at * a.row_parts + (keys == kBehind ? a.pre : 0) + y;
-  const bool parts = keys == kOwn ? splits > 1 : a.row_parts > 1;
+  else part_at = part_at * row_parts_of(a) + (keys == kBehind ? pre_of(a) : 0) + y;
+  const bool parts = keys == kOwn ? splits > 1 : row_parts_of(a) > 1;
   char* out_row = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1]);
   if (parts) {
     if (in && half == 0)

@@ -8,15 +8,15 @@ namespace {
 
 // References are raw scores here, whose differences are scaled: two products would
 // each be rounded, by up to 2^-8 at 2^16.
-__device__ inline float scale_of(const AttnArgs& a) {
+__device__ inline float scale_of(const PrefixArgs& a) {
   return a.softcap > 0.0f ? fold_scale<1>(a).c : fold_scale<0>(a).c;
 }
 
 // The keys that a sequence's last token sees behind the prefix, or all where no pass
 // takes the prefix: index i is key i + the prefix below `sinks`, and key i + skip
 // behind them.
-__device__ inline int32_t first_behind(const AttnArgs& a) { return a.pre > 0 ? a.prefix : 0; }
-__device__ inline Seen seen_behind(const AttnArgs& a, int32_t len) {
+__device__ inline int32_t first_behind(const PrefixArgs& a) { return a.pre > 0 ? a.prefix : 0; }
+__device__ inline Seen seen_behind(const PrefixArgs& a, int32_t len) {
   const int32_t from = first_behind(a);
   const int64_t cap = max((int64_t)a.b.width << a.p.page_shift, (int64_t)a.prefix);
   if (len < 0) len = 0;
@@ -29,6 +29,239 @@ __device__ inline Seen seen_behind(const AttnArgs& a, int32_t len) {
   return s;
 }
 
+// Sums of 16 heads over some keys. A lane has 4 values, 16 t + 4 (lane / 16) .., of head
+// lane % 16.
+template <int D> struct DecodeSums {
+  f32x4 o[D / 16];
+  float ref, sum;
+  bool any;  // has the wave seen a key?
+};
+
+// One wave's walk over the tiles first, first + STEP, ... below last of a run of n
+// keys of a kv head; key_of(i) is the position of key i, page_of(position) its page.
+//
+// A tile's scores are S^T = K Q^T on 16x16x32 matrix instructions: keys are
+// the rows, so K's 16-byte pieces go from memory straight into the operand,
+// and a lane ends with 4 keys each of one head. That is also where the second
+// product O^T = V^T P^T wants its weights: no weight crosses lanes. V^T comes
+// through LDS (written row by row, read transposed). K and V of the next tile
+// are in flight while a tile is computed.
+//
+// Weights are split in two 16-bit parts (hi + lo, both multiplied): the
+// matrix cores have time to spare, and two parts keep 16 bits of a weight in
+// bf16 and 22 in f16, well below the result's own rounding.
+// (attn_decode_kernel has this loop in its own body: through a function it takes 4
+// registers more.)
+template <class T, int D, int CAP, int STEP, class Key, class Page>
+__device__ __forceinline__ DecodeSums<D> decode_walk(const PrefixArgs& a, const Scale& sc, const u32x4 (&qf)[D / 32],
+                                                     int hk, int first, int last, int n, char* vt, Key key_of,
+                                                     Page page_of) {
+  constexpr int NS = dec_keys<D>() / 16, kKeys = 16 * NS, kStep = D / 32, kOut = D / 16, kRow = dec_row<D>();
+  const int lane = threadIdx.x & 63, m = lane & 15, j = lane >> 4;
+  const char* kbase = a.p.k + 2 * (hk * a.p.kst[2] + 8 * j);
+  const char* vbase = a.p.v + 2 * (hk * a.p.vst[2] + 8 * j);
+  // page of key i of the run (-1: none) and its place in the page
+  auto look_up = [&](int tile, int32_t* page, int32_t* at) {
+#pragma unroll
+    for (int h = 0; h < NS; ++h) {
+      const int i = tile * kKeys + 16 * h + m;
+      page[h] = -1;
+      at[h] = 0;
+      if (tile < last && i < n) {
+        const int32_t key = key_of(i);
+        page[h] = page_of(key);
+        at[h] = key & a.p.page_mask;
+      }
+    }
+  };
+  u32x4 kr[NS][kStep], vr[NS][kStep];
+  uint32_t there = 0;  // bit i: key i of the loaded tile exists
+  auto load = [&](const int32_t* page, const int32_t* at) {
+    there = 0;
+#pragma unroll
+    for (int h = 0; h < NS; ++h) {
+      const bool ok = (uint32_t)page[h] < (uint32_t)a.p.n_pages;
+      there |= (uint32_t)(__ballot(ok) & 0xffffu) << (16 * h);
+      // a key that does not exist reads the pool's first row, and is masked below
+      const int64_t pg = ok ? page[h] : 0, r = ok ? at[h] : 0;
+      const char* kp = kbase + 2 * (pg * a.p.kst[0] + r * a.p.kst[1]);
+      const char* vp = vbase + 2 * (pg * a.p.vst[0] + r * a.p.vst[1]);
+#pragma unroll
+      for (int s = 0; s < kStep; ++s) kr[h][s] = *reinterpret_cast<const u32x4*>(kp + 64 * s);
+#pragma unroll
+      for (int s = 0; s < kStep; ++s) vr[h][s] = *reinterpret_cast<const u32x4*>(vp + 64 * s);
+    }
+  };
+
+  DecodeSums<D> acc;
+  f32x4(&o)[kOut] = acc.o;
+#pragma unroll
+  for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
+  float ref = lowest_ref(sc.c), sum = 0.0f;
+  const float slack = Mx<T>::kDecSlack / sc.c;
+  bool any = false;
+  constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
+
+  int32_t page[NS], at[NS];
+  if (a.p.n_pages > 0 && first < last) {
+    look_up(first, page, at);
+    load(page, at);
+    look_up(first + STEP, page, at);
+    for (int tile = first; tile < last; tile += STEP) {
+      // scores
+      f32x4 s[NS];
+#pragma unroll
+      for (int h = 0; h < NS; ++h) {
+        s[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
+      }
+      const uint32_t now = there;
+      if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
+#pragma unroll
+        for (int h = 0; h < NS; ++h)
+          if (!((now >> (16 * h + m)) & 1))
+#pragma unroll
+            for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int h = 0; h < NS; ++h)
+#pragma unroll
+        for (int k = 0; k < kStep; ++k)
+          *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
+      if (tile + STEP < last) {
+        load(page, at);
+        look_up(tile + 2 * STEP, page, at);
+      }
+      // weights
+      float x[4 * NS], top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4 * NS; ++i) {
+        x[i] = s[i / 4][i % 4];
+        if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
+      }
+      const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
+      if (now != kAll) {
+#pragma unroll
+        for (int i = 0; i < 4 * NS; ++i)
+          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
+      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float to = top > ref + slack ? top : ref, f = lesser((ref - to) * sc.c);
+        sum *= f;
+#pragma unroll
+        for (int t = 0; t < kOut; ++t) o[t] *= f;
+        ref = to;
+      }
+      const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
+#pragma unroll
+      for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
+      any |= now != 0;
+      uint32_t hi[2 * NS], lo[2 * NS];
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
+        sum += x[2 * i] + x[2 * i + 1];
+        hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
+        lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
+      }
+      // O^T += V^T P^T
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int t = 0; t < kOut; ++t) {
+        const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
+        const u32x2 v0 = lds_transposed(p);
+        if constexpr (NS == 2) {
+          const u32x2 v1 = lds_transposed(p + 16 * kRow);
+          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
+          o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
+          o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
+        } else {
+          o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
+          o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
+  acc.ref = ref;
+  acc.sum = sum;
+  acc.any = any;
+  return acc;
+}
+
+// Did this lane's head's scores not fit the weights' form, or are its sums not finite?
+template <int D>
+__device__ __forceinline__ bool decode_odd(const Scale& sc, const DecodeSums<D>& x) {
+  float peak = x.sum;
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) peak = peak3(peak3(peak, x.o[t][0], x.o[t][1]), x.o[t][2], x.o[t][3]);
+  return x.any && !(fabsf(x.ref * sc.c) <= kBaseMax && peak < INFINITY);
+}
+
+// Such heads' keys once more, one after the other in f32. The reference is the
+// maximum, subtracted before the scale, and an infinity or NaN among the values
+// counts however small its key's weight is (the two parts of a weight would
+// not do: the lesser one may be zero or negative). Lane: head m, a quarter of D.
+// qp: the lane's head's q from its quarter on. Returns the head's reference and sum.
+template <class T, int D, int CAP, int STEP, class Key, class Page>
+__device__ __forceinline__ f32x2 decode_again(const PrefixArgs& a, const Scale& sc, const char* qp, int hk, int first,
+                                              int last, int n, Key key_of, Page page_of, float (&acc)[D / 4]) {
+  constexpr int kKeys = dec_keys<D>();
+  const int j = (threadIdx.x & 63) >> 4;
+  constexpr int kPieces = D / 32;
+  float r = lowest_ref(sc.c), l = 0.0f;
+#pragma unroll
+  for (int d = 0; d < D / 4; ++d) acc[d] = 0.0f;
+#pragma unroll 1
+  for (int i = first * kKeys; i < min(last * kKeys, n); i += (i + 1) % kKeys ? 1 : 1 + (STEP - 1) * kKeys) {
+    const int32_t key = key_of(i), pg = page_of(key);
+    if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
+    const int64_t row = key & a.p.page_mask;
+    const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
+    const char* vp = a.p.v + 2 * (hk * a.p.vst[2] + pg * a.p.vst[0] + row * a.p.vst[1] + j * (D / 4));
+    float x = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + 16 * c);
+      const u32x4 qw = *reinterpret_cast<const u32x4*>(qp + 16 * c);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t qq = (qw[w] & sc.keep) ^ sc.flip;
+        x = fmaf(T::hi(kw[w]), T::hi(qq), fmaf(T::lo(kw[w]), T::lo(qq), x));
+      }
+    }
+    x += __shfl_xor(x, 16);
+    x += __shfl_xor(x, 32);
+    if constexpr (CAP) x = cap_tanh<CAP>(x * sc.inner);
+    if (x > r) {
+      const float f = lesser((r - x) * sc.c);
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < D / 4; ++d) acc[d] *= f;
+      r = x;
+    }
+    const float w = __builtin_amdgcn_exp2f(fmaf(x - r, sc.c, Mx<T>::kDecBias));
+    const float odd = x == -INFINITY ? w : fmaxf(w, 1.0e-44f);
+    l += w;
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+      const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + 16 * c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = e & 1 ? T::hi(vw[e / 2]) : T::lo(vw[e / 2]);
+        acc[8 * c + e] = fmaf(v, fabsf(v) < INFINITY ? w : odd, acc[8 * c + e]);
+      }
+    }
+  }
+  return f32x2{r, l};
+}
+
 // Single tokens' own keys: WAVES waves have a chunk of a (sequence, kv head), for 16
 // of its query heads, and make one part of it.
 // lds: behind_lds<D, WAVES>() bytes, 16-byte aligned. x counts the blocks, y the 16s of
@@ -38,7 +271,7 @@ template <int D, int WAVES> constexpr int behind_lds() {
   return kTiles > kJoin ? kTiles : kJoin;
 }
 template <class T, int D, int CAP, int WAVES>
-__device__ __forceinline__ void attn_behind(const AttnArgs& a, char* lds, int block, int y) {
+__device__ __forceinline__ void attn_behind(const PrefixArgs& a, char* lds, int block, int y) {
   constexpr int kKeys = dec_keys<D>(), kStep = D / 32, kTile = kKeys * dec_row<D>();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, j = lane >> 4, step = WAVES > 1 ? wave : 0;
@@ -158,7 +391,7 @@ __device__ __forceinline__ void attn_behind(const AttnArgs& a, char* lds, int bl
 }
 
 template <class T, int D, int CAP, int WAVES>
-__global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(PrefixArgs a) {
   __shared__ __align__(16) char lds[behind_lds<D, WAVES>()];
   attn_behind<T, D, CAP, WAVES>(a, lds, blockIdx.x, blockIdx.y);
 }
@@ -169,7 +402,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(AttnArgs
 struct PrefixBlock {
   int x, grid_x, split;
 };
-__device__ inline PrefixBlock prefix_block(const AttnArgs& a, int id, int blocks) {
+__device__ inline PrefixBlock prefix_block(const PrefixArgs& a, int id, int blocks) {
   const int parts = a.pre * a.p.kv_heads, places = blocks / parts;
   int part = id / places, place = id - part * places;
   if (parts % 8 == 0) {
@@ -189,7 +422,7 @@ __device__ inline PrefixBlock prefix_block(const AttnArgs& a, int id, int blocks
 // heads of 256 (9 GFLOP, 117 MB): 54, as two 72; every sequence over a table of its
 // own (paged_attention's kernels): 496 and 149.
 template <class T, int D, int CAP>
-__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_kernel(AttnArgs a, int prefix_blocks,
+__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_kernel(PrefixArgs a, int prefix_blocks,
                                                                                           int behind_blocks) {
   static_assert(2 * kPromptRows == 64 * kDecWaves && prompt_lds<D>() >= behind_lds<D, 1>(), "one kind of block");
   __shared__ __align__(1024) char lds[prompt_lds<D>()];
@@ -207,7 +440,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared
 // Both passes of prompts in one launch. 32 sequences of up to 33 + 100 tokens behind
 // 16384, 32/8 heads of 128 f16 (148 GFLOP): 212 us with the join, 700 TFLOP/s.
 template <class T, int D, int CAP>
-__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_prompt_kernel(AttnArgs a,
+__global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_prompt_kernel(PrefixArgs a,
                                                                                                  int prefix_blocks,
                                                                                                  int behind_x) {
   __shared__ __align__(1024) char lds[prompt_lds<D>()];
@@ -229,7 +462,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared
 constexpr int kMaxParts = 256;
 template <int D, int G> constexpr int join_parts() { return G == 1 ? 4 : G == 2 ? 16 : kMaxParts; }
 template <class T, int D, int G, bool SINGLE>
-__global__ __launch_bounds__(256) void attn_prefix_join_kernel(AttnArgs a, uint32_t rows) {
+__global__ __launch_bounds__(256) void attn_prefix_join_kernel(PrefixArgs a, uint32_t rows) {
   constexpr uint32_t kLanes = D / 4, kRows = 256 / (kLanes * G), kShare = kLanes * G;
   constexpr uint32_t kMax = join_parts<D, G>(), kTurns = (kMax + kShare - 1) / kShare;
   __shared__ f32x4 vs[kRows][G][kLanes];
@@ -364,7 +597,7 @@ int check_prefix(const char* what, const KvView& p, int64_t width, int64_t prefi
 }
 
 template <class T, int D, int WAVES>
-void launch_behind(const AttnArgs& a, hipStream_t stream) {
+void launch_behind(const PrefixArgs& a, hipStream_t stream) {
   const int64_t units = (int64_t)a.b.batch * a.p.kv_heads * a.splits;
   const dim3 grid((unsigned)(WAVES > 1 ? units : (units + kDecWaves - 1) / kDecWaves), (a.group + 15) / 16);
   if (a.softcap > 0.0f)
@@ -374,7 +607,7 @@ void launch_behind(const AttnArgs& a, hipStream_t stream) {
 }
 
 template <class T, int D, bool SINGLE>
-void launch_prefix_join(const AttnArgs& a, hipStream_t stream) {
+void launch_prefix_join(const PrefixArgs& a, hipStream_t stream) {
   constexpr int kGroups = 256 / (D / 4);
   const uint32_t rows = (uint32_t)a.b.tokens * a.q_heads;
   auto grid = [&](int g) { const uint32_t n = kGroups / g; return dim3((rows + n - 1) / n); };
@@ -387,7 +620,7 @@ void launch_prefix_join(const AttnArgs& a, hipStream_t stream) {
 }
 
 template <class T, int D>
-void launch_shared(const AttnArgs& a, hipStream_t stream) {
+void launch_shared(const PrefixArgs& a, hipStream_t stream) {
   const int64_t units = (int64_t)a.b.batch * a.p.kv_heads * a.splits;
   const int prefix = (int)(a.p.kv_heads * prefix_tiles(a.b, a.group) * a.pre);
   const int behind = (int)((units + kDecWaves - 1) / kDecWaves), heads = (a.group + 15) / 16;
@@ -401,7 +634,7 @@ void launch_shared(const AttnArgs& a, hipStream_t stream) {
 }
 
 template <class T, int D>
-void launch_shared_prompts(const AttnArgs& a, hipStream_t stream) {
+void launch_shared_prompts(const PrefixArgs& a, hipStream_t stream) {
   const int prefix = (int)(a.p.kv_heads * prefix_tiles(a.b, a.group) * a.pre);
   const int behind = (int)(a.p.kv_heads * prompt_tiles(a.b, a.group));
   const dim3 grid(prefix + behind * a.splits), block(2 * kPromptRows);
@@ -414,7 +647,7 @@ void launch_shared_prompts(const AttnArgs& a, hipStream_t stream) {
 }
 
 template <class T, int D>
-int run_of(const AttnArgs& a, int waves, const char* what, hipStream_t stream) {
+int run_of(const PrefixArgs& a, int waves, const char* what, hipStream_t stream) {
   if (a.b.starts) {
     launch_shared_prompts<T, D>(a, stream);
   } else if (a.pre > 0) {
@@ -432,7 +665,7 @@ int run_of(const AttnArgs& a, int waves, const char* what, hipStream_t stream) {
 }
 
 template <class T>
-int run(const AttnArgs& a, int waves, const char* what, hipStream_t stream) {
+int run(const PrefixArgs& a, int waves, const char* what, hipStream_t stream) {
   switch (a.p.head_dim) {
     case 64: return run_of<T, 64>(a, waves, what, stream);
     case 96: return run_of<T, 96>(a, waves, what, stream);
@@ -466,7 +699,7 @@ extern "C" int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_
                                            void* stream) {
   const char* what = "hgk_shared_prefix_attention";
   clear_error();
-  AttnArgs a{};
+  PrefixArgs a{};
   if (int st = check_sizes(what, pages, batch, q_heads, window, sinks, &a.p, &a.b)) return st;
   if (int st = check_prefix(what, a.p, prefix_width, prefix_len)) return st;
   if (int st = check_scales(what, scale, softcap)) return st;
