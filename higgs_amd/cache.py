@@ -16,6 +16,7 @@ branches writes to a page that is only partly filled.
     t = cache.fork(s)                              # shares the prompt's pages
     cache.extend([s, t], [1, 1])                   # one new token each
     b = cache.batch([s, t])
+    o = cache.attend(layer, q, b, prefix=cache.shared_prefix([s, t]))  # the prompt read once
 """
 from __future__ import annotations
 
@@ -110,6 +111,18 @@ class PagedKVCache:
         f = self.new()
         self._seqs[f] = _Seq(array("i", s.pages), s.length)
         return f
+
+    def shared_prefix(self, seqs: Sequence[int]) -> int:
+        """How many tokens at their beginning all of seqs have on the same pages
+        (for attend's ``prefix``)."""
+        found = self._several(seqs, None)
+        if not found:
+            return 0
+        first, common = found[0].pages, min(len(s.pages) for s in found)
+        for s in found[1:]:
+            if first[:common] != s.pages[:common]:
+                common = next(i for i in range(common) if first[i] != s.pages[i])
+        return min(common * self.page_size, *(s.length for s in found))
 
     def _drop(self, page: int) -> None:
         self._refs[page] -= 1
@@ -213,8 +226,14 @@ class PagedKVCache:
         ops.kv_append(k, v, self.k_pages[layer], self.v_pages[layer], batch.block_table,
                       batch.kv_lens, q_starts=batch.q_starts)
 
-    def attend(self, layer: int, q: torch.Tensor, batch: KVBatch, **kw) -> torch.Tensor:
+    def attend(self, layer: int, q: torch.Tensor, batch: KVBatch, *, prefix: int = 0, **kw) -> torch.Tensor:
         """paged_attention over one layer's pages (scale, window, sinks,
-        softcap, out as there)."""
+        softcap, out as there). With ``prefix`` > 0 the batch's sequences have
+        their first ``prefix`` tokens on the same pages (shared_prefix), which are
+        read and multiplied once for all: shared_prefix_attention."""
+        if prefix:
+            pages = batch.block_table[:1].flatten()[:-(-prefix // self.page_size)]
+            return ops.shared_prefix_attention(q, self.k_pages[layer], self.v_pages[layer], batch.block_table,
+                                               batch.kv_lens, pages, prefix, q_starts=batch.q_starts, **kw)
         return ops.paged_attention(q, self.k_pages[layer], self.v_pages[layer], batch.block_table,
                                    batch.kv_lens, q_starts=batch.q_starts, **kw)

@@ -291,3 +291,36 @@ def test_route_experts_combine_in_one_graph(dev):
         assert torch.equal(e.cpu(), re)
         ref, bound = combine(y.cpu(), w.cpu(), shared.cpu(), gate.cpu())
         assert bool(((out.cpu().to(F64) - ref).abs() <= bound).all())
+
+
+def test_rows_far_apart(dev):
+    """Rows beyond 2^31 elements of each other."""
+    g = torch.Generator().manual_seed(10)
+    far = torch.empty((20 << 27) + 512, dtype=BF16, device=dev)
+    rows = far.as_strided((20, 128), (1 << 27, 1))
+    x = torch.randn((20, 128), generator=g).to(BF16)
+    rows.copy_(x)
+    w, e = H.moe_route(rows, 6, renormalize=True)
+    rw, re = route(x, 6, renormalize=True)
+    assert torch.equal(e.cpu(), re) and float((w.cpu().to(F64) - rw).abs().max()) < 1e-5
+    w = torch.rand((5, 4), generator=g)
+    want = check_combine(dev, x, w)
+    out = far.as_strided((5, 128), (5 << 27, 1), 256)
+    assert torch.equal(H.moe_combine(rows, w.to(dev), out=out), want)
+
+
+def test_on_another_stream(dev):
+    """Work goes to the current stream, behind what is on it."""
+    g = torch.Generator().manual_seed(11)
+    x = torch.randn((400, 256), generator=g).to(BF16)
+    y = torch.randn((400 * 4, 512), generator=g).to(BF16)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        xd, yd = x.to(dev, non_blocking=True), y.to(dev, non_blocking=True)
+        w, e = H.moe_route(xd, 4, renormalize=True)
+        out = H.moe_combine(yd, w)
+    s.synchronize()
+    rw, re = route(x, 4, renormalize=True)
+    assert torch.equal(e.cpu(), re)
+    ref, bound = combine(y, w.cpu())
+    assert bool(((out.cpu().to(F64) - ref).abs() <= bound).all())

@@ -224,3 +224,186 @@ def test_same_bits_every_time(dev):
     first = call(d, 2000)
     for _ in range(3):
         assert torch.equal(first, call(d, 2000))
+
+
+# ---------------------------------------------------------------- with a pass over the prefix
+# Such small batches as above read the prefix one by one. A pass of its own is made
+# from 40 MB of it on that it saves: enough sequences for that.
+def many(prefix, kv_heads, head_dim):
+    return 2 + (10 << 20) // (prefix * kv_heads * head_dim)
+
+
+def lens_of(prefix, n, prompts, longest=90):
+    """(lengths, new tokens) of n sequences behind the prefix."""
+    news = [1 + 5 * i % 4 for i in range(n)] if prompts else None
+    own = [(37 * i) % longest for i in range(n)]
+    return [prefix + own[i] + (news[i] if prompts else 1) for i in range(n)], news
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,head_dim", LAYOUTS)
+@pytest.mark.parametrize("prompts", [False, True])
+def test_pass_layouts(dev, heads, kv_heads, head_dim, dtype, prompts):
+    prefix = 1501
+    lens, news = lens_of(prefix, many(prefix, kv_heads, head_dim), prompts)
+    xy = make(21, prefix, lens, news=news, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page=16, dtype=dtype)
+    run(dev, xy, prefix)
+
+
+@pytest.mark.parametrize("page", [1, 8, 64, 4096])
+@pytest.mark.parametrize("prefix", [1023, 1024, 1087])
+@pytest.mark.parametrize("prompts", [False, True])
+def test_pass_page_sizes(dev, page, prefix, prompts):
+    lens, news = lens_of(prefix, many(prefix, 4, 128), prompts)
+    xy = make(22, prefix, lens, news=news, heads=8, kv_heads=4, head_dim=128, page=page, dtype=BF16)
+    run(dev, xy, prefix)
+
+
+@pytest.mark.parametrize("prompts", [False, True])
+@pytest.mark.parametrize("head_dim", [64, 256])
+def test_pass_over_shorter_sequences(dev, head_dim, prompts):
+    prefix, n = 2100, many(2100, 4, head_dim)
+    lens, news = lens_of(prefix, n, prompts)
+    for i, m in enumerate((0, 1, prefix, prefix - 1, 17, prefix // 2)):
+        lens[3 * i % n] = m
+    if prompts:
+        news = [min(a, b) for a, b in zip(news, lens)]
+        news[5] = 0
+    xy = make(23, prefix, lens, news=news, heads=8, kv_heads=4, head_dim=head_dim, page=16, dtype=BF16)
+    got = run(dev, xy, prefix)
+    if not prompts:
+        assert all(bool((got[b] == 0).all()) for b, m in enumerate(lens) if m == 0)
+
+
+@pytest.mark.parametrize("prompts", [False, True])
+@pytest.mark.parametrize("softcap", [0.0, 50.0, 200.0])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (900, 64), (1300, 4), (1600, 1500), (3000, 0), (2 ** 40, 0)])
+@pytest.mark.parametrize("head_dim", [128, 256])
+def test_pass_windows(dev, head_dim, window, sinks, softcap, prompts):
+    """Windows that end in the prefix or behind it; sinks past the prefix's end. (Those
+    that hide most of the prefix take no pass.)"""
+    prefix = 1400
+    lens, news = lens_of(prefix, 2 * many(prefix, 8, head_dim), prompts, 400)
+    xy = make(24, prefix, lens, news=news, heads=16, kv_heads=8, head_dim=head_dim, page=16, dtype=BF16, q_scale=2.0)
+    run(dev, xy, prefix, window=window, sinks=sinks, softcap=softcap)
+
+
+@pytest.mark.parametrize("prompts", [False, True])
+@pytest.mark.parametrize("scale", [None, -0.3, 0.0, 300.0])
+def test_pass_sharp_scores(dev, scale, prompts):
+    """Maxima in the prefix and behind it; scores whose exponents pass 2^16."""
+    prefix = 1500
+    lens, news = lens_of(prefix, many(prefix, 2, 128), prompts)
+    xy = make(25, prefix, lens, news=news, heads=8, kv_heads=2, head_dim=128, page=64, dtype=F16, q_scale=8.0)
+    run(dev, xy, prefix, scale=scale)
+
+
+@pytest.mark.parametrize("prompts", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_pass_values_that_are_not_finite(dev, head_dim, dtype, prompts):
+    prefix, n = 1320, many(1320, 4, head_dim)
+    lens, news = lens_of(prefix, n, prompts)
+    x, y = make(26, prefix, lens, news=news, heads=8, kv_heads=4, head_dim=head_dim, page=16, dtype=dtype)
+    v = x["v_pages"]
+    v[x["prefix_table"][3], 5, 0, 7] = float("inf")
+    v[x["prefix_table"][9], 1, 1, 9] = float("nan")
+    v[x["prefix_table"][82], 7, 2, 3] = float("-inf")  # the prefix's last token
+    v[y["table"][:, 82].long(), 7, 2, 3] = float("-inf")  # ... and its copies in the sequences' own pages
+    v[y["table"][1, 83], 0, 0, 11] = float("-inf")     # one sequence's own
+    run(dev, (x, y), prefix)
+    run(dev, (x, y), prefix, window=1300, sinks=16)
+
+
+def test_pass_places_and_layouts(dev):
+    """Rows of no sequence, strided operands, a window's dead pages and pages outside the pool."""
+    prefix = 1440
+    lens, news = lens_of(prefix, many(prefix, 2, 64), True)
+    x, y = make(27, prefix, lens, news=news, heads=4, kv_heads=2, head_dim=64, page=16, dtype=BF16, head_major=True)
+    x["prefix_table"][2], x["prefix_table"][70] = -1, 10 ** 6
+    y["table"][:, 2], y["table"][:, 70] = -1, 10 ** 6
+    rows = x["q"].shape[0]
+    d = R.to(x, dev)
+    pad = torch.zeros((rows + 7, 4, 128), dtype=BF16, device=dev)[:, :, 64:]
+    pad[3:3 + rows] = d["q"]
+    d["q"], d["starts"] = pad, d["starts"] + 3
+    out = torch.full((4, rows + 7, 64), 7.0, dtype=BF16, device=dev).transpose(0, 1)
+    call(d, prefix, out=out)
+    assert bool((out[:3] == 7).all()) and bool((out[3 + rows:] == 7).all())
+    R.check(out[3:3 + rows].cpu(), R.reference(y))
+
+
+@pytest.mark.parametrize("prompts", [False, True])
+def test_pass_in_a_graph_and_again(dev, prompts):
+    """Replays over changed lengths and queries; the same bits every time."""
+    prefix = 1600
+    lens, news = lens_of(prefix, many(prefix, 2, 256), prompts)
+    x, y = make(28, prefix, lens, news=news, heads=16, kv_heads=2, head_dim=256, page=32, dtype=BF16)
+    d = R.to(x, dev)
+    out = torch.empty_like(d["q"])
+    call(d, prefix, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(d, prefix, out=out)
+    for step in range(3):
+        x["q"] = (x["q"].float() * 0.9).to(BF16)
+        d["q"].copy_(x["q"])
+        if not prompts:
+            x["lens"] = (x["lens"] - step).clamp(min=0)
+            d["lens"].copy_(x["lens"])
+        y["lens"], y["q"] = x["lens"], x["q"]
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        R.check(out.cpu(), R.reference(y))
+        assert torch.equal(call(d, prefix), out)
+
+
+@pytest.mark.parametrize("prompts", [False, True])
+def test_pass_with_many_sequences_and_a_long_one(dev, prompts):
+    """700 sequences, empty ones among them, and one whose own part is split."""
+    prefix = 256
+    lens, news = lens_of(prefix, 700, prompts, 30)
+    lens[350] = prefix + 5000
+    if not prompts:
+        lens[0] = lens[699] = 0
+    xy = make(29, prefix, lens, news=news, heads=4, kv_heads=2, head_dim=64, page=16, dtype=BF16)
+    run(dev, xy, prefix)
+
+
+def test_pass_far_into_a_pool(dev):
+    """Pages beyond 2^31 elements of the pool (and 2^32 bytes), of the prefix and of sequences."""
+    prefix = 512
+    lens, _ = lens_of(prefix, many(prefix, 8, 256), False)
+    x, y = make(30, prefix, lens, heads=16, kv_heads=8, head_dim=256, page=64, dtype=BF16)
+    n = x["k_pages"].shape[0]
+    move = (1 << 31) // (64 * 8 * 256) + 11
+    assert (n + move) * 64 * 8 * 256 * 2 < 6 << 30
+    d = R.to({k: v for k, v in x.items() if "pages" not in k}, dev)
+    for name in ("k_pages", "v_pages"):
+        d[name] = torch.empty((n + move, 64, 8, 256), dtype=BF16, device=dev)
+        d[name][move:] = x[name].to(dev)
+    d["table"] = torch.where(d["table"] >= 0, d["table"] + move, d["table"])
+    d["prefix_table"] += move
+    R.check(call(d, prefix).cpu(), R.reference(y))
+
+
+def test_attend_of_a_cache_with_forks(dev):
+    """PagedKVCache.attend over forks, with the shared prefix it finds: as without."""
+    g = torch.Generator().manual_seed(31)
+    cache = H.PagedKVCache(1, 600, 16, 8, 128, device=dev)
+    a = cache.new()
+    cache.extend([a], [1030])
+    rand = lambda n, h: torch.randn((n, h, 128), generator=g).to(BF16).to(dev)
+    cache.append(0, rand(1030, 8), rand(1030, 8), cache.batch([a], [1030]))
+    seqs = [a] + [cache.fork(a) for _ in range(30)]
+    for step in range(3):
+        cache.extend(seqs, [1] * len(seqs))
+        b = cache.batch(seqs)
+        cache.append(0, rand(len(seqs), 8), rand(len(seqs), 8), b)
+        n = cache.shared_prefix(seqs)
+        assert n == 1024
+        q = rand(len(seqs), 32)
+        got = cache.attend(0, q, b, prefix=n).cpu()
+        k, v = cache.k_pages[0].cpu(), cache.v_pages[0].cpu()
+        R.check(got, R.attend(q.cpu(), k, v, b.block_table.cpu(), b.kv_lens.cpu()))
