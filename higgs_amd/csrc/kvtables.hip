@@ -354,7 +354,6 @@ extern "C" int hgk_kv_extend(const hgk_kv_tables* tables, const int32_t* seqs, c
   if (block_table && !seqs) return fail(HGK_ERR_ARG, "%s: a table of the batch's own needs the rows' numbers", what);
   if (block_table && batch > 1 && block_table_stride < a.t.width)
     return fail(HGK_ERR_ARG, "%s: rows of the batch's table overlap (stride %lld)", what, (long long)block_table_stride);
-  if (!seqs && batch > 0) block_table = nullptr;
   a.seqs = seqs;
   a.counts = counts;
   a.batch = (int32_t)batch;

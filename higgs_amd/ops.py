@@ -800,8 +800,9 @@ def kv_extend(tables: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor
     place), lens int32 [S] (their tokens), free_pages int32 [N] (a stack: its
     first n_free[0] entries are free), n_free int32 [1]. ``counts`` int32 [B]
     new tokens of the sequences in rows ``seqs`` (int32 [B], any order; without
-    it of every row). ``tokens`` rows is what the packed array of new tokens has;
-    those behind the last sequence's belong to none.
+    it of every row); the last page of one that has room for more is its own.
+    ``tokens`` rows is what the packed array of new tokens has; those behind the
+    last sequence's belong to none.
 
     Returns KVStep: block_table [B, W] (the tables themselves without seqs; else
     a copy of the batch's rows, -1 behind their last page), kv_lens [B],
@@ -879,7 +880,8 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scores: str = "softmax", bias
     sum of its two greatest (``group_top`` 1 or 2). Returns (weights f32 [..., top_k],
     experts int32 [..., top_k]): weights are scale * s, divided by the token's sum
     of them first with ``renormalize``. A NaN logit counts as -inf; a token without
-    any logit above -inf has weights of 0 (softmax). E up to 1024, top_k up to 64."""
+    any logit above -inf has weights of 0 (softmax). E up to 1024, top_k up to 64,
+    up to 64 groups, of at most 16 experts in each of a group's share of 64 lanes."""
     what = "moe_route"
     if logits.dim() < 1:
         raise HgkError(1, f"{what}: logits must have at least 1 dimension")

@@ -622,6 +622,8 @@ typedef enum {
  * seqs[i] (device int32 [batch]; NULL: row i, batch == rows), and what a call
  * over them takes. Sequence by sequence, position by position, each page that
  * is begun is taken from the top of the stack and written into the tables.
+ * A sequence's last page, if partly filled, takes its next tokens: it has to be the
+ * sequence's own (hgk_kv_copy_pages).
  *   lens_out [rows], n_free_out [1]: the new state. They may be lens and n_free.
  *   kv_lens [batch], q_starts [batch + 1]: as in hgk_kv_batch, of `tokens` rows,
  *     of which those from q_starts[batch] on belong to no sequence
