@@ -262,6 +262,44 @@ __device__ __forceinline__ f32x2 decode_again(const PrefixArgs& a, const Scale& 
   return f32x2{r, l};
 }
 
+// Which chunk a wave takes where sequences have several: the `want`-th of those that
+// there are, sequence by sequence, the whole ones first and then the sequences' last
+// ones, which are shorter. (A place for every chunk that a table allows, found or not,
+// left half the waves of ragged sequences' blocks without keys: 64 of up to 1500 behind
+// 8192, 16/2 heads of 256: 60 us, now 54.)
+struct Chunk {
+  int seq, at;  // seq -1: none
+};
+template <int KEYS>
+__device__ inline Chunk find_chunk(const PrefixArgs& a, int want) {
+  const int lane = threadIdx.x & 63, run = (a.b.batch + 63) / 64, i0 = lane * run;
+  // a sequence's whole chunks in the upper 16 bits, its last one in the lower (there
+  // are several to a sequence in batches of up to 2048, and 4096 in all)
+  auto chunks = [&](int i) {
+    const int tiles = min(decode_tiles<KEYS>(seen_behind(a, a.b.lens[i])), a.splits * a.chunk), whole = tiles / a.chunk;
+    return whole << 16 | (tiles > whole * a.chunk);
+  };
+  int mine = 0;
+  for (int i = i0; i < min(i0 + run, a.b.batch); ++i) mine += chunks(i);
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o);
+    if (lane >= o) upto += v;
+  }
+  const int whole = __builtin_amdgcn_readlane(upto, 63) >> 16, by = want < whole ? 16 : 0;
+  if (by == 0) want -= whole;
+  const uint64_t past = __ballot((upto >> by & 0xffff) > want);
+  if (!past) return Chunk{-1, 0};
+  const int owner = __builtin_ctzll(past);
+  int at = want - (__builtin_amdgcn_readlane(upto - mine, owner) >> by & 0xffff), seq = owner * run;
+  for (;; ++seq) {
+    const int c = chunks(seq), n = c >> by & 0xffff;
+    if (at < n) return Chunk{seq, by ? at : c >> 16};
+    at -= n;
+  }
+}
+
 // Single tokens' own keys: WAVES waves have a chunk of a (sequence, kv head), for 16
 // of its query heads, and make one part of it.
 // lds: behind_lds<D, WAVES>() bytes, 16-byte aligned. x counts the blocks, y the 16s of
@@ -275,11 +313,15 @@ __device__ __forceinline__ void attn_behind(const PrefixArgs& a, char* lds, int 
   constexpr int kKeys = dec_keys<D>(), kStep = D / 32, kTile = kKeys * dec_row<D>();
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int m = lane & 15, j = lane >> 4, step = WAVES > 1 ? wave : 0;
-  // chunks in the order of the sequences: those that are not there come last
-  const int unit = WAVES > 1 ? block : block * kDecWaves + wave, pairs = a.b.batch * a.p.kv_heads;
-  const int at_chunk = unit / pairs, pair = unit - at_chunk * pairs;
-  const int seq = pair / a.p.kv_heads, hk = pair - seq * a.p.kv_heads;
-  if (at_chunk >= a.splits) return;
+  const int unit = WAVES > 1 ? block : block * kDecWaves + wave;
+  int seq = unit / a.p.kv_heads, at_chunk = 0;
+  const int hk = unit - seq * a.p.kv_heads;
+  if (WAVES == 1 && a.splits > 1) {
+    const Chunk c = find_chunk<kKeys>(a, seq);
+    seq = c.seq;
+    at_chunk = c.at;
+  }
+  if ((uint32_t)seq >= (uint32_t)a.b.batch) return;
   Seen seen = seen_behind(a, a.b.lens[seq]);
   seen.n = __builtin_amdgcn_readfirstlane(seen.n);
   const int first = at_chunk * a.chunk, last = min(decode_tiles<kKeys>(seen), first + a.chunk);
@@ -418,8 +460,8 @@ __device__ inline PrefixBlock prefix_block(const PrefixArgs& a, int id, int bloc
 // the matrix instructions bound, and then those of the sequences' own keys, which the
 // memory does, so that either finds CUs, or places on them, that the other leaves.
 // With the join, in us: 256 sequences of up to 200 tokens behind 4001, 32/8 heads of
-// 128 (17 GFLOP, 126 MB): 47, as two launches 66; 64 of up to 1500 behind 8192, 16/2
-// heads of 256 (9 GFLOP, 117 MB): 54, as two 72; every sequence over a table of its
+// 128 (17 GFLOP, 126 MB): 56, as two launches 73; 64 of up to 1500 behind 8192, 16/2
+// heads of 256 (9 GFLOP, 117 MB): 54, as two 76; every sequence over a table of its
 // own (paged_attention's kernels): 496 and 149.
 template <class T, int D, int CAP>
 __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_kernel(PrefixArgs a, int prefix_blocks,
@@ -545,7 +587,7 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(PrefixArgs a, uin
 // one by one, much of it from the caches (8 sequences behind 1000 tokens, 8 kv heads
 // of 64, 14 MB: 20 us with the pass, 14.7 without; 16 behind 2000, 8 of 128, 123 MB:
 // 18.3, 32.8).
-constexpr int64_t kPassBytes = 40 << 20, kUnits = 2048;
+constexpr int64_t kPassBytes = 40 << 20;
 struct SharedPlan {
   int pre, splits, chunk, waves;
   int64_t rows() const { return pre + splits > 1 ? pre + splits : 0; }
@@ -581,9 +623,16 @@ SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, in
     s.chunk = (int)all;
     return s;
   }
-  // chunks of as many tiles as leave 2048 waves, two a SIMD, if every table is full
-  const int64_t most = std::clamp<int64_t>(kUnits / pairs, 1, kMaxParts - kMaxSplits);
-  s.chunk = (int)std::max<int64_t>((all + most - 1) / most, 4);
+  // Chunks of as many tiles as leave 4096 waves if every table is full: two turns of
+  // those that the chip has room for (rows of 256: four), so that ragged sequences end
+  // together. 100 of up to 1500 behind 2048, 24/8 heads of 96: 114 us with 2048 waves, 82
+  // with 4096, 80 with 8192; 64 behind 6000, 16/8 of 256: 116, 103, 101; 64 of up to 3000
+  // behind 8192, 32/8 of 128: 111, 98, 95. Rows of 64 are joined for as long as they are
+  // walked: 200 of up to 1500 behind 4096, 32/8 heads: 99, 107, 105. Nor do few tiles of
+  // many pairs gain (256 of up to 200 behind 4001, 32/8 of 128: 57, 58).
+  const int64_t units = p.head_dim > 64 ? 4096 : 2048;
+  const int64_t most = std::clamp<int64_t>(units / pairs, 1, kMaxParts - kMaxSplits);
+  s.chunk = (int)std::max<int64_t>((all + most - 1) / most, pairs >= 1024 ? 8 : 4);
   s.splits = (int)((all + s.chunk - 1) / s.chunk);
   return s;
 }

@@ -371,6 +371,21 @@ def test_pass_with_many_sequences_and_a_long_one(dev, prompts):
     run(dev, xy, prefix)
 
 
+@pytest.mark.parametrize("batch", [63, 65, 130, 200])
+@pytest.mark.parametrize("head_dim", [64, 256])
+def test_pass_with_chunks_of_ragged_sequences(dev, batch, head_dim):
+    """Own parts of no chunk, of a last one only, of whole ones only and of both, in
+    batches that a wave's lanes share out evenly and not."""
+    prefix = 512
+    own = [0, 1, 1500, 64, 0, 700, 128, 129, 33, 1024, 511, 2]
+    lens = [prefix + own[(5 * i + i // 12) % 12] for i in range(batch)]
+    lens[1] = lens[batch // 2] = 0
+    lens[2] = 100
+    xy = make(61, prefix, lens, heads=4, kv_heads=4 if head_dim == 64 else 2, head_dim=head_dim, page=16, dtype=BF16)
+    run(dev, xy, prefix)
+    run(dev, xy, prefix, window=900, sinks=5)
+
+
 def test_pass_far_into_a_pool(dev):
     """Pages beyond 2^31 elements of the pool (and 2^32 bytes), of the prefix and of sequences."""
     prefix = 512
