@@ -2,8 +2,10 @@
 panbanda/higgs' higgs-models (RMSNorm variants, RoPE variants, SwiGLU/GeGLU,
 the Qwen3-Next gated norm, the 4-bit QuantizedEmbedding gather, the fused
 residual-add + RMSNorm and embedding + RMSNorm forms, the 4-bit
-quantized_matmul / gather_qmm projections, the GatedDeltaNet recurrence, and
-the paged key-value cache with the attention over it), exposed
+quantized_matmul / gather_qmm projections, the GatedDeltaNet recurrence, the
+paged key-value cache with the attention over it, also of sequences that share a
+prefix, its tables' growth and release on the GPU, and the routing and combining
+of experts), exposed
 through the C ABI in include/higgs_hip.h and mirrored here for Python callers.
 """
 from ._lib import ACT_GELU_TANH, ACT_SILU, HgkError, LIB_PATH, lib  # noqa: F401

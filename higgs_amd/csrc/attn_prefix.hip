@@ -480,7 +480,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared
 }
 
 // Both passes of prompts in one launch. 32 sequences of up to 33 + 100 tokens behind
-// 16384, 32/8 heads of 128 f16 (148 GFLOP): 212 us with the join, 700 TFLOP/s.
+// 16384, 32/8 heads of 128 f16 (148 GFLOP): 215 us with the join, 690 TFLOP/s.
 template <class T, int D, int CAP>
 __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared_prompt_kernel(PrefixArgs a,
                                                                                                  int prefix_blocks,

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(kFill) void kv_release_kernel(PlanArgs a) {
 
 // A call in one launch: every block works the sums out for itself, which takes few
 // sequences no longer than a second launch, and the state must not be written where
-// other blocks still read it. (64 sequences of 1024-page tables: 4.9 us, in two
+// other blocks still read it. (64 sequences of 1024-page tables: 4.4 us, in two
 // launches 6.5.)
 template <bool RELEASE>
 __global__ __launch_bounds__(kFill) void kv_one_kernel(ExtendArgs x) {
