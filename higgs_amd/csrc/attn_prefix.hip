@@ -582,11 +582,10 @@ __global__ __launch_bounds__(256) void attn_prefix_join_kernel(PrefixArgs a, uin
 
 // The split of a call, from the sizes alone.
 //
-// A pass over the prefix costs a launch more and the writing and joining of its
-// parts, so it has to save the reading of 40 MB: below, the sequences read the prefix
-// one by one, much of it from the caches (8 sequences behind 1000 tokens, 8 kv heads
-// of 64, 14 MB: 20 us with the pass, 14.7 without; 16 behind 2000, 8 of 128, 123 MB:
-// 18.3, 32.8).
+// A pass over the prefix costs the writing and joining of its parts, a launch, so it
+// has to save the reading of 40 MB: below, the sequences read the prefix one by one,
+// much of it from the caches (8 sequences behind 1000 tokens, 8 kv heads of 64, 14 MB:
+// 20 us with the pass, 14.7 without; 16 behind 2000, 8 of 128, 123 MB: 18.3, 32.8).
 constexpr int64_t kPassBytes = 40 << 20;
 struct SharedPlan {
   int pre, splits, chunk, waves;
@@ -598,13 +597,14 @@ SharedPlan plan_shared(const KvView& p, const KvBatchView& b, int64_t prefix, in
   if (b.batch == 0 || b.tokens == 0) return s;
   const int64_t group = q_heads / p.kv_heads, width = (int64_t)b.width << p.page_shift;
   const int64_t seen = window > 0 && window < prefix && sinks < prefix - window ? window + sinks : prefix;
-  if ((b.batch - 1) * std::min(seen, width) * p.kv_heads * p.head_dim >= kPassBytes / 4) {
+  if ((double)(b.batch - 1) * std::min(seen, width) * p.kv_heads * p.head_dim >= kPassBytes / 4) {
     // Places on the chip, shared out by the two passes' work: a tile of 64 keys takes 3 us
-    // of a block with rows of 256, one a CU, and in proportion less of narrower ones, two
-    // a CU and 2.2 us each at 128; own keys, half of what the tables allow, come at 5 TB/s.
+    // of a block with rows of 256, one a CU, and 1 us and 1.2 a 128 values of narrower
+    // ones, two a CU; own keys, half of what the tables allow, come at 5 TB/s. (Within 3 %
+    // of the best number of parts at nine sizes with rows of 64 to 256.)
     const int64_t places = p.head_dim == 256 ? 256 : 512, tiles = p.kv_heads * prefix_tiles(b, group);
     const double own = (double)b.batch * std::max<int64_t>(width - prefix, 0) * p.kv_heads * p.head_dim * 2 / 5e6;
-    const double pass = (double)tiles * prefix / 64 * (p.head_dim == 256 ? 3.0 : 2.2 * p.head_dim / 128) / places;
+    const double pass = (double)tiles * prefix / 64 * (p.head_dim == 256 ? 3.0 : 1.0 + 1.2 * p.head_dim / 128) / places;
     const int64_t blocks = b.starts ? places : (int64_t)(places * pass / (pass + own));
     s.pre = (int)std::clamp<int64_t>((blocks + (b.starts ? 0 : tiles - 1)) / tiles, 1,
                                      std::max<int64_t>(std::min<int64_t>(prefix / kMinPart, kMaxSplits), 1));
