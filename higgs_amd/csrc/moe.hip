@@ -26,12 +26,21 @@ struct RouteArgs {
 
 constexpr float kLog2e = 1.44269504088896341f;
 
-// e^x to about 2^-22 of itself: x log2(e) in two parts, the lesser one put back
-// by its series (the product alone is off by up to 2^-17 of the result at x = -88).
+// e^x to about 2^-22 of itself for x >= -87, and zero below: x log2(e) in two parts, the
+// lesser one put back by its series (the product alone is off by up to 2^-17 of the
+// result at x = -88).
 __device__ inline float exp_f32(float x) {
   const float t = x * kLog2e, r = fmaf(x, kLog2e, -t) + x * 1.92596299e-8f;
   const float e = __builtin_amdgcn_exp2f(t);
   return x < -150.0f ? 0.0f : fmaf(e, r * 0.693147181f, e);
+}
+// ... where results below 2^-126 count too, which the hardware's exp2 has as zero: those
+// are 2^64 times as great until the last product, which rounds to the step of 2^-149.
+__device__ inline float exp_small(float x) {
+  const bool far = x < -80.0f;
+  const float t = x * kLog2e, r = fmaf(x, kLog2e, -t) + x * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(far ? t + 64.0f : t);
+  return x < -150.0f ? 0.0f : fmaf(e, r * 0.693147181f, e) * (far ? 0x1p-64f : 1.0f);
 }
 
 // Value of the lane that a DPP control pairs with this one.
@@ -427,13 +436,21 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
   const bool has = sub < a.top_k;
   float l = has ? load1<T>(row, expert) : -INFINITY, s;
   if (l != l) l = -INFINITY;
+  // Scores that are renormalised are taken from the greatest of the chosen logits on:
+  // all of them may be below what f32 holds (sigmoids of logits below -100, experts that
+  // a bias has put in front of others with logits far above). Where even 64 bits hold
+  // none of them (a logit masked by its type's lowest value) they are zero.
+  constexpr float kLeast = -745.0f;  // log 2^-1074
+  float most = 0.0f;
+  if (a.renormalize) most = fold<BITS>(l, [](float p, float q) { return fmaxf(p, q); });
   if (a.sigmoid) {
     // of a large negative logit the exponential is the score
-    const float f = exp_f32(-fabsf(l));
-    s = (l < 0.0f ? f : 1.0f) / (1.0f + f);
+    const float f = exp_small(-fabsf(l)), from = most > kLeast ? fminf(most, 0.0f) : 0.0f;
+    s = (l < 0.0f ? exp_small(l - from) : 1.0f) / (1.0f + f);
   } else {
     // (renormalised weights need no sum over all experts)
-    s = l == -INFINITY ? 0.0f : l == top ? 1.0f : exp_f32(l - top);
+    const float from = a.renormalize && most - top > kLeast ? most : top;
+    s = l == -INFINITY ? 0.0f : l == from ? 1.0f : exp_small(l - from);
     if (!a.renormalize) s = whole > 0.0f ? s / whole : 0.0f;
   }
   if (a.renormalize) {
