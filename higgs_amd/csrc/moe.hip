@@ -464,6 +464,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(RouteArgs a) {
 }
 
 constexpr int kRouteExperts = 1024, kRouteTopK = 64;
+constexpr int64_t kRouteBlocks = 1 << 23;  // of a launch
 
 // How a token's experts lie on lanes: 2^bits lanes, per of them each.
 struct RoutePlan {
@@ -486,8 +487,17 @@ void launch_route(RouteArgs a, hipStream_t stream) {
   a.pieces = a.group_size % V == 0 && a.row % V == 0 &&
              (reinterpret_cast<uintptr_t>(a.logits) & (V * T::kBytes - 1)) == 0;
   a.bias_pieces = a.pieces && aligned16(a.bias);
-  HGK_LAUNCH((moe_route_kernel<T, SUMS, BITS, PER>), dim3((unsigned)((a.tokens + kTokens - 1) / kTokens)), dim3(256), 0,
-             stream, a);
+  // (a launch has fewer than 2^32 threads)
+  const int64_t tokens = a.tokens;
+  for (int64_t t = 0; t < tokens; t += kRouteBlocks * kTokens) {
+    RouteArgs b = a;
+    b.logits += t * a.row * T::kBytes;
+    b.weights += t * a.top_k;
+    b.experts += t * a.top_k;
+    b.tokens = std::min(tokens - t, kRouteBlocks * kTokens);
+    HGK_LAUNCH((moe_route_kernel<T, SUMS, BITS, PER>), dim3((unsigned)((b.tokens + kTokens - 1) / kTokens)), dim3(256), 0,
+               stream, b);
+  }
 }
 template <class T, bool SUMS>
 void route_of(const RouteArgs& a, const RoutePlan& p, hipStream_t stream) {
