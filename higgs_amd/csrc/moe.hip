@@ -137,7 +137,8 @@ __device__ inline V group_score(const V* c, int gbits, int group_top) {
   if (gbits > 3) join(partner<3>(b1), partner<3>(b2));
   if constexpr (BITS > 4)
     if (gbits > 4) join(partner<4>(b1), partner<4>(b2));
-  return group_top == 2 ? b1 + b2 : b1;
+  const V sum = b1 + b2;
+  return group_top != 2 ? b1 : sum == sum ? sum : (V)-INFINITY;  // (infinities of both signs: NaN)
 }
 
 // The choice to the last bit: the keys hold all of it. c: -inf where a lane has no

@@ -668,7 +668,8 @@ typedef enum { HGK_SCORE_SOFTMAX = 0, HGK_SCORE_SIGMOID = 1 } hgk_score;
  *     the sum of those s first
  * Equal choices, and equal runs, go to the lower index. The order is that of the
  * logits themselves, or of sums in 64 bits where something is added to scores. A
- * NaN logit counts as -inf, of score 0; a NaN choice as the lowest. A token
+ * NaN logit counts as -inf, of score 0; a NaN choice, or sum of a run's two, as the
+ * lowest. A token
  * without a logit above -inf has softmax scores of 0. Scores below 2^-1074 (more than
  * 745 below zero, or below the greatest logit) count as zero where all of the chosen
  * are, and a sum of zero renormalises to zeros. At most 1024 experts, 64 groups (whose experts fill at most 16 in
