@@ -37,6 +37,18 @@ class KVBatch(NamedTuple):
     q_starts: Optional[torch.Tensor]
 
 
+class _CacheBatch(KVBatch):
+    """A batch of a cache's sequences, which knows what they share."""
+
+    def shared(self, page_size: int) -> int:
+        """The tokens that all of the batch's sequences have on the same pages at their beginning."""
+        if self._shared is None:
+            table, lengths = self._host
+            same = (table == table[:1]).all(0) if len(lengths) else np.zeros(1, bool)
+            self._shared = min(int(same.size if same.all() else same.argmin()) * page_size, *lengths, 2 ** 30)
+        return self._shared
+
+
 class _Seq:
     __slots__ = ("pages", "length")
 
@@ -219,7 +231,9 @@ class PagedKVCache:
         starts = None
         if counts is not None:
             starts = torch.from_numpy(np.cumsum([0, *counts]).astype(np.int32)).to(dev)
-        return KVBatch(torch.from_numpy(table).to(dev), lens, starts)
+        batch = _CacheBatch(torch.from_numpy(table).to(dev), lens, starts)
+        batch._host, batch._shared = (table, [s.length for s in found]), None
+        return batch
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch: KVBatch) -> None:
         """kv_append of one layer's keys and values."""
@@ -230,8 +244,12 @@ class PagedKVCache:
         """paged_attention over one layer's pages (scale, window, sinks,
         softcap, out as there). With ``prefix`` > 0 the batch's sequences have
         their first ``prefix`` tokens on the same pages (shared_prefix), which are
-        read and multiplied once for all: shared_prefix_attention."""
+        read and multiplied once for all: shared_prefix_attention. A ``prefix`` past
+        what the sequences of a batch() shared when it was made is refused."""
         if prefix:
+            if isinstance(batch, _CacheBatch) and prefix > batch.shared(self.page_size):
+                raise HgkError(1, f"PagedKVCache: prefix={prefix}, but the batch's sequences share "
+                                  f"{batch.shared(self.page_size)} tokens")
             pages = batch.block_table[:1].flatten()[:-(-prefix // self.page_size)]
             return ops.shared_prefix_attention(q, self.k_pages[layer], self.v_pages[layer], batch.block_table,
                                                batch.kv_lens, pages, prefix, q_starts=batch.q_starts, **kw)
