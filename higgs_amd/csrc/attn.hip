@@ -567,7 +567,10 @@ template <class T, int D, int BN, int CAP>
 __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt_kernel(AttnArgs a) {
   __shared__ __align__(1024) char lds[prompt_lds<D>()];
   __shared__ int words[kPromptWords];
-  attn_prompt<T, D, BN, CAP>(kOwn, a, lds, words, blockIdx.x, gridDim.x, blockIdx.y, a.splits);
+  constexpr Keys keys = kOwn;
+  const uint32_t x = blockIdx.x, grid_x = gridDim.x;
+  const int y = blockIdx.y, splits = a.splits;
+#include "attn_prompt.inl"
 }
 
 template <class T, int D, int BN>

@@ -438,6 +438,13 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(PrefixAr
   attn_behind<T, D, CAP, WAVES>(a, lds, blockIdx.x, blockIdx.y);
 }
 
+// A block of the prompts' kernel, over the prefix's keys or those behind them.
+template <class T, int D, int BN, int CAP>
+__device__ __forceinline__ void attn_prompt(Keys keys, const PrefixArgs& a, char* lds, int* words, uint32_t x,
+                                            uint32_t grid_x, int y, int splits) {
+#include "attn_prompt.inl"
+}
+
 // Which rows and which part of its keys block `id` of the pass over the prefix takes.
 // The blocks of a part are put on one XCD, whose L2 then holds its keys, where the
 // parts share out evenly.
