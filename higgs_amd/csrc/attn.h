@@ -386,6 +386,10 @@ constexpr int kPromptRows = 128;  // rows of a block: 32 a wave
 
 // Of attn_prompt.inl: the words and the bytes of LDS that it works in.
 constexpr int kPromptWords = 2 + 2 * (2 * kPromptRows / 64);
+template <int D, bool TWO> constexpr bool prompt_lean() { return TWO && D == 128; }
+template <int D, bool TWO> constexpr int prompt_words() {
+  return kPromptWords + (prompt_lean<D, TWO>() ? 3 * 2 * kPromptRows : 0);
+}
 template <int D> constexpr int prompt_lds() { return 4 * 64 * 2 * D; }
 
 // Sizes shared by the call and its workspace query.

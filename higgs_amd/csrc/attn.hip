@@ -568,6 +568,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_prompt
   __shared__ __align__(1024) char lds[prompt_lds<D>()];
   __shared__ int words[kPromptWords];
   constexpr Keys keys = kOwn;
+  constexpr bool TWO = false;
   const uint32_t x = blockIdx.x, grid_x = gridDim.x;
   const int y = blockIdx.y, splits = a.splits;
 #include "attn_prompt.inl"

@@ -439,7 +439,7 @@ __global__ __launch_bounds__(64 * kDecWaves, 2) void attn_behind_kernel(PrefixAr
 }
 
 // A block of the prompts' kernel, over the prefix's keys or those behind them.
-template <class T, int D, int BN, int CAP>
+template <class T, int D, int BN, int CAP, bool TWO>
 __device__ __forceinline__ void attn_prompt(Keys keys, const PrefixArgs& a, char* lds, int* words, uint32_t x,
                                             uint32_t grid_x, int y, int splits) {
 #include "attn_prompt.inl"
@@ -477,9 +477,14 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared
   __shared__ __align__(1024) char lds[prompt_lds<D>()];
   const int id = blockIdx.x;
   if (id < prefix_blocks) {
-    __shared__ int words[kPromptWords];
-    const PrefixBlock p = prefix_block(a, id, prefix_blocks);
-    attn_prompt<T, D, 64, CAP>(kPrefix, a, lds, words, p.x, p.grid_x, p.split, a.pre);
+    __shared__ int words[prompt_words<D, true>()];
+    const PrefixBlock block = prefix_block(a, id, prefix_blocks);
+    constexpr Keys keys = kPrefix;
+    constexpr bool TWO = true;
+    constexpr int BN = 64;
+    const uint32_t x = block.x, grid_x = block.grid_x;
+    const int y = block.split, splits = a.pre;
+#include "attn_prompt.inl"
   } else {
     const int b = id - prefix_blocks, y = b / behind_blocks;
     attn_behind<T, D, CAP == kNoCap ? kNoCap : kWideCap, 1>(a, lds, b - y * behind_blocks, y);
@@ -498,7 +503,7 @@ __global__ __launch_bounds__(2 * kPromptRows, D == 256 ? 1 : 2) void attn_shared
   const bool prefix = b < 0;
   PrefixBlock p{b % behind_x, behind_x, b / behind_x};
   if (prefix) p = prefix_block(a, id, prefix_blocks);
-  attn_prompt<T, D, 64, CAP>(prefix ? kPrefix : kBehind, a, lds, words, p.x, p.grid_x, p.split,
+  attn_prompt<T, D, 64, CAP, false>(prefix ? kPrefix : kBehind, a, lds, words, p.x, p.grid_x, p.split,
                              prefix ? a.pre : a.splits);
 }
 

@@ -24,6 +24,7 @@
 //   keys, a         which keys the block takes, the call's arguments
 //   lds, words      prompt_lds<D>() bytes, 1024-byte aligned, and kPromptWords
 //   x, grid_x, y, splits   the block's place, and the y there are
+//   TWO             are weights multiplied in two parts?
 // As a function of its arguments' type the kernel without a prefix was scheduled
 // otherwise, with 4 registers more, and took 1.5 % longer (8191 tokens in a window of
 // 4096, 16/8 heads of 256: 571 us for 562).
@@ -145,6 +146,16 @@
     koff[i] = 2 * ((r - r0) * (uint32_t)a.p.kst[1] + 8 * key_piece<D>(r, c));
     voff[i] = 2 * ((r - r0) * (uint32_t)a.p.vst[1] + 8 * value_place<D>(r, c));
   }
+  // Two parts of the weights of rows of 128 leave no register for what a lane needs a few
+  // times a tile, and to get it back from memory would wait for the tiles' loads: it is kept in LDS.
+  constexpr bool kLean = prompt_lean<D, TWO>();
+  static_assert(!kLean || kOffs == 1, "one offset");
+  int* const kept = words + kPromptWords + threadIdx.x;
+  if constexpr (kLean) {
+    kept[0] = koff[0];
+    kept[NT] = voff[0];
+    kept[2 * NT] = p;
+  }
   const uint32_t lds0 = lds_address(lds) + 1024 * wave;
   auto load = [&](int it, uint32_t to, int32_t page, const char* base, int64_t page_step, int64_t row_step,
                   const uint32_t* off, auto piece) {
@@ -171,18 +182,20 @@
   };
   // keys and values have two slots each: tile it0 + i lies in slot i % 2
   auto load_keys = [&](int it, int slot, int32_t page) {
-    load(it, lds0 + slot * kTile, page, kbase, a.p.kst[0], a.p.kst[1], koff, key_piece<D>);
+    load(it, lds0 + slot * kTile, page, kbase, a.p.kst[0], a.p.kst[1], kLean ? (uint32_t*)kept : koff, key_piece<D>);
   };
   auto load_values = [&](int it, int slot, int32_t page) {
-    load(it, lds0 + (2 + slot) * kTile, page, vbase, a.p.vst[0], a.p.vst[1], voff, value_place<D>);
+    load(it, lds0 + (2 + slot) * kTile, page, vbase, a.p.vst[0], a.p.vst[1], kLean ? (uint32_t*)kept + NT : voff, value_place<D>);
   };
   // does some row of this range see only a part of the tile?
   auto part_seen = [&](int key0, int first, int last) {
     return !(key0 + BN - 1 <= first &&
              (a.window == 0 || key0 > last - a.window || key0 + BN - 1 < a.sinks));
   };
+  auto position = [&]() { return kLean ? kept[2 * NT] : p; };
   // which keys of a tile this lane's row sees (bit i: key key0 + i)
   auto seen_keys = [&](int key0, uint64_t exist) {
+    const int p = position();
     auto below = [&](int key) {  // the tile's keys below `key`
       const int n = key - key0;
       return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1;
@@ -277,10 +290,10 @@
       top = top_of(x);
       if constexpr (CAP) top = cap_tanh<CAP>(top * sc.inner);
     }
-    moved = __any(top > ref + slack);
+    moved = kLean ? __any((top - ref) * sc.c > M::kSlack) : __any(top > ref + slack);
     if (moved) {  // a row's own scores alone decide for it
       top = halves_max(top);
-      const float to = top > ref + slack ? top : ref;
+      const float to = (kLean ? (top - ref) * sc.c > M::kSlack : top > ref + slack) ? top : ref;
       shrunk = lesser((ref - to) * sc.c);
       sum *= shrunk;
       ref = to;
@@ -298,10 +311,12 @@
   };
   // Weights of scores 2 i and 2 i + 1, rounded to the type: by half a step, as the
   // result is (a row's error against 64 bits is 1.3 times that of weights in f32).
-  // A second part, as single tokens have, would be half as many matrix
+  // A second part, as single tokens have (TWO: also of a pass over their prefix, so that
+  // a row's bits are as good as without one), is half as many matrix
   // instructions again and a conversion a weight, where the two bound the kernel.
   // The sum takes the rounded ones, so that a row's weights add up to one as used.
   float add[4];
+  uint32_t low;  // what the weights' first parts leave
   auto weigh = [&](const f32x16* x, int i) {
     float s0 = x[i / 8][2 * i % 16], s1 = x[i / 8][2 * i % 16 + 1];
     if constexpr (CAP) {
@@ -316,6 +331,10 @@
     const float w1 = __builtin_amdgcn_exp2f(fmaf(s1, sc.c, base));
     const uint32_t pair = M::pack(w0, w1);
     add[i & 3] = M::add_pair(pair, i < 4 ? 0.0f : add[i & 3]);
+    if constexpr (TWO) {
+      low = M::pack(w0 - T::lo(pair), w1 - T::hi(pair));
+      add[i & 3] = M::add_pair(low, add[i & 3]);
+    }
     return pair;
   };
   // Sums of what is not finite among a tile's values 32 t .. 32 t + 31 that the
@@ -390,7 +409,7 @@
   // the last one the scores are of stale keys and not used.
   // The operands of the matrix instructions are read kAhead ahead; nothing
   // moves across a pair of weights, or the reads would all come first and spill.
-  constexpr int kPairs = 8 * KT, kQ = KT * QS, kP = DT * 2 * KT;
+  constexpr int kPairs = 8 * KT, kQ = KT * QS, kP = DT * 2 * KT, kW = TWO ? 2 : 1;
   auto step = [&](const f32x16* x, f32x16* y, const u32x4* w, u32x4* wn, int slot) {
     u32x4 f[kAhead + 1];
     auto frag = [&](int n) {
@@ -402,18 +421,22 @@
     for (int i = 0; i < kPairs; ++i) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int n = i * (kQ + kP) / kPairs; n < (i + 1) * (kQ + kP) / kPairs; ++n) {
-        if (n + kAhead < kQ + kP) f[(n + kAhead) % (kAhead + 1)] = frag(n + kAhead);
+      for (int u = i * (kQ + kW * kP) / kPairs; u < (i + 1) * (kQ + kW * kP) / kPairs; ++u) {
+        // the product's pieces serve a weight's kW parts each
+        const int n = u < kW * kP ? u / kW : u - (kW - 1) * kP, part = u < kW * kP ? u % kW : 0;
+        if (part == 0 && n + kAhead < kQ + kP) f[(n + kAhead) % (kAhead + 1)] = frag(n + kAhead);
         const u32x4& v = f[n % (kAhead + 1)];
         const int j = n - kP;
         if (j < 0)
-          o[n % DT] = M::mma32x16(v, w[n / DT], o[n % DT]);
+          o[n % DT] = M::mma32x16(v, w[2 * KT * part + n / DT], o[n % DT]);
         else
           y[j / QS] = M::mma32x16(v, qf[j % QS], j % QS ? y[j / QS] : f32x16{});
       }
       wn[i / 4][i & 3] = weigh(x, i);
+      if constexpr (TWO) wn[2 * KT + i / 4][i & 3] = low;
       if (i % 4 == 3) {  // here, and not where they are used
         asm volatile("" : "+v"(wn[i / 4]));
+        if constexpr (TWO) asm volatile("" : "+v"(wn[2 * KT + i / 4]));
         asm volatile("" : "+v"(add[0]), "+v"(add[1]), "+v"(add[2]), "+v"(add[3]));
       }
     }
@@ -436,9 +459,9 @@
       *reinterpret_cast<u32x4*>(lds + 3 * kTile + 16 * (i * NT + threadIdx.x)) = u32x4{0, 0, 0, 0};
     landed_barrier();
     f32x16 xa[KT], xb[KT];
-    u32x4 wa[2 * KT], wb[2 * KT];
+    u32x4 wa[2 * KT * kW], wb[2 * KT * kW];  // all weights' first parts, then their second ones
 #pragma unroll
-    for (int k = 0; k < 2 * KT; ++k) wb[k] = u32x4{0, 0, 0, 0};
+    for (int k = 0; k < 2 * KT * kW; ++k) wb[k] = u32x4{0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       xa[t] = f32x16{};
@@ -469,6 +492,10 @@
             const uint32_t two = see[k / 2] >> (16 * (k & 1) + 8 * (i / 2) + 2 * (i & 1));
             wn[k][i] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
             sum = M::add_pair(wn[k][i], sum);
+            if constexpr (TWO) {
+              wn[2 * KT + k][i] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+              sum = M::add_pair(wn[2 * KT + k][i], sum);
+            }
           }
       }
       if (moved) {
@@ -482,7 +509,11 @@
     auto drain = [&](const u32x4* w, int slot) {
       odd_values(it1 - 1, slot, exist1, all_of(exist1));
 #pragma unroll
-      for (int j = 0; j < kP; ++j) o[j % DT] = M::mma32x16(value_frag(slot, j % DT, j / DT), w[j / DT], o[j % DT]);
+      for (int j = 0; j < kP; ++j) {
+        const u32x4 v = value_frag(slot, j % DT, j / DT);
+        o[j % DT] = M::mma32x16(v, w[j / DT], o[j % DT]);
+        if constexpr (TWO) o[j % DT] = M::mma32x16(v, w[2 * KT + j / DT], o[j % DT]);
+      }
     };
     // two turns a round, so that no score or weight is moved between registers
     int it = it0;

@@ -566,8 +566,7 @@ int hgk_kv_append_slots(const hgk_kv_pages* pages, const int64_t* slots, int64_t
  * of the prefix what it would see of its own table: a sequence shorter than
  * the prefix sees its beginning. The prefix may end inside a page; its last
  * tokens are then read from the prefix's page, those behind them from the
- * sequences' own. Everything else as hgk_paged_attention, but that the prefix's
- * part of a row has its weights rounded to the dtype once also for single tokens.
+ * sequences' own. Everything else as hgk_paged_attention.
  */
 int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_kv_batch* batch,
                                 const int32_t* prefix_table, int64_t prefix_width, int64_t prefix_len,
