@@ -37,14 +37,27 @@ struct AttnArgs {
 };
 
 // Of a call whose sequences share a prefix: its pages, which stand for the sequences'
-// own where key < prefix; the parts that a row has of a pass of its own over those
-// keys (0: there is none, and the sequences' pass takes all keys); and all parts of a
-// row, which lie at [row][row_parts], the prefix's first. (Not in AttnArgs: the kernels
-// without a prefix are compiled otherwise with it, and slower by up to 4 %.)
+// own where key < prefix; the most parts that a row has of a pass of its own over those
+// keys (0: there is none, and the sequences' pass takes all keys); and the parts of a
+// row that lie together, at [row][row_parts]: prompts' all, the prefix's first; single
+// tokens' of the prefix, behind which their other parts lie at [chunk][head]. (Not in
+// AttnArgs: the kernels without a prefix are compiled otherwise with it, and slower by
+// up to 4 %.)
 struct PrefixArgs : AttnArgs {
   const int32_t* prefix_table;
   int32_t prefix_width, prefix, pre, row_parts;
-  int32_t chunk;  // single tokens: tiles of a part
+  // Single tokens: what their work is dealt out by, once the device has the lengths.
+  // A chunk has at least `least` tiles, and else as many as give `chunks` of all
+  // sequences' tiles, or `most` of the longest one's, whichever is fewer (`chunks` 0: the
+  // tables have room for no more than `least`). The pass over
+  // the prefix gets its share of the places on the chip by time: `pass` us of it, and
+  // `own` us for a tile of the other keys, if all places were its; a part of it takes
+  // `rows` blocks.
+  int32_t least, most, chunks, rows, places;
+  float pass, own;
+  // A chunk's tiles, the prefix's parts, whether chunk i is sequence i's, and if not, of
+  // each sequence the numbers of its first whole chunk and of its last one, which is shorter.
+  int32_t* found;
 };
 __device__ inline int32_t prefix_of(const AttnArgs&) { return 0; }
 __device__ inline int32_t prefix_of(const PrefixArgs& a) { return a.prefix; }

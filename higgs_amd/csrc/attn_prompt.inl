@@ -554,7 +554,7 @@
   int64_t part_at = (int64_t)(s.first + qi) * a.q_heads + head;
   if (keys == kOwn) part_at = part_at * splits + y;
   else part_at = part_at * row_parts_of(a) + (keys == kBehind ? pre_of(a) : 0) + y;
-  const bool parts = keys == kOwn ? splits > 1 : row_parts_of(a) > 1;
+  const bool parts = keys == kOwn ? splits > 1 : keys == kPrefix || row_parts_of(a) > 1;
   char* out_row = a.out + 2 * ((int64_t)(s.first + qi) * a.ost[0] + head * a.ost[1]);
   if (parts) {
     if (in && half == 0)

@@ -1,0 +1,118 @@
+"""shared_prefix_attention over tables with room for far more than the sequences hold, and
+batches with one long sequence: what single tokens' work is dealt out by is the lengths."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import higgs_amd as H
+import kv_ref as R
+from test_gpu_shared_prefix import BF16, F16, call, make, many
+
+pytestmark = pytest.mark.gpu
+
+
+def widen(d, pages):
+    """The same with tables of `pages` entries."""
+    t = d["table"]
+    wide = torch.full((t.shape[0], max(pages, t.shape[1])), -1, dtype=torch.int32, device=t.device)
+    wide[:, :t.shape[1]] = t
+    return {**d, "table": wide}
+
+
+@pytest.mark.parametrize("heads,kv_heads,head_dim,dtype", [(16, 2, 256, BF16), (32, 8, 128, F16), (32, 8, 64, BF16), (6, 2, 96, BF16)])
+@pytest.mark.parametrize("longest", [40, 700])
+@pytest.mark.parametrize("passes", [False, True])
+def test_wide_tables_give_the_same_bits(dev, heads, kv_heads, head_dim, dtype, longest, passes):
+    """Without a pass over the prefix and with one."""
+    prefix = 1030
+    batch = many(prefix, kv_heads, head_dim) if passes else 3
+    lens = [prefix + 1 + (97 * i + longest - 1) % longest for i in range(batch)]
+    x, y = make(91, prefix, lens, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page=16, dtype=dtype)
+    d = R.to(x, dev)
+    want = call(d, prefix)
+    R.check(want.cpu(), R.reference(y))
+    for pages in (300, 2048, 16384):
+        got = call(widen(d, pages), prefix)
+        if passes:
+            assert torch.equal(got, want), pages
+        else:  # the walks of four waves a block give way to chunks
+            R.check(got.cpu(), R.reference(y), str(pages))
+
+
+@pytest.mark.parametrize("batch", [2, 60, 257, 300, 700])
+@pytest.mark.parametrize("head_dim", [64, 256])
+@pytest.mark.parametrize("pages", [0, 1024])
+def test_one_long_sequence(dev, batch, head_dim, pages):
+    """In batches of which a thread has one sequence, or several."""
+    prefix, kv_heads = 520, 2
+    own = [0, 1, 33, 260, 64, 128, 9, 300]
+    lens = [prefix + own[(3 * i + i // 8) % 8] for i in range(batch)]
+    lens[batch // 2] = prefix + 7000
+    if batch > 2:
+        lens[0], lens[5], lens[-1] = 0, 100, prefix
+    x, y = make(92, prefix, lens, heads=4, kv_heads=kv_heads, head_dim=head_dim, page=16, dtype=BF16)
+    d = widen(R.to(x, dev), pages)
+    for kw in ({}, {"window": 2000, "sinks": 530}):
+        got = call(d, prefix, **kw)
+        R.check(got.cpu(), R.reference(y, **kw), str(kw))
+        assert torch.equal(got, call(d, prefix, **kw))
+
+
+@pytest.mark.parametrize("batch", [2, 90, 600])
+def test_lengths_that_grow_under_a_graph(dev, batch):
+    """Captured over short sequences, replayed over others: chunks, the prefix's parts and
+    whether a sequence has more than one chunk are found out anew."""
+    prefix, room = 1024, 4096
+    x, y = make(93, prefix, [prefix + room] * 2 + [prefix + 200] * (batch - 2), heads=8, kv_heads=2, head_dim=128, page=32,
+                dtype=BF16)
+    d = R.to(x, dev)
+    full = d["lens"].clone()
+    out = torch.empty_like(d["q"])
+    d["lens"].copy_(torch.full_like(full, prefix + 1))
+    call(d, prefix, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(d, prefix, out=out)
+    rows = torch.arange(batch, device=dev, dtype=torch.int32)
+    for lens in (full, full * 0, torch.minimum(full, prefix + 1 + rows), full // 2, torch.where(rows == 1, full, prefix + 3),
+                 torch.full_like(full, prefix + 1)):
+        d["lens"].copy_(lens)
+        out.fill_(7)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call(d, prefix))
+        z = {**y, "lens": lens.cpu()}
+        if batch > 100:  # some of them against the definition
+            z = {**z, "q": z["q"][:40], "table": z["table"][:40], "lens": z["lens"][:40]}
+        R.check(out[:len(z["lens"])].cpu(), R.reference(z))
+
+
+def fastest(f):
+    f()
+    best = float("inf")
+    for _ in range(8):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        for _ in range(5):
+            f()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b))
+    return best
+
+
+def test_time_goes_by_the_lengths(dev):
+    """Tables of 32 times the room made these calls three times as long, and one sequence of
+    30000 tokens among 512 three times as long as without a shared prefix."""
+    prefix = 4096
+    lens = [prefix + 1 + 37 * i % 600 for i in range(64)]
+    d = R.to(make(94, prefix, lens, heads=16, kv_heads=2, head_dim=256, page=32, dtype=BF16)[0], dev)
+    wide = widen(d, 4096)
+    assert fastest(lambda: call(wide, prefix)) < 1.6 * fastest(lambda: call(d, prefix))
+    prefix = 1024
+    lens = [prefix + 1 + 37 * i % 90 for i in range(400)]
+    lens[7] = prefix + 20000
+    x, y = make(95, prefix, lens, heads=16, kv_heads=4, head_dim=128, page=32, dtype=BF16)
+    d, e = R.to(x, dev), R.to(y, dev)
+    assert fastest(lambda: call(d, prefix)) < fastest(lambda: R.call(H, e))
