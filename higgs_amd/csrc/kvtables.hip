@@ -9,8 +9,9 @@ namespace hgk {
 namespace {
 
 constexpr int kPlanThreads = 1024, kMaxRows = 1 << 18, kFill = 256, kNear = 4096;
-// Calls in one launch: at most so many sequences, resident ones and blocks.
-constexpr int kOneBatch = 1024, kOneRows = 1 << 15, kOneBlocks = 512;
+// Calls in one launch: at most so many sequences (releases of named ones: fewer),
+// resident ones and blocks.
+constexpr int kOneBatch = 1024, kOneNamed = 640, kOneRows = 1 << 15, kOneBlocks = 512;
 
 struct TablesView {
   int32_t* table;
@@ -261,10 +262,12 @@ __global__ __launch_bounds__(kFill) void kv_release_kernel(PlanArgs a) {
     release_row(a, i, a.lens_out[a.seqs ? a.seqs[i] : i], from, n, *a.n_free_out - a.page_starts[a.batch]);
 }
 
-// A call in one launch: every block works the sums out for itself, which takes few
-// sequences no longer than a second launch, and the state must not be written where
-// other blocks still read it. (64 sequences of 1024-page tables: 4.4 us, in two
-// launches 6.5.)
+// A call in one launch: every block works the sums out for itself, and the state must
+// not be written where other blocks still read it. In us, in a graph, in one launch and
+// in two: 64 sequences given a token each 4.4, 6.3; 512 6.1, 8.3; 1000 8.6, 9.5; up to 64
+// tokens each 4.5, 7.5; 6.2, 9.0; 8.8, 10.3. Releases 3.6, 6.3; 5.0, 6.6; 7.4, 7.6; of
+// named ones, which are looked up and marked in every block, 64 of 96 4.1, 6.6; 512 of
+// 768 6.2, 7.4; 768 of 1152 8.8, 7.9; 1000 of 1500 10.3, 8.7. (In place, always two.)
 template <bool RELEASE>
 __global__ __launch_bounds__(kFill) void kv_one_kernel(ExtendArgs x) {
   __shared__ int32_t pages[kOneBatch + 1], tokens[kOneBatch + 1];
@@ -328,9 +331,9 @@ int check_batch(const char* what, const TablesView& t, const int32_t* seqs, int6
   return HGK_OK;
 }
 
-// One launch will do: few sequences, and a state that is not written in place.
+// One launch is faster, and the state is not written in place.
 bool in_one(const PlanArgs& a) {
-  return a.batch <= kOneBatch && a.t.rows <= kOneRows && a.lens_out != a.t.lens && a.n_free_out != a.t.n_free;
+  return a.batch <= (a.release && a.seqs ? kOneNamed : kOneBatch) && a.t.rows <= kOneRows && a.lens_out != a.t.lens && a.n_free_out != a.t.n_free;
 }
 
 }  // namespace
