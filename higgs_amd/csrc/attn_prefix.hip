@@ -39,19 +39,6 @@ template <int D> struct DecodeSums {
 
 // One wave's walk over the tiles first, first + STEP, ... below last of a run of n
 // keys of a kv head; key_of(i) is the position of key i, page_of(position) its page.
-//
-// A tile's scores are S^T = K Q^T on 16x16x32 matrix instructions: keys are
-// the rows, so K's 16-byte pieces go from memory straight into the operand,
-// and a lane ends with 4 keys each of one head. That is also where the second
-// product O^T = V^T P^T wants its weights: no weight crosses lanes. V^T comes
-// through LDS (written row by row, read transposed). K and V of the next tile
-// are in flight while a tile is computed.
-//
-// Weights are split in two 16-bit parts (hi + lo, both multiplied): the
-// matrix cores have time to spare, and two parts keep 16 bits of a weight in
-// bf16 and 22 in f16, well below the result's own rounding.
-// (attn_decode_kernel has this loop in its own body: through a function it takes 4
-// registers more.)
 template <class T, int D, int CAP, int STEP, class Key, class Page>
 __device__ __forceinline__ DecodeSums<D> decode_walk(const PrefixArgs& a, const Scale& sc, const u32x4 (&qf)[D / 32],
                                                      int hk, int first, int last, int n, char* vt, Key key_of,
@@ -60,135 +47,13 @@ __device__ __forceinline__ DecodeSums<D> decode_walk(const PrefixArgs& a, const 
   const int lane = threadIdx.x & 63, m = lane & 15, j = lane >> 4;
   const char* kbase = a.p.k + 2 * (hk * a.p.kst[2] + 8 * j);
   const char* vbase = a.p.v + 2 * (hk * a.p.vst[2] + 8 * j);
-  // page of key i of the run (-1: none) and its place in the page
-  auto look_up = [&](int tile, int32_t* page, int32_t* at) {
-#pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      const int i = tile * kKeys + 16 * h + m;
-      page[h] = -1;
-      at[h] = 0;
-      if (tile < last && i < n) {
-        const int32_t key = key_of(i);
-        page[h] = page_of(key);
-        at[h] = key & a.p.page_mask;
-      }
-    }
-  };
-  u32x4 kr[NS][kStep], vr[NS][kStep];
-  uint32_t there = 0;  // bit i: key i of the loaded tile exists
-  auto load = [&](const int32_t* page, const int32_t* at) {
-    there = 0;
-#pragma unroll
-    for (int h = 0; h < NS; ++h) {
-      const bool ok = (uint32_t)page[h] < (uint32_t)a.p.n_pages;
-      there |= (uint32_t)(__ballot(ok) & 0xffffu) << (16 * h);
-      // a key that does not exist reads the pool's first row, and is masked below
-      const int64_t pg = ok ? page[h] : 0, r = ok ? at[h] : 0;
-      const char* kp = kbase + 2 * (pg * a.p.kst[0] + r * a.p.kst[1]);
-      const char* vp = vbase + 2 * (pg * a.p.vst[0] + r * a.p.vst[1]);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) kr[h][s] = *reinterpret_cast<const u32x4*>(kp + 64 * s);
-#pragma unroll
-      for (int s = 0; s < kStep; ++s) vr[h][s] = *reinterpret_cast<const u32x4*>(vp + 64 * s);
-    }
-  };
-
-  DecodeSums<D> acc;
-  f32x4(&o)[kOut] = acc.o;
-#pragma unroll
-  for (int t = 0; t < kOut; ++t) o[t] = f32x4{0, 0, 0, 0};
-  float ref = lowest_ref(sc.c), sum = 0.0f;
-  const float slack = Mx<T>::kDecSlack / sc.c;
-  bool any = false;
-  constexpr uint32_t kAll = NS == 2 ? 0xffffffffu : 0xffffu;
-
-  int32_t page[NS], at[NS];
-  if (a.p.n_pages > 0 && first < last) {
-    look_up(first, page, at);
-    load(page, at);
-    look_up(first + STEP, page, at);
-    for (int tile = first; tile < last; tile += STEP) {
-      // scores
-      f32x4 s[NS];
-#pragma unroll
-      for (int h = 0; h < NS; ++h) {
-        s[h] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < kStep; ++k) s[h] = Mx<T>::mma16x32(kr[h][k], qf[k], s[h]);
-      }
-      const uint32_t now = there;
-      if (now != kAll) {  // values that do not exist must not be multiplied by their zero weight
-#pragma unroll
-        for (int h = 0; h < NS; ++h)
-          if (!((now >> (16 * h + m)) & 1))
-#pragma unroll
-            for (int k = 0; k < kStep; ++k) vr[h][k] = u32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int h = 0; h < NS; ++h)
-#pragma unroll
-        for (int k = 0; k < kStep; ++k)
-          *reinterpret_cast<u32x4*>(vt + (16 * h + m) * kRow + 64 * k + 16 * j) = vr[h][k];
-      if (tile + STEP < last) {
-        load(page, at);
-        look_up(tile + 2 * STEP, page, at);
-      }
-      // weights
-      float x[4 * NS], top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) {
-        x[i] = s[i / 4][i % 4];
-        if constexpr (CAP) x[i] = cap_tanh<CAP>(x[i] * sc.inner);
-      }
-      const uint32_t mine = now >> (4 * j);  // this lane's keys: bits 0..3 and 16..19
-      if (now != kAll) {
-#pragma unroll
-        for (int i = 0; i < 4 * NS; ++i)
-          if (!((mine >> (16 * (i / 4) + i % 4)) & 1)) x[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) top = fmaxf(top, x[i]);
-      if (__any(top > ref + slack)) {  // a head's own scores alone decide for it
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float to = top > ref + slack ? top : ref, f = lesser((ref - to) * sc.c);
-        sum *= f;
-#pragma unroll
-        for (int t = 0; t < kOut; ++t) o[t] *= f;
-        ref = to;
-      }
-      const float base = fmaf(-ref, sc.c, Mx<T>::kDecBias);
-#pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], sc.c, base));
-      any |= now != 0;
-      uint32_t hi[2 * NS], lo[2 * NS];
-#pragma unroll
-      for (int i = 0; i < 2 * NS; ++i) {
-        sum += x[2 * i] + x[2 * i + 1];
-        hi[i] = Mx<T>::pack(x[2 * i], x[2 * i + 1]);
-        lo[i] = Mx<T>::pack(x[2 * i] - T::lo(hi[i]), x[2 * i + 1] - T::hi(hi[i]));
-      }
-      // O^T += V^T P^T
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int t = 0; t < kOut; ++t) {
-        const char* p = vt + (4 * j + m / 4) * kRow + 32 * t + 8 * (m & 3);
-        const u32x2 v0 = lds_transposed(p);
-        if constexpr (NS == 2) {
-          const u32x2 v1 = lds_transposed(p + 16 * kRow);
-          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-          o[t] = Mx<T>::mma16x32(v, u32x4{hi[0], hi[1], hi[2], hi[3]}, o[t]);
-          o[t] = Mx<T>::mma16x32(v, u32x4{lo[0], lo[1], lo[2], lo[3]}, o[t]);
-        } else {
-          o[t] = Mx<T>::mma16x16(v0, u32x2{hi[0], hi[1]}, o[t]);
-          o[t] = Mx<T>::mma16x16(v0, u32x2{lo[0], lo[1]}, o[t]);
-        }
-      }
-      __builtin_amdgcn_wave_barrier();
-    }
-  }
+  const int begin = first;
+#include "attn_walk.inl"
   sum += __shfl_xor(sum, 16);
   sum += __shfl_xor(sum, 32);
+  DecodeSums<D> acc;
+#pragma unroll
+  for (int t = 0; t < kOut; ++t) acc.o[t] = o[t];
   acc.ref = ref;
   acc.sum = sum;
   acc.any = any;
@@ -204,61 +69,15 @@ __device__ __forceinline__ bool decode_odd(const Scale& sc, const DecodeSums<D>&
   return x.any && !(fabsf(x.ref * sc.c) <= kBaseMax && peak < INFINITY);
 }
 
-// Such heads' keys once more, one after the other in f32. The reference is the
-// maximum, subtracted before the scale, and an infinity or NaN among the values
-// counts however small its key's weight is (the two parts of a weight would
-// not do: the lesser one may be zero or negative). Lane: head m, a quarter of D.
-// qp: the lane's head's q from its quarter on. Returns the head's reference and sum.
+// Such heads' keys once more. qp: the lane's head's q from its quarter of D on. Returns
+// the head's reference and sum.
 template <class T, int D, int CAP, int STEP, class Key, class Page>
 __device__ __forceinline__ f32x2 decode_again(const PrefixArgs& a, const Scale& sc, const char* qp, int hk, int first,
                                               int last, int n, Key key_of, Page page_of, float (&acc)[D / 4]) {
   constexpr int kKeys = dec_keys<D>();
   const int j = (threadIdx.x & 63) >> 4;
-  constexpr int kPieces = D / 32;
-  float r = lowest_ref(sc.c), l = 0.0f;
-#pragma unroll
-  for (int d = 0; d < D / 4; ++d) acc[d] = 0.0f;
-#pragma unroll 1
-  for (int i = first * kKeys; i < min(last * kKeys, n); i += (i + 1) % kKeys ? 1 : 1 + (STEP - 1) * kKeys) {
-    const int32_t key = key_of(i), pg = page_of(key);
-    if ((uint32_t)pg >= (uint32_t)a.p.n_pages) continue;
-    const int64_t row = key & a.p.page_mask;
-    const char* kp = a.p.k + 2 * (hk * a.p.kst[2] + pg * a.p.kst[0] + row * a.p.kst[1] + j * (D / 4));
-    const char* vp = a.p.v + 2 * (hk * a.p.vst[2] + pg * a.p.vst[0] + row * a.p.vst[1] + j * (D / 4));
-    float x = 0.0f;
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-      const u32x4 kw = *reinterpret_cast<const u32x4*>(kp + 16 * c);
-      const u32x4 qw = *reinterpret_cast<const u32x4*>(qp + 16 * c);
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const uint32_t qq = (qw[w] & sc.keep) ^ sc.flip;
-        x = fmaf(T::hi(kw[w]), T::hi(qq), fmaf(T::lo(kw[w]), T::lo(qq), x));
-      }
-    }
-    x += __shfl_xor(x, 16);
-    x += __shfl_xor(x, 32);
-    if constexpr (CAP) x = cap_tanh<CAP>(x * sc.inner);
-    if (x > r) {
-      const float f = lesser((r - x) * sc.c);
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < D / 4; ++d) acc[d] *= f;
-      r = x;
-    }
-    const float w = __builtin_amdgcn_exp2f(fmaf(x - r, sc.c, Mx<T>::kDecBias));
-    const float odd = x == -INFINITY ? w : fmaxf(w, 1.0e-44f);
-    l += w;
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-      const u32x4 vw = *reinterpret_cast<const u32x4*>(vp + 16 * c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = e & 1 ? T::hi(vw[e / 2]) : T::lo(vw[e / 2]);
-        acc[8 * c + e] = fmaf(v, fabsf(v) < INFINITY ? w : odd, acc[8 * c + e]);
-      }
-    }
-  }
+  const int begin = first;
+#include "attn_again.inl"
   return f32x2{r, l};
 }
 
