@@ -39,6 +39,7 @@ class KVBatch(NamedTuple):
 
 class _CacheBatch(KVBatch):
     """A batch of a cache's sequences, which knows what they share."""
+    _host = _shared = None
 
     def shared(self, page_size: int) -> int:
         """The tokens that all of the batch's sequences have on the same pages at their beginning."""
@@ -232,7 +233,7 @@ class PagedKVCache:
         if counts is not None:
             starts = torch.from_numpy(np.cumsum([0, *counts]).astype(np.int32)).to(dev)
         batch = _CacheBatch(torch.from_numpy(table).to(dev), lens, starts)
-        batch._host, batch._shared = (table, [s.length for s in found]), None
+        batch._host = table, [s.length for s in found]
         return batch
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch: KVBatch) -> None:
@@ -247,7 +248,7 @@ class PagedKVCache:
         read and multiplied once for all: shared_prefix_attention. A ``prefix`` past
         what the sequences of a batch() shared when it was made is refused."""
         if prefix:
-            if isinstance(batch, _CacheBatch) and prefix > batch.shared(self.page_size):
+            if isinstance(batch, _CacheBatch) and batch._host and prefix > batch.shared(self.page_size):
                 raise HgkError(1, f"PagedKVCache: prefix={prefix}, but the batch's sequences share "
                                   f"{batch.shared(self.page_size)} tokens")
             pages = batch.block_table[:1].flatten()[:-(-prefix // self.page_size)]

@@ -75,4 +75,5 @@ def test_batches_are_what_they_were(cache):
     assert table.tolist() == [c.pages(a), c.pages(b) + [-1, -1]]
     # a batch made otherwise is the caller's own affair
     c.attend(0, None, KVBatch(table, lens, None), prefix=33)
-    assert len(c.calls) == 1
+    c.attend(0, None, batch._replace(kv_lens=lens + 1), prefix=33)
+    assert len(c.calls) == 2

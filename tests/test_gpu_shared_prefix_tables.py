@@ -59,6 +59,18 @@ def test_one_long_sequence(dev, batch, head_dim, pages):
         assert torch.equal(got, call(d, prefix, **kw))
 
 
+def test_thousands_of_sequences(dev):
+    """20 of them a thread, a long one and empty ones among them."""
+    prefix, batch = 64, 5000
+    lens = [prefix + 7 * i % 150 for i in range(batch)]
+    lens[4321], lens[0], lens[4999] = prefix + 9000, 0, 0
+    x, y = make(96, prefix, lens, heads=2, kv_heads=1, head_dim=64, page=16, dtype=BF16)
+    d = R.to(x, dev)
+    got = call(d, prefix)
+    R.check(got.cpu(), R.reference(y))
+    assert torch.equal(got, call(widen(d, 1000), prefix))
+
+
 @pytest.mark.parametrize("batch", [2, 90, 600])
 def test_lengths_that_grow_under_a_graph(dev, batch):
     """Captured over short sequences, replayed over others: chunks, the prefix's parts and
