@@ -413,6 +413,20 @@
   auto step = [&](const f32x16* x, f32x16* y, const u32x4* w, u32x4* wn, int slot) {
     u32x4 f[kAhead + 1];
     auto frag = [&](int n) {
+      if constexpr (kLean && CAP) {  // with tanh no room for the places' variants either: worked out for each piece
+        auto other = [](uint32_t at, uint32_t mask) {
+          uint32_t r = at;
+          if (mask) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(r) : "v"(mask), "v"(at));
+          return r;
+        };
+        if (n < kP) {
+          const char* vt = lds + (2 + (slot ^ 1)) * kTile + 16 * (n / DT) * kRow + other(vat, 64 * (n % DT));
+          const u32x2 v0 = lds_transposed(vt), v1 = lds_transposed(vt + 8 * kRow);
+          return u32x4{v0[0], v0[1], v1[0], v1[1]};
+        }
+        const int j = n - kP;
+        return *reinterpret_cast<const u32x4*>(lds + (slot ^ 1) * kTile + 32 * (j / QS) * kRow + other(kat, 32 * (j % QS)));
+      }
       return n < kP ? value_frag(slot ^ 1, n % DT, n / DT) : key_frag(slot ^ 1, (n - kP) / QS, (n - kP) % QS);
     };
 #pragma unroll
