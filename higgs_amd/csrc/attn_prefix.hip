@@ -783,7 +783,7 @@ extern "C" int hgk_shared_prefix_attention(const hgk_kv_pages* pages, const hgk_
   a.chunks = s.chunks;
   a.rows = s.rows;
   a.places = s.places;
-  a.pass = s.pass;
+  a.pass = softcap > 0.0f ? 1.3f * s.pass : s.pass;  // (the tanh)
   a.own = s.own;
   a.part = static_cast<float*>(workspace);
   a.stat = parts > 0 ? a.part + parts * a.p.head_dim : nullptr;
